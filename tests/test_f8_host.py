@@ -1,0 +1,120 @@
+"""What the 8-bit operators refuse, through the C-ABI and the Python wrappers
+(no GPU: every call is rejected before a launch)."""
+
+import pytest
+import torch
+
+from tjkernels import _lib, ops
+from tjkernels._lib import BF16, E4M3, EINVAL, EUNSUPPORTED, F16, F32, TjkError
+
+FAKE = 1 << 20  # a pointer that is never followed
+
+
+def _norm(**kw):
+    a = dict(res=FAKE, res_dtype=F32, ld_res=256, delta=FAKE, delta_dtype=BF16, ld_delta=256, res_out=FAKE + 4096,
+             res_out_dtype=F32, ld_res_out=256, out=FAKE, out_dtype=E4M3, ld_out=256, scales=FAKE, ld_scales=2, gamma=FAKE,
+             rows=4, n=256, eps=1e-5, stream=None)
+    a.update(kw)
+    return _lib.load().tjk_add_rmsnorm(*a.values())
+
+
+def _quant(**kw):
+    a = dict(x=FAKE, x_dtype=BF16, ld_x=256, q=FAKE, ld_q=256, scales=FAKE, ld_scales=2, rows=4, n=256, block_rows=1,
+             stream=None)
+    a.update(kw)
+    return _lib.load().tjk_quantize_f8(*a.values())
+
+
+def _gemm(**kw):
+    a = dict(a=FAKE, lda=256, a_scales=FAKE, ld_as=2, w=FAKE, ldw=256, w_scales=FAKE, ld_ws=2, bias=FAKE, c=FAKE,
+             out_dtype=BF16, ldc=128, c_scales=None, ld_cs=0, m=4, n=128, k=256, epilogue=0, plan=-1, stream=None)
+    a.update(kw)
+    return _lib.load().tjk_gemm_f8(*a.values())
+
+
+def _said():
+    return _lib.load().tjk_last_error_string().decode()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(rows=-1), EINVAL, "shape"), (dict(n=0), EINVAL, "shape"), (dict(n=252), EUNSUPPORTED, "multiple of 8"),
+    (dict(n=32776), EUNSUPPORTED, "32768"), (dict(res=None), EINVAL, "null"), (dict(out=None), EINVAL, "null"),
+    (dict(gamma=None), EINVAL, "null"), (dict(scales=None), EINVAL, "null"),
+    (dict(res_dtype=E4M3), EINVAL, "dtype"), (dict(delta_dtype=9), EINVAL, "dtype"),
+    (dict(res_out_dtype=E4M3), EINVAL, "dtype"), (dict(out_dtype=4), EINVAL, "dtype"),
+    (dict(ld_res=248), EINVAL, "leading"), (dict(ld_out=255), EINVAL, "leading"), (dict(ld_delta=0), EINVAL, "leading"),
+    (dict(ld_scales=1), EINVAL, "leading"), (dict(ld_res=260), EUNSUPPORTED, "multiples of 8"),
+    (dict(ld_delta=257), EUNSUPPORTED, "multiples of 8"), (dict(res=FAKE + 8), EUNSUPPORTED, "misaligned"),
+    (dict(out=FAKE + 4), EUNSUPPORTED, "misaligned"), (dict(scales=FAKE + 2), EUNSUPPORTED, "misaligned"),
+    (dict(gamma=FAKE + 4), EUNSUPPORTED, "misaligned"), (dict(res_out=FAKE + 8), EUNSUPPORTED, "misaligned"),
+    (dict(res_out=FAKE, res_out_dtype=F16, delta=None), EINVAL, "alias"),
+    (dict(res_out=FAKE, ld_res_out=264, delta=None), EINVAL, "alias"),
+    (dict(res=FAKE + 64, res_out=FAKE), EINVAL, "alias"),  # fp32 into a bf16 delta
+    (dict(rows=1 << 31), EUNSUPPORTED, "int32"),
+])
+def test_norm_refusals(kw, status, word):
+    assert _norm(**kw) == status and word in _said()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(rows=-1), EINVAL, "shape"), (dict(n=-8), EINVAL, "shape"), (dict(block_rows=64), EINVAL, "block_rows"),
+    (dict(x_dtype=E4M3), EINVAL, "dtype"), (dict(n=100), EUNSUPPORTED, "multiple of 8"),
+    (dict(n=(1 << 20) + 8), EUNSUPPORTED, "2^20"), (dict(x=None), EINVAL, "null"), (dict(q=None), EINVAL, "null"),
+    (dict(scales=None), EINVAL, "null"), (dict(ld_x=200), EINVAL, "leading"), (dict(ld_q=200), EINVAL, "leading"),
+    (dict(ld_scales=1), EINVAL, "leading"), (dict(ld_x=260), EUNSUPPORTED, "multiples of 8"),
+    (dict(x=FAKE + 8), EUNSUPPORTED, "misaligned"), (dict(q=FAKE + 4), EUNSUPPORTED, "misaligned"),
+    (dict(rows=1 << 40), EUNSUPPORTED, "too many"), (dict(rows=1 << 40, block_rows=128), EUNSUPPORTED, "too many"),
+])
+def test_quantize_refusals(kw, status, word):
+    assert _quant(**kw) == status and word in _said()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(m=-1), EINVAL, "negative"), (dict(k=-16), EINVAL, "negative"), (dict(epilogue=2), EINVAL, "epilogue"),
+    (dict(epilogue=-1), EINVAL, "epilogue"), (dict(out_dtype=F32), EINVAL, "dtype"), (dict(out_dtype=7), EINVAL, "dtype"),
+    (dict(plan=-2), EINVAL, "plan"), (dict(plan=1000), EINVAL, "plan"), (dict(a=None), EINVAL, "null"),
+    (dict(w_scales=None), EINVAL, "null"), (dict(out_dtype=E4M3), EINVAL, "null"), (dict(c=None), EINVAL, "null"),
+    (dict(k=248), EUNSUPPORTED, "multiple of 16"), (dict(n=126), EUNSUPPORTED, "multiple of 4"),
+    (dict(lda=240), EINVAL, "leading"), (dict(ldw=0), EINVAL, "leading"), (dict(ldc=124), EINVAL, "leading"),
+    (dict(ld_as=1), EINVAL, "leading"), (dict(ld_ws=1), EINVAL, "leading"),
+    (dict(out_dtype=E4M3, c_scales=FAKE, n=256, ldc=256, ld_cs=1), EINVAL, "leading"),
+    (dict(lda=264), EUNSUPPORTED, "multiples of 16"), (dict(ldc=130), EUNSUPPORTED, "multiple of 4"),
+    (dict(lda=1 << 23), EUNSUPPORTED, "too large"), (dict(ld_as=1 << 21), EUNSUPPORTED, "too large"),
+    (dict(a=FAKE + 8), EUNSUPPORTED, "misaligned"), (dict(c=FAKE + 4), EUNSUPPORTED, "misaligned"),
+    (dict(bias=FAKE + 2), EUNSUPPORTED, "misaligned"), (dict(a_scales=FAKE + 1), EUNSUPPORTED, "misaligned"),
+    (dict(m=1 << 31), EUNSUPPORTED, "int32"),
+])
+def test_gemm_refusals(kw, status, word):
+    assert _gemm(**kw) == status and word in _said()
+
+
+def test_nothing_to_do_is_no_error():
+    assert _norm(rows=0, res=None) == 0
+    assert _quant(rows=0, x=None) == 0
+    assert _gemm(m=0, a=None) == 0
+    assert _gemm(n=0, w=None, ldc=0) == 0
+
+
+def test_wrappers_take_device_tensors_only():
+    x = torch.zeros(4, 128)
+    q, s = torch.zeros(4, 128, dtype=ops.F8), torch.zeros(4, 1)
+    with pytest.raises(TjkError, match="device tensors"):
+        ops.quantize_f8(x, q, s)
+    with pytest.raises(TjkError, match="device tensors"):
+        ops.add_rmsnorm(x, None, torch.ones(128), 1e-5, q, scales=s)
+    with pytest.raises(TjkError, match="device tensors"):
+        ops.gemm_f8(q, s, q, s, None, torch.zeros(4, 4, dtype=torch.bfloat16))
+
+
+def test_scale_layouts():
+    """Scales: fp32, enough rows and blocks, unit column stride, no row
+    repeated by a zero stride; one row or one block may have any stride."""
+    ok = ops._f8_scales
+    assert ok(torch.zeros(4, 3), 4, 260, "s") == 3
+    assert ok(torch.zeros(4, 8)[:, :3], 4, 260, "s") == 8
+    assert ok(torch.zeros(1, 3).t().contiguous().t(), 1, 260, "s") == 3
+    assert ok(torch.zeros(4, 8)[:, 2:3], 4, 128, "s") == 8
+    for bad in (None, torch.zeros(4, 2), torch.zeros(3, 3), torch.zeros(4, 3, dtype=torch.float64),
+                torch.zeros(3, 4).t(), torch.zeros(1, 3).expand(4, 3), torch.zeros(12)):
+        with pytest.raises(TjkError, match="float32"):
+            ok(bad, 4, 260, "s")

@@ -1,0 +1,350 @@
+"""The 8-bit operators against 64-bit results of the same inputs: the RMS
+norm and quantisation to e4m3 with block scales, and the block-scaled
+product.  Tolerances are bounds on the kernels' own roundings, derived
+beside each."""
+
+import math
+
+import pytest
+import torch
+
+from tjkernels import ops
+from tjkernels.ops import EPI_BIAS, EPI_BIAS_GELU, F8
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24  # half a unit in the last place of fp32, relative
+MIN_SCALE = 2.0 ** -126
+
+
+def _gen(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _inside(rows, cols, dtype, device, pad_cols=16, fill=None):
+    """A [rows, cols] view inside a larger buffer (its neighbours NaN unless
+    `fill` is given) and the buffer."""
+    lead = -(-cols // 16) * 16 + pad_cols
+    whole = torch.full((rows + 3, lead), float("nan") if fill is None else fill, device=device).to(dtype)
+    return whole[1:1 + rows, :cols], whole
+
+
+def _untouched(whole, rows, cols, fill):
+    """Whether everything of `whole` but its view holds `fill` (NaN: None)."""
+    keep = torch.ones(whole.shape, dtype=torch.bool)
+    keep[1:1 + rows, :cols] = False
+    w = whole.float().cpu()[keep]
+    return bool(torch.isnan(w).all()) if fill is None else bool((w == fill).all())
+
+
+def _half_step(v):
+    """Half a step of e4m3 at |v|: 2^-4 of its power of two, 2^-10 among the
+    subnormals."""
+    e = torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -40)))
+    return torch.maximum(torch.exp2(e - 4), torch.full_like(v, 2.0 ** -10))
+
+
+def _check_quantised(q, scales, y, block_rows, y_err):
+    """q, scales (of the device) against the 64-bit y, known to the kernel to
+    within y_err (absolute, per element).  The scale is the largest kernel
+    value times 1 / 448 (two roundings); q the kernel value times a reciprocal
+    of the scale good to one unit in the last place, so another 4 U, then
+    rounded to nearest."""
+    rows, n = y.shape
+    q, scales = q.float().double().cpu(), scales.double().cpu()
+    assert scales.shape == (-(-rows // block_rows), _blocks(n))
+    for b in range(_blocks(n)):
+        part, err, got = y[:, 128 * b:128 * b + 128], y_err[:, 128 * b:128 * b + 128], q[:, 128 * b:128 * b + 128]
+        top = torch.stack([t.abs().max() for t in part.split(block_rows)])
+        slack = torch.stack([t.max() for t in err.split(block_rows)])
+        s = scales[:, b]
+        assert ((s - (top / 448).clamp(min=MIN_SCALE)).abs() <= slack / 448 + 2 * 2 * U * s).all()
+        each = s.repeat_interleave(block_rows)[:rows, None]
+        v = part / each
+        bad = ~((got - v).abs() <= _half_step(v) + err / each + 8 * U * v.abs())
+        assert not bad.any(), f"block {b}: {int(bad.sum())} values off"
+
+
+# -------------------------------------------------------------- quantisation
+
+@pytest.mark.parametrize("rows,n", [(1, 8), (1, 128), (3, 120), (7, 136), (129, 1008), (64, 512), (257, 2600), (5, 8192)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize(device, rows, n, dt, block_rows):
+    g = _gen(rows * n)
+    x = torch.randn(rows, n, generator=g) * torch.exp(torch.randn(rows, 1, generator=g))
+    x[rows // 2] = 0
+    view, _ = _inside(rows, n, DT[dt], device)
+    view.copy_(x)
+    q, whole = _inside(rows, n, F8, device, fill=2.0)
+    rb = -(-rows // block_rows)
+    scales = torch.full((rb + 2, _blocks(n) + 3), 7.0, device=device)
+    ops.quantize_f8(view, q, scales[1:1 + rb, :_blocks(n)], block_rows=block_rows)
+    torch.cuda.synchronize()
+    y = x.to(DT[dt]).double()
+    _check_quantised(q, scales[1:1 + rb, :_blocks(n)], y, block_rows, torch.zeros_like(y))
+    assert _untouched(whole, rows, n, 2.0)
+    outside = scales.clone()
+    outside[1:1 + rb, :_blocks(n)] = 7.0
+    assert (outside == 7.0).all()
+
+
+def test_quantize_is_exact_where_it_can_be(device):
+    """Every finite e4m3 value times a power of two, with 448 in each block,
+    comes back as it was."""
+    vals = torch.arange(256, dtype=torch.uint8).view(F8).float()
+    vals = vals[torch.isfinite(vals)]
+    row = torch.cat([vals, torch.full((2,), 448.0)])  # 256: the second block ends in +448s
+    row[0] = 448.0
+    x = torch.stack([row * 2.0 ** e for e in (-20, -3, 0, 5, 60)])
+    q = torch.empty(x.shape, dtype=F8, device=device)
+    s = torch.empty(5, 2, device=device)
+    ops.quantize_f8(x.to(device), q, s)
+    got = q.float().cpu() * s.cpu().repeat_interleave(128, dim=1)
+    # 1 / 448 is rounded: a scale is off its power of two by one unit at most
+    assert ((got - x).abs() <= 2 * 2 * U * x.abs()).all()
+    assert torch.equal(q.float().cpu(), row.expand(5, -1))
+
+
+def test_quantize_special_values(device):
+    """A NaN stays one and does not reach the scale; an infinity makes its
+    block's scale infinite; zeros and the smallest numbers keep a normal
+    scale; other blocks are not touched by either."""
+    x = torch.ones(6, 256)
+    x[0, 5] = float("nan")
+    x[1, 130] = float("inf")
+    x[2, :128] = 0
+    x[3, :128] = 2.0 ** -149
+    x[4] = 3e38
+    x[5, 128:] = -0.0
+    q = torch.empty(x.shape, dtype=F8, device=device)
+    s = torch.empty(6, 2, device=device)
+    ops.quantize_f8(x.to(device), q, s)
+    q, s = q.float().cpu(), s.cpu()
+    one = torch.tensor(1 / 448)
+    assert torch.isnan(q[0, 5]) and torch.isfinite(q[0]).sum() == 255
+    assert torch.allclose(s[0], one.expand(2), rtol=4 * U)
+    assert s[1, 1] == float("inf") and (q[1, 131:] == 0).all() and torch.isnan(q[1, 130])
+    assert (q[1, :128] == 448).all()
+    assert s[2, 0] == MIN_SCALE and (q[2, :128] == 0).all()
+    assert s[3, 0] == MIN_SCALE and (q[3, :128] == 0).all()
+    assert torch.isfinite(s[4]).all() and (q[4] == 448).all()
+    assert s[5, 1] == MIN_SCALE and (q[5, 128:] == 0).all()
+
+
+def test_quantize_nothing(device):
+    q = torch.empty(0, 128, dtype=F8, device=device)
+    ops.quantize_f8(torch.empty(0, 128, device=device), q, torch.empty(0, 1, device=device))
+
+
+# ------------------------------------------------------------------ RMS norm
+
+# Relative error of y before its last rounding: at most 32 + 6 + 16 additions
+# in a sum of squares, halved by the root; mean, eps, root, reciprocal and two
+# products add 7 more.
+Y_ERR = (27 + 8) * U
+
+
+def _norm_case(rows, n, res_dt, delta_dt, seed, device):
+    g = _gen(seed)
+    res, res_whole = _inside(rows, n, DT[res_dt], device)
+    res.copy_(torch.randn(rows, n, generator=g) * torch.exp(torch.randn(rows, 1, generator=g)))
+    delta = None
+    if delta_dt is not None:
+        delta, _ = _inside(rows, n, DT[delta_dt], device, pad_cols=32)
+        delta.copy_(torch.randn(rows, n, generator=g))
+    gamma = 1 + 0.2 * torch.randn(n, generator=g)
+    x = res.float().cpu() + (0 if delta is None else delta.float().cpu())  # one fp32 addition
+    y = x.double() / (x.double().square().mean(dim=1, keepdim=True) + 1e-5).sqrt() * gamma.double()
+    return res, delta, gamma.to(device), x, y
+
+
+@pytest.mark.parametrize("rows,n", [(1, 8), (5, 120), (3, 512), (37, 520), (9, 1024), (6, 1032), (4, 2048), (3, 4096),
+                                    (2, 5000), (2, 8192), (3, 8200), (2, 16384), (1, 32768)])
+@pytest.mark.parametrize("res_dt,delta_dt", [("f32", "bf16"), ("bf16", "bf16"), ("f16", None), ("f32", "f32"),
+                                             ("bf16", "f16")])
+def test_add_rmsnorm_f8(device, rows, n, res_dt, delta_dt):
+    res, delta, gamma, x, y = _norm_case(rows, n, res_dt, delta_dt, rows + n, device)
+    q, whole = _inside(rows, n, F8, device, fill=2.0)
+    res_out, ro_whole = _inside(rows, n, DT[res_dt], device)
+    scales = torch.full((rows, _blocks(n)), 7.0, device=device)
+    ops.add_rmsnorm(res, delta, gamma, 1e-5, q, res_out=res_out, scales=scales)
+    torch.cuda.synchronize()
+    _check_quantised(q, scales, y, 1, Y_ERR * y.abs())
+    assert torch.equal(res_out.cpu(), x.to(DT[res_dt]))  # one fp32 addition, one rounding
+    assert _untouched(whole, rows, n, 2.0) and _untouched(ro_whole, rows, n, None)
+
+
+@pytest.mark.parametrize("out_dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,n", [(5, 8), (33, 1024), (3, 4104), (1, 20000)])
+def test_add_rmsnorm_wide_outputs(device, out_dt, rows, n):
+    res, delta, gamma, x, y = _norm_case(rows, n, "f32", "bf16", n, device)
+    out, whole = _inside(rows, n, DT[out_dt], device)
+    ops.add_rmsnorm(res, delta, gamma, 1e-5, out)
+    torch.cuda.synchronize()
+    half = torch.finfo(DT[out_dt]).eps / 2
+    err = (out.double().cpu() - y).abs()
+    # the last rounding takes half a step (fp16 subnormals: 2^-25)
+    assert (err <= (Y_ERR + half * (1 + Y_ERR)) * y.abs() + 2.0 ** -25).all()
+    assert _untouched(whole, rows, n, None)
+
+
+def test_add_rmsnorm_in_place_and_special_rows(device):
+    """The residual updated in place, in res or in delta; a row of zeros is
+    zeros (eps), a row with a NaN or an infinity is NaN and leaves its
+    neighbours alone."""
+    n = 1024
+    g = _gen(3)
+    res, delta = torch.randn(6, n, generator=g), torch.randn(6, n, generator=g)
+    res[1], delta[1] = 0, 0
+    res[3, 17] = float("nan")
+    res[4, 900] = float("inf")
+    gamma = torch.ones(n, device=device)
+    want_q, want_s, want_r = (torch.empty(6, n, dtype=F8, device=device), torch.empty(6, 8, device=device),
+                              torch.empty(6, n, device=device))
+    ops.add_rmsnorm(res.to(device), delta.to(device), gamma, 1e-5, want_q, res_out=want_r, scales=want_s)
+    for into in (0, 1):
+        pair = [res.to(device), delta.to(device)]
+        q, s = torch.empty_like(want_q), torch.empty_like(want_s)
+        ops.add_rmsnorm(pair[0], pair[1], gamma, 1e-5, q, res_out=pair[into], scales=s)
+        assert torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
+        assert torch.equal(s.nan_to_num(7), want_s.nan_to_num(7))
+        assert torch.equal(pair[into].nan_to_num(7), want_r.nan_to_num(7))
+    q, s = want_q.float().cpu(), want_s.cpu()
+    assert (q[1] == 0).all() and (s[1] == MIN_SCALE).all()
+    assert torch.isnan(q[3]).all()
+    # x inf: 1 / rms is 0, so the finite values are 0 and the infinity NaN
+    assert torch.isnan(q[4, 900]) and (q[4, :900] == 0).all()
+    for r in (0, 2, 5):
+        assert torch.isfinite(q[r]).all() and torch.isfinite(s[r]).all()
+
+
+# ------------------------------------------------------------------- product
+
+def _operands(m, n, k, seed, device):
+    """e4m3 operands and scales inside larger buffers, and their 64-bit
+    values."""
+    g = _gen(seed)
+
+    def matrix(rows, cols, block_rows, pad):
+        q, _ = _inside(rows, cols, F8, device, pad_cols=pad)
+        q.copy_((torch.randn(rows, cols, generator=g) * 100).clamp(-448, 448).to(F8))
+        sr = -(-rows // block_rows)
+        whole = torch.full((sr + 2, _blocks(cols) + 3), float("nan"), device=device)
+        s = whole[1:1 + sr, :_blocks(cols)]
+        s.copy_(torch.exp(torch.randn(s.shape, generator=g)) * 0.01)
+        val = q.float().double().cpu()
+        val = val * s.double().cpu().repeat_interleave(block_rows, 0)[:rows].repeat_interleave(128, 1)[:, :cols]
+        return q, s, val
+
+    return matrix(m, k, 1, 16), matrix(n, k, 128, 48)
+
+
+def _product(a, w, bias):
+    """(64-bit result, bound on the kernel's error).
+
+    gfx950's matrix unit sums the eight products of k = 8 i .. 8 i + 7 in
+    fixed point: bits below 2^-13 of the power of two of the largest are
+    dropped, so each of the seven others is off by less than 2^-13 of the
+    largest product.  The groups' sums, the blocks' (each times its scales: two
+    more roundings) and the bias then enter fp32 additions, each off by at most one
+    unit in the last place (truncated) of a partial sum, no larger than the
+    sum of magnitudes."""
+    v = a @ w.t()
+    mag = a.abs() @ w.abs().t()
+    err = torch.zeros_like(v)
+    k = a.shape[1]
+    for i in range(0, k, 8):
+        largest = torch.zeros_like(v)
+        for j in range(i, min(i + 8, k)):
+            torch.maximum(largest, a[:, j].abs()[:, None] * w[:, j].abs()[None, :], out=largest)
+        err += 7 * 2.0 ** -13 * largest
+    if bias is not None:
+        v, mag = v + bias, mag + bias.abs()
+    return v, err + (16 + _blocks(k) + 4) * 2 * U * mag
+
+
+def _gelu(v):
+    return 0.5 * v * torch.special.erfc(-v * math.sqrt(0.5))
+
+
+# GELU's slope is at most 1.13; the kernel's erfc is within 3e-7 (a
+# polynomial's 16th power and an approximate reciprocal: 40 roundings more)
+def _gelu_err(v, err):
+    return 1.13 * err + v.abs() * (1.5e-7 + 40 * U)
+
+
+SHAPES = [(1, 4, 16), (1, 128, 128), (8, 2048, 512), (15, 12, 112), (16, 132, 144), (17, 260, 1008), (33, 64, 1168),
+          (64, 512, 2064), (100, 1000, 256), (128, 128, 4112), (130, 516, 272), (300, 388, 1024), (513, 1028, 400)]
+
+
+PLANS = list(range(-1, 8))
+
+
+@pytest.fixture(scope="module")
+def problem(device):
+    """Operands of one shape, and their 64-bit product with its bound (kept for
+    the next test of the same shape)."""
+    kept = {}
+
+    def get(m, n, k):
+        if (m, n, k) not in kept:
+            kept.clear()
+            a, w = _operands(m, n, k, m * n + k, device)
+            bias = torch.randn(n, generator=_gen(k)).half().bfloat16().float()
+            kept[m, n, k] = a[:2], w[:2], bias, _product(a[2], w[2], bias.double())
+        return kept[m, n, k]
+
+    return get
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("plan", PLANS)
+def test_gemm(device, problem, m, n, k, plan):
+    """Every tile, output type and epilogue at odd sizes, operands and outputs
+    inside larger buffers whose other elements are NaN (operands) or kept
+    (outputs)."""
+    if plan >= ops.gemm_f8_plan_count():
+        pytest.skip("no such plan")
+    (a, a_s), (w, w_s), bias, (v0, err0) = problem(m, n, k)
+    for out_dt, epi, with_bias in (("bf16", EPI_BIAS, True), ("f16", EPI_BIAS_GELU, True), ("bf16", EPI_BIAS_GELU, False),
+                                   ("f16", EPI_BIAS, False)):
+        dt = DT[out_dt]
+        v, err = v0 if with_bias else v0 - bias.double(), err0
+        if epi == EPI_BIAS_GELU:
+            err, v = _gelu_err(v, err), _gelu(v)
+        out, whole = _inside(m, n, dt, device, pad_cols=20)
+        ops.gemm_f8(a, a_s, w, w_s, bias.to(dt).to(device) if with_bias else None, out, epi, plan=plan)
+        torch.cuda.synchronize()
+        got = out.double().cpu()
+        half = torch.finfo(dt).eps / 2
+        over = got.abs() == float("inf")  # fp16 results past its range
+        assert (v.abs()[over] >= 65504).all()
+        bad = ~((got - v).abs() <= err + half * (v.abs() + err) + 2.0 ** -25) & ~over
+        assert not bad.any(), f"{out_dt} epilogue {epi}: {int(bad.sum())} of {m * n} off"
+        assert _untouched(whole, m, n, None)
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("epi", [EPI_BIAS, EPI_BIAS_GELU])
+def test_gemm_f8_output(device, problem, m, n, k, epi, plan):
+    if plan >= ops.gemm_f8_plan_count():
+        pytest.skip("no such plan")
+    (a, a_s), (w, w_s), bias, (v, err) = problem(m, n, k)
+    if epi == EPI_BIAS_GELU:
+        err, v = _gelu_err(v, err), _gelu(v)
+    out, whole = _inside(m, n, F8, device, fill=2.0)
+    scales = torch.full((m + 1, _blocks(n) + 2), 7.0, device=device)
+    ops.gemm_f8(a, a_s, w, w_s, bias.to(device), out, epi, out_scales=scales[:m, :_blocks(n)], plan=plan)
+    torch.cuda.synchronize()
+    _check_quantised(out, scales[:m, :_blocks(n)], v, 1, err)
+    assert _untouched(whole, m, n, 2.0)
+    assert (scales[m] == 7.0).all() and (scales[:, _blocks(n):] == 7.0).all()

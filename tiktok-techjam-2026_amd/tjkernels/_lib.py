@@ -15,9 +15,9 @@ from pathlib import Path
 import torch  # noqa: F401  (must precede the library load; see module docstring)
 
 LIB_PATH = Path(__file__).with_name("libtjk.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, E4M3 = 0, 1, 2, 3
 OK, EINVAL, EUNSUPPORTED = 0, -1, -2
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL = 0, 1, 2
 
@@ -60,6 +60,12 @@ _SIGNATURES = {
                            _i32, _vp]),
     "tjk_gemm_ln_supported": (_i32, [_i64, _i32]),
     "tjk_gemm_ln_plan_count": (_i32, []),
+    "tjk_add_rmsnorm": (_i32, [_vp, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _i64, _vp, _i32, _i64, _vp, _i64, _vp,
+                               _i64, _i64, _f32, _vp]),
+    "tjk_quantize_f8": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp]),
+    "tjk_gemm_f8": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _i64, _i64,
+                           _i64, _i32, _i32, _vp]),
+    "tjk_gemm_f8_plan_count": (_i32, []),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

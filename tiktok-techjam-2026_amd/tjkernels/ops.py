@@ -12,6 +12,7 @@ Mirrors of the reference's kernel dispatch layer
 
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -395,6 +396,136 @@ def attn_block(x: torch.Tensor, w_qkv: torch.Tensor, b_qkv: Optional[torch.Tenso
         float(hd ** -0.5 if scale is None else scale), int(bool(causal)), _code(x), _stream(x))
     check(status, "tjk_attn_block")
     return parts
+
+
+F8 = torch.float8_e4m3fn
+F8_BLOCK = 128
+
+
+def _f8_scales(t: Optional[torch.Tensor], rows: int, cols: int, name: str) -> int:
+    """Leading dimension of the fp32 scales of a quantised matrix: at least
+    ``rows`` x ceil(cols / 128), unit column stride."""
+    need = -(-cols // F8_BLOCK)
+    if t is None or t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] < rows or t.shape[1] < need \
+            or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < need):
+        raise TjkError(f"{name} must be a float32 [{rows}, {need}] matrix with unit column stride")
+    return t.stride(0) if t.shape[0] > 1 else need
+
+
+def _one_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """Refuses tensors of several devices; a context in which ``first``'s
+    device is the current one (a launch goes to the current device)."""
+    _require_gpu(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise TjkError(f"tensors on {first.device} and {t.device}")
+    if first.device.index in (None, torch.cuda.current_device()):
+        return nullcontext()
+    return torch.cuda.device(first.device)
+
+
+def _wide(t: Optional[torch.Tensor], name: str) -> int:
+    if t is None:
+        return 0
+    return _code(t) if t.dtype in _lib.DTYPE_CODES else _bad_dtype(t, name)
+
+
+def _bad_dtype(t: torch.Tensor, name: str) -> int:
+    raise TjkError(f"{name}: unsupported dtype {t.dtype}")
+
+
+def add_rmsnorm(res: torch.Tensor, delta: Optional[torch.Tensor], gamma: torch.Tensor, eps: float,
+                out: torch.Tensor, res_out: Optional[torch.Tensor] = None,
+                scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x = res (+ delta) in fp32; res_out <- x (optional, in its own dtype);
+    out <- x * rsqrt(mean(x^2) + eps) * gamma of the unrounded x.
+
+    With a float8_e4m3fn ``out`` the result is quantised: ``scales`` (fp32
+    [rows, ceil(n / 128)]) receives one scale per row and 128 columns, as
+    ``gemm_f8`` takes them.  res_out may be res or delta itself."""
+    device = _one_device(res, delta, gamma, out, res_out, scales)
+    ld_res = _rowmajor(res, "res")
+    rows, n = res.shape
+    for name, t in (("delta", delta), ("out", out), ("res_out", res_out)):
+        if t is not None and (t.dim() != 2 or t.shape[0] < rows or t.shape[1] != n):
+            raise TjkError(f"{name} must be [{rows}, {n}], got {tuple(t.shape)}")
+    if gamma.dtype != torch.float32 or gamma.shape != (n,) or not gamma.is_contiguous():
+        raise TjkError(f"gamma must be a contiguous float32 vector of {n} elements")
+    f8 = out.dtype == F8
+    if scales is not None and not f8:
+        raise TjkError("scales belong to a float8_e4m3fn out")
+    ld_scales = _f8_scales(scales, rows, n, "scales") if f8 else 0
+    with device:
+        status = _lib.load().tjk_add_rmsnorm(
+            res.data_ptr(), _wide(res, "res"), ld_res,
+            _ptr(delta), _wide(delta, "delta"), _rowmajor(delta, "delta") if delta is not None else 0,
+            _ptr(res_out), _wide(res_out, "res_out"), _rowmajor(res_out, "res_out") if res_out is not None else 0,
+            out.data_ptr(), _lib.E4M3 if f8 else _wide(out, "out"), _rowmajor(out, "out"),
+            _ptr(scales), ld_scales, gamma.data_ptr(), rows, n, float(eps), _stream(res))
+    check(status, "tjk_add_rmsnorm")
+    return out
+
+
+def quantize_f8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> torch.Tensor:
+    """Quantises x [rows, n] to float8_e4m3fn: ``out`` [rows, n] and the fp32
+    ``scales`` of its blocks, of one row (activations) or 128 rows (weights;
+    ``block_rows=128``) and 128 columns."""
+    device = _one_device(x, out, scales)
+    ld_x = _rowmajor(x, "x")
+    rows, n = x.shape
+    if out.dtype != F8 or out.dim() != 2 or out.shape[0] < rows or out.shape[1] != n:
+        raise TjkError(f"out must be a float8_e4m3fn [{rows}, {n}] matrix, got {out.dtype} {tuple(out.shape)}")
+    if block_rows not in (1, F8_BLOCK):
+        raise TjkError(f"block_rows must be 1 or {F8_BLOCK}, got {block_rows}")
+    ld_scales = _f8_scales(scales, -(-rows // block_rows), n, "scales")
+    with device:
+        status = _lib.load().tjk_quantize_f8(x.data_ptr(), _wide(x, "x"), ld_x, out.data_ptr(), _rowmajor(out, "out"),
+                                             scales.data_ptr(), ld_scales, rows, n, block_rows, _stream(x))
+    check(status, "tjk_quantize_f8")
+    return out
+
+
+def gemm_f8_plan_count() -> int:
+    return int(_lib.load().tjk_gemm_f8_plan_count())
+
+
+def gemm_f8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor,
+            bias: Optional[torch.Tensor], out: torch.Tensor, epilogue: int = EPI_BIAS,
+            out_scales: Optional[torch.Tensor] = None, plan: int = -1) -> torch.Tensor:
+    """out = epi(a @ w.T + bias) of float8_e4m3fn operands with fp32 scales:
+    ``a`` [m, k] with one per row and 128 columns, ``w`` in nn.Linear [n, k]
+    layout with one per 128 x 128 block (``quantize_f8``).
+
+    ``out`` is float16, bfloat16, or float8_e4m3fn with ``out_scales``
+    [m, ceil(n / 128)]; ``bias`` has a 2-byte out's dtype, else float32.
+    Epilogues EPI_BIAS and EPI_BIAS_GELU: a 2-byte output is added to an fp32
+    residual by the next ``add_rmsnorm`` or ``add_layernorm``, as its delta."""
+    device = _one_device(a, a_scales, w, w_scales, bias, out, out_scales)
+    if a.dtype != F8 or w.dtype != F8:
+        raise TjkError(f"gemm_f8 operands must be float8_e4m3fn, got {a.dtype} and {w.dtype}")
+    lda, ldw, ldc = _rowmajor(a, "a"), _rowmajor(w, "w"), _rowmajor(out, "out")
+    m, k = a.shape
+    n, k2 = w.shape
+    if k != k2 or tuple(out.shape) != (m, n):
+        raise TjkError(f"gemm_f8 shape mismatch a{tuple(a.shape)} w{tuple(w.shape)} out{tuple(out.shape)}")
+    if out.dtype not in (torch.float16, torch.bfloat16, F8):
+        raise TjkError(f"gemm_f8 out must be float16, bfloat16 or float8_e4m3fn, got {out.dtype}")
+    ld_as = _f8_scales(a_scales, m, k, "a_scales")
+    ld_ws = _f8_scales(w_scales, -(-n // F8_BLOCK), k, "w_scales")
+    f8 = out.dtype == F8
+    if out_scales is not None and not f8:
+        raise TjkError("out_scales belong to a float8_e4m3fn out")
+    ld_cs = _f8_scales(out_scales, m, n, "out_scales") if f8 else 0
+    if bias is not None and (bias.dtype != (torch.float32 if f8 else out.dtype) or bias.shape != (n,)
+                             or not bias.is_contiguous()):
+        raise TjkError(f"bias must be a contiguous vector of {n} elements, in a 2-byte out's dtype, else float32")
+    with device:
+        status = _lib.load().tjk_gemm_f8(
+            a.data_ptr(), lda, a_scales.data_ptr(), ld_as, w.data_ptr(), ldw, w_scales.data_ptr(), ld_ws,
+            _ptr(bias), out.data_ptr(), _lib.E4M3 if f8 else _code(out), ldc, _ptr(out_scales), ld_cs, m, n, k,
+            epilogue, plan, _stream(a))
+    check(status, "tjk_gemm_f8")
+    return out
 
 
 def gemm_plans(dtype: torch.dtype):

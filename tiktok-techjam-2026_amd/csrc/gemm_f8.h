@@ -35,8 +35,27 @@ struct F8GemmArgs {
   int m, n, k;
 };
 
-__device__ __forceinline__ f32x4 f8_mma(const i32x8& w, const i32x8& a) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+// In inline asm, volatile, so that the products and the FMAs that read them
+// stay in the order written: as a builtin the compiler put each FMA right behind
+// its product, which then waited out the matrix pipe.  The compiler does not see
+// an MFMA here and inserts no wait states: 12 have to lie between the MFMA (8
+// passes) and a read of its result on gfx950.
+__device__ __forceinline__ void f8_mma(f32x4& d, const i32x8& w, const i32x8& a) {
+  asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, 0" : "=&v"(d) : "v"(w), "v"(a));
+}
+
+// Chunk of a 128-byte tile row: the 16-byte chunk c of row r lies at
+// c ^ f8_swz(r).  A fragment read takes chunk q or q + 4 of 16 rows in 4 lane
+// groups.  Bits 0, 1, 2 of the row map to independent masks, and so do 1, 2, 3, and 2,
+// 3 with mask 1: 8 rows x 1 chunk, 16 x 1 over two rows of banks and 16 x 2 over
+// four all hit different banks, whichever of them the LDS serves at once.
+__device__ __forceinline__ int f8_swz(int r) {
+  return ((r & 1) << 2) ^ ((r >> 1) & 1) ^ (((r >> 2) & 1) << 1) ^ (((r >> 3) & 1) << 2);
+}
+
+// lds_dma16 at voff + soff.
+__device__ __forceinline__ void lds_dma16_at(u32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds_addr) {
+  asm volatile("buffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voff), "s"(rsrc), "s"(soff), "{m0}"(lds_addr));
 }
 
 // One LDS DMA of 4 bytes per lane: lane's word at voff of the descriptor's
@@ -76,16 +95,15 @@ struct F8Geom {
 // has met at a barrier.
 //
 // Tiles reach LDS by DMA, rows of 128 bytes with the 16-byte chunk c of row r
-// at c ^ swz(r).  Lane (l16, q) of a fragment reads chunks q and q + 4 of row
+// at c ^ f8_swz(r).  Lane (l16, q) of a fragment reads chunks q and q + 4 of row
 // l16: any assignment of K to lanes is right that both operands share.
 //
-// Pipeline: MFMAs run in slots of GP (one 16-row tile of A with GP tiles of
-// W); the FMAs of a slot's products follow the next slot's MFMAs, so no FMA
-// waits for the matrix pipe.  Fragments of the next GP tiles of W are read one
-// group ahead.  Before the last group of a K tile everything of it is in
-// registers: there the waves meet, the tile's slot is handed to the DMA of
-// tile it + STAGES, and each A fragment is replaced by the next tile's as soon
-// as its last MFMA is issued.
+// Pipeline: the FMAs of a product run behind the third MFMA after it, four
+// per MFMA, so none waits for the matrix pipe (and 15 instructions lie between).
+// Fragments of the next GP tiles of W are read one group ahead.  Before the last
+// group of a K tile everything of it is in registers: there the waves meet, the
+// tile's slot is handed to the DMA of tile it + STAGES, and each A fragment is
+// replaced by the next tile's as soon as its last MFMA is issued.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x4 (&acc)[G::NT][G::MT]) {
@@ -107,18 +125,27 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 
   // DMA instruction i fills rows (i NW + wave) 8 .. + 7; lane l lands in row
   // l / 8, physical chunk l % 8.  NW is even, so the chunk is the same for all.
+  // A lane's offset stays the same over the K tiles, whose own offset is a
+  // scalar: it takes no vector instruction next to the FMAs.
   const int line0 = wave * 8 + lane / 8;
-  const uint32_t lcb = (uint32_t)(((lane & 7) ^ swz<128>(line0)) << 4);
-  const uint32_t va = (uint32_t)line0 * (uint32_t)p.lda + lcb, vw = (uint32_t)line0 * (uint32_t)p.ldw + lcb;
-  const uint32_t ia = 8u * NW * (uint32_t)p.lda, iw = 8u * NW * (uint32_t)p.ldw;
+  const uint32_t lcb = (uint32_t)(((lane & 7) ^ f8_swz(line0)) << 4);
+  uint32_t voff[G::NDMA];
+#pragma unroll
+  for (int i = 0; i < G::NDMA; ++i)
+    voff[i] = i < G::DA ? (uint32_t)(line0 + 8 * NW * i) * (uint32_t)p.lda + lcb
+                        : (uint32_t)(line0 + 8 * NW * (i - G::DA)) * (uint32_t)p.ldw + lcb;
   auto dma = [&](int it, int i) __attribute__((always_inline)) {
-    const uint32_t kb = (uint32_t)(it * KG + kg) * 128u;
-    const uint32_t ko = kb + lcb < (uint32_t)p.k ? kb : kPastEnd;
     const uint32_t slot = lds0 + (uint32_t)(it % S) * G::STAGE;
-    if (i < G::DA)
-      lds_dma16(rsa, va + ko + (uint32_t)i * ia, slot + (i * NW + wave) * 1024);
-    else
-      lds_dma16(rsw, vw + ko + (uint32_t)(i - G::DA) * iw, slot + G::BM * 128 + ((i - G::DA) * NW + wave) * 1024);
+    const uint32_t dst = slot + (i < G::DA ? (i * NW + wave) * 1024 : G::BM * 128 + ((i - G::DA) * NW + wave) * 1024);
+    lds_dma16_at(i < G::DA ? rsa : rsw, voff[i], (uint32_t)(it * KG + kg) * 128u, dst);
+  };
+  // Called before the DMA of K tile `it`: from the K tile that is not whole on,
+  // the chunks past K lie outside the buffer ranges, from the first one past
+  // the end on all do (they arrive as zeros).
+  auto past_end = [&](int it) __attribute__((always_inline)) {
+    const uint32_t out = (uint32_t)(it * KG + kg) * 128u + lcb < (uint32_t)p.k ? 0u : kPastEnd;
+#pragma unroll
+    for (int i = 0; i < G::NDMA; ++i) voff[i] |= out;
   };
   // scales of K tiles 8 c .. 8 c + 7 of this group, into half c & 1 of the table
   auto scale_dma = [&](int c) __attribute__((always_inline)) {
@@ -136,7 +163,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     }
   };
 
-  const int sw = (q16 ^ swz<128>(l16)) << 4;
+  const int sw = (q16 ^ f8_swz(l16)) << 4;
   const char* const fa0 = gsm + (wm * 16 * MT + l16) * 128;
   const char* const fw0 = gsm + G::BM * 128 + (wn * 16 * NT + l16) * 128;
   auto frag = [&](const char* rows) __attribute__((always_inline)) {
@@ -146,78 +173,111 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   const float* const tab = reinterpret_cast<const float*>(gsm + G::TAB) + wm * 16 * MT + l16;
   const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * 16 * NT) / 128 - nb0) * 8;
 
+  // The rows of A of K tile it are all in registers by its second group, where
+  // a second meeting (MEET) hands their part of the slot to the DMA of tile
+  // it + S, so that the DMA spreads over the K tile: A's over the groups in the
+  // middle, W's in the last one.
+  constexpr bool MEET = NG >= 3;
+  constexpr int NMID = MEET ? (NG - 2) * MT : 1;
   scale_dma(0);
 #pragma unroll
-  for (int t = 0; t < S; ++t)
+  for (int t = 0; t < S; ++t) {
+    past_end(t);
 #pragma unroll
     for (int i = 0; i < G::NDMA; ++i) dma(t, i);
+  }
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * G::NDMA) : "memory");
   asm volatile("s_barrier" ::: "memory");
 
   i32x8 fa[MT], fw[2][GP];
-  f32x4 part[2][GP];
-  float raw[MT], raw_w, s[MT], s_last = 0.f;
+  f32x4 part[4];
+  float raw[MT], raw_w, s[MT], s_last[MT];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) fa[j] = frag(fa0 + j * 2048);
-#pragma unroll
-  for (int i = 0; i < GP; ++i) {
-    fw[0][i] = frag(fw0 + i * 2048);
-    part[1][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < MT; ++j) {
+    fa[j] = frag(fa0 + j * 2048);
+    raw[j] = tab[16 * j];
+    s_last[j] = 0.f;
   }
 #pragma unroll
-  for (int j = 0; j < MT; ++j) raw[j] = tab[16 * j];
+  for (int i = 0; i < GP; ++i) fw[0][i] = frag(fw0 + i * 2048);
   raw_w = tabw[0];
-
-  auto add = [&](f32x4& c, const f32x4& v, float f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) c[r] = fmaf(v[r], f, c[r]);
+  for (int j = 0; j < MT; ++j) s[j] = raw[j] * raw_w;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) part[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // Product v of a K tile: group v / (MT GP), 16-row tile j, W tile i.  The FMAs
+  // of the product three back (of the previous K tile for v < 3).
+  constexpr int TILES = MT * NT;
+  static_assert(TILES % 4 == 0, "ring of four products");
+  auto join = [&](int v, const float (&f)[MT]) __attribute__((always_inline)) {
+    f32x4& p4 = part[v & 3];
+    asm volatile("" : "+v"(p4));  // not before the MFMAs above
+    const int j = v % (MT * GP) / GP;
+    f32x4& c = acc[v / (MT * GP) * GP + v % GP][j];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c[r] = fmaf(p4[r], f[j], c[r]);
   };
 
   for (int it = 0; it < nit; ++it) {
     const int st = (it % S) * G::STAGE, nx = ((it + 1) % S) * G::STAGE;
-#pragma unroll
-    for (int j = 0; j < MT; ++j) s[j] = raw[j] * raw_w;
     if ((it & 7) == 0) scale_dma((it >> 3) + 1);
+    if (((it + S) * KG + kg + 1) * 128 > p.k) past_end(it + S);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const bool last = g + 1 == NG;
       if (last) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * G::NDMA) : "memory");  // tile it + 1 landed
+        // tile it + 1 landed
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * G::NDMA + (MEET ? G::DA : 0)) : "memory");
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      } else if (MEET && g == 1) {
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const int u = (g * MT + j) & 1;
 #pragma unroll
-        for (int i = 0; i < GP; ++i) part[u][i] = f8_mma(fw[g & 1][i], fa[j]);
+        for (int i = 0; i < GP; ++i) {
+          const int v = (g * MT + j) * GP + i;
+          f8_mma(part[v & 3], fw[g & 1][i], fa[j]);
+          if (v < 3) join(v + TILES - 3, s_last);
+          else join(v - 3, s);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         if (last) {
-          fa[j] = frag(fa0 + nx + j * 2048);
-          if (j < GP) fw[0][j] = frag(fw0 + nx + j * 2048);
-          if (j + 1 == MT) {
+          if (j == 0) {
             const int o = (it + 1) & 15;
 #pragma unroll
             for (int jj = 0; jj < MT; ++jj) raw[jj] = tab[o * G::BM + 16 * jj];
             raw_w = tabw[(o >> 3) * 64 + (o & 7)];
           }
+          fa[j] = frag(fa0 + nx + j * 2048);
+          if (j < GP) fw[0][j] = frag(fw0 + nx + j * 2048);
+          constexpr int D0 = MEET ? G::DA : 0, ND = G::NDMA - D0;
 #pragma unroll
-          for (int d = j * G::NDMA / MT; d < (j + 1) * G::NDMA / MT; ++d) dma(it + S, d);
+          for (int d = j * ND / MT; d < (j + 1) * ND / MT; ++d) dma(it + S, D0 + d);
         } else if (j < GP) {
           fw[(g + 1) & 1][j] = frag(fw0 + st + ((g + 1) * GP + j) * 2048);
         }
-        // the slot before this one
-        const int gp = j > 0 ? g : g > 0 ? g - 1 : NG - 1, jp = j > 0 ? j - 1 : MT - 1;
-        const float f = g == 0 && j == 0 ? s_last : s[jp];
+        if (MEET && g >= 1 && !last) {
+          const int u = (g - 1) * MT + j;
 #pragma unroll
-        for (int i = 0; i < GP; ++i) add(acc[gp * GP + i][jp], part[u ^ 1][i], f);
+          for (int d = u * G::DA / NMID; d < (u + 1) * G::DA / NMID; ++d) dma(it + S, d);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    s_last = s[MT - 1];
-  }
 #pragma unroll
-  for (int i = 0; i < GP; ++i) add(acc[(NG - 1) * GP + i][MT - 1], part[1][i], s_last);
+    for (int j = 0; j < MT; ++j) {
+      s_last[j] = s[j];
+      s[j] = raw[j] * raw_w;
+    }
+  }
+  asm volatile("s_nop 7\n\ts_nop 3" : "+v"(part[1]), "+v"(part[2]), "+v"(part[3]));
+#pragma unroll
+  for (int v = TILES - 3; v < TILES; ++v) join(v, s_last);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }

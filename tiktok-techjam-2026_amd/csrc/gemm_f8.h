@@ -1,13 +1,19 @@
 // Block-scaled e4m3 GEMM: C = epi(sum_b sa[m, b] sw[n / 128, b] P_b[m, n] +
 // bias), P_b the product over the b-th block of 128 along K.
 //
-// One v_mfma_f32_16x16x128_f8f6f4 contracts a whole block, so P_b of 16 x 16
-// outputs is one instruction with a zero addend (its scale operands are left
-// at 1) and the two scales cost one fp32 FMA per output and block,
-// acc += P_b (sa sw).  W is the first operand, so a lane holds four
-// consecutive columns of one row: the row's scale is one register per 16
-// rows, and the weights' scale is the same for the whole wave (its columns lie
-// in one block of 128).
+// Two v_mfma_f32_32x32x64_f8f6f4 contract a block: P_b of 32 x 32 outputs
+// starts from a zero addend and takes the two scales as one fp32 FMA per output
+// and block, acc += P_b (sa sw).  W is the first operand, so a lane holds four
+// consecutive columns of one row: the row's scale is one register per 32 rows,
+// and the weights' scale is the same for the whole wave (its columns lie in one
+// block of 128).
+//
+// What bounds it: an f8f6f4 MFMA keeps the vector issue of its SIMD for 16
+// cycles, whatever its shape (it reads 16 operand registers), a vector
+// instruction for 4; measured with loops of nothing else.  With 16 x 16 x 128 MFMAs
+// (32 cycles each) the four FMAs that belong to one fill the rest of it, and
+// every address or scale instruction more delays the matrix unit.  With 32 x 32 x 64
+// (64 cycles) the eight FMAs leave four issue slots.
 #pragma once
 
 #include "f8_common.h"
@@ -35,22 +41,27 @@ struct F8GemmArgs {
   int m, n, k;
 };
 
-// In inline asm, volatile, so that the products and the FMAs that read them
-// stay in the order written: as a builtin the compiler put each FMA right behind
-// its product, which then waited out the matrix pipe.  The compiler does not see
-// an MFMA here and inserts no wait states: 12 have to lie between the MFMA (8
-// passes) and a read of its result on gfx950.
-__device__ __forceinline__ void f8_mma(f32x4& d, const i32x8& w, const i32x8& a) {
-  asm volatile("v_mfma_f32_16x16x128_f8f6f4 %0, %1, %2, 0" : "=&v"(d) : "v"(w), "v"(a));
+// The product of one block.  In inline asm, volatile, so that the products and
+// the FMAs that read them stay in the order written: as a builtin the compiler
+// put each FMA right behind its product, which then waited out the matrix pipe.
+// The compiler does not see an MFMA here and inserts no wait states: 20 have to
+// lie between the second MFMA (16 passes) and a read of its result on gfx950.
+__device__ __forceinline__ void f8_mma(f32x16& d, const i32x8 (&w)[2], const i32x8 (&a)[2]) {
+  asm volatile(
+      "v_mfma_f32_32x32x64_f8f6f4 %0, %1, %3, 0\n\t"
+      "v_mfma_f32_32x32x64_f8f6f4 %0, %2, %4, %0\n\t"
+      "s_nop 1"
+      : "=&v"(d)
+      : "v"(w[0]), "v"(w[1]), "v"(a[0]), "v"(a[1]));
 }
 
 // Chunk of a 128-byte tile row: the 16-byte chunk c of row r lies at
-// c ^ f8_swz(r).  A fragment read takes chunk q or q + 4 of 16 rows in 4 lane
-// groups.  Bits 0, 1, 2 of the row map to independent masks, and so do 1, 2, 3, and 2,
-// 3 with mask 1: 8 rows x 1 chunk, 16 x 1 over two rows of banks and 16 x 2 over
-// four all hit different banks, whichever of them the LDS serves at once.
+// c ^ f8_swz(r).  A fragment read takes one chunk of 32 rows in each lane half.
+// Row bits 0, 1, 2 map to independent masks, and so do 1, 2, 3, and 2, 3, 4: 8
+// rows, 16 over two rows of banks and 32 over four all hit different banks,
+// whichever of them the LDS serves at once.  Measured: no conflicts.
 __device__ __forceinline__ int f8_swz(int r) {
-  return ((r & 1) << 2) ^ ((r >> 1) & 1) ^ (((r >> 2) & 1) << 1) ^ (((r >> 3) & 1) << 2);
+  return ((r & 1) << 1) ^ ((r & 2) << 1) ^ ((r >> 2) & 1) ^ (((r >> 3) & 1) << 1) ^ (((r >> 4) & 1) << 2);
 }
 
 // lds_dma16 at voff + soff.
@@ -64,14 +75,14 @@ __device__ __forceinline__ void lds_dma4(u32x4 rsrc, uint32_t voff, uint32_t lds
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(lds_addr));
 }
 
-// WM x WN waves of (16 MT) x (16 NT) outputs, KG groups of them along K
+// WM x WN waves of (32 FM) x (32 FN) outputs, KG groups of them along K
 // (group g takes K tiles g, g + KG, ...), each with a ring of STAGES K tiles
 // of 128 and a table of the scales of 16 K tiles.
-template <int MT_, int NT_, int WM_, int WN_, int KG_, int STAGES_>
+template <int FM_, int FN_, int WM_, int WN_, int KG_, int STAGES_>
 struct F8Geom {
-  static constexpr int MT = MT_, NT = NT_, WM = WM_, WN = WN_, KG = KG_, STAGES = STAGES_;
+  static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, KG = KG_, STAGES = STAGES_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW * KG;
-  static constexpr int BM = 16 * MT * WM, BN = 16 * NT * WN;
+  static constexpr int WTM = 32 * FM, WTN = 32 * FN, BM = WTM * WM, BN = WTN * WN;
   static constexpr int DA = BM / (8 * NW), DW = BN / (8 * NW), NDMA = DA + DW;  // DMA instructions per wave per K tile
   static constexpr int STAGE = (BM + BN) * 128;
   static constexpr int TAB = STAGES * STAGE;         // byte of the row scales, [16][BM]
@@ -79,39 +90,37 @@ struct F8Geom {
   static constexpr int GROUP = TABW + 512;           // bytes per K group
   static constexpr int PARTS = (KG - 1) * BM * BN * 4;  // K groups' sums, over the rings
   static constexpr int LDS = KG * GROUP > PARTS ? KG * GROUP : PARTS;
-  static constexpr int GP = NT % 4 == 0 ? 2 : 1;     // 16-column tiles whose W fragments are held at once
-  static constexpr int NG = NT / GP;
   static_assert(DA * 8 * NW == BM && DW * 8 * NW == BN, "tile rows must split over the waves");
-  static_assert(NW % 2 == 0, "row parity of the DMA instructions");
-  static_assert(NG % 2 == 0 && MT % 2 == 0, "fragment double buffer; 32-row epilogue blocks");
-  static_assert(128 % (16 * NT) == 0, "a wave's columns lie in one block");
+  static_assert(FN % 2 == 0, "fragment double buffer, ring of two products");
+  static_assert(128 % WTN == 0, "a wave's columns lie in one block");
   static_assert(STAGES >= 2 && STAGES <= 8, "a chunk of scales lands within 8 K tiles");
   static_assert((STAGES - 1) * NDMA + DA + 1 <= 63, "vmcnt range");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-// acc += the block-scaled product for this wave's (16 MT) x (16 NT) outputs
+// acc += the block-scaled product for this wave's (32 FM) x (32 FN) outputs
 // of the tile at (m0, n0).  On return every DMA has landed and the workgroup
 // has met at a barrier.
 //
 // Tiles reach LDS by DMA, rows of 128 bytes with the 16-byte chunk c of row r
-// at c ^ f8_swz(r).  Lane (l16, q) of a fragment reads chunks q and q + 4 of row
-// l16: any assignment of K to lanes is right that both operands share.
+// at c ^ f8_swz(r).  Lane (l32, hi) of a fragment's half h reads chunks
+// 4 h + hi and 4 h + 2 + hi of row l32: any assignment of K to lanes is right
+// that both operands share.
 //
-// Pipeline: the FMAs of a product run behind the third MFMA after it, four
-// per MFMA, so none waits for the matrix pipe (and 15 instructions lie between).
-// Fragments of the next GP tiles of W are read one group ahead.  Before the last
-// group of a K tile everything of it is in registers: there the waves meet, the
-// tile's slot is handed to the DMA of tile it + STAGES, and each A fragment is
-// replaced by the next tile's as soon as its last MFMA is issued.
+// Pipeline: the FMAs of a product run behind the two MFMAs of the next one, so
+// none waits for the matrix pipe (18 instructions and a pause of two lie
+// between).  W's fragments are read one 32-column tile ahead.  Before the last
+// tile of W everything of a K tile is in registers: there the waves meet, the K
+// tile's slot is handed to the DMA of K tile it + STAGES, and each A fragment is
+// replaced by the next K tile's as soon as its last MFMA is issued.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
-                                              f32x4 (&acc)[G::NT][G::MT]) {
-  constexpr int MT = G::MT, NT = G::NT, NW = G::NW, KG = G::KG, S = G::STAGES, GP = G::GP, NG = G::NG;
+                                              f32x16 (&acc)[G::FN][G::FM]) {
+  constexpr int FM = G::FM, FN = G::FN, NW = G::NW, KG = G::KG, S = G::STAGES;
   const int lane = threadIdx.x & 63;
   const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = gw / NW, wave = gw % NW, wm = wave / G::WN, wn = wave % G::WN;
-  const int l16 = lane & 15, q16 = lane >> 4;
+  const int l32 = lane & 31, hi = lane >> 5;
   char* const gsm = smem + kg * G::GROUP;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)gsm;
   const int nkt = (p.k + 127) / 128, nit = (nkt + KG - 1) / KG;
@@ -123,17 +132,20 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   const int nb0 = n0 / 128, nbs = (p.n + 127) / 128;
   const u32x4 rsws = lds_dma_rsrc(p.ws + (int64_t)nb0 * p.ld_ws, (int64_t)(nbs - nb0) * p.ld_ws * 4);
 
-  // DMA instruction i fills rows (i NW + wave) 8 .. + 7; lane l lands in row
-  // l / 8, physical chunk l % 8.  NW is even, so the chunk is the same for all.
-  // A lane's offset stays the same over the K tiles, whose own offset is a
-  // scalar: it takes no vector instruction next to the FMAs.
-  const int line0 = wave * 8 + lane / 8;
-  const uint32_t lcb = (uint32_t)(((lane & 7) ^ f8_swz(line0)) << 4);
+  // DMA instruction i fills rows (i NW + wave) 8 .. + 7 of A (of W from i = DA);
+  // lane l lands in row l / 8, physical chunk l % 8.  A lane's offset stays the
+  // same over the K tiles, whose own offset is a scalar: it takes no vector
+  // instruction next to the FMAs.
+  auto dma_row = [&](int i) __attribute__((always_inline)) {
+    return ((i < G::DA ? i : i - G::DA) * NW + wave) * 8 + lane / 8;
+  };
+  auto dma_chunk = [&](int i) __attribute__((always_inline)) {
+    return (uint32_t)(((lane & 7) ^ f8_swz(dma_row(i))) << 4);
+  };
   uint32_t voff[G::NDMA];
 #pragma unroll
   for (int i = 0; i < G::NDMA; ++i)
-    voff[i] = i < G::DA ? (uint32_t)(line0 + 8 * NW * i) * (uint32_t)p.lda + lcb
-                        : (uint32_t)(line0 + 8 * NW * (i - G::DA)) * (uint32_t)p.ldw + lcb;
+    voff[i] = (uint32_t)dma_row(i) * (uint32_t)(i < G::DA ? p.lda : p.ldw) + dma_chunk(i);
   auto dma = [&](int it, int i) __attribute__((always_inline)) {
     const uint32_t slot = lds0 + (uint32_t)(it % S) * G::STAGE;
     const uint32_t dst = slot + (i < G::DA ? (i * NW + wave) * 1024 : G::BM * 128 + ((i - G::DA) * NW + wave) * 1024);
@@ -143,9 +155,9 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   // the chunks past K lie outside the buffer ranges, from the first one past
   // the end on all do (they arrive as zeros).
   auto past_end = [&](int it) __attribute__((always_inline)) {
-    const uint32_t out = (uint32_t)(it * KG + kg) * 128u + lcb < (uint32_t)p.k ? 0u : kPastEnd;
 #pragma unroll
-    for (int i = 0; i < G::NDMA; ++i) voff[i] |= out;
+    for (int i = 0; i < G::NDMA; ++i)
+      voff[i] |= (uint32_t)(it * KG + kg) * 128u + dma_chunk(i) < (uint32_t)p.k ? 0u : kPastEnd;
   };
   // scales of K tiles 8 c .. 8 c + 7 of this group, into half c & 1 of the table
   auto scale_dma = [&](int c) __attribute__((always_inline)) {
@@ -163,22 +175,23 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     }
   };
 
-  const int sw = (q16 ^ f8_swz(l16)) << 4;
-  const char* const fa0 = gsm + (wm * 16 * MT + l16) * 128;
-  const char* const fw0 = gsm + G::BM * 128 + (wn * 16 * NT + l16) * 128;
-  auto frag = [&](const char* rows) __attribute__((always_inline)) {
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(rows + sw), hi = *reinterpret_cast<const i32x4*>(rows + (sw ^ 64));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  const int sw = (hi ^ f8_swz(l32)) << 4;
+  const char* const fa0 = gsm + (wm * G::WTM + l32) * 128;
+  const char* const fw0 = gsm + G::BM * 128 + (wn * G::WTN + l32) * 128;
+  auto frag = [&](const char* rows, int h) __attribute__((always_inline)) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64)));
+    const i32x4 up = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64 + 32)));
+    return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  const float* const tab = reinterpret_cast<const float*>(gsm + G::TAB) + wm * 16 * MT + l16;
-  const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * 16 * NT) / 128 - nb0) * 8;
+  const float* const tab = reinterpret_cast<const float*>(gsm + G::TAB) + wm * G::WTM + l32;
+  const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * G::WTN) / 128 - nb0) * 8;
 
-  // The rows of A of K tile it are all in registers by its second group, where
-  // a second meeting (MEET) hands their part of the slot to the DMA of tile
-  // it + S, so that the DMA spreads over the K tile: A's over the groups in the
+  // The rows of A of K tile it are all in registers by its second W tile, where
+  // a second meeting (MEET) hands their part of the slot to the DMA of K tile
+  // it + S, so that the DMA spreads over the K tile: A's over the W tiles in the
   // middle, W's in the last one.
-  constexpr bool MEET = NG >= 3;
-  constexpr int NMID = MEET ? (NG - 2) * MT : 1;
+  constexpr bool MEET = FN >= 4;
+  constexpr int NMID = MEET ? (FN - 2) * FM : 1;
   scale_dma(0);
 #pragma unroll
   for (int t = 0; t < S; ++t) {
@@ -189,34 +202,31 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * G::NDMA) : "memory");
   asm volatile("s_barrier" ::: "memory");
 
-  i32x8 fa[MT], fw[2][GP];
-  f32x4 part[4];
-  float raw[MT], raw_w, s[MT], s_last[MT];
+  i32x8 fa[FM][2], fw[2][2];
+  f32x16 part[2];
+  float raw[FM], raw_w, s[FM], s_last = 0.f;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    fa[j] = frag(fa0 + j * 2048);
-    raw[j] = tab[16 * j];
-    s_last[j] = 0.f;
+  for (int j = 0; j < FM; ++j) {
+    fa[j][0] = frag(fa0 + j * 4096, 0);
+    fa[j][1] = frag(fa0 + j * 4096, 1);
+    raw[j] = tab[32 * j];
   }
-#pragma unroll
-  for (int i = 0; i < GP; ++i) fw[0][i] = frag(fw0 + i * 2048);
+  fw[0][0] = frag(fw0, 0);
+  fw[0][1] = frag(fw0, 1);
   raw_w = tabw[0];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) s[j] = raw[j] * raw_w;
+  for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) part[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < 16; ++r) part[1][r] = 0.f;
 
-  // Product v of a K tile: group v / (MT GP), 16-row tile j, W tile i.  The FMAs
-  // of the product three back (of the previous K tile for v < 3).
-  constexpr int TILES = MT * NT;
-  static_assert(TILES % 4 == 0, "ring of four products");
-  auto join = [&](int v, const float (&f)[MT]) __attribute__((always_inline)) {
-    f32x4& p4 = part[v & 3];
-    asm volatile("" : "+v"(p4));  // not before the MFMAs above
-    const int j = v % (MT * GP) / GP;
-    f32x4& c = acc[v / (MT * GP) * GP + v % GP][j];
+  // The FMAs of product v = i FM + j (the last of the K tile before: v = -1).
+  constexpr int TILES = FM * FN;
+  auto join = [&](int v, float f) __attribute__((always_inline)) {
+    f32x16& d = part[v & 1];
+    asm volatile("" : "+v"(d));  // not before the MFMAs above
+    f32x16& c = acc[(v + TILES) % TILES / FM][(v + TILES) % FM];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) c[r] = fmaf(p4[r], f[j], c[r]);
+    for (int r = 0; r < 16; ++r) c[r] = fmaf(d[r], f, c[r]);
   };
 
   for (int it = 0; it < nit; ++it) {
@@ -225,59 +235,56 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     if (((it + S) * KG + kg + 1) * 128 > p.k) past_end(it + S);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const bool last = g + 1 == NG;
+    for (int i = 0; i < FN; ++i) {
+      const bool last = i + 1 == FN;
       if (last) {
-        // tile it + 1 landed
+        // K tile it + 1 landed
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * G::NDMA + (MEET ? G::DA : 0)) : "memory");
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-      } else if (MEET && g == 1) {
+      } else if (MEET && i == 1) {
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-#pragma unroll
-        for (int i = 0; i < GP; ++i) {
-          const int v = (g * MT + j) * GP + i;
-          f8_mma(part[v & 3], fw[g & 1][i], fa[j]);
-          if (v < 3) join(v + TILES - 3, s_last);
-          else join(v - 3, s);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      for (int j = 0; j < FM; ++j) {
+        const int v = i * FM + j;
+        f8_mma(part[v & 1], fw[i & 1], fa[j]);
         if (last) {
           if (j == 0) {
             const int o = (it + 1) & 15;
 #pragma unroll
-            for (int jj = 0; jj < MT; ++jj) raw[jj] = tab[o * G::BM + 16 * jj];
+            for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
             raw_w = tabw[(o >> 3) * 64 + (o & 7)];
           }
-          fa[j] = frag(fa0 + nx + j * 2048);
-          if (j < GP) fw[0][j] = frag(fw0 + nx + j * 2048);
-          constexpr int D0 = MEET ? G::DA : 0, ND = G::NDMA - D0;
-#pragma unroll
-          for (int d = j * ND / MT; d < (j + 1) * ND / MT; ++d) dma(it + S, D0 + d);
-        } else if (j < GP) {
-          fw[(g + 1) & 1][j] = frag(fw0 + st + ((g + 1) * GP + j) * 2048);
+          fa[j][0] = frag(fa0 + nx + j * 4096, 0);
+          fa[j][1] = frag(fa0 + nx + j * 4096, 1);
         }
-        if (MEET && g >= 1 && !last) {
-          const int u = (g - 1) * MT + j;
+        // fragments of the next W tile, a half after each MFMA pair (both after
+        // the only one)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (j == min(h, FM - 1))
+            fw[(i + 1) & 1][h] = last ? frag(fw0 + nx, h) : frag(fw0 + st + (i + 1) * 4096, h);
+        constexpr int D0 = MEET ? G::DA : 0, ND = G::NDMA - D0;
+        if (last) {
+#pragma unroll
+          for (int d = j * ND / FM; d < (j + 1) * ND / FM; ++d) dma(it + S, D0 + d);
+        } else if (MEET && i >= 1) {
+          const int u = (i - 1) * FM + j;
 #pragma unroll
           for (int d = u * G::DA / NMID; d < (u + 1) * G::DA / NMID; ++d) dma(it + S, d);
         }
+        join(v - 1, v == 0 ? s_last : s[(v - 1) % FM]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    s_last = s[FM - 1];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      s_last[j] = s[j];
-      s[j] = raw[j] * raw_w;
-    }
+    for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
   }
-  asm volatile("s_nop 7\n\ts_nop 3" : "+v"(part[1]), "+v"(part[2]), "+v"(part[3]));
-#pragma unroll
-  for (int v = TILES - 3; v < TILES; ++v) join(v, s_last);
+  asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[1]));
+  join(-1, s_last);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }
@@ -285,28 +292,36 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 // Adds the K groups' sums in group order into group 0's accumulators, through
 // LDS.  True for the waves that hold the result.
 template <typename G>
-__device__ __forceinline__ bool f8_join_groups(char* smem, f32x4 (&acc)[G::NT][G::MT]) {
+__device__ __forceinline__ bool f8_join_groups(char* smem, f32x16 (&acc)[G::FN][G::FM]) {
   if constexpr (G::KG > 1) {
     const int gw = threadIdx.x >> 6, kg = gw / G::NW, lane = threadIdx.x & 63;
-    constexpr int TILES = G::MT * G::NT;
-    float4* const base = reinterpret_cast<float4*>(smem) + (gw % G::NW) * TILES * 64 + lane;
-    constexpr int STEP = G::NW * TILES * 64;
+    constexpr int QUADS = G::FM * G::FN * 4;  // of a lane
+    float4* const base = reinterpret_cast<float4*>(smem) + (gw % G::NW) * QUADS * 64 + lane;
+    constexpr int STEP = G::NW * QUADS * 64;
     if (kg > 0) {
 #pragma unroll
-      for (int i = 0; i < G::NT; ++i)
+      for (int i = 0; i < G::FN; ++i)
 #pragma unroll
-        for (int j = 0; j < G::MT; ++j)
-          base[(kg - 1) * STEP + (i * G::MT + j) * 64] = __builtin_bit_cast(float4, acc[i][j]);
+        for (int j = 0; j < G::FM; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            base[(kg - 1) * STEP + ((i * G::FM + j) * 4 + q) * 64] =
+                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
     }
     __syncthreads();
     if (kg == 0) {
 #pragma unroll
       for (int o = 0; o < G::KG - 1; ++o)
 #pragma unroll
-        for (int i = 0; i < G::NT; ++i)
+        for (int i = 0; i < G::FN; ++i)
 #pragma unroll
-          for (int j = 0; j < G::MT; ++j)
-            acc[i][j] += __builtin_bit_cast(f32x4, base[o * STEP + (i * G::MT + j) * 64]);
+          for (int j = 0; j < G::FM; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float4 v = base[o * STEP + ((i * G::FM + j) * 4 + q) * 64];
+              acc[i][j][4 * q] += v.x; acc[i][j][4 * q + 1] += v.y;
+              acc[i][j][4 * q + 2] += v.z; acc[i][j][4 * q + 3] += v.w;
+            }
     }
     __syncthreads();
     return kg == 0;
@@ -319,80 +334,91 @@ __device__ __forceinline__ bool f8_join_groups(char* smem, f32x4 (&acc)[G::NT][G
 // columns, after the bias (and GELU).
 constexpr int kEpiF8 = 8, kEpiF8Gelu = 9;
 
-// e4m3 output of a wave's (16 MT) x (16 NT) outputs at (mw, nw).  Lane (l16,
-// q) holds columns 16 i + 4 q .. + 3 of rows 16 j + l16, so a row's largest
-// magnitude over the wave's columns takes two lane exchanges; where a block of
-// 128 columns spans several waves they trade theirs through LDS (`red`, BM x WN
-// floats; every wave of the workgroup calls this).  Words are put in rows through
-// `stage` (16 MT x 16 NT bytes of the wave's own), the 16-byte piece i of row r
-// at i ^ x(r), and leave as whole pieces.
+// e4m3 output of a wave's (32 FM) x (32 FN) outputs at (mw, nw).  Lane (l32,
+// hi) holds columns 32 i + 8 g + 4 hi .. + 3 of rows 32 j + l32, so a row's
+// largest magnitude over the wave's columns takes one lane exchange; where a
+// block of 128 columns spans several waves they trade theirs through LDS (`red`,
+// BM x WN floats; every wave of the workgroup calls this).  Words are put in rows
+// through `stage` (1024 FM FN bytes of the wave's own), the 16-byte piece c of
+// row r at c ^ x(r), and leave as whole pieces.
 template <bool GELU, typename G>
-__device__ __forceinline__ void f8_epilogue(const F8GemmArgs& p, f32x4 (&acc)[G::NT][G::MT], int mw, int nw, int wm,
+__device__ __forceinline__ void f8_epilogue(const F8GemmArgs& p, f32x16 (&acc)[G::FN][G::FM], int mw, int nw, int wm,
                                             int wn, int lane, bool holds, float* red, char* stage) {
-  constexpr int MT = G::MT, NT = G::NT, WPB = 128 / (16 * NT);
-  const int l16 = lane & 15, q16 = lane >> 4;
-  float top[MT];
+  constexpr int FM = G::FM, FN = G::FN, WPB = 128 / G::WTN;
+  const int l32 = lane & 31, hi = lane >> 5;
+  float top[FM];
   if (holds) {
     const float* const bias = static_cast<const float*>(p.bias);
-    float4 b[NT];
+    float4 b[FN][4];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) b[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) b[i][g] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (bias != nullptr) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) b[i] = *reinterpret_cast<const float4*>(bias + min(nw + 16 * i + 4 * q16, p.n - 4));
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          b[i][g] = *reinterpret_cast<const float4*>(bias + min(nw + 32 * i + 8 * g + 4 * hi, p.n - 4));
     }
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
+    for (int j = 0; j < FM; ++j) {
       top[j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        f32x4 v = acc[i][j];
-        v[0] += b[i].x; v[1] += b[i].y; v[2] += b[i].z; v[3] += b[i].w;
-        const bool in = nw + 16 * i + 4 * q16 < p.n;
+      for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (GELU) v[r] = gelu_erf(v[r]);
-          top[j] = fmaxf(top[j], in ? fabsf(v[r]) : 0.f);
+        for (int g = 0; g < 4; ++g) {
+          const bool in = nw + 32 * i + 8 * g + 4 * hi < p.n;
+          const float add[4] = {b[i][g].x, b[i][g].y, b[i][g].z, b[i][g].w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v = acc[i][j][4 * g + r] + add[r];
+            if (GELU) v = gelu_erf(v);
+            acc[i][j][4 * g + r] = v;
+            top[j] = fmaxf(top[j], in ? fabsf(v) : 0.f);
+          }
         }
-        acc[i][j] = v;
-      }
-      top[j] = fmaxf(top[j], __shfl_xor(top[j], 16));
       top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
     }
   }
   if constexpr (WPB > 1) {
-    if (holds && q16 == 0) {
+    if (holds && hi == 0) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) red[wn * G::BM + wm * 16 * MT + 16 * j + l16] = top[j];
+      for (int j = 0; j < FM; ++j) red[wn * G::BM + wm * G::WTM + 32 * j + l32] = top[j];
     }
     __syncthreads();
     if (holds) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j)
+      for (int j = 0; j < FM; ++j)
 #pragma unroll
         for (int o = 0; o < WPB; ++o)
-          top[j] = fmaxf(top[j], red[(wn / WPB * WPB + o) * G::BM + wm * 16 * MT + 16 * j + l16]);
+          top[j] = fmaxf(top[j], red[(wn / WPB * WPB + o) * G::BM + wm * G::WTM + 32 * j + l32]);
     }
   }
   if (!holds) return;
-  auto x = [](int r) { return NT >= 8 ? r & 7 : (r >> 1) & (NT - 1); };
+  constexpr int LPR = 2 * FN;  // pieces per row: 8 or 4
+  static_assert(LPR == 8 || LPR == 4, "staged rows of 128 or 64 bytes");
+  auto x = [](int r) { return LPR == 8 ? r & 7 : (r >> 1) & 3; };
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
+  for (int j = 0; j < FM; ++j) {
     const float s = f8_scale(top[j]), inv = __builtin_amdgcn_rcpf(s);
-    const int m = mw + 16 * j + l16;
-    if (q16 == 0 && wn % WPB == 0 && m < p.m && nw < p.n) p.cs[(int64_t)m * p.ld_cs + nw / 128] = s;
+    const int m = mw + 32 * j + l32;
+    if (hi == 0 && wn % WPB == 0 && m < p.m && nw < p.n) p.cs[(int64_t)m * p.ld_cs + nw / 128] = s;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-      *reinterpret_cast<uint32_t*>(stage + (16 * j + l16) * 16 * NT + ((i ^ x(l16)) << 4) + 4 * q16) =
-          f8_pack4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], inv);
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint32_t*>(stage + (32 * j + l32) * 16 * LPR + (((2 * i + (g >> 1)) ^ x(l32)) << 4) +
+                                     8 * (g & 1) + 4 * hi) =
+            f8_pack4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3], inv);
   }
   uint8_t* const c = static_cast<uint8_t*>(p.c);
   const bool a16 = ((uintptr_t)c & 15) == 0 && p.ldc % 16 == 0;
-  constexpr int NPC = 16 * MT * NT;
+  constexpr int NPC = 32 * FM * LPR;
 #pragma unroll
   for (int it = 0; it < NPC / 64; ++it) {
-    const int pc = lane + 64 * it, r = pc / NT, i = pc % NT;
-    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 16 * NT + ((i ^ x(r & 15)) << 4));
+    const int pc = lane + 64 * it, r = pc / LPR, i = pc % LPR;
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 16 * LPR + ((i ^ x(r & 31)) << 4));
     const int m = mw + r, n = nw + 16 * i;
     if (m < p.m && n < p.n) {
       uint8_t* const o = c + (int64_t)m * p.ldc + n;
@@ -415,27 +441,25 @@ __global__ __launch_bounds__(G::THREADS, G::THREADS >= 512 ? 2 : 1) void gemm_f8
   int pid_m, pid_n;
   tile_coords(blockIdx.x, (p.m + G::BM - 1) / G::BM, (p.n + G::BN - 1) / G::BN, pid_m, pid_n);
   const int m0 = pid_m * G::BM, n0 = pid_n * G::BN;
-  f32x4 acc[G::NT][G::MT];
-#pragma unroll
-  for (int i = 0; i < G::NT; ++i)
-#pragma unroll
-    for (int j = 0; j < G::MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x16 acc[G::FN][G::FM];
+  zero_acc<float, G::FM, G::FN>(acc);
   f8_accumulate<G>(smem, p, m0, n0, acc);
   const bool holds = f8_join_groups<G>(smem, acc);
   const int lane = threadIdx.x & 63;
   const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = gw % G::NW;
   const int wm = wave / G::WN, wn = wave % G::WN;
-  const int mw = m0 + wm * 16 * G::MT, nw = n0 + wn * 16 * G::NT;
+  const int mw = m0 + wm * G::WTM, nw = n0 + wn * G::WTN;
   if constexpr (EPI == kEpiF8 || EPI == kEpiF8Gelu) {
     constexpr int RED = G::BM * G::WN * 4;
+    static_assert(RED + G::BM * G::BN <= G::LDS, "epilogue staging");
     f8_epilogue<EPI == kEpiF8Gelu, G>(p, acc, mw, nw, wm, wn, lane, holds, reinterpret_cast<float*>(smem),
-                                      smem + RED + wave * 256 * G::MT * G::NT);
+                                      smem + RED + wave * 1024 * G::FM * G::FN);
   } else {
-    constexpr int FM = G::MT / 2, FN = G::NT / 2;
-    static_assert(EpiStage<T, EPI, FN>::BYTES * G::NW <= G::LDS, "epilogue staging");
+    typedef EpiStage<T, EPI, G::FN> E;
+    static_assert(E::BYTES * G::NW <= G::LDS, "epilogue staging");
     if (holds)
-      epilogue<T, EPI, FM, FN, NoPrefetch, kResBatch, true>(acc, static_cast<const T*>(p.bias), p.c, p.ldc, p.m, p.n,
-                                                            mw, nw, lane, smem + wave * EpiStage<T, EPI, FN>::BYTES);
+      epilogue<T, EPI, G::FM, G::FN>(acc, static_cast<const T*>(p.bias), p.c, p.ldc, p.m, p.n, mw, nw, lane,
+                                     smem + wave * E::BYTES);
   }
 }
 

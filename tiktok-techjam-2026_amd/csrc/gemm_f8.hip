@@ -5,11 +5,11 @@
 
 namespace tjk {
 
-//                  MT NT WM WN KG STAGES
-typedef F8Geom<4, 8, 4, 2, 1, 2> Tile256;
-typedef F8Geom<4, 4, 2, 2, 1, 2> Tile128;
-typedef F8Geom<2, 4, 2, 2, 2, 2> Tile64x128;
-typedef F8Geom<2, 2, 2, 2, 4, 2> Tile64;
+//             FM FN WM WN KG STAGES
+typedef F8Geom<2, 4, 4, 2, 1, 2> Tile256;
+typedef F8Geom<2, 2, 2, 2, 1, 2> Tile128;
+typedef F8Geom<1, 2, 2, 2, 2, 2> Tile64x128;
+typedef F8Geom<1, 2, 2, 1, 4, 2> Tile64;
 
 template <typename T, int EPI, typename G>
 static int run_tile(const F8GemmArgs& p, hipStream_t s) {

@@ -75,26 +75,32 @@ __device__ __forceinline__ void lds_dma4(u32x4 rsrc, uint32_t voff, uint32_t lds
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(lds_addr));
 }
 
-// WM x WN waves of (32 FM) x (32 FN) outputs, KG groups of them along K
-// (group g takes K tiles g, g + KG, ...), each with a ring of STAGES K tiles
-// of 128 and a table of the scales of 16 K tiles.
-template <int FM_, int FN_, int WM_, int WN_, int KG_, int STAGES_>
+// W x W waves of (32 FM) x (32 FN) outputs, KG groups of them along K (group g
+// takes K tiles g, g + KG, ...).  A K tile (128 deep) is PPS panels: panel j <
+// FM of A holds every wave row's j-th 32 rows, panel FM + i of W every wave
+// column's i-th 32 columns.  Each group has a ring of R panels and a table of the
+// scales of 8 K tiles.
+template <int FM_, int FN_, int W_, int KG_, int R_>
 struct F8Geom {
-  static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, KG = KG_, STAGES = STAGES_;
-  static constexpr int NW = WM * WN, THREADS = 64 * NW * KG;
-  static constexpr int WTM = 32 * FM, WTN = 32 * FN, BM = WTM * WM, BN = WTN * WN;
-  static constexpr int DA = BM / (8 * NW), DW = BN / (8 * NW), NDMA = DA + DW;  // DMA instructions per wave per K tile
-  static constexpr int STAGE = (BM + BN) * 128;
-  static constexpr int TAB = STAGES * STAGE;         // byte of the row scales, [16][BM]
-  static constexpr int TABW = TAB + 16 * BM * 4;     // byte of the weight scales, [2][8 blocks][8]
-  static constexpr int GROUP = TABW + 512;           // bytes per K group
+  static constexpr int FM = FM_, FN = FN_, W = W_, KG = KG_, R = R_;
+  static constexpr int NW = W * W, THREADS = 64 * NW * KG;
+  static constexpr int WTM = 32 * FM, WTN = 32 * FN, BM = WTM * W, BN = WTN * W;
+  static constexpr int PPS = FM + FN, PANEL = 32 * W * 128;
+  static constexpr int DP = 4 / W, ND = PPS * DP;  // DMA instructions per wave: of a panel, of a K tile
+  static constexpr int DS = 2 * FM / W;            // of the row scales of four K tiles
+  static constexpr int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+  static constexpr int PHASES = R / gcd(R, PPS);   // K tiles until the ring's slots repeat
+  static constexpr int TAB = R * PANEL;            // byte of the row scales, [8][BM]
+  static constexpr int TABW = TAB + 8 * BM * 4;    // byte of the weight scales, [2][16 blocks][4]
+  static constexpr int GROUP = TABW + 512;         // bytes per K group
   static constexpr int PARTS = (KG - 1) * BM * BN * 4;  // K groups' sums, over the rings
   static constexpr int LDS = KG * GROUP > PARTS ? KG * GROUP : PARTS;
-  static_assert(DA * 8 * NW == BM && DW * 8 * NW == BN, "tile rows must split over the waves");
+  static_assert(W == 1 || W == 2, "4 / W DMA instructions per panel");
   static_assert(FN % 2 == 0, "fragment double buffer, ring of two products");
   static_assert(128 % WTN == 0, "a wave's columns lie in one block");
-  static_assert(STAGES >= 2 && STAGES <= 8, "a chunk of scales lands within 8 K tiles");
-  static_assert((STAGES - 1) * NDMA + DA + 1 <= 63, "vmcnt range");
+  static_assert(DS * W == 2 * FM, "scales must split over the waves");
+  static_assert(R >= PPS + FM + 1 && PHASES <= 4, "the panels that are read together fit beside those of a K tile");
+  static_assert(R * DP + ND <= 63, "vmcnt range");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -102,24 +108,28 @@ struct F8Geom {
 // of the tile at (m0, n0).  On return every DMA has landed and the workgroup
 // has met at a barrier.
 //
-// Tiles reach LDS by DMA, rows of 128 bytes with the 16-byte chunk c of row r
+// Panels reach LDS by DMA, rows of 128 bytes with the 16-byte chunk c of row r
 // at c ^ f8_swz(r).  Lane (l32, hi) of a fragment's half h reads chunks
 // 4 h + hi and 4 h + 2 + hi of row l32: any assignment of K to lanes is right
 // that both operands share.
 //
-// Pipeline: the FMAs of a product run behind the two MFMAs of the next one, so
-// none waits for the matrix pipe (18 instructions and a pause of two lie
-// between).  W's fragments are read one 32-column tile ahead.  Before the last
-// tile of W everything of a K tile is in registers: there the waves meet, the K
-// tile's slot is handed to the DMA of K tile it + STAGES, and each A fragment is
-// replaced by the next K tile's as soon as its last MFMA is issued.
+// Pipeline.  A K tile runs as FN W tiles of FM products.  The FMAs of a product
+// run behind the two MFMAs of the next one, so none waits for the matrix pipe (18
+// instructions and a pause of two lie between).  Fragments are read one W tile
+// ahead: W's i + 1 during tile i, and during the last one A's and W's first of
+// the next K tile, each A fragment in place of the one whose last MFMA has been
+// issued.  Panels are read in the order A0 .. W0 W1 .. of each K tile, so the ring
+// is a queue: at the meeting before a W tile the panels read during the one
+// before are free, and those about to be read have landed.  A K tile's ND DMA
+// instructions, each into the slot of a panel read at least one meeting ago, are
+// spread evenly over its products: a burst stalls the waves that issue it.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x16 (&acc)[G::FN][G::FM]) {
-  constexpr int FM = G::FM, FN = G::FN, NW = G::NW, KG = G::KG, S = G::STAGES;
+  constexpr int FM = G::FM, FN = G::FN, NW = G::NW, KG = G::KG, R = G::R, PPS = G::PPS, DP = G::DP;
   const int lane = threadIdx.x & 63;
   const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kg = gw / NW, wave = gw % NW, wm = wave / G::WN, wn = wave % G::WN;
+  const int kg = gw / NW, wave = gw % NW, wm = wave / G::W, wn = wave % G::W;
   const int l32 = lane & 31, hi = lane >> 5;
   char* const gsm = smem + kg * G::GROUP;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)gsm;
@@ -132,74 +142,70 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   const int nb0 = n0 / 128, nbs = (p.n + 127) / 128;
   const u32x4 rsws = lds_dma_rsrc(p.ws + (int64_t)nb0 * p.ld_ws, (int64_t)(nbs - nb0) * p.ld_ws * 4);
 
-  // DMA instruction i fills rows (i NW + wave) 8 .. + 7 of A (of W from i = DA);
-  // lane l lands in row l / 8, physical chunk l % 8.  A lane's offset stays the
-  // same over the K tiles, whose own offset is a scalar: it takes no vector
-  // instruction next to the FMAs.
-  auto dma_row = [&](int i) __attribute__((always_inline)) {
-    return ((i < G::DA ? i : i - G::DA) * NW + wave) * 8 + lane / 8;
+  // DMA instruction d of a panel fills its rows (d NW + wave) 8 .. + 7: with
+  // two wave rows instruction d the d-th one's.  Lane l lands in row l / 8,
+  // physical chunk l % 8.  A lane's offset stays the same over the K tiles, whose
+  // own offset is a scalar: it takes no vector instruction next to the FMAs.
+  uint32_t voff[PPS][DP];
+  auto dma_chunk = [&](int d) __attribute__((always_inline)) {
+    return (uint32_t)(((lane & 7) ^ f8_swz((d * NW + wave) * 8 + lane / 8)) << 4);
   };
-  auto dma_chunk = [&](int i) __attribute__((always_inline)) {
-    return (uint32_t)(((lane & 7) ^ f8_swz(dma_row(i))) << 4);
-  };
-  uint32_t voff[G::NDMA];
 #pragma unroll
-  for (int i = 0; i < G::NDMA; ++i)
-    voff[i] = (uint32_t)dma_row(i) * (uint32_t)(i < G::DA ? p.lda : p.ldw) + dma_chunk(i);
-  auto dma = [&](int it, int i) __attribute__((always_inline)) {
-    const uint32_t slot = lds0 + (uint32_t)(it % S) * G::STAGE;
-    const uint32_t dst = slot + (i < G::DA ? (i * NW + wave) * 1024 : G::BM * 128 + ((i - G::DA) * NW + wave) * 1024);
-    lds_dma16_at(i < G::DA ? rsa : rsw, voff[i], (uint32_t)(it * KG + kg) * 128u, dst);
-  };
-  // Called before the DMA of K tile `it`: from the K tile that is not whole on,
-  // the chunks past K lie outside the buffer ranges, from the first one past
-  // the end on all do (they arrive as zeros).
-  auto past_end = [&](int it) __attribute__((always_inline)) {
+  for (int y = 0; y < PPS; ++y)
 #pragma unroll
-    for (int i = 0; i < G::NDMA; ++i)
-      voff[i] |= (uint32_t)(it * KG + kg) * 128u + dma_chunk(i) < (uint32_t)p.k ? 0u : kPastEnd;
+    for (int d = 0; d < DP; ++d) {
+      const int r = (d * NW + wave) * 8 + lane / 8;
+      const int row = y < FM ? r / 32 * G::WTM + y * 32 + r % 32 : r / 32 * G::WTN + (y - FM) * 32 + r % 32;
+      voff[y][d] = (uint32_t)row * (uint32_t)(y < FM ? p.lda : p.ldw) + dma_chunk(d);
+    }
+  // instruction d of panel y of K tile `it` into a slot
+  auto dma = [&](int it, int y, int d, int slot) __attribute__((always_inline)) {
+    lds_dma16_at(y < FM ? rsa : rsw, voff[y][d], (uint32_t)(it * KG + kg) * 128u,
+                 lds0 + slot * G::PANEL + (d * NW + wave) * 1024);
   };
-  // scales of K tiles 8 c .. 8 c + 7 of this group, into half c & 1 of the table
+  // Called before the DMA of panel y of K tile `it`: from the K tile that is not
+  // whole on, the chunks past K lie outside the buffer ranges, from the first
+  // one past the end on all do (they arrive as zeros).
+  auto past_end = [&](int it, int y) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DP; ++d)
+      voff[y][d] |= (uint32_t)(it * KG + kg) * 128u + dma_chunk(d) < (uint32_t)p.k ? 0u : kPastEnd;
+  };
+  // scales of K tiles 4 c .. 4 c + 3 of this group, into half c & 1 of the table
   auto scale_dma = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < G::DA; ++d) {
+    for (int d = 0; d < G::DS; ++d) {
       const int f0 = (d * NW + wave) * 64, f = f0 + lane, i = f / G::BM, row = f % G::BM;
-      const int kt = (8 * c + i) * KG + kg;
+      const int kt = (4 * c + i) * KG + kg;
       const uint32_t off = kt < nkt ? ((uint32_t)row * (uint32_t)p.ld_as + (uint32_t)kt) * 4u : kPastEnd;
-      lds_dma4(rsas, off, lds0 + G::TAB + (c & 1) * 8 * G::BM * 4 + f0 * 4);
+      lds_dma4(rsas, off, lds0 + G::TAB + (c & 1) * 4 * G::BM * 4 + f0 * 4);
     }
     if (wave == 0) {
-      const int nb = lane >> 3, kt = (8 * c + (lane & 7)) * KG + kg;
+      const int nb = lane >> 2, kt = (4 * c + (lane & 3)) * KG + kg;
       const uint32_t off = kt < nkt ? ((uint32_t)nb * (uint32_t)p.ld_ws + (uint32_t)kt) * 4u : kPastEnd;
       lds_dma4(rsws, off, lds0 + G::TABW + (c & 1) * 256);
     }
   };
 
   const int sw = (hi ^ f8_swz(l32)) << 4;
-  const char* const fa0 = gsm + (wm * G::WTM + l32) * 128;
-  const char* const fw0 = gsm + G::BM * 128 + (wn * G::WTN + l32) * 128;
-  auto frag = [&](const char* rows, int h) __attribute__((always_inline)) {
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64)));
-    const i32x4 up = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64 + 32)));
+  const char* const fa0 = gsm + (wm * 32 + l32) * 128;
+  const char* const fw0 = gsm + (wn * 32 + l32) * 128;
+  auto frag = [&](const char* rows, int slot, int h) __attribute__((always_inline)) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64)) + slot * G::PANEL);
+    const i32x4 up = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64 + 32)) + slot * G::PANEL);
     return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   const float* const tab = reinterpret_cast<const float*>(gsm + G::TAB) + wm * G::WTM + l32;
-  const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * G::WTN) / 128 - nb0) * 8;
+  const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * G::WTN) / 128 - nb0) * 4;
 
-  // The rows of A of K tile it are all in registers by its second W tile, where
-  // a second meeting (MEET) hands their part of the slot to the DMA of K tile
-  // it + S, so that the DMA spreads over the K tile: A's over the W tiles in the
-  // middle, W's in the last one.
-  constexpr bool MEET = FN >= 4;
-  constexpr int NMID = MEET ? (FN - 2) * FM : 1;
   scale_dma(0);
 #pragma unroll
-  for (int t = 0; t < S; ++t) {
-    past_end(t);
+  for (int q = 0; q < R; ++q) {
+    past_end(q / PPS, q % PPS);
 #pragma unroll
-    for (int i = 0; i < G::NDMA; ++i) dma(t, i);
+    for (int d = 0; d < DP; ++d) dma(q / PPS, q % PPS, d, q);
   }
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * G::NDMA) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R - FM - 1) * DP) : "memory");
   asm volatile("s_barrier" ::: "memory");
 
   i32x8 fa[FM][2], fw[2][2];
@@ -207,12 +213,12 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   float raw[FM], raw_w, s[FM], s_last = 0.f;
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
-    fa[j][0] = frag(fa0 + j * 4096, 0);
-    fa[j][1] = frag(fa0 + j * 4096, 1);
+    fa[j][0] = frag(fa0, j, 0);
+    fa[j][1] = frag(fa0, j, 1);
     raw[j] = tab[32 * j];
   }
-  fw[0][0] = frag(fw0, 0);
-  fw[0][1] = frag(fw0, 1);
+  fw[0][0] = frag(fw0, FM, 0);
+  fw[0][1] = frag(fw0, FM, 1);
   raw_w = tabw[0];
 #pragma unroll
   for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
@@ -229,52 +235,47 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     for (int r = 0; r < 16; ++r) c[r] = fmaf(d[r], f, c[r]);
   };
 
-  for (int it = 0; it < nit; ++it) {
-    const int st = (it % S) * G::STAGE, nx = ((it + 1) % S) * G::STAGE;
-    if ((it & 7) == 0) scale_dma((it >> 3) + 1);
-    if (((it + S) * KG + kg + 1) * 128 > p.k) past_end(it + S);
+  // One K tile, its panels in slots PH PPS .. (mod R).
+  auto step = [&](auto PH, int it) __attribute__((always_inline)) {
+    constexpr int q0 = decltype(PH)::value * PPS;
+    if ((it & 3) == 0) scale_dma((it >> 2) + 1);
+    if (((it + (PPS - 1 + R) / PPS) * KG + kg + 1) * 128 > p.k) {
+#pragma unroll
+      for (int y = 0; y < PPS; ++y) past_end(it + (y + R) / PPS, (y + R) % PPS);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
       const bool last = i + 1 == FN;
-      if (last) {
-        // K tile it + 1 landed
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * G::NDMA + (MEET ? G::DA : 0)) : "memory");
-        asm volatile("s_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-      } else if (MEET && i == 1) {
-        asm volatile("s_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      // Landed: the panels read during this W tile; in flight at most what was
+      // issued after them.
+      constexpr int ISSUED = R * DP;  // before this K tile, from its own first panel on
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(ISSUED + i * FM * G::ND / TILES -
+                                                         DP * (last ? PPS + FM + 1 : FM + i + 2))
+                   : "memory");
+      asm volatile("s_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int v = i * FM + j;
         f8_mma(part[v & 1], fw[i & 1], fa[j]);
         if (last) {
           if (j == 0) {
-            const int o = (it + 1) & 15;
+            const int o = (it + 1) & 7;
 #pragma unroll
             for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
-            raw_w = tabw[(o >> 3) * 64 + (o & 7)];
+            raw_w = tabw[(o >> 2) * 64 + (o & 3)];
           }
-          fa[j][0] = frag(fa0 + nx + j * 4096, 0);
-          fa[j][1] = frag(fa0 + nx + j * 4096, 1);
+          fa[j][0] = frag(fa0, (q0 + PPS + j) % R, 0);
+          fa[j][1] = frag(fa0, (q0 + PPS + j) % R, 1);
         }
-        // fragments of the next W tile, a half after each MFMA pair (both after
-        // the only one)
+        // fragments of the next W tile, a half after each product
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (j == min(h, FM - 1))
-            fw[(i + 1) & 1][h] = last ? frag(fw0 + nx, h) : frag(fw0 + st + (i + 1) * 4096, h);
-        constexpr int D0 = MEET ? G::DA : 0, ND = G::NDMA - D0;
-        if (last) {
+          if (j == min(h, FM - 1)) fw[(i + 1) & 1][h] = frag(fw0, (q0 + FM + (last ? PPS : i + 1)) % R, h);
 #pragma unroll
-          for (int d = j * ND / FM; d < (j + 1) * ND / FM; ++d) dma(it + S, D0 + d);
-        } else if (MEET && i >= 1) {
-          const int u = (i - 1) * FM + j;
-#pragma unroll
-          for (int d = u * G::DA / NMID; d < (u + 1) * G::DA / NMID; ++d) dma(it + S, d);
-        }
+        for (int d = v * G::ND / TILES; d < (v + 1) * G::ND / TILES; ++d)
+          dma(it + (d / DP + R) / PPS, (d / DP + R) % PPS, d % DP, (q0 + d / DP) % R);
         join(v - 1, v == 0 ? s_last : s[(v - 1) % FM]);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -282,6 +283,22 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     s_last = s[FM - 1];
 #pragma unroll
     for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
+  };
+  for (int it = 0; it < nit;) {
+    step(IntC<0>{}, it);
+    if (++it >= nit) break;
+    if constexpr (G::PHASES > 1) {
+      step(IntC<1>{}, it);
+      if (++it >= nit) break;
+    }
+    if constexpr (G::PHASES > 2) {
+      step(IntC<2>{}, it);
+      if (++it >= nit) break;
+    }
+    if constexpr (G::PHASES > 3) {
+      step(IntC<3>{}, it);
+      ++it;
+    }
   }
   asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[1]));
   join(-1, s_last);
@@ -338,7 +355,7 @@ constexpr int kEpiF8 = 8, kEpiF8Gelu = 9;
 // hi) holds columns 32 i + 8 g + 4 hi .. + 3 of rows 32 j + l32, so a row's
 // largest magnitude over the wave's columns takes one lane exchange; where a
 // block of 128 columns spans several waves they trade theirs through LDS (`red`,
-// BM x WN floats; every wave of the workgroup calls this).  Words are put in rows
+// BM x W floats; every wave of the workgroup calls this).  Words are put in rows
 // through `stage` (1024 FM FN bytes of the wave's own), the 16-byte piece c of
 // row r at c ^ x(r), and leave as whole pieces.
 template <bool GELU, typename G>
@@ -436,7 +453,7 @@ __device__ __forceinline__ void f8_epilogue(const F8GemmArgs& p, f32x16 (&acc)[G
 
 // T: the bias's type, and the output's unless that is e4m3
 template <typename T, int EPI, typename G>
-__global__ __launch_bounds__(G::THREADS, G::THREADS >= 512 ? 2 : 1) void gemm_f8_kernel(F8GemmArgs p) {
+__global__ __launch_bounds__(G::THREADS, G::THREADS <= 256 && G::LDS > 80 * 1024 ? 1 : 2) void gemm_f8_kernel(F8GemmArgs p) {
   __shared__ __align__(16) char smem[G::LDS];
   int pid_m, pid_n;
   tile_coords(blockIdx.x, (p.m + G::BM - 1) / G::BM, (p.n + G::BN - 1) / G::BN, pid_m, pid_n);
@@ -447,10 +464,10 @@ __global__ __launch_bounds__(G::THREADS, G::THREADS >= 512 ? 2 : 1) void gemm_f8
   const bool holds = f8_join_groups<G>(smem, acc);
   const int lane = threadIdx.x & 63;
   const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = gw % G::NW;
-  const int wm = wave / G::WN, wn = wave % G::WN;
+  const int wm = wave / G::W, wn = wave % G::W;
   const int mw = m0 + wm * G::WTM, nw = n0 + wn * G::WTN;
   if constexpr (EPI == kEpiF8 || EPI == kEpiF8Gelu) {
-    constexpr int RED = G::BM * G::WN * 4;
+    constexpr int RED = G::BM * G::W * 4;
     static_assert(RED + G::BM * G::BN <= G::LDS, "epilogue staging");
     f8_epilogue<EPI == kEpiF8Gelu, G>(p, acc, mw, nw, wm, wn, lane, holds, reinterpret_cast<float*>(smem),
                                       smem + RED + wave * 1024 * G::FM * G::FN);

@@ -5,11 +5,11 @@
 
 namespace tjk {
 
-//             FM FN WM WN KG STAGES
-typedef F8Geom<2, 4, 4, 2, 1, 2> Tile256;
-typedef F8Geom<2, 2, 2, 2, 1, 2> Tile128;
-typedef F8Geom<1, 2, 2, 2, 2, 2> Tile64x128;
-typedef F8Geom<1, 2, 2, 1, 4, 2> Tile64;
+//             FM FN W KG R
+typedef F8Geom<2, 4, 2, 1, 9> Tile128x256;
+typedef F8Geom<2, 2, 2, 1, 8> Tile128;
+typedef F8Geom<1, 2, 2, 2, 9> Tile64x128;
+typedef F8Geom<1, 2, 1, 4, 9> Tile32x64;
 
 template <typename T, int EPI, typename G>
 static int run_tile(const F8GemmArgs& p, hipStream_t s) {
@@ -23,18 +23,18 @@ struct F8Plan {
   int bm, bn, threads, k_groups;
 };
 #define TJK_F8_PLAN(G) {G::BM, G::BN, G::THREADS, G::KG}
-static const F8Plan kPlans[] = {TJK_F8_PLAN(Tile256), TJK_F8_PLAN(Tile128), TJK_F8_PLAN(Tile64x128), TJK_F8_PLAN(Tile64)};
+static const F8Plan kPlans[] = {TJK_F8_PLAN(Tile128x256), TJK_F8_PLAN(Tile128), TJK_F8_PLAN(Tile64x128), TJK_F8_PLAN(Tile32x64)};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]);
 
 template <typename T, int EPI>
 static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
   switch (plan) {
-    case 0: return run_tile<T, EPI, Tile256>(p, s);
+    case 0: return run_tile<T, EPI, Tile128x256>(p, s);
     case 1: return run_tile<T, EPI, Tile128>(p, s);
     case 2: return run_tile<T, EPI, Tile64x128>(p, s);
     default:
       if constexpr (EPI == kEpiF8 || EPI == kEpiF8Gelu) return run_tile<T, EPI, Tile64x128>(p, s);
-      else return run_tile<T, EPI, Tile64>(p, s);
+      else return run_tile<T, EPI, Tile32x64>(p, s);
   }
 }
 

@@ -75,32 +75,85 @@ __device__ __forceinline__ void lds_dma4(u32x4 rsrc, uint32_t voff, uint32_t lds
   asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(lds_addr));
 }
 
-// W x W waves of (32 FM) x (32 FN) outputs, KG groups of them along K (group g
-// takes K tiles g, g + KG, ...).  A K tile (128 deep) is PPS panels: panel j <
-// FM of A holds every wave row's j-th 32 rows, panel FM + i of W every wave
-// column's i-th 32 columns.  Each group has a ring of R panels and a table of the
-// scales of 8 K tiles.
-template <int FM_, int FN_, int W_, int KG_, int R_>
+// WM x WN waves of (32 FM) x (32 FN) outputs, KG groups of them along K (group
+// g takes K tiles g, g + KG, ...).  A K tile (128 deep) is PPS panels: panel
+// j < FM of A holds every wave row's j-th 32 rows, panel FM + i of W every wave
+// column's i-th 32 columns.  Each group has a ring of RA panels of A, one of RW
+// panels of W, and a table of the scales of 8 K tiles.  MEETINGS: bit i, the
+// waves meet before the i-th W tile (0 and the last are among them).
+template <int FM_, int FN_, int WM_, int WN_, int KG_, int RA_, int RW_, int MEETINGS_ = -1>
 struct F8Geom {
-  static constexpr int FM = FM_, FN = FN_, W = W_, KG = KG_, R = R_;
-  static constexpr int NW = W * W, THREADS = 64 * NW * KG;
-  static constexpr int WTM = 32 * FM, WTN = 32 * FN, BM = WTM * W, BN = WTN * W;
-  static constexpr int PPS = FM + FN, PANEL = 32 * W * 128;
-  static constexpr int DP = 4 / W, ND = PPS * DP;  // DMA instructions per wave: of a panel, of a K tile
-  static constexpr int DS = 2 * FM / W;            // of the row scales of four K tiles
+  static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, KG = KG_, RA = RA_, RW = RW_;
+  static constexpr int NW = WM * WN, THREADS = 64 * NW * KG, TILES = FM * FN;
+  static constexpr int WTM = 32 * FM, WTN = 32 * FN, BM = WTM * WM, BN = WTN * WN;
+  static constexpr int PPS = FM + FN, PA = 32 * WM * 128, PW = 32 * WN * 128;  // panel bytes
+  static constexpr int DPA = 4 / WN, DPW = 4 / WM;        // DMA instructions per wave: of a panel
+  static constexpr int ND = FM * DPA + FN * DPW;          // of a K tile
+  static constexpr int DS = 2 * FM / WN;                  // of the row scales of four K tiles
   static constexpr int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
-  static constexpr int PHASES = R / gcd(R, PPS);   // K tiles until the ring's slots repeat
-  static constexpr int TAB = R * PANEL;            // byte of the row scales, [8][BM]
-  static constexpr int TABW = TAB + 8 * BM * 4;    // byte of the weight scales, [2][16 blocks][4]
-  static constexpr int GROUP = TABW + 512;         // bytes per K group
+  static constexpr int lcm(int a, int b) { return a / gcd(a, b) * b; }
+  static constexpr int PHASES = lcm(RA / gcd(RA, FM), RW / gcd(RW, FN));  // K tiles until the slots repeat
+  static constexpr int RINGW = RA * PA;                // byte of W's ring
+  static constexpr int TAB = RINGW + RW * PW;          // of the row scales, [8][BM]
+  static constexpr int TABW = TAB + 8 * BM * 4;        // of the weight scales, [2][16 blocks][4]
+  static constexpr int BIAS = TABW + 512;              // of the bias, as it is stored
+  static constexpr int GROUP = BIAS + BN * 4;          // bytes per K group
   static constexpr int PARTS = (KG - 1) * BM * BN * 4;  // K groups' sums, over the rings
   static constexpr int LDS = KG * GROUP > PARTS ? KG * GROUP : PARTS;
-  static_assert(W == 1 || W == 2, "4 / W DMA instructions per panel");
+
+  // Panel y (A: y < FM) of a K tile: the first of its DMA instructions, their
+  // number; the panel that goes into its slot when it has been read, and how many
+  // K tiles later that one is.
+  static constexpr int first(int y) { return y < FM ? y * DPA : FM * DPA + (y - FM) * DPW; }
+  static constexpr int count(int y) { return y < FM ? DPA : DPW; }
+  static constexpr int panel(int d) { return d < FM * DPA ? d / DPA : FM + (d - FM * DPA) / DPW; }
+  static constexpr int next(int y) { return y < FM ? (y + RA) % FM : FM + (y - FM + RW) % FN; }
+  static constexpr int ahead(int y) { return y < FM ? (y + RA) / FM : (y - FM + RW) / FN; }
+  static constexpr int AHEAD = ahead(FM - 1) > ahead(PPS - 1) ? ahead(FM - 1) : ahead(PPS - 1);
+  // Whether the waves meet before W tile i, and the W tile of the meeting after.
+  static constexpr bool meets(int i) { return i == 0 || i == FN - 1 || (MEETINGS_ >> i & 1); }
+  static constexpr int until(int i) { return i + 1 >= FN || meets(i + 1) ? i + 1 : until(i + 1); }
+  static constexpr int since(int i) { return meets(i) ? i : since(i - 1); }
+  // DMA instructions of a K tile issued before its product v: evenly spread, but
+  // only into slots whose panel was read before the last meeting (A's and W's
+  // first during the K tile before, W's i + 1 during W tile i).
+  static constexpr int issued(int v) {
+    return v == 0 ? 0
+                  : v * ND / TILES < FM * DPA + (since((v - 1) / FM) + 1) * DPW
+                        ? v * ND / TILES
+                        : FM * DPA + (since((v - 1) / FM) + 1) * DPW;
+  }
+  // DMA instructions issued up to W tile i after those of panel y of the K tile
+  // `later` K tiles on.
+  static constexpr int after(int i, int y, int later) {
+    for (int z = 0; z < PPS; ++z)
+      if (next(z) == y) return issued(i * FM) - (later - ahead(z)) * ND - first(z) - count(z);
+    return 0;
+  }
+  // How many may be in flight at the meeting before W tile i: what was issued
+  // after the last of the panels that are read until the next meeting.
+  static constexpr int in_flight(int i) {
+    int n = 63;
+    for (int t = i; t < until(i); ++t)
+      for (int y = 0; y < PPS; ++y)
+        if (t + 1 < FN ? y == FM + t + 1 : y <= FM) {
+          const int a = after(i, y, t + 1 < FN ? 0 : 1);
+          if (a < n) n = a;
+        }
+    return n;
+  }
+  static constexpr bool valid() {
+    for (int i = 0; i < FN; ++i)
+      if (meets(i) && in_flight(i) < 0) return false;
+    return issued(TILES) == ND;
+  }
+  static_assert(DPA * WN == 4 && DPW * WM == 4, "panels must split over the waves");
   static_assert(FN % 2 == 0, "fragment double buffer, ring of two products");
   static_assert(128 % WTN == 0, "a wave's columns lie in one block");
-  static_assert(DS * W == 2 * FM, "scales must split over the waves");
-  static_assert(R >= PPS + FM + 1 && PHASES <= 4, "the panels that are read together fit beside those of a K tile");
-  static_assert(R * DP + ND <= 63, "vmcnt range");
+  static_assert(DS * WN == 2 * FM, "scales must split over the waves");
+  static_assert(RA >= FM && RW >= FN && PHASES <= 4, "rings of whole K tiles at least");
+  static_assert(valid(), "panels land before they are read");
+  static_assert(RA / FM * FM * DPA + RW / FN * FN * DPW + 2 * ND <= 63, "vmcnt range");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -118,18 +171,17 @@ struct F8Geom {
 // instructions and a pause of two lie between).  Fragments are read one W tile
 // ahead: W's i + 1 during tile i, and during the last one A's and W's first of
 // the next K tile, each A fragment in place of the one whose last MFMA has been
-// issued.  Panels are read in the order A0 .. W0 W1 .. of each K tile, so the ring
-// is a queue: at the meeting before a W tile the panels read during the one
-// before are free, and those about to be read have landed.  A K tile's ND DMA
-// instructions, each into the slot of a panel read at least one meeting ago, are
-// spread evenly over its products: a burst stalls the waves that issue it.
+// issued.  At a meeting of the waves the panels read since the last one are free,
+// and those about to be read have landed.  A K tile's ND DMA instructions, each
+// into the slot of a panel read before the last meeting, are spread over its
+// products: a burst stalls the waves that issue it.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x16 (&acc)[G::FN][G::FM]) {
-  constexpr int FM = G::FM, FN = G::FN, NW = G::NW, KG = G::KG, R = G::R, PPS = G::PPS, DP = G::DP;
+  constexpr int FM = G::FM, FN = G::FN, NW = G::NW, KG = G::KG, PPS = G::PPS;
   const int lane = threadIdx.x & 63;
   const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kg = gw / NW, wave = gw % NW, wm = wave / G::W, wn = wave % G::W;
+  const int kg = gw / NW, wave = gw % NW, wm = wave / G::WN, wn = wave % G::WN;
   const int l32 = lane & 31, hi = lane >> 5;
   char* const gsm = smem + kg * G::GROUP;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)gsm;
@@ -142,34 +194,37 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   const int nb0 = n0 / 128, nbs = (p.n + 127) / 128;
   const u32x4 rsws = lds_dma_rsrc(p.ws + (int64_t)nb0 * p.ld_ws, (int64_t)(nbs - nb0) * p.ld_ws * 4);
 
-  // DMA instruction d of a panel fills its rows (d NW + wave) 8 .. + 7: with
-  // two wave rows instruction d the d-th one's.  Lane l lands in row l / 8,
-  // physical chunk l % 8.  A lane's offset stays the same over the K tiles, whose
-  // own offset is a scalar: it takes no vector instruction next to the FMAs.
-  uint32_t voff[PPS][DP];
-  auto dma_chunk = [&](int d) __attribute__((always_inline)) {
+  // DMA instruction d of a panel fills its rows (d NW + wave) 8 .. + 7; lane l
+  // lands in row l / 8, physical chunk l % 8.  A lane's offset stays the same
+  // over the K tiles, whose own offset is a scalar: it takes no vector
+  // instruction next to the FMAs.
+  uint32_t voff[G::ND];
+  auto dma_chunk = [&](int i) __attribute__((always_inline)) {
+    const int d = i - G::first(G::panel(i));
     return (uint32_t)(((lane & 7) ^ f8_swz((d * NW + wave) * 8 + lane / 8)) << 4);
   };
 #pragma unroll
-  for (int y = 0; y < PPS; ++y)
-#pragma unroll
-    for (int d = 0; d < DP; ++d) {
-      const int r = (d * NW + wave) * 8 + lane / 8;
-      const int row = y < FM ? r / 32 * G::WTM + y * 32 + r % 32 : r / 32 * G::WTN + (y - FM) * 32 + r % 32;
-      voff[y][d] = (uint32_t)row * (uint32_t)(y < FM ? p.lda : p.ldw) + dma_chunk(d);
-    }
-  // instruction d of panel y of K tile `it` into a slot
-  auto dma = [&](int it, int y, int d, int slot) __attribute__((always_inline)) {
-    lds_dma16_at(y < FM ? rsa : rsw, voff[y][d], (uint32_t)(it * KG + kg) * 128u,
-                 lds0 + slot * G::PANEL + (d * NW + wave) * 1024);
+  for (int i = 0; i < G::ND; ++i) {
+    const int y = G::panel(i), r = ((i - G::first(y)) * NW + wave) * 8 + lane / 8;
+    const int row = y < FM ? r / 32 * G::WTM + y * 32 + r % 32 : r / 32 * G::WTN + (y - FM) * 32 + r % 32;
+    voff[i] = (uint32_t)row * (uint32_t)(y < FM ? p.lda : p.ldw) + dma_chunk(i);
+  }
+  // byte in its ring of the slot that panel y of K tile ph (mod PHASES) lies in
+  auto slot = [](int ph, int y) __attribute__((always_inline)) {
+    return y < FM ? (ph * FM + y) % G::RA * G::PA : (ph * FN + y - FM) % G::RW * G::PW;
+  };
+  // DMA instruction i of K tile `it` into the slot at byte `to` of its ring
+  auto dma = [&](int it, int i, int to) __attribute__((always_inline)) {
+    lds_dma16_at(i < FM * G::DPA ? rsa : rsw, voff[i], (uint32_t)(it * KG + kg) * 128u,
+                 lds0 + (i < FM * G::DPA ? 0 : G::RINGW) + to + ((i - G::first(G::panel(i))) * NW + wave) * 1024);
   };
   // Called before the DMA of panel y of K tile `it`: from the K tile that is not
   // whole on, the chunks past K lie outside the buffer ranges, from the first
   // one past the end on all do (they arrive as zeros).
   auto past_end = [&](int it, int y) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < DP; ++d)
-      voff[y][d] |= (uint32_t)(it * KG + kg) * 128u + dma_chunk(d) < (uint32_t)p.k ? 0u : kPastEnd;
+    for (int i = G::first(y); i < G::first(y) + G::count(y); ++i)
+      voff[i] |= (uint32_t)(it * KG + kg) * 128u + dma_chunk(i) < (uint32_t)p.k ? 0u : kPastEnd;
   };
   // scales of K tiles 4 c .. 4 c + 3 of this group, into half c & 1 of the table
   auto scale_dma = [&](int c) __attribute__((always_inline)) {
@@ -189,23 +244,31 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 
   const int sw = (hi ^ f8_swz(l32)) << 4;
   const char* const fa0 = gsm + (wm * 32 + l32) * 128;
-  const char* const fw0 = gsm + (wn * 32 + l32) * 128;
-  auto frag = [&](const char* rows, int slot, int h) __attribute__((always_inline)) {
-    const i32x4 lo = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64)) + slot * G::PANEL);
-    const i32x4 up = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64 + 32)) + slot * G::PANEL);
+  const char* const fw0 = gsm + G::RINGW + (wn * 32 + l32) * 128;
+  auto frag = [&](const char* rows, int at, int h) __attribute__((always_inline)) {
+    const i32x4 lo = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64)) + at);
+    const i32x4 up = *reinterpret_cast<const i32x4*>(rows + (sw ^ (h * 64 + 32)) + at);
     return __builtin_shufflevector(lo, up, 0, 1, 2, 3, 4, 5, 6, 7);
   };
   const float* const tab = reinterpret_cast<const float*>(gsm + G::TAB) + wm * G::WTM + l32;
   const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * G::WTN) / 128 - nb0) * 4;
 
+  // The panels that fill the rings, in the order in which K tiles before the
+  // first would have issued them.
   scale_dma(0);
 #pragma unroll
-  for (int q = 0; q < R; ++q) {
-    past_end(q / PPS, q % PPS);
+  for (int t = -G::AHEAD; t < 0; ++t)
 #pragma unroll
-    for (int d = 0; d < DP; ++d) dma(q / PPS, q % PPS, d, q);
-  }
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((R - FM - 1) * DP) : "memory");
+    for (int z = 0; z < PPS; ++z)
+      if (t + G::ahead(z) >= 0) {
+        const int y = G::next(z), it = t + G::ahead(z);
+        past_end(it, y);
+#pragma unroll
+        for (int d = 0; d < G::count(y); ++d) dma(it, G::first(y) + d, slot(it, y));
+      }
+  // (as before the last W tile of a K tile -1)
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::in_flight(FN - 1) + G::issued(G::TILES) - G::issued((FN - 1) * FM))
+               : "memory");
   asm volatile("s_barrier" ::: "memory");
 
   i32x8 fa[FM][2], fw[2][2];
@@ -213,12 +276,12 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   float raw[FM], raw_w, s[FM], s_last = 0.f;
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
-    fa[j][0] = frag(fa0, j, 0);
-    fa[j][1] = frag(fa0, j, 1);
+    fa[j][0] = frag(fa0, slot(0, j), 0);
+    fa[j][1] = frag(fa0, slot(0, j), 1);
     raw[j] = tab[32 * j];
   }
-  fw[0][0] = frag(fw0, FM, 0);
-  fw[0][1] = frag(fw0, FM, 1);
+  fw[0][0] = frag(fw0, slot(0, FM), 0);
+  fw[0][1] = frag(fw0, slot(0, FM), 1);
   raw_w = tabw[0];
 #pragma unroll
   for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
@@ -226,7 +289,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   for (int r = 0; r < 16; ++r) part[1][r] = 0.f;
 
   // The FMAs of product v = i FM + j (the last of the K tile before: v = -1).
-  constexpr int TILES = FM * FN;
+  constexpr int TILES = G::TILES;
   auto join = [&](int v, float f) __attribute__((always_inline)) {
     f32x16& d = part[v & 1];
     asm volatile("" : "+v"(d));  // not before the MFMAs above
@@ -235,26 +298,24 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     for (int r = 0; r < 16; ++r) c[r] = fmaf(d[r], f, c[r]);
   };
 
-  // One K tile, its panels in slots PH PPS .. (mod R).
+  // One K tile, PH = it mod PHASES.
   auto step = [&](auto PH, int it) __attribute__((always_inline)) {
-    constexpr int q0 = decltype(PH)::value * PPS;
+    constexpr int ph = decltype(PH)::value;
     if ((it & 3) == 0) scale_dma((it >> 2) + 1);
-    if (((it + (PPS - 1 + R) / PPS) * KG + kg + 1) * 128 > p.k) {
+    if (((it + G::AHEAD) * KG + kg + 1) * 128 > p.k) {
 #pragma unroll
-      for (int y = 0; y < PPS; ++y) past_end(it + (y + R) / PPS, (y + R) % PPS);
+      for (int z = 0; z < PPS; ++z) past_end(it + G::ahead(z), G::next(z));
     }
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < FN; ++i) {
-      const bool last = i + 1 == FN;
-      // Landed: the panels read during this W tile; in flight at most what was
-      // issued after them.
-      constexpr int ISSUED = R * DP;  // before this K tile, from its own first panel on
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(ISSUED + i * FM * G::ND / TILES -
-                                                         DP * (last ? PPS + FM + 1 : FM + i + 2))
-                   : "memory");
-      asm volatile("s_barrier" ::: "memory");
-      __builtin_amdgcn_sched_barrier(0);
+    auto tile = [&](auto I) __attribute__((always_inline)) {
+      constexpr int i = decltype(I)::value;
+      constexpr bool last = i + 1 == FN;
+      if constexpr (G::meets(i)) {
+        constexpr int in_flight = G::in_flight(i);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(in_flight) : "memory");
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int v = i * FM + j;
@@ -266,19 +327,28 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
             for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
             raw_w = tabw[(o >> 2) * 64 + (o & 3)];
           }
-          fa[j][0] = frag(fa0, (q0 + PPS + j) % R, 0);
-          fa[j][1] = frag(fa0, (q0 + PPS + j) % R, 1);
+          fa[j][0] = frag(fa0, slot(ph + 1, j), 0);
+          fa[j][1] = frag(fa0, slot(ph + 1, j), 1);
         }
         // fragments of the next W tile, a half after each product
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (j == min(h, FM - 1)) fw[(i + 1) & 1][h] = frag(fw0, (q0 + FM + (last ? PPS : i + 1)) % R, h);
+          if (j == min(h, FM - 1))
+            fw[(i + 1) & 1][h] = frag(fw0, last ? slot(ph + 1, FM) : slot(ph, FM + i + 1), h);
 #pragma unroll
-        for (int d = v * G::ND / TILES; d < (v + 1) * G::ND / TILES; ++d)
-          dma(it + (d / DP + R) / PPS, (d / DP + R) % PPS, d % DP, (q0 + d / DP) % R);
-        join(v - 1, v == 0 ? s_last : s[(v - 1) % FM]);
+        for (int d = G::issued(v); d < G::issued(v + 1); ++d) {
+          const int z = G::panel(d), y = G::next(z);
+          dma(it + G::ahead(z), G::first(y) + d - G::first(z), slot(ph, z));
+        }
+        join(v - 1, v == 0 ? s_last : s[(v - 1 + FM) % FM]);
         __builtin_amdgcn_sched_barrier(0);
       }
+    };
+    tile(IntC<0>{});
+    tile(IntC<1>{});
+    if constexpr (FN > 2) {
+      tile(IntC<2>{});
+      tile(IntC<3>{});
     }
     s_last = s[FM - 1];
 #pragma unroll
@@ -347,56 +417,140 @@ __device__ __forceinline__ bool f8_join_groups(char* smem, f32x16 (&acc)[G::FN][
   }
 }
 
-// Internal epilogue modes: the output in e4m3 with scales per row and 128
-// columns, after the bias (and GELU).
-constexpr int kEpiF8 = 8, kEpiF8Gelu = 9;
+// Two values rounded to nearest even in a 2-byte type, one word.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), t2));
+}
 
-// e4m3 output of a wave's (32 FM) x (32 FN) outputs at (mw, nw).  Lane (l32,
-// hi) holds columns 32 i + 8 g + 4 hi .. + 3 of rows 32 j + l32, so a row's
-// largest magnitude over the wave's columns takes one lane exchange; where a
-// block of 128 columns spans several waves they trade theirs through LDS (`red`,
-// BM x W floats; every wave of the workgroup calls this).  Words are put in rows
-// through `stage` (1024 FM FN bytes of the wave's own), the 16-byte piece c of
-// row r at c ^ x(r), and leave as whole pieces.
-template <bool GELU, typename G>
-__device__ __forceinline__ void f8_epilogue(const F8GemmArgs& p, f32x16 (&acc)[G::FN][G::FM], int mw, int nw, int wm,
-                                            int wn, int lane, bool holds, float* red, char* stage) {
+// The output rows of a wave, (32 FM) x (32 FN) elements of ES bytes from the
+// wave-uniform (mw, nw): stores at byte offsets of a buffer range that ends with
+// the last row and column, so that rows past M are dropped; columns past N go
+// past the range.
+struct F8Rows {
+  __amdgpu_buffer_rsrc_t r;
+  uint32_t pitch;
+  int cols;  // columns from nw on
+  template <int AUX>
+  __device__ __forceinline__ void put16(int row, int col, int es, const uint4& v) const {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at(row, col, 16 / es, es), 0, AUX);
+  }
+  __device__ __forceinline__ void put8(int row, int col, int es, uint32_t x, uint32_t y) const {
+    __builtin_amdgcn_raw_buffer_store_b64(u32x2{x, y}, r, at(row, col, 8 / es, es), 0, 0);
+  }
+  __device__ __forceinline__ void put4(int row, int col, int es, uint32_t x) const {
+    __builtin_amdgcn_raw_buffer_store_b32(x, r, at(row, col, 4 / es, es), 0, 0);
+  }
+  __device__ __forceinline__ uint32_t at(int row, int col, int n, int es) const {
+    return col + n <= cols ? (uint32_t)row * pitch + (uint32_t)(col * es) : kPastEnd;
+  }
+};
+
+template <typename G>
+__device__ __forceinline__ F8Rows f8_rows(const F8GemmArgs& p, int mw, int nw, int es) {
+  const int rows = min(G::WTM, p.m - mw), cols = min(G::WTN, p.n - nw);
+  const int64_t bytes = rows > 0 && cols > 0 ? ((int64_t)(rows - 1) * p.ldc + cols) * es : 0;
+  return F8Rows{wave_rsrc(static_cast<char*>(p.c) + ((int64_t)mw * p.ldc + nw) * es, bytes), (uint32_t)(p.ldc * es), cols};
+}
+
+// acc <- epilogue(acc + bias) of a wave's outputs; the bias of the tile's
+// columns lies in LDS, in T.
+template <typename T, bool GELU, typename G>
+__device__ __forceinline__ void f8_values(const char* smem, f32x16 (&acc)[G::FN][G::FM], int wn, int hi) {
+  const T* const bias = reinterpret_cast<const T*>(smem + G::BIAS) + wn * G::WTN + 4 * hi;
+#pragma unroll
+  for (int i = 0; i < G::FN; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 b = Quad<T>::to(*reinterpret_cast<const typename Quad<T>::raw*>(bias + 32 * i + 8 * g));
+      const float add[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < G::FM; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = acc[i][j][4 * g + r] + add[r];
+          acc[i][j][4 * g + r] = GELU ? gelu_erf(v) : v;
+        }
+    }
+}
+
+// Outputs in a 2-byte type T.  Lane (l32, hi) holds columns 32 i + 8 g + 4 hi
+// .. + 3 of rows 32 j + l32: the lane halves trade quads, so that each holds whole
+// 16-byte pieces, which go through `stage` (64 WTN bytes of the wave's own; piece c
+// of row r at c ^ x(r), EpiStage's conflict-free order) to leave as row segments.
+// All of a 32-row block's pieces are read before the first is stored.
+template <typename T, typename G>
+__device__ __forceinline__ void f8_store(const F8GemmArgs& p, const f32x16 (&acc)[G::FN][G::FM], int mw, int nw,
+                                         int lane, char* stage) {
+  typedef EpiStage<T, TJK_EPI_BIAS, G::FN> E;
+  constexpr int LPR = E::LPR, NIT = 32 * LPR / 64;
+  const int l32 = lane & 31, hi = lane >> 5;
+  const F8Rows out = f8_rows<G>(p, mw, nw, 2);
+  const bool whole = (((uintptr_t)p.c & 15) | (p.ldc & 7) | (p.n & 7)) == 0;
+  const bool wt = (int64_t)p.m * p.n * 2 >= kWtMinBytes;
+#pragma unroll
+  for (int j = 0; j < G::FM; ++j) {
+#pragma unroll
+    for (int i = 0; i < G::FN; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const f32x16& a = acc[i][j];
+        const int r = 8 * k;
+        const auto s0 = __builtin_amdgcn_permlane32_swap(pack2<T>(a[r], a[r + 1]), pack2<T>(a[r + 4], a[r + 5]), false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(pack2<T>(a[r + 2], a[r + 3]), pack2<T>(a[r + 6], a[r + 7]), false, false);
+        *reinterpret_cast<uint4*>(stage + E::at(l32, 4 * i + 2 * k + hi)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+      }
+    uint4 v[NIT];
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int pc = lane + 64 * it;
+      v[it] = *reinterpret_cast<const uint4*>(stage + E::at(pc / LPR, pc % LPR));
+    }
+    auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int pc = lane + 64 * it;
+        f(32 * j + pc / LPR, pc % LPR * 8, v[it]);
+      }
+    };
+    if (!whole) {
+      each([&](int row, int col, const uint4& x) __attribute__((always_inline)) {
+        out.put8(row, col, 2, x.x, x.y);
+        out.put8(row, col + 4, 2, x.z, x.w);
+      });
+    } else if (wt) {
+      each([&](int row, int col, const uint4& x) __attribute__((always_inline)) { out.put16<kStoreWt>(row, col, 2, x); });
+    } else {
+      each([&](int row, int col, const uint4& x) __attribute__((always_inline)) { out.put16<0>(row, col, 2, x); });
+    }
+  }
+}
+
+// Outputs in e4m3.  A row's largest magnitude over the wave's columns takes one
+// lane exchange; where a block of 128 columns spans several waves they trade
+// theirs through LDS (`red`, BM x WN floats; every wave of the workgroup calls
+// this).  Words are put in rows through `stage` (1024 FM FN bytes of the wave's own),
+// the 16-byte piece c of row r at c ^ x(r).
+template <typename G>
+__device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&acc)[G::FN][G::FM], int mw, int nw,
+                                            int wm, int wn, int lane, bool holds, float* red, char* stage) {
   constexpr int FM = G::FM, FN = G::FN, WPB = 128 / G::WTN;
   const int l32 = lane & 31, hi = lane >> 5;
   float top[FM];
-  if (holds) {
-    const float* const bias = static_cast<const float*>(p.bias);
-    float4 b[FN][4];
+#pragma unroll
+  for (int j = 0; j < FM; ++j) {
+    top[j] = 0.f;
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) b[i][g] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (bias != nullptr) {
+      for (int g = 0; g < 4; ++g) {
+        float t = 0.f;
 #pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          b[i][g] = *reinterpret_cast<const float4*>(bias + min(nw + 32 * i + 8 * g + 4 * hi, p.n - 4));
-    }
-#pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      top[j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const bool in = nw + 32 * i + 8 * g + 4 * hi < p.n;
-          const float add[4] = {b[i][g].x, b[i][g].y, b[i][g].z, b[i][g].w};
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = acc[i][j][4 * g + r] + add[r];
-            if (GELU) v = gelu_erf(v);
-            acc[i][j][4 * g + r] = v;
-            top[j] = fmaxf(top[j], in ? fabsf(v) : 0.f);
-          }
-        }
-      top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
-    }
+        for (int r = 0; r < 4; ++r) t = fmaxf(t, fabsf(acc[i][j][4 * g + r]));
+        top[j] = fmaxf(top[j], nw + 32 * i + 8 * g + 4 * hi < p.n ? t : 0.f);
+      }
+    top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
   }
   if constexpr (WPB > 1) {
     if (holds && hi == 0) {
@@ -404,13 +558,11 @@ __device__ __forceinline__ void f8_epilogue(const F8GemmArgs& p, f32x16 (&acc)[G
       for (int j = 0; j < FM; ++j) red[wn * G::BM + wm * G::WTM + 32 * j + l32] = top[j];
     }
     __syncthreads();
-    if (holds) {
 #pragma unroll
-      for (int j = 0; j < FM; ++j)
+    for (int j = 0; j < FM; ++j)
 #pragma unroll
-        for (int o = 0; o < WPB; ++o)
-          top[j] = fmaxf(top[j], red[(wn / WPB * WPB + o) * G::BM + wm * G::WTM + 32 * j + l32]);
-    }
+      for (int o = 0; o < WPB; ++o)
+        top[j] = fmaxf(top[j], red[(wn / WPB * WPB + o) * G::BM + wm * G::WTM + 32 * j + l32]);
   }
   if (!holds) return;
   constexpr int LPR = 2 * FN;  // pieces per row: 8 or 4
@@ -429,54 +581,91 @@ __device__ __forceinline__ void f8_epilogue(const F8GemmArgs& p, f32x16 (&acc)[G
                                      8 * (g & 1) + 4 * hi) =
             f8_pack4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3], inv);
   }
-  uint8_t* const c = static_cast<uint8_t*>(p.c);
-  const bool a16 = ((uintptr_t)c & 15) == 0 && p.ldc % 16 == 0;
-  constexpr int NPC = 32 * FM * LPR;
+  const F8Rows out = f8_rows<G>(p, mw, nw, 1);
+  const bool whole = (((uintptr_t)p.c & 15) | (p.ldc & 15) | (p.n & 15)) == 0;
+  const bool wt = (int64_t)p.m * p.n >= kWtMinBytes;
+  constexpr int NIT = 32 * FM * LPR / 64;
+  uint4 v[NIT];
 #pragma unroll
-  for (int it = 0; it < NPC / 64; ++it) {
-    const int pc = lane + 64 * it, r = pc / LPR, i = pc % LPR;
-    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 16 * LPR + ((i ^ x(r & 31)) << 4));
-    const int m = mw + r, n = nw + 16 * i;
-    if (m < p.m && n < p.n) {
-      uint8_t* const o = c + (int64_t)m * p.ldc + n;
-      if (a16 && n + 16 <= p.n) {
-        *reinterpret_cast<uint4*>(o) = v;
-      } else {  // N and ldc are multiples of 4
-        reinterpret_cast<uint32_t*>(o)[0] = v.x;
-        if (n + 4 < p.n) reinterpret_cast<uint32_t*>(o)[1] = v.y;
-        if (n + 8 < p.n) reinterpret_cast<uint32_t*>(o)[2] = v.z;
-        if (n + 12 < p.n) reinterpret_cast<uint32_t*>(o)[3] = v.w;
-      }
+  for (int it = 0; it < NIT; ++it) {
+    const int pc = lane + 64 * it, r = pc / LPR;
+    v[it] = *reinterpret_cast<const uint4*>(stage + r * 16 * LPR + ((pc % LPR ^ x(r & 31)) << 4));
+  }
+  auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int pc = lane + 64 * it;
+      f(pc / LPR, pc % LPR * 16, v[it]);
     }
+  };
+  if (!whole) {  // N and ldc are multiples of 4
+    each([&](int row, int col, const uint4& q) __attribute__((always_inline)) {
+      out.put4(row, col, 1, q.x);
+      out.put4(row, col + 4, 1, q.y);
+      out.put4(row, col + 8, 1, q.z);
+      out.put4(row, col + 12, 1, q.w);
+    });
+  } else if (wt) {
+    each([&](int row, int col, const uint4& q) __attribute__((always_inline)) { out.put16<kStoreWt>(row, col, 1, q); });
+  } else {
+    each([&](int row, int col, const uint4& q) __attribute__((always_inline)) { out.put16<0>(row, col, 1, q); });
   }
 }
 
-// T: the bias's type, and the output's unless that is e4m3
-template <typename T, int EPI, typename G>
+// Tile of workgroup `bid`: XCD-contiguous ranges of a raster in groups of 1024
+// rows, so that the tiles that an XCD has at work at a time (one or two per CU)
+// lie in a block near a square, whose operands take the least traffic into its L2.
+template <int BM>
+__device__ __forceinline__ void f8_tile_coords(int bid, int tiles_m, int tiles_n, int& pid_m, int& pid_n) {
+  constexpr int ROWS = BM < 1024 ? 1024 / BM : 1;
+  const int t = xcd_remap(bid, tiles_m * tiles_n), group = t / (ROWS * tiles_n);
+  const int rows = min(tiles_m - group * ROWS, ROWS), in = t - group * (ROWS * tiles_n);
+  pid_m = group * ROWS + in % rows;
+  pid_n = in / rows;
+}
+
+// T: the bias's type, and the output's unless that is e4m3 (F8)
+template <typename T, bool GELU, bool F8, typename G>
 __global__ __launch_bounds__(G::THREADS, G::THREADS <= 256 && G::LDS > 80 * 1024 ? 1 : 2) void gemm_f8_kernel(F8GemmArgs p) {
   __shared__ __align__(16) char smem[G::LDS];
   int pid_m, pid_n;
-  tile_coords(blockIdx.x, (p.m + G::BM - 1) / G::BM, (p.n + G::BN - 1) / G::BN, pid_m, pid_n);
+  f8_tile_coords<G::BM>(blockIdx.x, (p.m + G::BM - 1) / G::BM, (p.n + G::BN - 1) / G::BN, pid_m, pid_n);
   const int m0 = pid_m * G::BM, n0 = pid_n * G::BN;
+  const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = gw % G::NW;
+  // the bias of the tile's columns; zeros past N, and without one
+  {
+    const int lane = threadIdx.x & 63;
+    const u32x4 r = lds_dma_rsrc(static_cast<const T*>(p.bias) + n0,
+                                 p.bias != nullptr ? (int64_t)(p.n - n0) * (int64_t)sizeof(T) : 0);
+    constexpr int NI = G::BN * (int)sizeof(T) / 256 > 0 ? G::BN * (int)sizeof(T) / 256 : 1;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      if (i % (G::NW * G::KG) == gw) {
+        const int at = i * 256 + lane * 4;
+        lds_dma4(r, at < G::BN * (int)sizeof(T) ? at : kPastEnd,
+                 (uint32_t)(uintptr_t)(lds_void*)smem + G::BIAS + i * 256);
+      }
+  }
+  static_assert(G::PARTS <= G::BIAS, "the K groups' sums leave group 0's bias alone");
   f32x16 acc[G::FN][G::FM];
   zero_acc<float, G::FM, G::FN>(acc);
   f8_accumulate<G>(smem, p, m0, n0, acc);
   const bool holds = f8_join_groups<G>(smem, acc);
-  const int lane = threadIdx.x & 63;
-  const int gw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = gw % G::NW;
-  const int wm = wave / G::W, wn = wave % G::W;
+  // (an empty asm: nothing derived from the lane stays in a register through the main loop)
+  int lane = threadIdx.x;
+  asm volatile("" : "+v"(lane));
+  lane &= 63;
+  const int wm = wave / G::WN, wn = wave % G::WN;
   const int mw = m0 + wm * G::WTM, nw = n0 + wn * G::WTN;
-  if constexpr (EPI == kEpiF8 || EPI == kEpiF8Gelu) {
-    constexpr int RED = G::BM * G::W * 4;
-    static_assert(RED + G::BM * G::BN <= G::LDS, "epilogue staging");
-    f8_epilogue<EPI == kEpiF8Gelu, G>(p, acc, mw, nw, wm, wn, lane, holds, reinterpret_cast<float*>(smem),
-                                      smem + RED + wave * 1024 * G::FM * G::FN);
+  if (holds) f8_values<T, GELU, G>(smem, acc, wn, lane >> 5);
+  if constexpr (F8) {
+    constexpr int RED = G::BM * G::WN * 4;
+    static_assert(RED + G::BM * G::BN <= G::BIAS, "epilogue staging");
+    f8_quantise<G>(p, acc, mw, nw, wm, wn, lane, holds, reinterpret_cast<float*>(smem),
+                   smem + RED + wave * 1024 * G::FM * G::FN);
   } else {
-    typedef EpiStage<T, EPI, G::FN> E;
-    static_assert(E::BYTES * G::NW <= G::LDS, "epilogue staging");
-    if (holds)
-      epilogue<T, EPI, G::FM, G::FN>(acc, static_cast<const T*>(p.bias), p.c, p.ldc, p.m, p.n, mw, nw, lane,
-                                     smem + wave * E::BYTES);
+    static_assert(64 * G::WTN * G::NW <= G::BIAS, "epilogue staging");
+    if (holds) f8_store<T, G>(p, acc, mw, nw, lane, smem + wave * 64 * G::WTN);
   }
 }
 

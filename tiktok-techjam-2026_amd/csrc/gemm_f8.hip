@@ -5,17 +5,18 @@
 
 namespace tjk {
 
-//             FM FN W KG R
-typedef F8Geom<2, 4, 2, 1, 9> Tile128x256;
-typedef F8Geom<2, 2, 2, 1, 8> Tile128;
-typedef F8Geom<1, 2, 2, 2, 9> Tile64x128;
-typedef F8Geom<1, 2, 1, 4, 9> Tile32x64;
+//             FM FN WM WN KG RA RW
+typedef F8Geom<2, 4, 4, 2, 1, 4, 8, 9> Tile256;
+typedef F8Geom<2, 4, 4, 2, 1, 4, 8> Tile256b;
+typedef F8Geom<2, 4, 2, 2, 1, 3, 6> Tile128x256;
+typedef F8Geom<2, 2, 2, 2, 1, 4, 4> Tile128;
+typedef F8Geom<1, 2, 2, 2, 2, 3, 6> Tile64x128;
 
-template <typename T, int EPI, typename G>
+template <typename T, bool GELU, bool F8, typename G>
 static int run_tile(const F8GemmArgs& p, hipStream_t s) {
   const int64_t tiles = (int64_t)((p.m + G::BM - 1) / G::BM) * ((p.n + G::BN - 1) / G::BN);
   if (tiles * G::THREADS > UINT32_MAX) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: %lld tiles are too many", (long long)tiles);
-  gemm_f8_kernel<T, EPI, G><<<(unsigned)tiles, G::THREADS, 0, s>>>(p);
+  gemm_f8_kernel<T, GELU, F8, G><<<(unsigned)tiles, G::THREADS, 0, s>>>(p);
   return check_launch("tjk_gemm_f8");
 }
 
@@ -23,18 +24,17 @@ struct F8Plan {
   int bm, bn, threads, k_groups;
 };
 #define TJK_F8_PLAN(G) {G::BM, G::BN, G::THREADS, G::KG}
-static const F8Plan kPlans[] = {TJK_F8_PLAN(Tile128x256), TJK_F8_PLAN(Tile128), TJK_F8_PLAN(Tile64x128), TJK_F8_PLAN(Tile32x64)};
+static const F8Plan kPlans[] = {TJK_F8_PLAN(Tile256), TJK_F8_PLAN(Tile256b), TJK_F8_PLAN(Tile128x256), TJK_F8_PLAN(Tile128), TJK_F8_PLAN(Tile64x128)};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]);
 
-template <typename T, int EPI>
+template <typename T, bool GELU, bool F8>
 static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
   switch (plan) {
-    case 0: return run_tile<T, EPI, Tile128x256>(p, s);
-    case 1: return run_tile<T, EPI, Tile128>(p, s);
-    case 2: return run_tile<T, EPI, Tile64x128>(p, s);
-    default:
-      if constexpr (EPI == kEpiF8 || EPI == kEpiF8Gelu) return run_tile<T, EPI, Tile64x128>(p, s);
-      else return run_tile<T, EPI, Tile32x64>(p, s);
+    case 0: return run_tile<T, GELU, F8, Tile256>(p, s);
+    case 1: return run_tile<T, GELU, F8, Tile256b>(p, s);
+    case 2: return run_tile<T, GELU, F8, Tile128x256>(p, s);
+    case 3: return run_tile<T, GELU, F8, Tile128>(p, s);
+    default: return run_tile<T, GELU, F8, Tile64x128>(p, s);
   }
 }
 
@@ -66,8 +66,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
     return fail(TJK_EINVAL, "tjk_gemm_f8: leading dimension too small");
   if (lda % 16 || ldw % 16) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: lda/ldw must be multiples of 16");
   if (ldc % 4) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: ldc must be a multiple of 4");
-  // 256 rows of an operand, or of its scales, within 31-bit byte offsets
-  if (lda > INT32_MAX / 256 || ldw > INT32_MAX / 256 || ld_as > INT32_MAX / 1024 || ld_ws > INT32_MAX / 1024)
+  // 256 rows of an operand, of its scales, or 64 of the output within 31-bit byte offsets
+  if (ldc > INT32_MAX / 256 || lda > INT32_MAX / 256 || ldw > INT32_MAX / 256 || ld_as > INT32_MAX / 1024 || ld_ws > INT32_MAX / 1024)
     return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: leading dimension too large");
   const uintptr_t need_c = f8 ? 3 : 7, need_bias = f8 ? 15 : 7;
   if (((uintptr_t)a & 15) || ((uintptr_t)w & 15) || ((uintptr_t)c & need_c) || ((uintptr_t)bias & need_bias) ||
@@ -78,8 +78,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int plan = plan_id >= 0 ? plan_id : 0;
   const bool gelu = epilogue == TJK_EPI_BIAS_GELU;
-  if (f8) return gelu ? run_plan<float, kEpiF8Gelu>(plan, p, s) : run_plan<float, kEpiF8>(plan, p, s);
+  if (f8) return gelu ? run_plan<float, true, true>(plan, p, s) : run_plan<float, false, true>(plan, p, s);
   if (out_dtype == TJK_F16)
-    return gelu ? run_plan<f16, TJK_EPI_BIAS_GELU>(plan, p, s) : run_plan<f16, TJK_EPI_BIAS>(plan, p, s);
-  return gelu ? run_plan<bf16, TJK_EPI_BIAS_GELU>(plan, p, s) : run_plan<bf16, TJK_EPI_BIAS>(plan, p, s);
+    return gelu ? run_plan<f16, true, false>(plan, p, s) : run_plan<f16, false, false>(plan, p, s);
+  return gelu ? run_plan<bf16, true, false>(plan, p, s) : run_plan<bf16, false, false>(plan, p, s);
 }

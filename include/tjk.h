@@ -394,7 +394,9 @@ int tjk_quantize_f8(const void* x, int x_dtype, int64_t ld_x, void* q, int64_t l
  * residual.
  * Requires k % 16 == 0, n % 4 == 0, lda and ldw multiples of 16 (below 2^23),
  * ldc of 4, 16-byte aligned a and w, and bias and c aligned to 4 elements.
- * plan_id: -1 chooses, else one of tjk_gemm_f8_plan_count() tiles.
+ * plan_id: -1 chooses, else one of tjk_gemm_f8_plan_count() tiles (an e4m3
+ * output takes those of 128 columns or more).  Tiles that split K over groups of
+ * waves add up in another order, always the same.
  */
 int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, int64_t ld_as,
                 const void* w, int64_t ldw, const float* w_scales, int64_t ld_ws,
@@ -402,6 +404,8 @@ int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, int64_t ld_as
                 float* c_scales, int64_t ld_cs, int64_t m, int64_t n, int64_t k,
                 int epilogue, int plan_id, void* stream);
 int tjk_gemm_f8_plan_count(void);
+/* The plan that plan_id -1 takes (host only). */
+int tjk_gemm_f8_default_plan(int64_t m, int64_t n, int64_t k, int out_dtype, int epilogue);
 
 #ifdef __cplusplus
 }

@@ -285,7 +285,8 @@ SHAPES = [(1, 4, 16), (1, 128, 128), (8, 2048, 512), (15, 12, 112), (16, 132, 14
           (64, 512, 2064), (100, 1000, 256), (128, 128, 4112), (130, 516, 272), (300, 388, 1024), (513, 1028, 400)]
 
 
-PLANS = list(range(-1, 8))
+PLANS = list(range(-1, 8))  # every tile, and the rule's choice
+NARROW = 7
 
 
 @pytest.fixture(scope="module")
@@ -311,8 +312,6 @@ def test_gemm(device, problem, m, n, k, plan):
     """Every tile, output type and epilogue at odd sizes, operands and outputs
     inside larger buffers whose other elements are NaN (operands) or kept
     (outputs)."""
-    if plan >= ops.gemm_f8_plan_count():
-        pytest.skip("no such plan")
     (a, a_s), (w, w_s), bias, (v0, err0) = problem(m, n, k)
     for out_dt, epi, with_bias in (("bf16", EPI_BIAS, True), ("f16", EPI_BIAS_GELU, True), ("bf16", EPI_BIAS_GELU, False),
                                    ("f16", EPI_BIAS, False)):
@@ -336,8 +335,8 @@ def test_gemm(device, problem, m, n, k, plan):
 @pytest.mark.parametrize("plan", PLANS)
 @pytest.mark.parametrize("epi", [EPI_BIAS, EPI_BIAS_GELU])
 def test_gemm_f8_output(device, problem, m, n, k, epi, plan):
-    if plan >= ops.gemm_f8_plan_count():
-        pytest.skip("no such plan")
+    if plan == NARROW:
+        pytest.skip("a tile of 64 columns has no whole block of an e4m3 output")
     (a, a_s), (w, w_s), bias, (v, err) = problem(m, n, k)
     if epi == EPI_BIAS_GELU:
         err, v = _gelu_err(v, err), _gelu(v)

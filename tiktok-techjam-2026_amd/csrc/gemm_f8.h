@@ -41,18 +41,17 @@ struct F8GemmArgs {
   int m, n, k;
 };
 
-// The product of one block.  In inline asm, volatile, so that the products and
-// the FMAs that read them stay in the order written: as a builtin the compiler
-// put each FMA right behind its product, which then waited out the matrix pipe.
-// The compiler does not see an MFMA here and inserts no wait states: 20 have to
-// lie between the second MFMA (16 passes) and a read of its result on gfx950.
-__device__ __forceinline__ void f8_mma(f32x16& d, const i32x8 (&w)[2], const i32x8 (&a)[2]) {
-  asm volatile(
-      "v_mfma_f32_32x32x64_f8f6f4 %0, %1, %3, 0\n\t"
-      "v_mfma_f32_32x32x64_f8f6f4 %0, %2, %4, %0\n\t"
-      "s_nop 1"
-      : "=&v"(d)
-      : "v"(w[0]), "v"(w[1]), "v"(a[0]), "v"(a[1]));
+// The two halves of a block's product.  In inline asm, volatile, so that the
+// products and the FMAs that read them stay in the order written: as a builtin the
+// compiler put each FMA right behind its product, which then waited out the
+// matrix pipe.  The compiler does not see an MFMA here and inserts no wait
+// states: 20 have to lie between the second half (16 passes) and a read of the
+// result on gfx950.
+__device__ __forceinline__ void f8_mma0(f32x16& d, const i32x8& w, const i32x8& a) {
+  asm volatile("v_mfma_f32_32x32x64_f8f6f4 %0, %1, %2, 0" : "=&v"(d) : "v"(w), "v"(a));
+}
+__device__ __forceinline__ void f8_mma1(f32x16& d, const i32x8& w, const i32x8& a) {
+  asm volatile("v_mfma_f32_32x32x64_f8f6f4 %0, %1, %2, %0\n\ts_nop 1" : "+v"(d) : "v"(w), "v"(a));
 }
 
 // Chunk of a 128-byte tile row: the 16-byte chunk c of row r lies at
@@ -89,6 +88,7 @@ struct F8Geom {
   static constexpr int PPS = FM + FN, PA = 32 * WM * 128, PW = 32 * WN * 128;  // panel bytes
   static constexpr int DPA = 4 / WN, DPW = 4 / WM;        // DMA instructions per wave: of a panel
   static constexpr int ND = FM * DPA + FN * DPW;          // of a K tile
+  static constexpr bool SPLIT = FN < 4;                   // reads and DMA between a product's MFMAs
   static constexpr int DS = 2 * FM / WN;                  // of the row scales of four K tiles
   static constexpr int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
   static constexpr int lcm(int a, int b) { return a / gcd(a, b) * b; }
@@ -96,10 +96,10 @@ struct F8Geom {
   static constexpr int RINGW = RA * PA;                // byte of W's ring
   static constexpr int TAB = RINGW + RW * PW;          // of the row scales, [8][BM]
   static constexpr int TABW = TAB + 8 * BM * 4;        // of the weight scales, [2][16 blocks][4]
-  static constexpr int BIAS = TABW + 512;              // of the bias, as it is stored
-  static constexpr int GROUP = BIAS + BN * 4;          // bytes per K group
+  static constexpr int GROUP = TABW + 512;             // bytes per K group
   static constexpr int PARTS = (KG - 1) * BM * BN * 4;  // K groups' sums, over the rings
-  static constexpr int LDS = KG * GROUP > PARTS ? KG * GROUP : PARTS;
+  static constexpr int BIAS = KG * GROUP > PARTS ? KG * GROUP : PARTS;  // byte of the bias, as it is stored
+  static constexpr int LDS = BIAS + BN * 4;
 
   // Panel y (A: y < FM) of a K tile: the first of its DMA instructions, their
   // number; the panel that goes into its slot when it has been read, and how many
@@ -166,9 +166,16 @@ struct F8Geom {
 // 4 h + hi and 4 h + 2 + hi of row l32: any assignment of K to lanes is right
 // that both operands share.
 //
-// Pipeline.  A K tile runs as FN W tiles of FM products.  The FMAs of a product
-// run behind the two MFMAs of the next one, so none waits for the matrix pipe (18
-// instructions and a pause of two lie between).  Fragments are read one W tile
+// Pipeline.  A K tile runs as FN W tiles of FM products of two MFMAs (64 cycles
+// each).  The FMAs of a product run behind the second MFMA of the next one, so none
+// waits for the matrix pipe (18 instructions and a pause of two lie between).
+// Between the MFMAs (SPLIT) or behind them come the fragment reads and the DMA
+// instructions; a DMA that cannot issue yet stalls its wave, and each takes 16 cycles
+// of the CU, so four waves that issue one at once hold each other up for 64: under
+// the first MFMA that costs nothing.  1024 x 1024 x 4096 in 128 x 128 tiles, one
+// wave per SIMD: 19.2 us, against 21.4 behind both; the tiles of four W tiles have
+// no registers for it (they spilled, 133 -> 143 us at 8192 x 8192 x 2048).
+// Fragments are read one W tile
 // ahead: W's i + 1 during tile i, and during the last one A's and W's first of
 // the next K tile, each A fragment in place of the one whose last MFMA has been
 // issued.  At a meeting of the waves the panels read since the last one are free,
@@ -194,20 +201,22 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   const int nb0 = n0 / 128, nbs = (p.n + 127) / 128;
   const u32x4 rsws = lds_dma_rsrc(p.ws + (int64_t)nb0 * p.ld_ws, (int64_t)(nbs - nb0) * p.ld_ws * 4);
 
-  // DMA instruction d of a panel fills its rows (d NW + wave) 8 .. + 7; lane l
-  // lands in row l / 8, physical chunk l % 8.  A lane's offset stays the same
-  // over the K tiles, whose own offset is a scalar: it takes no vector
+  // DMA instruction d of a panel fills its rows u .. u + 7, u = (d NW + wave) 8;
+  // lane l lands in row u + l / 8, physical chunk l % 8.  A lane's offset stays
+  // the same over the K tiles, whose own offset is a scalar: it takes no vector
   // instruction next to the FMAs.
   uint32_t voff[G::ND];
-  auto dma_chunk = [&](int i) __attribute__((always_inline)) {
-    const int d = i - G::first(G::panel(i));
-    return (uint32_t)(((lane & 7) ^ f8_swz((d * NW + wave) * 8 + lane / 8)) << 4);
-  };
+  auto dma_u = [&](int i) __attribute__((always_inline)) { return ((i - G::first(G::panel(i))) * NW + wave) * 8; };
+  const int lane_chunk = (lane & 7) ^ f8_swz(lane / 8);
+  auto dma_chunk = [&](int i) __attribute__((always_inline)) { return (uint32_t)((lane_chunk ^ f8_swz(dma_u(i) & 31)) << 4); };
+  {
+    const uint32_t ra = (uint32_t)(lane / 8) * (uint32_t)p.lda, rw = (uint32_t)(lane / 8) * (uint32_t)p.ldw;
 #pragma unroll
-  for (int i = 0; i < G::ND; ++i) {
-    const int y = G::panel(i), r = ((i - G::first(y)) * NW + wave) * 8 + lane / 8;
-    const int row = y < FM ? r / 32 * G::WTM + y * 32 + r % 32 : r / 32 * G::WTN + (y - FM) * 32 + r % 32;
-    voff[i] = (uint32_t)row * (uint32_t)(y < FM ? p.lda : p.ldw) + dma_chunk(i);
+    for (int i = 0; i < G::ND; ++i) {
+      const int y = G::panel(i), u = dma_u(i);
+      const uint32_t row = u / 32 * (y < FM ? G::WTM : G::WTN) + (y < FM ? y : y - FM) * 32 + u % 32;
+      voff[i] = row * (uint32_t)(y < FM ? p.lda : p.ldw) + ((y < FM ? ra : rw) + dma_chunk(i));
+    }
   }
   // byte in its ring of the slot that panel y of K tile ph (mod PHASES) lies in
   auto slot = [](int ph, int y) __attribute__((always_inline)) {
@@ -254,7 +263,8 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   const float* const tabw = reinterpret_cast<const float*>(gsm + G::TABW) + ((n0 + wn * G::WTN) / 128 - nb0) * 4;
 
   // The panels that fill the rings, in the order in which K tiles before the
-  // first would have issued them.
+  // first would have issued them; then a wait as before the last W tile of a K
+  // tile -1.
   scale_dma(0);
 #pragma unroll
   for (int t = -G::AHEAD; t < 0; ++t)
@@ -266,7 +276,6 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
         for (int d = 0; d < G::count(y); ++d) dma(it, G::first(y) + d, slot(it, y));
       }
-  // (as before the last W tile of a K tile -1)
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::in_flight(FN - 1) + G::issued(G::TILES) - G::issued((FN - 1) * FM))
                : "memory");
   asm volatile("s_barrier" ::: "memory");
@@ -319,18 +328,22 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int v = i * FM + j;
-        f8_mma(part[v & 1], fw[i & 1], fa[j]);
+        f8_mma0(part[v & 1], fw[i & 1][0], fa[j][0]);
+        if constexpr (!G::SPLIT) f8_mma1(part[v & 1], fw[i & 1][1], fa[j][1]);
+        __builtin_amdgcn_sched_barrier(0);
         if (last) {
           if (j == 0) {
             const int o = (it + 1) & 7;
 #pragma unroll
             for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
             raw_w = tabw[(o >> 2) * 64 + (o & 3)];
+          } else if (G::SPLIT) {
+            fa[j - 1][1] = frag(fa0, slot(ph + 1, j - 1), 1);
           }
           fa[j][0] = frag(fa0, slot(ph + 1, j), 0);
-          fa[j][1] = frag(fa0, slot(ph + 1, j), 1);
+          if (!G::SPLIT) fa[j][1] = frag(fa0, slot(ph + 1, j), 1);
         }
-        // fragments of the next W tile, a half after each product
+        // fragments of the next W tile, a half per product
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (j == min(h, FM - 1))
@@ -339,6 +352,11 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
         for (int d = G::issued(v); d < G::issued(v + 1); ++d) {
           const int z = G::panel(d), y = G::next(z);
           dma(it + G::ahead(z), G::first(y) + d - G::first(z), slot(ph, z));
+        }
+        if constexpr (G::SPLIT) {
+          __builtin_amdgcn_sched_barrier(0);
+          f8_mma1(part[v & 1], fw[i & 1][1], fa[j][1]);
+          if (last && j + 1 == FM) fa[j][1] = frag(fa0, slot(ph + 1, j), 1);
         }
         join(v - 1, v == 0 ? s_last : s[(v - 1 + FM) % FM]);
         __builtin_amdgcn_sched_barrier(0);
@@ -354,6 +372,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
     for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
   };
+#pragma unroll 1
   for (int it = 0; it < nit;) {
     step(IntC<0>{}, it);
     if (++it >= nit) break;
@@ -612,16 +631,21 @@ __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&
   }
 }
 
-// Tile of workgroup `bid`: XCD-contiguous ranges of a raster in groups of 1024
-// rows, so that the tiles that an XCD has at work at a time (one or two per CU)
+// Tile of workgroup `bid`: XCD-contiguous ranges of a raster in groups of about
+// 1024 rows, so that the tiles that an XCD has at work at a time (one or two per CU)
 // lie in a block near a square, whose operands take the least traffic into its L2.
 template <int BM>
 __device__ __forceinline__ void f8_tile_coords(int bid, int tiles_m, int tiles_n, int& pid_m, int& pid_n) {
-  constexpr int ROWS = BM < 1024 ? 1024 / BM : 1;
+  constexpr int ROWS = BM >= 256 ? 4 : BM >= 128 ? 8 : BM >= 64 ? 16 : 32;
   const int t = xcd_remap(bid, tiles_m * tiles_n), group = t / (ROWS * tiles_n);
   const int rows = min(tiles_m - group * ROWS, ROWS), in = t - group * (ROWS * tiles_n);
-  pid_m = group * ROWS + in % rows;
-  pid_n = in / rows;
+  if (rows == ROWS) {
+    pid_m = group * ROWS + in % ROWS;
+    pid_n = in / ROWS;
+  } else {
+    pid_m = group * ROWS + in % rows;
+    pid_n = in / rows;
+  }
 }
 
 // T: the bias's type, and the output's unless that is e4m3 (F8)
@@ -646,7 +670,6 @@ __global__ __launch_bounds__(G::THREADS, G::THREADS <= 256 && G::LDS > 80 * 1024
                  (uint32_t)(uintptr_t)(lds_void*)smem + G::BIAS + i * 256);
       }
   }
-  static_assert(G::PARTS <= G::BIAS, "the K groups' sums leave group 0's bias alone");
   f32x16 acc[G::FN][G::FM];
   zero_acc<float, G::FM, G::FN>(acc);
   f8_accumulate<G>(smem, p, m0, n0, acc);

@@ -7,10 +7,13 @@ namespace tjk {
 
 //             FM FN WM WN KG RA RW
 typedef F8Geom<2, 4, 4, 2, 1, 4, 8, 9> Tile256;
-typedef F8Geom<2, 4, 4, 2, 1, 4, 8> Tile256b;
 typedef F8Geom<2, 4, 2, 2, 1, 3, 6> Tile128x256;
+typedef F8Geom<3, 2, 2, 2, 1, 6, 4> Tile192x128;
 typedef F8Geom<2, 2, 2, 2, 1, 4, 4> Tile128;
-typedef F8Geom<1, 2, 2, 2, 2, 3, 6> Tile64x128;
+typedef F8Geom<1, 2, 2, 2, 1, 3, 6> Tile64x128;
+typedef F8Geom<1, 2, 2, 2, 2, 3, 6> Tile64x128k2;
+typedef F8Geom<1, 2, 1, 2, 4, 3, 3> Tile32x128k4;
+typedef F8Geom<1, 2, 1, 1, 4, 2, 4> Tile32x64k4;
 
 template <typename T, bool GELU, bool F8, typename G>
 static int run_tile(const F8GemmArgs& p, hipStream_t s) {
@@ -20,21 +23,69 @@ static int run_tile(const F8GemmArgs& p, hipStream_t s) {
   return check_launch("tjk_gemm_f8");
 }
 
+// Estimated microseconds of a launch on MI355X, as gemm.hip's estimate: with
+// `tiles` workgroups, `per_cu` of them resident per CU, a launch is `rounds`
+// fillings of the chip, in which the fullest CU runs `load` workgroups in all,
+// each of `steps` K tiles (per K group), and stores `mb` MB of output:
+//   c0 + c1 rounds + c2 rounds steps + c3 load + c4 load steps + c5 mb + c6 load (GELU)
+// (mb at 5 TB/s).  Non-negative least squares, by relative error and weighted
+// towards tiles near the best of their launch, over the 337 launches of
+// profiles/gemm_f8_tiles.csv (1 to 16384 rows, widths and K from 64 and 128 to
+// 8192).  The tile with the least estimate is 0.3% slower than the best of the
+// eight (geometric mean), three launches more than 10% (at most 21%, one round of
+// 256 x 256 tiles taken for two of 128 x 128).  Without one of the tiles the best
+// would be slower by 0.1 to 1.2%, without 32 x 64 by 9%.
 struct F8Plan {
-  int bm, bn, threads, k_groups;
+  int bm, bn, per_cu, k_groups;
+  float c[7];
 };
-#define TJK_F8_PLAN(G) {G::BM, G::BN, G::THREADS, G::KG}
-static const F8Plan kPlans[] = {TJK_F8_PLAN(Tile256), TJK_F8_PLAN(Tile256b), TJK_F8_PLAN(Tile128x256), TJK_F8_PLAN(Tile128), TJK_F8_PLAN(Tile64x128)};
+static const F8Plan kPlans[] = {
+    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {0.999f, 4.118f, 1.405f, 0.000f, 0.000f, 0.624f, 5.777f}},
+    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.656f, 3.243f, 0.195f, 0.000f, 0.745f, 0.451f, 2.977f}},
+    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {1.043f, 3.430f, 0.000f, 0.000f, 0.680f, 0.393f, 2.274f}},
+    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {2.196f, 2.048f, 0.006f, 0.000f, 0.456f, 0.420f, 1.353f}},
+    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {2.749f, 1.398f, 0.086f, 0.000f, 0.272f, 0.620f, 0.484f}},
+    {Tile64x128k2::BM, Tile64x128k2::BN, 1, Tile64x128k2::KG, {1.434f, 3.160f, 0.496f, 0.000f, 0.000f, 1.550f, 0.790f}},
+    {Tile32x128k4::BM, Tile32x128k4::BN, 1, Tile32x128k4::KG, {1.563f, 3.566f, 0.758f, 0.000f, 0.000f, 2.399f, 0.743f}},
+    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.296f, 0.000f, 0.000f, 3.204f, 0.483f, 2.052f, 0.736f}}};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]);
+
+// The tile with the least estimate.  (An e4m3 output's blocks of 128 columns
+// need tiles as wide.)
+static int auto_plan(int64_t m, int64_t n, int64_t k, bool f8, bool gelu) {
+  int best = 0;
+  float best_us = 0.f;
+  for (int i = 0; i < kPlanCount; ++i) {
+    const F8Plan& q = kPlans[i];
+    if (f8 && q.bn < kF8Block) continue;
+    const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n + q.bn - 1) / q.bn), slots = 256 * q.per_cu;
+    const int64_t full = tiles / slots, rest = tiles % slots;
+    const float rounds = (float)(full + (rest > 0)), load = (float)(full * q.per_cu + (rest + 255) / 256);
+    const float steps = (float)(((k + 127) / 128 + q.k_groups - 1) / q.k_groups);
+    const float mb = (float)m * (float)n * (f8 ? 1.f : 2.f) / 5e6f;
+    const float us = q.c[0] + rounds * (q.c[1] + q.c[2] * steps) + load * (q.c[3] + q.c[4] * steps) + q.c[5] * mb +
+                     (gelu ? q.c[6] * load : 0.f);
+    if (i == 0 || us < best_us) {
+      best = i;
+      best_us = us;
+    }
+  }
+  return best;
+}
 
 template <typename T, bool GELU, bool F8>
 static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
   switch (plan) {
     case 0: return run_tile<T, GELU, F8, Tile256>(p, s);
-    case 1: return run_tile<T, GELU, F8, Tile256b>(p, s);
-    case 2: return run_tile<T, GELU, F8, Tile128x256>(p, s);
+    case 1: return run_tile<T, GELU, F8, Tile128x256>(p, s);
+    case 2: return run_tile<T, GELU, F8, Tile192x128>(p, s);
     case 3: return run_tile<T, GELU, F8, Tile128>(p, s);
-    default: return run_tile<T, GELU, F8, Tile64x128>(p, s);
+    case 4: return run_tile<T, GELU, F8, Tile64x128>(p, s);
+    case 5: return run_tile<T, GELU, F8, Tile64x128k2>(p, s);
+    case 6: return run_tile<T, GELU, F8, Tile32x128k4>(p, s);
+    default:
+      if constexpr (!F8) return run_tile<T, GELU, F8, Tile32x64k4>(p, s);
+      return TJK_EUNSUPPORTED;
   }
 }
 
@@ -43,6 +94,16 @@ static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
 using namespace tjk;
 
 extern "C" int tjk_gemm_f8_plan_count(void) { return kPlanCount; }
+
+extern "C" int tjk_gemm_f8_default_plan(int64_t m, int64_t n, int64_t k, int out_dtype, int epilogue) {
+  if (m <= 0 || n <= 0 || k < 0 || m > INT32_MAX || n > INT32_MAX || k > INT32_MAX)
+    return fail(TJK_EINVAL, "tjk_gemm_f8_default_plan: bad shape");
+  if (out_dtype != TJK_F16 && out_dtype != TJK_BF16 && out_dtype != TJK_E4M3)
+    return fail(TJK_EINVAL, "tjk_gemm_f8_default_plan: bad output dtype %d", out_dtype);
+  if (epilogue != TJK_EPI_BIAS && epilogue != TJK_EPI_BIAS_GELU)
+    return fail(TJK_EINVAL, "tjk_gemm_f8_default_plan: bad epilogue %d", epilogue);
+  return auto_plan(m, n, k, out_dtype == TJK_E4M3, epilogue == TJK_EPI_BIAS_GELU);
+}
 
 extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, int64_t ld_as, const void* w, int64_t ldw,
                            const float* w_scales, int64_t ld_ws, const void* bias, void* c, int out_dtype, int64_t ldc,
@@ -57,6 +118,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
     return fail(TJK_EINVAL, "tjk_gemm_f8: plan %d out of range [-1,%d)", plan_id, kPlanCount);
   if (m == 0 || n == 0) return TJK_OK;
   const bool f8 = out_dtype == TJK_E4M3;
+  if (f8 && plan_id >= 0 && kPlans[plan_id].bn < kF8Block)
+    return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: plan %d has no whole block of an e4m3 output", plan_id);
   if (!a || !w || !a_scales || !w_scales || !c || (f8 && !c_scales)) return fail(TJK_EINVAL, "tjk_gemm_f8: null pointer");
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: shape exceeds int32");
   if (k % 16) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: k=%lld must be a multiple of 16", (long long)k);
@@ -76,8 +139,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
   const F8GemmArgs p{static_cast<const uint8_t*>(a), lda, a_scales, ld_as, static_cast<const uint8_t*>(w), ldw,
                      w_scales, ld_ws, bias, c, ldc, c_scales, ld_cs, (int)m, (int)n, (int)k};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const int plan = plan_id >= 0 ? plan_id : 0;
   const bool gelu = epilogue == TJK_EPI_BIAS_GELU;
+  const int plan = plan_id >= 0 ? plan_id : auto_plan(m, n, k, f8, gelu);
   if (f8) return gelu ? run_plan<float, true, true>(plan, p, s) : run_plan<float, false, true>(plan, p, s);
   if (out_dtype == TJK_F16)
     return gelu ? run_plan<f16, true, false>(plan, p, s) : run_plan<f16, false, false>(plan, p, s);

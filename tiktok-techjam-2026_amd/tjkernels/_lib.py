@@ -66,6 +66,7 @@ _SIGNATURES = {
     "tjk_gemm_f8": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _i64, _i64,
                            _i64, _i32, _i32, _vp]),
     "tjk_gemm_f8_plan_count": (_i32, []),
+    "tjk_gemm_f8_default_plan": (_i32, [_i64, _i64, _i64, _i32, _i32]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -54,6 +54,23 @@ __device__ __forceinline__ void f8_mma1(f32x16& d, const i32x8& w, const i32x8& 
   asm volatile("v_mfma_f32_32x32x64_f8f6f4 %0, %1, %2, %0\n\ts_nop 1" : "+v"(d) : "v"(w), "v"(a));
 }
 
+// A fragment half (32 e4m3 values of one row per lane) in fp16, which holds
+// every e4m3 value exactly (NaN stays NaN): four operands of a 32x32x16 MFMA.
+__device__ __forceinline__ void f8_widen(const i32x8& f, f16x8 (&w)[4]) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * q + d], 1.0f, false);
+      const f16x2 up = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * q + d], 1.0f, true);
+      w[q][4 * d] = lo[0];
+      w[q][4 * d + 1] = lo[1];
+      w[q][4 * d + 2] = up[0];
+      w[q][4 * d + 3] = up[1];
+    }
+}
+
 // Chunk of a 128-byte tile row: the 16-byte chunk c of row r lies at
 // c ^ f8_swz(r).  A fragment read takes one chunk of 32 rows in each lane half.
 // Row bits 0, 1, 2 map to independent masks, and so do 1, 2, 3, and 2, 3, 4: 8
@@ -79,9 +96,11 @@ __device__ __forceinline__ void lds_dma4(u32x4 rsrc, uint32_t voff, uint32_t lds
 // j < FM of A holds every wave row's j-th 32 rows, panel FM + i of W every wave
 // column's i-th 32 columns.  Each group has a ring of RA panels of A, one of RW
 // panels of W, and a table of the scales of 8 K tiles.  MEETINGS: bit i, the
-// waves meet before the i-th W tile (0 and the last are among them).
-template <int FM_, int FN_, int WM_, int WN_, int KG_, int RA_, int RW_, int MEETINGS_ = -1>
+// waves meet before the i-th W tile (0 and the last are among them).  EXACT:
+// exact products, in fp16.
+template <int FM_, int FN_, int WM_, int WN_, int KG_, int RA_, int RW_, int MEETINGS_ = -1, bool EXACT_ = false>
 struct F8Geom {
+  static constexpr bool EXACT = EXACT_;
   static constexpr int FM = FM_, FN = FN_, WM = WM_, WN = WN_, KG = KG_, RA = RA_, RW = RW_;
   static constexpr int NW = WM * WN, THREADS = 64 * NW * KG, TILES = FM * FN;
   static constexpr int WTM = 32 * FM, WTN = 32 * FN, BM = WTM * WM, BN = WTN * WN;
@@ -182,6 +201,16 @@ struct F8Geom {
 // and those about to be read have landed.  A K tile's ND DMA instructions, each
 // into the slot of a panel read before the last meeting, are spread over its
 // products: a burst stalls the waves that issue it.
+//
+// EXACT.  The e4m3 MFMAs drop low bits of products (1.0e-5 of an output's scale
+// was lost, against 1e-7 here); an e4m3 output's scales are fp32 results, so
+// its sums are formed of fragments widened to fp16 in registers, 8 products of 32
+// cycles in place of 2 of 64, with the same panels, rings and meetings.  A is
+// widened once per K tile, W once per wave column: with 192 conversions and FMAs
+// per 32 products of 32 cycles the vector unit is as busy as the matrix unit, and
+// wider wave tiles have no registers left.  5430 x 4096 x 1024 with GELU: 57 us (36
+// with the e4m3 MFMAs); 4096^3: 122 us, 1.12 PFLOP/s.  Spreading the conversions
+// between the MFMAs by hand cost 38 registers more and time (125 us).
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x16 (&acc)[G::FN][G::FM]) {
@@ -307,6 +336,16 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     for (int r = 0; r < 16; ++r) c[r] = fmaf(d[r], f, c[r]);
   };
 
+  f16x8 ah[G::EXACT ? FM : 1][2][4];
+  auto widen_a = [&]() __attribute__((always_inline)) {
+    if constexpr (G::EXACT)
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) f8_widen(fa[j][h], ah[j][h]);
+  };
+  widen_a();
+
   // One K tile, PH = it mod PHASES.
   auto step = [&](auto PH, int it) __attribute__((always_inline)) {
     constexpr int ph = decltype(PH)::value;
@@ -324,6 +363,40 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(in_flight) : "memory");
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (G::EXACT) {
+        f32x16 d[FM];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f16x8 wh[4];
+          f8_widen(fw[0][h], wh);
+          fw[0][h] = frag(fw0, last ? slot(ph + 1, FM) : slot(ph, FM + i + 1), h);
+          if (last) {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) fa[j][h] = frag(fa0, slot(ph + 1, j), h);
+          }
+#pragma unroll
+          for (int j = 0; j < FM; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              d[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wh[q], ah[j][h][q], h + q == 0 ? f32x16{} : d[j], 0, 0, 0);
+        }
+        if (last) {
+          const int o = (it + 1) & 7;
+#pragma unroll
+          for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
+          raw_w = tabw[(o >> 2) * 64 + (o & 3)];
+        }
+#pragma unroll
+        for (int n = G::issued(i * FM); n < G::issued((i + 1) * FM); ++n) {
+          const int z = G::panel(n), y = G::next(z);
+          dma(it + G::ahead(z), G::first(y) + n - G::first(z), slot(ph, z));
+        }
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(d[j][r], s[j], acc[i][j][r]);
+        return;
       }
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
@@ -371,6 +444,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     s_last = s[FM - 1];
 #pragma unroll
     for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
+    widen_a();
   };
 #pragma unroll 1
   for (int it = 0; it < nit;) {
@@ -389,8 +463,10 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
       ++it;
     }
   }
-  asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[1]));
-  join(-1, s_last);
+  if constexpr (!G::EXACT) {
+    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[1]));
+    join(-1, s_last);
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }

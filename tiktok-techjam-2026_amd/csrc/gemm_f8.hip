@@ -14,6 +14,12 @@ typedef F8Geom<1, 2, 2, 2, 1, 3, 6> Tile64x128;
 typedef F8Geom<1, 2, 2, 2, 2, 3, 6> Tile64x128k2;
 typedef F8Geom<1, 2, 1, 2, 4, 3, 3> Tile32x128k4;
 typedef F8Geom<1, 2, 1, 1, 4, 2, 4> Tile32x64k4;
+// of e4m3 outputs
+typedef F8Geom<2, 2, 2, 4, 1, 4, 4, -1, true> Exact128x256;
+typedef F8Geom<2, 2, 2, 2, 1, 4, 4, -1, true> Exact128;
+typedef F8Geom<1, 2, 2, 2, 1, 3, 6, -1, true> Exact64x128;
+typedef F8Geom<1, 2, 2, 2, 2, 3, 6, -1, true> Exact64x128k2;
+typedef F8Geom<1, 2, 1, 2, 4, 3, 3, -1, true> Exact32x128k4;
 
 template <typename T, bool GELU, bool F8, typename G>
 static int run_tile(const F8GemmArgs& p, hipStream_t s) {
@@ -29,35 +35,41 @@ static int run_tile(const F8GemmArgs& p, hipStream_t s) {
 // each of `steps` K tiles (per K group), and stores `mb` MB of output:
 //   c0 + c1 rounds + c2 rounds steps + c3 load + c4 load steps + c5 mb + c6 load (GELU)
 // (mb at 5 TB/s).  Non-negative least squares, by relative error and weighted
-// towards tiles near the best of their launch, over the 337 launches of
+// towards tiles near the best of their launch, over the 336 launches of
 // profiles/gemm_f8_tiles.csv (1 to 16384 rows, widths and K from 64 and 128 to
-// 8192).  The tile with the least estimate is 0.3% slower than the best of the
-// eight (geometric mean), three launches more than 10% (at most 21%, one round of
+// 8192), for e4m3 outputs over the 262 of profiles/gemm_f8_e4m3_tiles.csv.  The
+// tile with the least estimate is 0.3% slower than the best of its list (geometric
+// mean), three launches of either list more than 10% (at most 21%, one round of
 // 256 x 256 tiles taken for two of 128 x 128).  Without one of the tiles the best
-// would be slower by 0.1 to 1.2%, without 32 x 64 by 9%.
+// would be slower by 0.1 to 1.3%, without 32 x 64 by 9%; of the e4m3 list
+// by 0.1 to 2.9%, without 32 x 128 by 9%.
 struct F8Plan {
   int bm, bn, per_cu, k_groups;
   float c[7];
 };
 static const F8Plan kPlans[] = {
-    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {0.999f, 4.118f, 1.405f, 0.000f, 0.000f, 0.624f, 5.777f}},
-    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.656f, 3.243f, 0.195f, 0.000f, 0.745f, 0.451f, 2.977f}},
-    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {1.043f, 3.430f, 0.000f, 0.000f, 0.680f, 0.393f, 2.274f}},
-    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {2.196f, 2.048f, 0.006f, 0.000f, 0.456f, 0.420f, 1.353f}},
-    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {2.749f, 1.398f, 0.086f, 0.000f, 0.272f, 0.620f, 0.484f}},
-    {Tile64x128k2::BM, Tile64x128k2::BN, 1, Tile64x128k2::KG, {1.434f, 3.160f, 0.496f, 0.000f, 0.000f, 1.550f, 0.790f}},
-    {Tile32x128k4::BM, Tile32x128k4::BN, 1, Tile32x128k4::KG, {1.563f, 3.566f, 0.758f, 0.000f, 0.000f, 2.399f, 0.743f}},
-    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.296f, 0.000f, 0.000f, 3.204f, 0.483f, 2.052f, 0.736f}}};
-constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]);
+    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {1.102f, 0.000f, 1.404f, 4.009f, 0.000f, 0.635f, 5.457f}},
+    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.642f, 3.257f, 0.196f, 0.000f, 0.745f, 0.450f, 2.988f}},
+    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {1.056f, 3.417f, 0.000f, 0.000f, 0.680f, 0.396f, 2.268f}},
+    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {2.189f, 2.054f, 0.005f, 0.000f, 0.456f, 0.419f, 1.355f}},
+    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {2.775f, 1.372f, 0.087f, 0.000f, 0.271f, 0.631f, 0.480f}},
+    {Tile64x128k2::BM, Tile64x128k2::BN, 1, Tile64x128k2::KG, {1.446f, 3.147f, 0.496f, 0.000f, 0.000f, 1.552f, 0.789f}},
+    {Tile32x128k4::BM, Tile32x128k4::BN, 1, Tile32x128k4::KG, {1.568f, 3.561f, 0.758f, 0.000f, 0.000f, 2.400f, 0.742f}},
+    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.278f, 0.000f, 0.000f, 3.222f, 0.483f, 2.045f, 0.737f}}};
+static const F8Plan kPlansF8[] = {
+    {Exact128x256::BM, Exact128x256::BN, 1, Exact128x256::KG, {1.332f, 3.368f, 1.632f, 0.000f, 0.000f, 1.352f, 2.407f}},
+    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.899f, 0.506f, 0.145f, 0.000f, 0.811f, 1.250f, 1.468f}},
+    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.603f, 0.401f, 0.288f, 0.183f, 0.391f, 1.734f, 0.653f}},
+    {Exact64x128k2::BM, Exact64x128k2::BN, 1, Exact64x128k2::KG, {1.163f, 0.000f, 0.942f, 3.782f, 0.000f, 2.293f, 0.699f}},
+    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {0.613f, 0.000f, 1.025f, 4.843f, 0.000f, 4.092f, 0.777f}}};
+constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]), kPlanCountF8 = sizeof(kPlansF8) / sizeof(kPlansF8[0]);
 
-// The tile with the least estimate.  (An e4m3 output's blocks of 128 columns
-// need tiles as wide.)
+// The tile with the least estimate.
 static int auto_plan(int64_t m, int64_t n, int64_t k, bool f8, bool gelu) {
   int best = 0;
   float best_us = 0.f;
-  for (int i = 0; i < kPlanCount; ++i) {
-    const F8Plan& q = kPlans[i];
-    if (f8 && q.bn < kF8Block) continue;
+  for (int i = 0; i < (f8 ? kPlanCountF8 : kPlanCount); ++i) {
+    const F8Plan& q = f8 ? kPlansF8[i] : kPlans[i];
     const int64_t tiles = ((m + q.bm - 1) / q.bm) * ((n + q.bn - 1) / q.bn), slots = 256 * q.per_cu;
     const int64_t full = tiles / slots, rest = tiles % slots;
     const float rounds = (float)(full + (rest > 0)), load = (float)(full * q.per_cu + (rest + 255) / 256);
@@ -73,19 +85,28 @@ static int auto_plan(int64_t m, int64_t n, int64_t k, bool f8, bool gelu) {
   return best;
 }
 
-template <typename T, bool GELU, bool F8>
+template <typename T, bool GELU>
 static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
   switch (plan) {
-    case 0: return run_tile<T, GELU, F8, Tile256>(p, s);
-    case 1: return run_tile<T, GELU, F8, Tile128x256>(p, s);
-    case 2: return run_tile<T, GELU, F8, Tile192x128>(p, s);
-    case 3: return run_tile<T, GELU, F8, Tile128>(p, s);
-    case 4: return run_tile<T, GELU, F8, Tile64x128>(p, s);
-    case 5: return run_tile<T, GELU, F8, Tile64x128k2>(p, s);
-    case 6: return run_tile<T, GELU, F8, Tile32x128k4>(p, s);
-    default:
-      if constexpr (!F8) return run_tile<T, GELU, F8, Tile32x64k4>(p, s);
-      return TJK_EUNSUPPORTED;
+    case 0: return run_tile<T, GELU, false, Tile256>(p, s);
+    case 1: return run_tile<T, GELU, false, Tile128x256>(p, s);
+    case 2: return run_tile<T, GELU, false, Tile192x128>(p, s);
+    case 3: return run_tile<T, GELU, false, Tile128>(p, s);
+    case 4: return run_tile<T, GELU, false, Tile64x128>(p, s);
+    case 5: return run_tile<T, GELU, false, Tile64x128k2>(p, s);
+    case 6: return run_tile<T, GELU, false, Tile32x128k4>(p, s);
+    default: return run_tile<T, GELU, false, Tile32x64k4>(p, s);
+  }
+}
+
+template <bool GELU>
+static int run_plan_f8(int plan, const F8GemmArgs& p, hipStream_t s) {
+  switch (plan) {
+    case 0: return run_tile<float, GELU, true, Exact128x256>(p, s);
+    case 1: return run_tile<float, GELU, true, Exact128>(p, s);
+    case 2: return run_tile<float, GELU, true, Exact64x128>(p, s);
+    case 3: return run_tile<float, GELU, true, Exact64x128k2>(p, s);
+    default: return run_tile<float, GELU, true, Exact32x128k4>(p, s);
   }
 }
 
@@ -118,8 +139,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
     return fail(TJK_EINVAL, "tjk_gemm_f8: plan %d out of range [-1,%d)", plan_id, kPlanCount);
   if (m == 0 || n == 0) return TJK_OK;
   const bool f8 = out_dtype == TJK_E4M3;
-  if (f8 && plan_id >= 0 && kPlans[plan_id].bn < kF8Block)
-    return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: plan %d has no whole block of an e4m3 output", plan_id);
+  if (f8 && plan_id >= kPlanCountF8)
+    return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: an e4m3 output has plans 0 to %d, not %d", kPlanCountF8 - 1, plan_id);
   if (!a || !w || !a_scales || !w_scales || !c || (f8 && !c_scales)) return fail(TJK_EINVAL, "tjk_gemm_f8: null pointer");
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: shape exceeds int32");
   if (k % 16) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: k=%lld must be a multiple of 16", (long long)k);
@@ -141,8 +162,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const bool gelu = epilogue == TJK_EPI_BIAS_GELU;
   const int plan = plan_id >= 0 ? plan_id : auto_plan(m, n, k, f8, gelu);
-  if (f8) return gelu ? run_plan<float, true, true>(plan, p, s) : run_plan<float, false, true>(plan, p, s);
+  if (f8) return gelu ? run_plan_f8<true>(plan, p, s) : run_plan_f8<false>(plan, p, s);
   if (out_dtype == TJK_F16)
-    return gelu ? run_plan<f16, true, false>(plan, p, s) : run_plan<f16, false, false>(plan, p, s);
-  return gelu ? run_plan<bf16, true, false>(plan, p, s) : run_plan<bf16, false, false>(plan, p, s);
+    return gelu ? run_plan<f16, true>(plan, p, s) : run_plan<f16, false>(plan, p, s);
+  return gelu ? run_plan<bf16, true>(plan, p, s) : run_plan<bf16, false>(plan, p, s);
 }

@@ -108,16 +108,86 @@ def test_wrappers_take_device_tensors_only():
 
 def test_scale_layouts():
     """Scales: fp32, enough rows and blocks, unit column stride, no row
-    repeated by a zero stride; one row or one block may have any stride."""
-    ok = ops._f8_scales
-    assert ok(torch.zeros(4, 3), 4, 260, "s") == 3
-    assert ok(torch.zeros(4, 8)[:, :3], 4, 260, "s") == 8
-    assert ok(torch.zeros(1, 3).t().contiguous().t(), 1, 260, "s") == 3
-    assert ok(torch.zeros(4, 8)[:, 2:3], 4, 128, "s") == 8
-    for bad in (None, torch.zeros(4, 2), torch.zeros(3, 3), torch.zeros(4, 3, dtype=torch.float64),
+    repeated by a zero stride; one row or one block may have any stride.  (What
+    is well formed is refused last, for its device.)"""
+    def call(s, rows, cols):
+        x, q = torch.zeros(rows, cols), torch.zeros(rows, cols, dtype=ops.F8)
+        ops.quantize_f8(x, q, s)
+
+    for s, rows, cols in ((torch.zeros(4, 3), 4, 260), (torch.zeros(4, 8)[:, :3], 4, 260), (torch.zeros(5, 8), 4, 260),
+                          (torch.zeros(1, 3).t().contiguous().t(), 1, 260), (torch.zeros(4, 8)[:, 2:3], 4, 128)):
+        with pytest.raises(TjkError, match="device tensors"):
+            call(s, rows, cols)
+    for bad in (torch.zeros(4, 2), torch.zeros(3, 3), torch.zeros(4, 3, dtype=torch.float64),
                 torch.zeros(3, 4).t(), torch.zeros(1, 3).expand(4, 3), torch.zeros(12)):
         with pytest.raises(TjkError, match="float32"):
-            ok(bad, 4, 260, "s")
+            call(bad, 4, 260)
+
+
+def _bf16(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+def _e4m3(*shape):
+    return torch.zeros(*shape, dtype=ops.F8)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(res=torch.zeros(4, 256).t()), "row-major"), (dict(res=torch.zeros(256)), "row-major"),
+    (dict(res=torch.zeros(4, 256, dtype=torch.float64)), "dtype"), (dict(res=[1.0]), "must be a tensor"),
+    (dict(res=None), "must be a tensor"), (dict(delta=_bf16(3, 256)), "delta must be"),
+    (dict(delta=_bf16(4, 264)), "delta must be"), (dict(delta=torch.zeros(4, 256, dtype=torch.int32)), "dtype"),
+    (dict(out=_bf16(4, 248), scales=None), "out must be"), (dict(res_out=torch.zeros(2, 256)), "res_out must be"),
+    (dict(gamma=torch.ones(255)), "gamma"), (dict(gamma=_bf16(256)), "gamma"), (dict(gamma=torch.ones(1, 256)), "gamma"),
+    (dict(gamma=torch.ones(512)[::2]), "gamma"), (dict(scales=None), "float32"), (dict(scales=torch.zeros(4, 1)), "float32"),
+    (dict(out=_bf16(4, 256)), "belong to"), (dict(), "device tensors"),
+])
+def test_norm_wrapper_refusals(kw, word):
+    a = dict(res=torch.zeros(4, 256), delta=_bf16(4, 256), gamma=torch.ones(256), eps=1e-5, out=_e4m3(4, 256),
+             res_out=torch.zeros(4, 256), scales=torch.zeros(4, 2))
+    a.update(kw)
+    with pytest.raises(TjkError, match=word):
+        ops.add_rmsnorm(**a)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(out=_bf16(130, 256)), "out must be"), (dict(out=_e4m3(129, 256)), "out must be"),
+    (dict(out=_e4m3(130, 264)), "out must be"), (dict(block_rows=64), "block_rows"), (dict(block_rows=1 << 40), "range"),
+    (dict(scales=None), "must be a tensor"), (dict(scales=torch.zeros(1, 2)), "float32"),
+    (dict(x=torch.zeros(130, 256, dtype=torch.int8)), "dtype"), (dict(x=torch.zeros(256, 130).t()), "row-major"),
+    (dict(), "device tensors"),
+])
+def test_quantize_wrapper_refusals(kw, word):
+    a = dict(x=torch.zeros(130, 256), out=_e4m3(130, 256), scales=torch.zeros(2, 2), block_rows=128)
+    a.update(kw)
+    with pytest.raises(TjkError, match=word):
+        ops.quantize_f8(**a)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(a=_bf16(4, 256)), "must be float8"), (dict(w=_bf16(132, 256)), "must be float8"),
+    (dict(w=_e4m3(132, 240)), "mismatch"), (dict(out=_bf16(5, 132)), "mismatch"), (dict(out=_bf16(4, 128)), "mismatch"),
+    (dict(out=torch.zeros(4, 132)), "out must be"), (dict(out=_e4m3(4, 132), bias=torch.zeros(132)), "out_scales must be"),
+    (dict(out_scales=torch.zeros(4, 2)), "belong to"), (dict(a_scales=torch.zeros(3, 2)), "a_scales"),
+    (dict(w_scales=torch.zeros(1, 2)), "w_scales"), (dict(w_scales=torch.zeros(2, 1)), "w_scales"),
+    (dict(bias=torch.zeros(132)), "bias"), (dict(bias=_bf16(131)), "bias"), (dict(bias=_bf16(264)[::2]), "bias"),
+    (dict(out=_e4m3(4, 132), out_scales=torch.zeros(4, 2)), "bias"), (dict(a=_e4m3(256, 4).t()), "row-major"),
+    (dict(plan=1 << 32), "range"), (dict(epilogue=-(1 << 40)), "range"), (dict(bias=None), "device tensors"),
+])
+def test_gemm_wrapper_refusals(kw, word):
+    a = dict(a=_e4m3(4, 256), a_scales=torch.zeros(4, 2), w=_e4m3(132, 256), w_scales=torch.zeros(2, 2), bias=_bf16(132),
+             out=_bf16(4, 132))
+    a.update(kw)
+    with pytest.raises(TjkError, match=word):
+        ops.gemm_f8(**a)
+
+
+def test_wrapper_argument_types():
+    a = (torch.zeros(4, 256), None, torch.ones(256), "eps", _bf16(4, 256))
+    with pytest.raises(TypeError):
+        ops.add_rmsnorm(*a)
+    with pytest.raises(TypeError):
+        ops.quantize_f8(torch.zeros(4, 256), _e4m3(4, 256), torch.zeros(4, 2), block_rows="1")
 
 
 def test_every_tile_is_some_shapes_choice():

@@ -141,7 +141,7 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
   const bool f8 = out_dtype == TJK_E4M3;
   if (f8 && plan_id >= kPlanCountF8)
     return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: an e4m3 output has plans 0 to %d, not %d", kPlanCountF8 - 1, plan_id);
-  if (!a || !w || !a_scales || !w_scales || !c || (f8 && !c_scales)) return fail(TJK_EINVAL, "tjk_gemm_f8: null pointer");
+  if ((k && (!a || !w || !a_scales || !w_scales)) || !c || (f8 && !c_scales)) return fail(TJK_EINVAL, "tjk_gemm_f8: null pointer");
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: shape exceeds int32");
   if (k % 16) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: k=%lld must be a multiple of 16", (long long)k);
   if (n % 4) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: n=%lld must be a multiple of 4", (long long)n);

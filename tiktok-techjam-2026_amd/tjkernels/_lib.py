@@ -15,6 +15,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must precede the library load; see module docstring)
 
 LIB_PATH = Path(__file__).with_name("libtjk.so")
+F8_PATH = Path(__file__).with_name("_f8.so")
 ABI_VERSION = 11
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
@@ -96,6 +97,17 @@ def load() -> ctypes.CDLL:
         raise TjkError(f"libtjk ABI version {version}, expected {ABI_VERSION}")
     _lib = lib
     return lib
+
+
+def load_f8():
+    """Import (once) the Python calls of the 8-bit operators, which go past
+    ctypes; raises if they are not built."""
+    load()
+    if not F8_PATH.exists():
+        raise TjkError(f"{F8_PATH} is not built: run `make -C {LIB_PATH.parent.parent / 'csrc'}` "
+                       "or __graft_entry__.build(); tjkernels has no non-HIP fallback")
+    from . import _f8
+    return _f8
 
 
 def check(status: int, what: str) -> None:

@@ -398,64 +398,18 @@ def attn_block(x: torch.Tensor, w_qkv: torch.Tensor, b_qkv: Optional[torch.Tenso
 
 
 F8 = torch.float8_e4m3fn
-F8_BLOCK = 128
-_F8_CODES = {**_lib.DTYPE_CODES, F8: _lib.E4M3}
+F8_BLOCK = 128  # columns (of a weight: and rows) that share a scale
+
+_f8_calls = None
 
 
-# The wrappers of the 8-bit operators look at each tensor's shape, strides and
-# device once: on a call for a few tokens the host's share is the longer one.
-
-def _matrix(t: torch.Tensor, name: str):
-    """(rows, columns, leading dimension) of a 2-D row-major view."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 2 or stride[1] != 1:
-        raise TjkError(f"{name} must be a 2-D row-major view, got shape {tuple(shape)} strides {stride}")
-    return shape[0], shape[1], stride[0]
-
-
-def _f8_scales(t: Optional[torch.Tensor], rows: int, cols: int, name: str) -> int:
-    """Leading dimension of the fp32 scales of a quantised matrix: at least
-    ``rows`` x ceil(cols / 128), unit column stride."""
-    need = -(-cols // F8_BLOCK)
-    if t is not None and t.dtype is torch.float32:
-        shape, stride = t.shape, t.stride()
-        if len(shape) == 2 and shape[0] >= rows and shape[1] >= need and (stride[1] == 1 or shape[1] == 1):
-            if shape[0] == 1:
-                return need
-            if stride[0] >= need:
-                return stride[0]
-    raise TjkError(f"{name} must be a float32 [{rows}, {need}] matrix with unit column stride")
-
-
-def _f8_code(t: torch.Tensor, name: str) -> int:
-    code = _F8_CODES.get(t.dtype)
-    if code is None:
-        raise TjkError(f"{name}: unsupported dtype {t.dtype}")
-    return code
-
-
-def _one_device(*ts: Optional[torch.Tensor]) -> int:
-    """The device that all tensors lie on."""
-    device = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != device:
-            raise TjkError(f"tensors on {ts[0].device} and {t.device}")
-    if device < 0:
-        raise TjkError("tjkernels ops need ROCm device tensors (no CPU path)")
-    return device
-
-
-def _launch_on(device: int, what: str, *args) -> None:
-    """Calls an entry point on the current stream of ``device``, with that as
-    the current device (a launch goes to the current one)."""
-    fn = getattr(_lib.load(), what)
-    if device == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(device) if _raw_stream else torch.cuda.current_stream(device).cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    if status:
-        check(status, what)
+def _f8():
+    """The 8-bit operators' calls (csrc/binding_f8.cpp): they check the tensors
+    and launch, raising TjkError."""
+    global _f8_calls
+    if _f8_calls is None:
+        _f8_calls = _lib.load_f8()
+    return _f8_calls
 
 
 def add_rmsnorm(res: torch.Tensor, delta: Optional[torch.Tensor], gamma: torch.Tensor, eps: float,
@@ -467,31 +421,7 @@ def add_rmsnorm(res: torch.Tensor, delta: Optional[torch.Tensor], gamma: torch.T
     With a float8_e4m3fn ``out`` the result is quantised: ``scales`` (fp32
     [rows, ceil(n / 128)]) receives one scale per row and 128 columns, as
     ``gemm_f8`` takes them.  res_out may be res or delta itself."""
-    device = _one_device(res, delta, gamma, out, res_out, scales)
-    rows, n, ld_res = _matrix(res, "res")
-
-    def like(t: torch.Tensor, name: str) -> int:
-        r, c, ld = _matrix(t, name)
-        if r < rows or c != n:
-            raise TjkError(f"{name} must be [{rows}, {n}], got {tuple(t.shape)}")
-        return ld
-
-    ld_out = like(out, "out")
-    ld_delta = ld_ro = delta_code = ro_code = 0
-    if delta is not None:
-        ld_delta, delta_code = like(delta, "delta"), _f8_code(delta, "delta")
-    if res_out is not None:
-        ld_ro, ro_code = like(res_out, "res_out"), _f8_code(res_out, "res_out")
-    if gamma.dtype is not torch.float32 or gamma.shape != (n,) or not gamma.is_contiguous():
-        raise TjkError(f"gamma must be a contiguous float32 vector of {n} elements")
-    ld_scales = 0
-    if out.dtype is F8:
-        ld_scales = _f8_scales(scales, rows, n, "scales")
-    elif scales is not None:
-        raise TjkError("scales belong to a float8_e4m3fn out")
-    _launch_on(device, "tjk_add_rmsnorm", res.data_ptr(), _f8_code(res, "res"), ld_res, _ptr(delta), delta_code, ld_delta,
-               _ptr(res_out), ro_code, ld_ro, out.data_ptr(), _f8_code(out, "out"), ld_out, _ptr(scales), ld_scales,
-               gamma.data_ptr(), rows, n, eps)
+    _f8().add_rmsnorm(res, delta, gamma, eps, out, res_out, scales)
     return out
 
 
@@ -499,16 +429,7 @@ def quantize_f8(x: torch.Tensor, out: torch.Tensor, scales: torch.Tensor, block_
     """Quantises x [rows, n] to float8_e4m3fn: ``out`` [rows, n] and the fp32
     ``scales`` of its blocks, of one row (activations) or 128 rows (weights;
     ``block_rows=128``) and 128 columns."""
-    device = _one_device(x, out, scales)
-    rows, n, ld_x = _matrix(x, "x")
-    out_rows, out_n, ld_out = _matrix(out, "out")
-    if out.dtype is not F8 or out_rows < rows or out_n != n:
-        raise TjkError(f"out must be a float8_e4m3fn [{rows}, {n}] matrix, got {out.dtype} {tuple(out.shape)}")
-    if block_rows not in (1, F8_BLOCK):
-        raise TjkError(f"block_rows must be 1 or {F8_BLOCK}, got {block_rows}")
-    ld_scales = _f8_scales(scales, -(-rows // block_rows), n, "scales")
-    _launch_on(device, "tjk_quantize_f8", x.data_ptr(), _f8_code(x, "x"), ld_x, out.data_ptr(), ld_out,
-               scales.data_ptr(), ld_scales, rows, n, block_rows)
+    _f8().quantize_f8(x, out, scales, block_rows)
     return out
 
 
@@ -526,31 +447,11 @@ def gemm_f8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: 
     ``out`` is float16, bfloat16, or float8_e4m3fn with ``out_scales``
     [m, ceil(n / 128)]; ``bias`` has a 2-byte out's dtype, else float32.
     Epilogues EPI_BIAS and EPI_BIAS_GELU: a 2-byte output is added to an fp32
-    residual by the next ``add_rmsnorm`` or ``add_layernorm``, as its delta."""
-    device = _one_device(a, a_scales, w, w_scales, bias, out, out_scales)
-    dtype = out.dtype
-    if a.dtype is not F8 or w.dtype is not F8:
-        raise TjkError(f"gemm_f8 operands must be float8_e4m3fn, got {a.dtype} and {w.dtype}")
-    m, k, lda = _matrix(a, "a")
-    n, k2, ldw = _matrix(w, "w")
-    out_m, out_n, ldc = _matrix(out, "out")
-    if k != k2 or out_m != m or out_n != n:
-        raise TjkError(f"gemm_f8 shape mismatch a{tuple(a.shape)} w{tuple(w.shape)} out{tuple(out.shape)}")
-    ld_as = _f8_scales(a_scales, m, k, "a_scales")
-    ld_ws = _f8_scales(w_scales, -(-n // F8_BLOCK), k, "w_scales")
-    ld_cs = 0
-    if dtype is F8:
-        ld_cs = _f8_scales(out_scales, m, n, "out_scales")
-    elif dtype is not torch.bfloat16 and dtype is not torch.float16:
-        raise TjkError(f"gemm_f8 out must be float16, bfloat16 or float8_e4m3fn, got {dtype}")
-    elif out_scales is not None:
-        raise TjkError("out_scales belong to a float8_e4m3fn out")
-    if bias is not None and (bias.dtype is not (torch.float32 if dtype is F8 else dtype) or bias.shape != (n,)
-                             or not bias.is_contiguous()):
-        raise TjkError(f"bias must be a contiguous vector of {n} elements, in a 2-byte out's dtype, else float32")
-    _launch_on(device, "tjk_gemm_f8", a.data_ptr(), lda, a_scales.data_ptr(), ld_as, w.data_ptr(), ldw,
-               w_scales.data_ptr(), ld_ws, _ptr(bias), out.data_ptr(), _F8_CODES[dtype], ldc, _ptr(out_scales), ld_cs,
-               m, n, k, epilogue, plan)
+    residual by the next ``add_rmsnorm`` or ``add_layernorm``, as its delta.
+
+    The sums of a 2-byte output are 1.5e-5 off, relative to their 2-norm, those
+    of a float8_e4m3fn output 1e-7."""
+    _f8().gemm_f8(a, a_scales, w, w_scales, bias, out, epilogue, out_scales, plan)
     return out
 
 

@@ -116,8 +116,13 @@ struct F8Geom {
   static constexpr int TAB = RINGW + RW * PW;          // of the row scales, [8][BM]
   static constexpr int TABW = TAB + 8 * BM * 4;        // of the weight scales, [2][16 blocks][4]
   static constexpr int GROUP = TABW + 512;             // bytes per K group
-  static constexpr int PARTS = (KG - 1) * BM * BN * 4;  // K groups' sums, over the rings
+  static constexpr int PITCH = BN + 4;                 // floats between rows of the K groups' sums
+  static constexpr int PARTS = KG > 1 ? KG * BM * PITCH * 4 : 0;  // which lie over the rings
   static constexpr int BIAS = KG * GROUP > PARTS ? KG * GROUP : PARTS;  // byte of the bias, as it is stored
+  // No DMA past the last K tile, in workgroups whose every wave is a K group: each
+  // takes few K tiles, and two past them cost 0.2 of 4.1 us (K = 512).  Not where
+  // waves share K tiles: branches in the K loop cost 4 to 15% of a K tile.
+  static constexpr bool TRIM = KG > 1 && NW == 1;
   static constexpr int LDS = BIAS + BN * 4;
 
   // Panel y (A: y < FM) of a K tile: the first of its DMA instructions, their
@@ -167,7 +172,7 @@ struct F8Geom {
     return issued(TILES) == ND;
   }
   static_assert(DPA * WN == 4 && DPW * WM == 4, "panels must split over the waves");
-  static_assert(FN % 2 == 0, "fragment double buffer, ring of two products");
+  static_assert(FN % 2 == 0 || (FM == 1 && FN == 1 && PHASES % 2 == 0), "fragment double buffer, ring of two products");
   static_assert(128 % WTN == 0, "a wave's columns lie in one block");
   static_assert(DS * WN == 2 * FM, "scales must split over the waves");
   static_assert(RA >= FM && RW >= FN && PHASES <= 4, "rings of whole K tiles at least");
@@ -301,12 +306,16 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     for (int z = 0; z < PPS; ++z)
       if (t + G::ahead(z) >= 0) {
         const int y = G::next(z), it = t + G::ahead(z);
+        if (G::TRIM && it >= nit) continue;
         past_end(it, y);
 #pragma unroll
         for (int d = 0; d < G::count(y); ++d) dma(it, G::first(y) + d, slot(it, y));
       }
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::in_flight(FN - 1) + G::issued(G::TILES) - G::issued((FN - 1) * FM))
-               : "memory");
+  if (G::TRIM && nit < G::AHEAD)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::in_flight(FN - 1) + G::issued(G::TILES) - G::issued((FN - 1) * FM))
+                 : "memory");
   asm volatile("s_barrier" ::: "memory");
 
   i32x8 fa[FM][2], fw[2][2];
@@ -326,10 +335,11 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
   for (int r = 0; r < 16; ++r) part[1][r] = 0.f;
 
-  // The FMAs of product v = i FM + j (the last of the K tile before: v = -1).
+  // The FMAs of product v = i FM + j (the last of the K tile before: v = -1), of a
+  // K tile that begins with part `odd`.
   constexpr int TILES = G::TILES;
-  auto join = [&](int v, float f) __attribute__((always_inline)) {
-    f32x16& d = part[v & 1];
+  auto join = [&](int v, int odd, float f) __attribute__((always_inline)) {
+    f32x16& d = part[(v + odd) & 1];
     asm volatile("" : "+v"(d));  // not before the MFMAs above
     f32x16& c = acc[(v + TILES) % TILES / FM][(v + TILES) % FM];
 #pragma unroll
@@ -349,7 +359,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   // One K tile, PH = it mod PHASES.
   auto step = [&](auto PH, int it) __attribute__((always_inline)) {
     constexpr int ph = decltype(PH)::value;
-    if ((it & 3) == 0) scale_dma((it >> 2) + 1);
+    if ((it & 3) == 0 && (!G::TRIM || it + 4 < nit)) scale_dma((it >> 2) + 1);
     if (((it + G::AHEAD) * KG + kg + 1) * 128 > p.k) {
 #pragma unroll
       for (int z = 0; z < PPS; ++z) past_end(it + G::ahead(z), G::next(z));
@@ -360,7 +370,10 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
       constexpr bool last = i + 1 == FN;
       if constexpr (G::meets(i)) {
         constexpr int in_flight = G::in_flight(i);
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(in_flight) : "memory");
+        if (G::TRIM && it + G::AHEAD >= nit)  // fewer in flight
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(in_flight) : "memory");
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -390,7 +403,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
         for (int n = G::issued(i * FM); n < G::issued((i + 1) * FM); ++n) {
           const int z = G::panel(n), y = G::next(z);
-          dma(it + G::ahead(z), G::first(y) + n - G::first(z), slot(ph, z));
+          if (!G::TRIM || it + G::ahead(z) < nit) dma(it + G::ahead(z), G::first(y) + n - G::first(z), slot(ph, z));
         }
 #pragma unroll
         for (int j = 0; j < FM; ++j)
@@ -401,8 +414,9 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
       for (int j = 0; j < FM; ++j) {
         const int v = i * FM + j;
-        f8_mma0(part[v & 1], fw[i & 1][0], fa[j][0]);
-        if constexpr (!G::SPLIT) f8_mma1(part[v & 1], fw[i & 1][1], fa[j][1]);
+        constexpr int odd = TILES % 2 ? ph & 1 : 0, w = (i + odd) & 1;
+        f8_mma0(part[(v + odd) & 1], fw[w][0], fa[j][0]);
+        if constexpr (!G::SPLIT) f8_mma1(part[(v + odd) & 1], fw[w][1], fa[j][1]);
         __builtin_amdgcn_sched_barrier(0);
         if (last) {
           if (j == 0) {
@@ -420,23 +434,23 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (j == min(h, FM - 1))
-            fw[(i + 1) & 1][h] = frag(fw0, last ? slot(ph + 1, FM) : slot(ph, FM + i + 1), h);
+            fw[w ^ 1][h] = frag(fw0, last ? slot(ph + 1, FM) : slot(ph, FM + i + 1), h);
 #pragma unroll
         for (int d = G::issued(v); d < G::issued(v + 1); ++d) {
           const int z = G::panel(d), y = G::next(z);
-          dma(it + G::ahead(z), G::first(y) + d - G::first(z), slot(ph, z));
+          if (!G::TRIM || it + G::ahead(z) < nit) dma(it + G::ahead(z), G::first(y) + d - G::first(z), slot(ph, z));
         }
         if constexpr (G::SPLIT) {
           __builtin_amdgcn_sched_barrier(0);
-          f8_mma1(part[v & 1], fw[i & 1][1], fa[j][1]);
+          f8_mma1(part[(v + odd) & 1], fw[w][1], fa[j][1]);
           if (last && j + 1 == FM) fa[j][1] = frag(fa0, slot(ph + 1, j), 1);
         }
-        join(v - 1, v == 0 ? s_last : s[(v - 1 + FM) % FM]);
+        join(v - 1, odd, v == 0 ? s_last : s[(v - 1 + FM) % FM]);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
     tile(IntC<0>{});
-    tile(IntC<1>{});
+    if constexpr (FN > 1) tile(IntC<1>{});
     if constexpr (FN > 2) {
       tile(IntC<2>{});
       tile(IntC<3>{});
@@ -464,52 +478,16 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     }
   }
   if constexpr (!G::EXACT) {
-    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[1]));
-    join(-1, s_last);
+    if (TILES % 2 && (nit & 1)) {
+      asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[0]));
+      join(-1, 1, s_last);
+    } else {
+      asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[1]));
+      join(-1, 0, s_last);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-}
-
-// Adds the K groups' sums in group order into group 0's accumulators, through
-// LDS.  True for the waves that hold the result.
-template <typename G>
-__device__ __forceinline__ bool f8_join_groups(char* smem, f32x16 (&acc)[G::FN][G::FM]) {
-  if constexpr (G::KG > 1) {
-    const int gw = threadIdx.x >> 6, kg = gw / G::NW, lane = threadIdx.x & 63;
-    constexpr int QUADS = G::FM * G::FN * 4;  // of a lane
-    float4* const base = reinterpret_cast<float4*>(smem) + (gw % G::NW) * QUADS * 64 + lane;
-    constexpr int STEP = G::NW * QUADS * 64;
-    if (kg > 0) {
-#pragma unroll
-      for (int i = 0; i < G::FN; ++i)
-#pragma unroll
-        for (int j = 0; j < G::FM; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            base[(kg - 1) * STEP + ((i * G::FM + j) * 4 + q) * 64] =
-                make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-    }
-    __syncthreads();
-    if (kg == 0) {
-#pragma unroll
-      for (int o = 0; o < G::KG - 1; ++o)
-#pragma unroll
-        for (int i = 0; i < G::FN; ++i)
-#pragma unroll
-          for (int j = 0; j < G::FM; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float4 v = base[o * STEP + ((i * G::FM + j) * 4 + q) * 64];
-              acc[i][j][4 * q] += v.x; acc[i][j][4 * q + 1] += v.y;
-              acc[i][j][4 * q + 2] += v.z; acc[i][j][4 * q + 3] += v.w;
-            }
-    }
-    __syncthreads();
-    return kg == 0;
-  } else {
-    return true;
-  }
 }
 
 // Two values rounded to nearest even in a 2-byte type, one word.
@@ -568,6 +546,73 @@ __device__ __forceinline__ void f8_values(const char* smem, f32x16 (&acc)[G::FN]
           acc[i][j][4 * g + r] = GELU ? gelu_erf(v) : v;
         }
     }
+}
+
+// Epilogue of K groups: their sums go to LDS in rows, and every thread takes
+// pieces of 8 columns, adds the groups' in group order, and stores the result.
+// 16 lanes hold an e4m3 block.  128 x 2048 x 512 with GELU in 32 x 64 tiles: 4.3 us,
+// against 5.5 with the join and the epilogue by group 0's wave alone.
+template <typename T, bool GELU, bool F8, typename G>
+__device__ __forceinline__ void f8_join(const F8GemmArgs& p, char* smem, const f32x16 (&acc)[G::FN][G::FM], int m0, int n0) {
+  const int tid = threadIdx.x, lane = tid & 63, gw = tid >> 6;
+  const int kg = gw / G::NW, wm = gw % G::NW / G::WN, wn = gw % G::WN;
+  float* const parts = reinterpret_cast<float*>(smem);
+  {
+    float* const to = parts + (kg * G::BM + wm * G::WTM + (lane & 31)) * G::PITCH + wn * G::WTN + 4 * (lane >> 5);
+#pragma unroll
+    for (int i = 0; i < G::FN; ++i)
+#pragma unroll
+      for (int j = 0; j < G::FM; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(to + 32 * j * G::PITCH + 32 * i + 8 * g) =
+              make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+  }
+  __syncthreads();
+  constexpr int ES = F8 ? 1 : 2, PPR = G::BN / 8, NIT = (G::BM * PPR + G::THREADS - 1) / G::THREADS;
+  static_assert(G::BM * PPR % 64 == 0 && (!F8 || PPR == 16), "whole waves of pieces");
+  const int rows = min(G::BM, p.m - m0), cols = min(G::BN, p.n - n0);
+  const F8Rows out{wave_rsrc(static_cast<char*>(p.c) + ((int64_t)m0 * p.ldc + n0) * ES, ((int64_t)(rows - 1) * p.ldc + cols) * ES),
+                   (uint32_t)(p.ldc * ES), cols};
+  const bool whole = (((uintptr_t)p.c & (8 * ES - 1)) | (p.ldc & 7) | (p.n & 7)) == 0;
+#pragma unroll
+  for (int it = 0; it < NIT; ++it) {
+    const int pc = tid + it * G::THREADS, row = pc / PPR, col = pc % PPR * 8;
+    if (pc >= G::BM * PPR) break;
+    float v[8], o[8];
+    Oct<float>::to(Oct<float>::load(parts + row * G::PITCH + col), v);
+#pragma unroll
+    for (int g = 1; g < G::KG; ++g) {
+      Oct<float>::to(Oct<float>::load(parts + (g * G::BM + row) * G::PITCH + col), o);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] += o[r];
+    }
+    Oct<T>::to(Oct<T>::load(reinterpret_cast<const T*>(smem + G::BIAS) + col), o);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) v[r] = GELU ? gelu_erf(v[r] + o[r]) : v[r] + o[r];
+    if constexpr (F8) {
+      float top = 0.f;  // N is a multiple of 4
+#pragma unroll
+      for (int r = 0; r < 8; ++r) top = fmaxf(top, col + (r & 4) < cols ? fabsf(v[r]) : 0.f);
+      const float s = f8_scale(row16_max(top)), inv = __builtin_amdgcn_rcpf(s);
+      const uint32_t x = f8_pack4(v[0], v[1], v[2], v[3], inv), y = f8_pack4(v[4], v[5], v[6], v[7], inv);
+      if (col == 0 && row < rows) p.cs[(int64_t)(m0 + row) * p.ld_cs + n0 / 128] = s;
+      if (whole) {
+        out.put8(row, col, 1, x, y);
+      } else {
+        out.put4(row, col, 1, x);
+        out.put4(row, col + 4, 1, y);
+      }
+    } else {
+      const uint4 q = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      if (whole) {
+        out.put16<0>(row, col, 2, q);
+      } else {
+        out.put8(row, col, 2, q.x, q.y);
+        out.put8(row, col + 4, 2, q.z, q.w);
+      }
+    }
+  }
 }
 
 // Outputs in a 2-byte type T.  Lane (l32, hi) holds columns 32 i + 8 g + 4 hi
@@ -629,7 +674,7 @@ __device__ __forceinline__ void f8_store(const F8GemmArgs& p, const f32x16 (&acc
 // the 16-byte piece c of row r at c ^ x(r).
 template <typename G>
 __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&acc)[G::FN][G::FM], int mw, int nw,
-                                            int wm, int wn, int lane, bool holds, float* red, char* stage) {
+                                            int wm, int wn, int lane, float* red, char* stage) {
   constexpr int FM = G::FM, FN = G::FN, WPB = 128 / G::WTN;
   const int l32 = lane & 31, hi = lane >> 5;
   float top[FM];
@@ -648,7 +693,7 @@ __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&
     top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
   }
   if constexpr (WPB > 1) {
-    if (holds && hi == 0) {
+    if (hi == 0) {
 #pragma unroll
       for (int j = 0; j < FM; ++j) red[wn * G::BM + wm * G::WTM + 32 * j + l32] = top[j];
     }
@@ -659,7 +704,6 @@ __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&
       for (int o = 0; o < WPB; ++o)
         top[j] = fmaxf(top[j], red[(wn / WPB * WPB + o) * G::BM + wm * G::WTM + 32 * j + l32]);
   }
-  if (!holds) return;
   constexpr int LPR = 2 * FN;  // pieces per row: 8 or 4
   static_assert(LPR == 8 || LPR == 4, "staged rows of 128 or 64 bytes");
   auto x = [](int r) { return LPR == 8 ? r & 7 : (r >> 1) & 3; };
@@ -749,22 +793,24 @@ __global__ __launch_bounds__(G::THREADS, G::THREADS <= 256 && G::LDS > 80 * 1024
   f32x16 acc[G::FN][G::FM];
   zero_acc<float, G::FM, G::FN>(acc);
   f8_accumulate<G>(smem, p, m0, n0, acc);
-  const bool holds = f8_join_groups<G>(smem, acc);
+  if constexpr (G::KG > 1) {
+    f8_join<T, GELU, F8, G>(p, smem, acc, m0, n0);
+    return;
+  }
   // (an empty asm: nothing derived from the lane stays in a register through the main loop)
   int lane = threadIdx.x;
   asm volatile("" : "+v"(lane));
   lane &= 63;
   const int wm = wave / G::WN, wn = wave % G::WN;
   const int mw = m0 + wm * G::WTM, nw = n0 + wn * G::WTN;
-  if (holds) f8_values<T, GELU, G>(smem, acc, wn, lane >> 5);
+  f8_values<T, GELU, G>(smem, acc, wn, lane >> 5);
   if constexpr (F8) {
     constexpr int RED = G::BM * G::WN * 4;
     static_assert(RED + G::BM * G::BN <= G::BIAS, "epilogue staging");
-    f8_quantise<G>(p, acc, mw, nw, wm, wn, lane, holds, reinterpret_cast<float*>(smem),
-                   smem + RED + wave * 1024 * G::FM * G::FN);
+    f8_quantise<G>(p, acc, mw, nw, wm, wn, lane, reinterpret_cast<float*>(smem), smem + RED + wave * 1024 * G::FM * G::FN);
   } else {
     static_assert(64 * G::WTN * G::NW <= G::BIAS, "epilogue staging");
-    if (holds) f8_store<T, G>(p, acc, mw, nw, lane, smem + wave * 64 * G::WTN);
+    f8_store<T, G>(p, acc, mw, nw, lane, smem + wave * 64 * G::WTN);
   }
 }
 

@@ -12,8 +12,9 @@ typedef F8Geom<3, 2, 2, 2, 1, 6, 4> Tile192x128;
 typedef F8Geom<2, 2, 2, 2, 1, 4, 4> Tile128;
 typedef F8Geom<1, 2, 2, 2, 1, 3, 6> Tile64x128;
 typedef F8Geom<1, 2, 2, 2, 2, 3, 6> Tile64x128k2;
-typedef F8Geom<1, 2, 1, 2, 4, 3, 3> Tile32x128k4;
 typedef F8Geom<1, 2, 1, 1, 4, 2, 4> Tile32x64k4;
+typedef F8Geom<1, 1, 1, 1, 4, 2, 2> Tile32k4;
+typedef F8Geom<1, 1, 1, 1, 8, 2, 2> Tile32k8;
 // of e4m3 outputs
 typedef F8Geom<2, 2, 2, 4, 1, 4, 4, -1, true> Exact128x256;
 typedef F8Geom<2, 2, 2, 2, 1, 4, 4, -1, true> Exact128;
@@ -38,30 +39,30 @@ static int run_tile(const F8GemmArgs& p, hipStream_t s) {
 // towards tiles near the best of their launch, over the 336 launches of
 // profiles/gemm_f8_tiles.csv (1 to 16384 rows, widths and K from 64 and 128 to
 // 8192), for e4m3 outputs over the 262 of profiles/gemm_f8_e4m3_tiles.csv.  The
-// tile with the least estimate is 0.3% slower than the best of its list (geometric
-// mean), three launches of either list more than 10% (at most 21%, one round of
-// 256 x 256 tiles taken for two of 128 x 128).  Without one of the tiles the best
-// would be slower by 0.1 to 1.3%, without 32 x 64 by 9%; of the e4m3 list
-// by 0.1 to 2.9%, without 32 x 128 by 9%.
+// tile with the least estimate is 0.2% (e4m3: 0.3%) slower than the best of its
+// list (geometric mean), none of the first list more than 10%, two of the second
+// (at most 28%, 7206 x 576 x 8128).  Without one of the tiles the best would be
+// slower by 0.1 to 2.4%; of the e4m3 list by 0.2 to 1.7%, without 32 x 128 by 14%.
 struct F8Plan {
   int bm, bn, per_cu, k_groups;
   float c[7];
 };
 static const F8Plan kPlans[] = {
-    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {1.102f, 0.000f, 1.404f, 4.009f, 0.000f, 0.635f, 5.457f}},
-    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.642f, 3.257f, 0.196f, 0.000f, 0.745f, 0.450f, 2.988f}},
-    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {1.056f, 3.417f, 0.000f, 0.000f, 0.680f, 0.396f, 2.268f}},
-    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {2.189f, 2.054f, 0.005f, 0.000f, 0.456f, 0.419f, 1.355f}},
-    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {2.775f, 1.372f, 0.087f, 0.000f, 0.271f, 0.631f, 0.480f}},
-    {Tile64x128k2::BM, Tile64x128k2::BN, 1, Tile64x128k2::KG, {1.446f, 3.147f, 0.496f, 0.000f, 0.000f, 1.552f, 0.789f}},
-    {Tile32x128k4::BM, Tile32x128k4::BN, 1, Tile32x128k4::KG, {1.568f, 3.561f, 0.758f, 0.000f, 0.000f, 2.400f, 0.742f}},
-    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.278f, 0.000f, 0.000f, 3.222f, 0.483f, 2.045f, 0.737f}}};
+    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {0.576f, 4.117f, 1.458f, 0.000f, 0.000f, 0.599f, 5.392f}},
+    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.090f, 3.263f, 0.219f, 0.000f, 0.752f, 0.426f, 2.788f}},
+    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {0.558f, 3.352f, 0.702f, 0.000f, 0.000f, 0.366f, 2.266f}},
+    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {1.682f, 1.884f, 0.044f, 0.000f, 0.455f, 0.461f, 1.384f}},
+    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {2.201f, 1.001f, 0.176f, 0.000f, 0.225f, 0.876f, 0.664f}},
+    {Tile64x128k2::BM, Tile64x128k2::BN, 1, Tile64x128k2::KG, {1.058f, 2.724f, 0.543f, 0.000f, 0.000f, 1.509f, 0.718f}},
+    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.071f, 1.934f, 0.575f, 0.000f, 0.000f, 1.663f, 0.219f}},
+    {Tile32k4::BM, Tile32k4::BN, 2, Tile32k4::KG, {1.761f, 1.161f, 0.184f, 0.000f, 0.260f, 2.475f, 0.192f}},
+    {Tile32k8::BM, Tile32k8::BN, 1, Tile32k8::KG, {1.044f, 2.321f, 0.671f, 0.000f, 0.000f, 3.387f, 0.192f}}};
 static const F8Plan kPlansF8[] = {
-    {Exact128x256::BM, Exact128x256::BN, 1, Exact128x256::KG, {1.332f, 3.368f, 1.632f, 0.000f, 0.000f, 1.352f, 2.407f}},
-    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.899f, 0.506f, 0.145f, 0.000f, 0.811f, 1.250f, 1.468f}},
-    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.603f, 0.401f, 0.288f, 0.183f, 0.391f, 1.734f, 0.653f}},
-    {Exact64x128k2::BM, Exact64x128k2::BN, 1, Exact64x128k2::KG, {1.163f, 0.000f, 0.942f, 3.782f, 0.000f, 2.293f, 0.699f}},
-    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {0.613f, 0.000f, 1.025f, 4.843f, 0.000f, 4.092f, 0.777f}}};
+    {Exact128x256::BM, Exact128x256::BN, 1, Exact128x256::KG, {0.562f, 3.399f, 0.000f, 0.000f, 1.667f, 1.261f, 2.696f}},
+    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.144f, 0.738f, 0.171f, 0.000f, 0.807f, 1.112f, 1.510f}},
+    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.053f, 0.225f, 0.320f, 0.269f, 0.378f, 1.438f, 0.734f}},
+    {Exact64x128k2::BM, Exact64x128k2::BN, 1, Exact64x128k2::KG, {0.883f, 0.000f, 0.960f, 3.401f, 0.000f, 1.939f, 0.672f}},
+    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {0.664f, 3.664f, 0.000f, 0.000f, 1.035f, 4.012f, 0.265f}}};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]), kPlanCountF8 = sizeof(kPlansF8) / sizeof(kPlansF8[0]);
 
 // The tile with the least estimate.
@@ -94,8 +95,9 @@ static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
     case 3: return run_tile<T, GELU, false, Tile128>(p, s);
     case 4: return run_tile<T, GELU, false, Tile64x128>(p, s);
     case 5: return run_tile<T, GELU, false, Tile64x128k2>(p, s);
-    case 6: return run_tile<T, GELU, false, Tile32x128k4>(p, s);
-    default: return run_tile<T, GELU, false, Tile32x64k4>(p, s);
+    case 6: return run_tile<T, GELU, false, Tile32x64k4>(p, s);
+    case 7: return run_tile<T, GELU, false, Tile32k4>(p, s);
+    default: return run_tile<T, GELU, false, Tile32k8>(p, s);
   }
 }
 

@@ -316,7 +316,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
   else
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::in_flight(FN - 1) + G::issued(G::TILES) - G::issued((FN - 1) * FM))
                  : "memory");
-  asm volatile("s_barrier" ::: "memory");
+  if constexpr (NW > 1) asm volatile("s_barrier" ::: "memory");
 
   i32x8 fa[FM][2], fw[2][2];
   f32x16 part[2];
@@ -374,7 +374,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         else
           asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(in_flight) : "memory");
-        asm volatile("s_barrier" ::: "memory");
+        if constexpr (NW > 1) asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (G::EXACT) {

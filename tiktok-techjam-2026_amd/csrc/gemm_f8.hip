@@ -11,10 +11,9 @@ typedef F8Geom<2, 4, 2, 2, 1, 3, 6> Tile128x256;
 typedef F8Geom<3, 2, 2, 2, 1, 6, 4> Tile192x128;
 typedef F8Geom<2, 2, 2, 2, 1, 4, 4> Tile128;
 typedef F8Geom<1, 2, 2, 2, 1, 3, 6> Tile64x128;
-typedef F8Geom<1, 2, 2, 2, 2, 3, 6> Tile64x128k2;
 typedef F8Geom<1, 2, 1, 1, 4, 2, 4> Tile32x64k4;
 typedef F8Geom<1, 1, 1, 1, 4, 2, 2> Tile32k4;
-typedef F8Geom<1, 1, 1, 1, 8, 2, 2> Tile32k8;
+typedef F8Geom<1, 1, 1, 1, 4, 4, 4> Tile32k4d;
 // of e4m3 outputs
 typedef F8Geom<2, 2, 2, 4, 1, 4, 4, -1, true> Exact128x256;
 typedef F8Geom<2, 2, 2, 2, 1, 4, 4, -1, true> Exact128;
@@ -38,31 +37,31 @@ static int run_tile(const F8GemmArgs& p, hipStream_t s) {
 // (mb at 5 TB/s).  Non-negative least squares, by relative error and weighted
 // towards tiles near the best of their launch, over the 336 launches of
 // profiles/gemm_f8_tiles.csv (1 to 16384 rows, widths and K from 64 and 128 to
-// 8192), for e4m3 outputs over the 262 of profiles/gemm_f8_e4m3_tiles.csv.  The
-// tile with the least estimate is 0.2% (e4m3: 0.3%) slower than the best of its
-// list (geometric mean), none of the first list more than 10%, two of the second
-// (at most 28%, 7206 x 576 x 8128).  Without one of the tiles the best would be
-// slower by 0.1 to 2.4%; of the e4m3 list by 0.2 to 1.7%, without 32 x 128 by 14%.
+// 8192, weights from memory), for e4m3 outputs over the 262 of
+// profiles/gemm_f8_e4m3_tiles.csv.  The tile with the least estimate is 0.4% slower
+// than the best of its list (e4m3: 0.3%, geometric means), none of the first list
+// more than 10%, one of the second (12%).  Without one of the tiles
+// the best would be slower by 0.2 to 1.9%; of the e4m3 list by 0.1 to 1.7%, without
+// 32 x 128 by 10%.
 struct F8Plan {
   int bm, bn, per_cu, k_groups;
   float c[7];
 };
 static const F8Plan kPlans[] = {
-    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {0.576f, 4.117f, 1.458f, 0.000f, 0.000f, 0.599f, 5.392f}},
-    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.090f, 3.263f, 0.219f, 0.000f, 0.752f, 0.426f, 2.788f}},
-    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {0.558f, 3.352f, 0.702f, 0.000f, 0.000f, 0.366f, 2.266f}},
-    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {1.682f, 1.884f, 0.044f, 0.000f, 0.455f, 0.461f, 1.384f}},
-    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {2.201f, 1.001f, 0.176f, 0.000f, 0.225f, 0.876f, 0.664f}},
-    {Tile64x128k2::BM, Tile64x128k2::BN, 1, Tile64x128k2::KG, {1.058f, 2.724f, 0.543f, 0.000f, 0.000f, 1.509f, 0.718f}},
-    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.071f, 1.934f, 0.575f, 0.000f, 0.000f, 1.663f, 0.219f}},
-    {Tile32k4::BM, Tile32k4::BN, 2, Tile32k4::KG, {1.761f, 1.161f, 0.184f, 0.000f, 0.260f, 2.475f, 0.192f}},
-    {Tile32k8::BM, Tile32k8::BN, 1, Tile32k8::KG, {1.044f, 2.321f, 0.671f, 0.000f, 0.000f, 3.387f, 0.192f}}};
+    {Tile256::BM, Tile256::BN, 1, Tile256::KG, {1.408f, 3.649f, 1.439f, 0.000f, 0.000f, 0.686f, 5.396f}},
+    {Tile128x256::BM, Tile128x256::BN, 2, Tile128x256::KG, {1.817f, 2.973f, 0.243f, 0.000f, 0.732f, 0.440f, 2.809f}},
+    {Tile192x128::BM, Tile192x128::BN, 1, Tile192x128::KG, {1.171f, 3.204f, 0.000f, 0.000f, 0.739f, 0.328f, 2.255f}},
+    {Tile128::BM, Tile128::BN, 2, Tile128::KG, {2.333f, 1.434f, 0.168f, 0.000f, 0.389f, 0.551f, 1.409f}},
+    {Tile64x128::BM, Tile64x128::BN, 2, Tile64x128::KG, {3.106f, 0.299f, 0.211f, 0.000f, 0.224f, 1.179f, 0.696f}},
+    {Tile32x64k4::BM, Tile32x64k4::BN, 1, Tile32x64k4::KG, {1.627f, 1.496f, 0.658f, 0.000f, 0.000f, 3.162f, 0.274f}},
+    {Tile32k4::BM, Tile32k4::BN, 2, Tile32k4::KG, {2.111f, 0.736f, 0.476f, 0.000f, 0.158f, 4.547f, 0.232f}},
+    {Tile32k4d::BM, Tile32k4d::BN, 1, Tile32k4d::KG, {1.935f, 0.000f, 0.513f, 1.199f, 0.000f, 5.940f, 0.253f}}};
 static const F8Plan kPlansF8[] = {
-    {Exact128x256::BM, Exact128x256::BN, 1, Exact128x256::KG, {0.562f, 3.399f, 0.000f, 0.000f, 1.667f, 1.261f, 2.696f}},
-    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.144f, 0.738f, 0.171f, 0.000f, 0.807f, 1.112f, 1.510f}},
-    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.053f, 0.225f, 0.320f, 0.269f, 0.378f, 1.438f, 0.734f}},
-    {Exact64x128k2::BM, Exact64x128k2::BN, 1, Exact64x128k2::KG, {0.883f, 0.000f, 0.960f, 3.401f, 0.000f, 1.939f, 0.672f}},
-    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {0.664f, 3.664f, 0.000f, 0.000f, 1.035f, 4.012f, 0.265f}}};
+    {Exact128x256::BM, Exact128x256::BN, 1, Exact128x256::KG, {1.592f, 3.007f, 1.662f, 0.000f, 0.000f, 1.534f, 2.579f}},
+    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.912f, 0.210f, 0.323f, 0.000f, 0.719f, 1.525f, 1.421f}},
+    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.790f, 0.000f, 0.398f, 0.016f, 0.331f, 2.658f, 0.657f}},
+    {Exact64x128k2::BM, Exact64x128k2::BN, 1, Exact64x128k2::KG, {2.089f, 2.557f, 1.004f, 0.000f, 0.000f, 3.057f, 0.571f}},
+    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {2.520f, 0.000f, 1.375f, 1.839f, 0.000f, 5.725f, 0.182f}}};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]), kPlanCountF8 = sizeof(kPlansF8) / sizeof(kPlansF8[0]);
 
 // The tile with the least estimate.
@@ -94,10 +93,9 @@ static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
     case 2: return run_tile<T, GELU, false, Tile192x128>(p, s);
     case 3: return run_tile<T, GELU, false, Tile128>(p, s);
     case 4: return run_tile<T, GELU, false, Tile64x128>(p, s);
-    case 5: return run_tile<T, GELU, false, Tile64x128k2>(p, s);
-    case 6: return run_tile<T, GELU, false, Tile32x64k4>(p, s);
-    case 7: return run_tile<T, GELU, false, Tile32k4>(p, s);
-    default: return run_tile<T, GELU, false, Tile32k8>(p, s);
+    case 5: return run_tile<T, GELU, false, Tile32x64k4>(p, s);
+    case 6: return run_tile<T, GELU, false, Tile32k4>(p, s);
+    default: return run_tile<T, GELU, false, Tile32k4d>(p, s);
   }
 }
 

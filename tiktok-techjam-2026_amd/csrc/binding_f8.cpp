@@ -57,7 +57,7 @@ int dtype_code(const at::Tensor& t, const char* name) {
   }
 }
 
-// A 2-D row-major view.  (A dimension of one element may have any stride.)
+// A 2-D row-major view.  (A single row, and an empty one, may have any stride.)
 struct Matrix {
   int64_t rows, cols, ld;
   int dtype;
@@ -67,7 +67,7 @@ struct Matrix {
 Matrix matrix(const at::Tensor& t, const char* name) {
   if (t.dim() != 2 || (t.stride(1) != 1 && t.size(1) != 1))
     refuse("%s must be a 2-D row-major view", name);
-  return {t.size(0), t.size(1), t.size(0) > 1 ? t.stride(0) : t.size(1), dtype_code(t, name), t.data_ptr()};
+  return {t.size(0), t.size(1), t.size(0) > 1 && t.size(1) > 0 ? t.stride(0) : t.size(1), dtype_code(t, name), t.data_ptr()};
 }
 
 // The fp32 scales of a quantised matrix: at least rows x ceil(cols / 128).

@@ -395,7 +395,7 @@ int tjk_quantize_f8(const void* x, int x_dtype, int64_t ld_x, void* q, int64_t l
  * tjk_add_layernorm add a 2-byte output to an fp32 residual.
  * Requires k % 16 == 0, n % 4 == 0, lda and ldw multiples of 16 (below 2^23),
  * ldc of 4, 16-byte aligned a and w, and bias and c aligned to 4 elements.
- * plan_id: -1 chooses, else one of tjk_gemm_f8_plan_count() tiles (0 to 4 for an
+ * plan_id: -1 chooses, else one of tjk_gemm_f8_plan_count() tiles (0 to 2 for an
  * e4m3 output).  Tiles that split K over groups of
  * waves add up in another order, always the same.
  */

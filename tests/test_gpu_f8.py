@@ -289,7 +289,7 @@ SHAPES = [(1, 4, 16), (1, 128, 128), (8, 2048, 512), (15, 12, 112), (16, 132, 14
 
 
 PLANS = list(range(-1, 8))  # every tile, and the rule's choice
-PLANS_F8 = list(range(-1, 5))
+PLANS_F8 = list(range(-1, 3))
 
 
 @pytest.fixture(scope="module")

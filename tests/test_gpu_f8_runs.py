@@ -167,7 +167,7 @@ def test_no_depth(device, plan):
     assert torch.equal(out.cpu(), bias.bfloat16().expand(m, n))
     ops.gemm_f8(a, a_s, w, w_s, None, out, plan=plan)
     assert (out == 0).all()
-    if plan < 5:
+    if plan < 3:
         q, s = torch.empty(m, n, dtype=F8, device=device), torch.empty(m, 2, device=device)
         ops.gemm_f8(a, a_s, w, w_s, bias.to(device), q, out_scales=s, plan=plan)
         y = bias.double().expand(m, n)
@@ -204,7 +204,7 @@ def test_nan_stays_in_its_row_and_column(device, plan):
     assert torch.isnan(got[33]).all() and torch.isnan(got[5]).all() and torch.isnan(got[:, 101]).all()
     got[33], got[5], got[:, 101] = want[33], want[5], want[:, 101]
     assert torch.equal(want, got)
-    if plan < 5:
+    if plan < 3:
         outs = []
         for s in (args, bad):
             q, s_out = torch.empty(m, n, dtype=F8, device=device), torch.empty(m, 2, device=device)

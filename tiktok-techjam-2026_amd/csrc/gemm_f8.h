@@ -56,19 +56,19 @@ __device__ __forceinline__ void f8_mma1(f32x16& d, const i32x8& w, const i32x8& 
 
 // A fragment half (32 e4m3 values of one row per lane) in fp16, which holds
 // every e4m3 value exactly (NaN stays NaN): four operands of a 32x32x16 MFMA.
-__device__ __forceinline__ void f8_widen(const i32x8& f, f16x8 (&w)[4]) {
+__device__ __forceinline__ f16x8 f8_widen(const i32x8& f, int q) {
   typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  f16x8 w;
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-#pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * q + d], 1.0f, false);
-      const f16x2 up = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * q + d], 1.0f, true);
-      w[q][4 * d] = lo[0];
-      w[q][4 * d + 1] = lo[1];
-      w[q][4 * d + 2] = up[0];
-      w[q][4 * d + 3] = up[1];
-    }
+  for (int d = 0; d < 2; ++d) {
+    const f16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * q + d], 1.0f, false);
+    const f16x2 up = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * q + d], 1.0f, true);
+    w[4 * d] = lo[0];
+    w[4 * d + 1] = lo[1];
+    w[4 * d + 2] = up[0];
+    w[4 * d + 3] = up[1];
+  }
+  return w;
 }
 
 // Chunk of a 128-byte tile row: the 16-byte chunk c of row r lies at
@@ -173,6 +173,7 @@ struct F8Geom {
   }
   static_assert(DPA * WN == 4 && DPW * WM == 4, "panels must split over the waves");
   static_assert(FN % 2 == 0 || (FM == 1 && FN == 1 && PHASES % 2 == 0), "fragment double buffer, ring of two products");
+  static_assert(!EXACT || (FN == 2 && FM <= 2), "two W tiles, two A fragments");
   static_assert(128 % WTN == 0, "a wave's columns lie in one block");
   static_assert(DS * WN == 2 * FM, "scales must split over the waves");
   static_assert(RA >= FM && RW >= FN && PHASES <= 4, "rings of whole K tiles at least");
@@ -210,12 +211,15 @@ struct F8Geom {
 // EXACT.  The e4m3 MFMAs drop low bits of products (1.0e-5 of an output's scale
 // was lost, against 1e-7 here); an e4m3 output's scales are fp32 results, so
 // its sums are formed of fragments widened to fp16 in registers, 8 products of 32
-// cycles in place of 2 of 64, with the same panels, rings and meetings.  A is
-// widened once per K tile, W once per wave column: with 192 conversions and FMAs
-// per 32 products of 32 cycles the vector unit is as busy as the matrix unit, and
-// wider wave tiles have no registers left.  5430 x 4096 x 1024 with GELU: 57 us (36
-// with the e4m3 MFMAs); 4096^3: 122 us, 1.12 PFLOP/s.  Spreading the conversions
-// between the MFMAs by hand cost 38 registers more and time (125 us).
+// cycles in place of 2 of 64, with the same panels, rings and meetings.  Behind each
+// MFMA stand two FMAs of the product before and four or eight conversions, each
+// into the registers of an operand that was used for the last time: W's next tile
+// behind its last row block, A's next K tile behind its last W tile and, the second
+// fragment, behind the next K tile's first product (its registers are free then).
+// 2048 x 1024 x 4096, one wave per SIMD: 30.5 us, against 35.0 with the conversions
+// in one piece.  5430 x 4096 x 1024 with GELU, two waves: 57 us either way (36 with
+// the e4m3 MFMAs), and 4096^3 119 us, 1.15 PFLOP/s: there the clock falls with the
+// power that fp16 products take (a bf16 library product of 8192^3 reaches 1.38).
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x16 (&acc)[G::FN][G::FM]) {
@@ -346,15 +350,14 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     for (int r = 0; r < 16; ++r) c[r] = fmaf(d[r], f, c[r]);
   };
 
-  f16x8 ah[G::EXACT ? FM : 1][2][4];
-  auto widen_a = [&]() __attribute__((always_inline)) {
-    if constexpr (G::EXACT)
+  f16x8 ah[G::EXACT ? FM : 1][8], wh[8];
+  if constexpr (G::EXACT) {
 #pragma unroll
-      for (int j = 0; j < FM; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) f8_widen(fa[j][h], ah[j][h]);
-  };
-  widen_a();
+    for (int q = 0; q < 8; ++q) {
+      ah[0][q] = f8_widen(fa[0][q >> 2], q & 3);
+      wh[q] = f8_widen(fw[0][q >> 2], q & 3);
+    }
+  }
 
   // One K tile, PH = it mod PHASES.
   auto step = [&](auto PH, int it) __attribute__((always_inline)) {
@@ -378,37 +381,72 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
         __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (G::EXACT) {
-        f32x16 d[FM];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          f16x8 wh[4];
-          f8_widen(fw[0][h], wh);
+        auto raw_w_half = [&](int h) __attribute__((always_inline)) {
           fw[0][h] = frag(fw0, last ? slot(ph + 1, FM) : slot(ph, FM + i + 1), h);
-          if (last) {
+        };
+        auto widen_w = [&](int q) __attribute__((always_inline)) {
+          wh[q] = f8_widen(fw[0][q >> 2], q & 3);
+          asm volatile("" : "+v"(wh[q]));
+        };
+        auto widen_a = [&](int j, int q) __attribute__((always_inline)) {
+          ah[j][q] = f8_widen(fa[j][q >> 2], q & 3);
+          asm volatile("" : "+v"(ah[j][q]));
+        };
 #pragma unroll
-            for (int j = 0; j < FM; ++j) fa[j][h] = frag(fa0, slot(ph + 1, j), h);
+        for (int j = 0; j < FM; ++j) {
+          const int v = i * FM + j;
+          f32x16& d = part[v & 1];
+          const f32x16& e = part[~v & 1];
+          f32x16& c = acc[(v - 1 + TILES) % TILES / FM][(v - 1 + TILES) % FM];
+          const float f = v == 0 ? s_last : s[(v - 1 + FM) % FM];
+          if (j == 0) {
+            raw_w_half(0);
+            raw_w_half(1);
           }
+          if (last && j == 0) {
+            fa[0][0] = frag(fa0, slot(ph + 1, 0), 0);
+            fa[0][1] = frag(fa0, slot(ph + 1, 0), 1);
+            const int o = (it + 1) & 7;
 #pragma unroll
-          for (int j = 0; j < FM; ++j)
+            for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
+            raw_w = tabw[(o >> 2) * 64 + (o & 3)];
+          }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              d[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(wh[q], ah[j][h][q], h + q == 0 ? f32x16{} : d[j], 0, 0, 0);
+          for (int q = 0; q < 8; ++q) {
+            d = __builtin_amdgcn_mfma_f32_32x32x16_f16(wh[q], ah[j][q], q ? d : f32x16{}, 0, 0, 0);
+            if (q == 1 || q == 5) {  // half of the product's DMA instructions each
+              const int n0 = G::issued(v), n1 = G::issued(v + 1), mid = (n0 + n1 + 1) / 2;
+#pragma unroll
+              for (int n = q == 1 ? n0 : mid; n < (q == 1 ? mid : n1); ++n) {
+                const int z = G::panel(n), y = G::next(z);
+                dma(it + G::ahead(z), G::first(y) + n - G::first(z), slot(ph, z));
+              }
+            }
+            if (q > 0)  // not at once behind the product that they read
+#pragma unroll
+              for (int r = (q - 1) * 16 / 7; r < q * 16 / 7; ++r) c[r] = fmaf(e[r], f, c[r]);
+            if constexpr (FM == 2) {
+              if (v == 0) widen_a(1, q);
+              if (j == 1) widen_w(q);
+              if (last && j == 0 && q >= 4) widen_a(0, q - 4);
+              if (last && j == 1 && q < 4) widen_a(0, q + 4);
+              if (last && j == 1 && (q == 4 || q == 7)) fa[1][q == 7] = frag(fa0, slot(ph + 1, 1), q == 7);
+            } else if (q >= 4) {
+              widen_w(q - 4);
+              if (last) widen_a(0, q - 4);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if constexpr (FM == 1) {
+#pragma unroll
+            for (int q = 4; q < 8; ++q) {
+              widen_w(q);
+              if (last) widen_a(0, q);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
-        if (last) {
-          const int o = (it + 1) & 7;
-#pragma unroll
-          for (int jj = 0; jj < FM; ++jj) raw[jj] = tab[o * G::BM + 32 * jj];
-          raw_w = tabw[(o >> 2) * 64 + (o & 3)];
-        }
-#pragma unroll
-        for (int n = G::issued(i * FM); n < G::issued((i + 1) * FM); ++n) {
-          const int z = G::panel(n), y = G::next(z);
-          if (!G::TRIM || it + G::ahead(z) < nit) dma(it + G::ahead(z), G::first(y) + n - G::first(z), slot(ph, z));
-        }
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][j][r] = fmaf(d[j][r], s[j], acc[i][j][r]);
         return;
       }
 #pragma unroll
@@ -458,7 +496,6 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
     s_last = s[FM - 1];
 #pragma unroll
     for (int j = 0; j < FM; ++j) s[j] = raw[j] * raw_w;
-    widen_a();
   };
 #pragma unroll 1
   for (int it = 0; it < nit;) {
@@ -477,7 +514,9 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
       ++it;
     }
   }
-  if constexpr (!G::EXACT) {
+  if constexpr (G::EXACT) {
+    join(-1, 0, s_last);
+  } else {
     if (TILES % 2 && (nit & 1)) {
       asm volatile("s_nop 15\n\ts_nop 3" : "+v"(part[0]));
       join(-1, 1, s_last);

@@ -15,10 +15,8 @@ typedef F8Geom<1, 2, 1, 1, 4, 2, 4> Tile32x64k4;
 typedef F8Geom<1, 1, 1, 1, 4, 2, 2> Tile32k4;
 typedef F8Geom<1, 1, 1, 1, 4, 4, 4> Tile32k4d;
 // of e4m3 outputs
-typedef F8Geom<2, 2, 2, 4, 1, 4, 4, -1, true> Exact128x256;
 typedef F8Geom<2, 2, 2, 2, 1, 4, 4, -1, true> Exact128;
 typedef F8Geom<1, 2, 2, 2, 1, 3, 6, -1, true> Exact64x128;
-typedef F8Geom<1, 2, 2, 2, 2, 3, 6, -1, true> Exact64x128k2;
 typedef F8Geom<1, 2, 1, 2, 4, 3, 3, -1, true> Exact32x128k4;
 
 template <typename T, bool GELU, bool F8, typename G>
@@ -39,10 +37,9 @@ static int run_tile(const F8GemmArgs& p, hipStream_t s) {
 // profiles/gemm_f8_tiles.csv (1 to 16384 rows, widths and K from 64 and 128 to
 // 8192, weights from memory), for e4m3 outputs over the 262 of
 // profiles/gemm_f8_e4m3_tiles.csv.  The tile with the least estimate is 0.4% slower
-// than the best of its list (e4m3: 0.3%, geometric means), none of the first list
-// more than 10%, one of the second (12%).  Without one of the tiles
-// the best would be slower by 0.2 to 1.9%; of the e4m3 list by 0.1 to 1.7%, without
-// 32 x 128 by 10%.
+// than the best of its list (e4m3: 0.2%, geometric means), none more than 10%.
+// Without one of the tiles the best would be slower by 0.2 to 1.9%; of the e4m3
+// list by 3 to 4%, without 32 x 128 by 12%.
 struct F8Plan {
   int bm, bn, per_cu, k_groups;
   float c[7];
@@ -57,11 +54,9 @@ static const F8Plan kPlans[] = {
     {Tile32k4::BM, Tile32k4::BN, 2, Tile32k4::KG, {2.111f, 0.736f, 0.476f, 0.000f, 0.158f, 4.547f, 0.232f}},
     {Tile32k4d::BM, Tile32k4d::BN, 1, Tile32k4d::KG, {1.935f, 0.000f, 0.513f, 1.199f, 0.000f, 5.940f, 0.253f}}};
 static const F8Plan kPlansF8[] = {
-    {Exact128x256::BM, Exact128x256::BN, 1, Exact128x256::KG, {1.592f, 3.007f, 1.662f, 0.000f, 0.000f, 1.534f, 2.579f}},
-    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.912f, 0.210f, 0.323f, 0.000f, 0.719f, 1.525f, 1.421f}},
-    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.790f, 0.000f, 0.398f, 0.016f, 0.331f, 2.658f, 0.657f}},
-    {Exact64x128k2::BM, Exact64x128k2::BN, 1, Exact64x128k2::KG, {2.089f, 2.557f, 1.004f, 0.000f, 0.000f, 3.057f, 0.571f}},
-    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {2.520f, 0.000f, 1.375f, 1.839f, 0.000f, 5.725f, 0.182f}}};
+    {Exact128::BM, Exact128::BN, 2, Exact128::KG, {3.624f, 0.704f, 0.055f, 0.000f, 0.803f, 1.675f, 1.438f}},
+    {Exact64x128::BM, Exact64x128::BN, 2, Exact64x128::KG, {3.737f, 0.331f, 0.169f, 0.000f, 0.437f, 2.551f, 0.668f}},
+    {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {2.543f, 0.000f, 1.264f, 2.301f, 0.000f, 5.372f, 0.163f}}};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]), kPlanCountF8 = sizeof(kPlansF8) / sizeof(kPlansF8[0]);
 
 // The tile with the least estimate.
@@ -102,10 +97,8 @@ static int run_plan(int plan, const F8GemmArgs& p, hipStream_t s) {
 template <bool GELU>
 static int run_plan_f8(int plan, const F8GemmArgs& p, hipStream_t s) {
   switch (plan) {
-    case 0: return run_tile<float, GELU, true, Exact128x256>(p, s);
-    case 1: return run_tile<float, GELU, true, Exact128>(p, s);
-    case 2: return run_tile<float, GELU, true, Exact64x128>(p, s);
-    case 3: return run_tile<float, GELU, true, Exact64x128k2>(p, s);
+    case 0: return run_tile<float, GELU, true, Exact128>(p, s);
+    case 1: return run_tile<float, GELU, true, Exact64x128>(p, s);
     default: return run_tile<float, GELU, true, Exact32x128k4>(p, s);
   }
 }

@@ -103,7 +103,7 @@ def kernels(tmp_path_factory):
 def test_gemm_f8_reads_products_after_their_wait(kernels):
     """Every instance: no read or copy of a product before its MFMAs are done,
     and no scratch (a spilled product is such a read)."""
-    assert len(kernels) == 8 * 4 + 3 * 2  # tiles x (two 2-byte types x GELU or not), x (e4m3 x GELU or not)
+    assert len(kernels) == 9 * 4 + 3 * 2  # tiles x (two 2-byte types x GELU or not), x (e4m3 x GELU or not)
     for name, code in kernels.items():
         assert sum(l.startswith("v_mfma") for l in code) >= 4, name
         e4m3 = {"f8f6f4" in l for l in code if l.startswith("v_mfma")}

@@ -194,15 +194,15 @@ def test_every_tile_is_some_shapes_choice():
     """The rule reaches every tile of either list (the second is of e4m3
     outputs), with K groups only where there are few tiles."""
     lib = _lib.load()
-    assert lib.tjk_gemm_f8_plan_count() == 8
+    assert lib.tjk_gemm_f8_plan_count() == 9
     shapes = [(m, n, k) for m in (1, 8, 64, 128, 256, 512, 1024, 2443, 5430, 8192, 16384)
               for n in (128, 512, 1024, 2600, 4096, 8192) for k in (128, 512, 1024, 2048, 4096, 8192)]
     for out in (BF16, E4M3):
         got = {lib.tjk_gemm_f8_default_plan(m, n, k, out, e) for m, n, k in shapes for e in (0, 1)}
-        assert got == (set(range(8)) if out == BF16 else set(range(3)))
+        assert got == (set(range(9)) if out == BF16 else set(range(3)))
     assert lib.tjk_gemm_f8_default_plan(8192, 8192, 8192, BF16, 0) == 0
     assert lib.tjk_gemm_f8_default_plan(8, 8192, 2048, BF16, 0) == 7
     for bad in ((0, 8, 16, BF16, 0), (8, 8, -1, BF16, 0), (8, 8, 16, F32, 0), (8, 8, 16, BF16, 2)):
         assert lib.tjk_gemm_f8_default_plan(*bad) == EINVAL
-    for plan in (3, 7):
+    for plan in (3, 8):
         assert _gemm(out_dtype=E4M3, c_scales=FAKE, ld_cs=1, plan=plan) == EUNSUPPORTED and "0 to 2" in _said()

@@ -288,7 +288,7 @@ SHAPES = [(1, 4, 16), (1, 128, 128), (8, 2048, 512), (15, 12, 112), (16, 132, 14
           (64, 512, 2064), (100, 1000, 256), (128, 128, 4112), (130, 516, 272), (300, 388, 1024), (513, 1028, 400)]
 
 
-PLANS = list(range(-1, 8))  # every tile, and the rule's choice
+PLANS = list(range(-1, 9))  # every tile, and the rule's choice
 PLANS_F8 = list(range(-1, 3))
 
 

@@ -155,7 +155,7 @@ def test_streams(device):
     assert all(_same(a.state(), b.state()) for a, b in zip(alone, layers))
 
 
-@pytest.mark.parametrize("plan", range(8))
+@pytest.mark.parametrize("plan", range(9))
 def test_no_depth(device, plan):
     """K = 0: the epilogue of the bias alone, and no operand is read."""
     m, n = 37, 132
@@ -183,7 +183,7 @@ def test_nothing_to_multiply(device):
     torch.cuda.synchronize()
 
 
-@pytest.mark.parametrize("plan", range(-1, 8))
+@pytest.mark.parametrize("plan", range(-1, 9))
 def test_nan_stays_in_its_row_and_column(device, plan):
     """A NaN in a row of a (or its scale) makes that row of the output NaN, one
     in a row of w that column, and nothing else differs."""

@@ -13,7 +13,13 @@
 // instruction for 4; measured with loops of nothing else.  With 16 x 16 x 128 MFMAs
 // (32 cycles each) the four FMAs that belong to one fill the rest of it, and
 // every address or scale instruction more delays the matrix unit.  With 32 x 32 x 64
-// (64 cycles) the eight FMAs leave four issue slots.
+// (64 cycles) the eight FMAs leave four issue slots.  One wave issues an instruction
+// every 7 cycles at most, so a SIMD with one wave falls behind its products; with
+// two the matrix unit is the bound, and in large launches the clock that their power
+// leaves: 8192^3 takes 457 us (2.4 PFLOP/s; matrix unit busy for 66% of the cycles at
+// 1.74 GHz), its MFMAs alone 290, and 412 a library product with one scale per
+// tensor.  8192 x 8192 x 2048: 137 us.  Few rows are bound by the latency of the
+// weights: 8 x 8192 x 2048 in 6.2 us, 2.7 TB/s.
 #pragma once
 
 #include "f8_common.h"
@@ -216,10 +222,11 @@ struct F8Geom {
 // into the registers of an operand that was used for the last time: W's next tile
 // behind its last row block, A's next K tile behind its last W tile and, the second
 // fragment, behind the next K tile's first product (its registers are free then).
-// 2048 x 1024 x 4096, one wave per SIMD: 30.5 us, against 35.0 with the conversions
-// in one piece.  5430 x 4096 x 1024 with GELU, two waves: 57 us either way (36 with
-// the e4m3 MFMAs), and 4096^3 119 us, 1.15 PFLOP/s: there the clock falls with the
-// power that fp16 products take (a bf16 library product of 8192^3 reaches 1.38).
+// 2048 x 1024 x 4096, one wave per SIMD: 30.1 us, against 35.0 with the conversions
+// in one piece.  Two waves: 4096^3 117 us (1.17 PFLOP/s, the matrix unit busy for
+// 57% of the cycles at 1.95 GHz), 5430 x 4096 x 1024 with GELU 55 us (36 with the
+// e4m3 MFMAs).  Of a K tile there the DMA takes 16% and the conversions 18% beside
+// the products; with neither it is the products' own time.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x16 (&acc)[G::FN][G::FM]) {

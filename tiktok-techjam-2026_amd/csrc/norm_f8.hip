@@ -14,6 +14,13 @@ namespace tjk {
 // pieces t, t + T, ... in registers, so the row is read once.  A block of
 // 128 columns is 16 neighbouring lanes, one DPP row: its largest magnitude
 // needs no LDS.
+//
+// Bound by memory: residual, addend, sum and quantised row pass once, 7 bytes per
+// element with 2-byte ones.  32768 x 4096 bf16: 165 us, 5.7 TB/s (a copy of 1 GB
+// reaches 4.8); 5430 x 1024 with an fp32 residual: 11.2 us, 5.5 TB/s, as quick from
+// one wave per row (four rows a workgroup) as it gets.  8 x 2048: 2.6 us in a graph,
+// a launch and two passages of memory latency.  gamma is loaded where it is used:
+// requested with the row it takes registers, and 2 to 4% longer.
 
 struct NormArgs {
   const void* res;
@@ -159,9 +166,10 @@ static int launch_norm(const NormArgs& a, hipStream_t s) {
 // -------------------------------------------------------------- quantisation
 //
 // Blocks of one row and 128 columns: 16 lanes hold a block, 8 elements each.
-// The blocks of the matrix are numbered row by row; a wave takes kBlocks of
+// The blocks of the matrix are numbered row by row; a wave takes kQuantBlocks of
 // them, four at a time, so narrow rows share a wave and every load of the
-// wave goes out before the first is used.
+// wave goes out before the first is used.  Bound by memory: 8192 x 8192 bf16 in
+// 37.2 us, 5.5 TB/s.
 
 constexpr int kQuantBlocks = 16;
 
@@ -212,7 +220,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 }
 
 // Blocks of 128 rows and 128 columns: one workgroup holds a block in
-// registers, 16 rows at a time over its 256 threads.
+// registers, 16 rows at a time over its 256 threads.  2600 x 1008 fp32: 4.1 us,
+// 3.2 TB/s from 168 workgroups, a launch and one round of loads.
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_tiles_kernel(const T* __restrict__ x, int64_t ld, uint8_t* __restrict__ q,
                                                              int64_t ld_q, float* __restrict__ scales, int64_t ld_s,

@@ -18,8 +18,9 @@
 // two the matrix unit is the bound, and in large launches the clock that their power
 // leaves: 8192^3 takes 457 us (2.4 PFLOP/s; matrix unit busy for 66% of the cycles at
 // 1.74 GHz), its MFMAs alone 290, and 412 a library product with one scale per
-// tensor.  8192 x 8192 x 2048: 137 us.  Few rows are bound by the latency of the
-// weights: 8 x 8192 x 2048 in 6.2 us, 2.7 TB/s.
+// tensor.  8192 x 8192 x 2048: 137 us.  Few rows are bound by the passage of the
+// weights: 8 x 8192 x 2048 in 6.0 us, 2.8 TB/s, of which 2.5 us are launch, latency
+// and join.
 #pragma once
 
 #include "f8_common.h"
@@ -322,8 +323,20 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
 #pragma unroll
         for (int d = 0; d < G::count(y); ++d) dma(it, G::first(y) + d, slot(it, y));
       }
+  // TRIM, near the end: waits until no more than `tiles` K tiles are in flight (DMA
+  // instructions land in order, K tile by K tile; of several W tiles: until all have).
+  static_assert(!G::TRIM || FN > 1 || (G::ahead(0) == G::AHEAD && G::ahead(FM) == G::AHEAD && G::AHEAD <= 4),
+                "the panels of a K tile are in flight together, with three more K tiles at most");
+  auto wait_tiles = [&](int tiles) __attribute__((always_inline)) {
+    if (FN > 1 || tiles <= 0)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else if (tiles == 1)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(G::ND) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * G::ND) : "memory");
+  };
   if (G::TRIM && nit < G::AHEAD)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_tiles(nit - 1);
   else
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(G::in_flight(FN - 1) + G::issued(G::TILES) - G::issued((FN - 1) * FM))
                  : "memory");
@@ -381,7 +394,7 @@ __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, i
       if constexpr (G::meets(i)) {
         constexpr int in_flight = G::in_flight(i);
         if (G::TRIM && it + G::AHEAD >= nit)  // fewer in flight
-          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          wait_tiles(nit - 2 - it);
         else
           asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(in_flight) : "memory");
         if constexpr (NW > 1) asm volatile("s_barrier" ::: "memory");

@@ -220,24 +220,29 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 }
 
 // Blocks of 128 rows and 128 columns: one workgroup holds a block in
-// registers, 16 rows at a time over its 256 threads.  2600 x 1008 fp32: 4.1 us,
-// 3.2 TB/s from 168 workgroups, a launch and one round of loads.
+// registers, 32 rows at a time over its 512 threads (4096 x 1024 fp32: 5.6 us,
+// with 256 threads 6.1, with 1024 5.9).  2600 x 1008 fp32: a launch and one round
+// of loads of 168 workgroups.  8192 x 8192 bf16: 37.1 us, 5.4 TB/s.
+constexpr int kQuantThreads = 512;
+
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_tiles_kernel(const T* __restrict__ x, int64_t ld, uint8_t* __restrict__ q,
-                                                             int64_t ld_q, float* __restrict__ scales, int64_t ld_s,
-                                                             int64_t rows, int n, int nb) {
-  __shared__ float part[4];
+__global__ __launch_bounds__(kQuantThreads) void quantize_tiles_kernel(const T* __restrict__ x, int64_t ld,
+                                                                       uint8_t* __restrict__ q, int64_t ld_q,
+                                                                       float* __restrict__ scales, int64_t ld_s,
+                                                                       int64_t rows, int n, int nb) {
+  constexpr int STEP = kQuantThreads / 16, U = kF8Block / STEP;  // rows at a time, how often
+  __shared__ float part[kQuantThreads / 64];
   const int t = threadIdx.x, l16 = t & 15;
   const int64_t rb = blockIdx.x / nb;
   const int cb = (int)(blockIdx.x - rb * nb);
   const int64_t r0 = rb * kF8Block + (t >> 4);
   const int col = cb * kF8Block + 8 * l16;
-  typename Oct<T>::raw raw[8];
+  typename Oct<T>::raw raw[U];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) raw[u] = Oct<T>::load(x + min(r0 + 16 * u, rows - 1) * ld + min(col, n - 8));
+  for (int u = 0; u < U; ++u) raw[u] = Oct<T>::load(x + min(r0 + STEP * u, rows - 1) * ld + min(col, n - 8));
   float top = 0.f;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
+  for (int u = 0; u < U; ++u) {
     float v[8];
     Oct<T>::to(raw[u], v);
     // rows and columns past the end repeat values of this block, so they
@@ -250,12 +255,14 @@ __global__ __launch_bounds__(256) void quantize_tiles_kernel(const T* __restrict
   top = fmaxf(top, __shfl_xor(top, 32));
   if ((t & 63) == 0) part[t >> 6] = top;
   __syncthreads();
-  const float s = f8_scale(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+#pragma unroll
+  for (int w = 0; w < kQuantThreads / 64; ++w) top = fmaxf(top, part[w]);
+  const float s = f8_scale(top);
   const float inv = __builtin_amdgcn_rcpf(s);
   if (t == 0) scales[rb * ld_s + cb] = s;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const int64_t r = r0 + 16 * u;
+  for (int u = 0; u < U; ++u) {
+    const int64_t r = r0 + STEP * u;
     if (r < rows && col < n) {
       float v[8];
       Oct<T>::to(raw[u], v);
@@ -272,14 +279,14 @@ static int launch_quantize(const void* x, int64_t ld, void* q, int64_t ld_q, flo
   if (rows > ((int64_t)1 << 38)) return fail(TJK_EUNSUPPORTED, "tjk_quantize_f8: %lld rows are too many", (long long)rows);
   const int64_t blocks = (block_rows == 1 ? rows : (rows + kF8Block - 1) / kF8Block) * nb;
   const int64_t grid = block_rows == 1 ? (blocks + 4 * kQuantBlocks - 1) / (4 * kQuantBlocks) : blocks;
-  if (grid > (int64_t)UINT32_MAX / 256)
+  if (grid > (int64_t)UINT32_MAX / kQuantThreads)
     return fail(TJK_EUNSUPPORTED, "tjk_quantize_f8: %lld blocks are too many", (long long)blocks);
   const T* xt = static_cast<const T*>(x);
   uint8_t* qt = static_cast<uint8_t*>(q);
   if (block_rows == 1)
     quantize_rows_kernel<T><<<(unsigned)grid, 256, 0, s>>>(xt, ld, qt, ld_q, scales, ld_s, rows, (int)n, (int)nb);
   else
-    quantize_tiles_kernel<T><<<(unsigned)grid, 256, 0, s>>>(xt, ld, qt, ld_q, scales, ld_s, rows, (int)n, (int)nb);
+    quantize_tiles_kernel<T><<<(unsigned)grid, kQuantThreads, 0, s>>>(xt, ld, qt, ld_q, scales, ld_s, rows, (int)n, (int)nb);
   return check_launch("tjk_quantize_f8");
 }
 

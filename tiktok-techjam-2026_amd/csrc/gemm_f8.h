@@ -130,7 +130,9 @@ struct F8Geom {
   // takes few K tiles, and two past them cost 0.2 of 4.1 us (K = 512).  Not where
   // waves share K tiles: branches in the K loop cost 4 to 15% of a K tile.
   static constexpr bool TRIM = KG > 1 && NW == 1;
-  static constexpr int LDS = BIAS + BN * 4;
+  // (whole LDS DMA instructions bring the bias: 64 words each, zeros past the tile)
+  static constexpr int BIAS_BYTES = BN * 4 > 256 ? BN * 4 : 256;
+  static constexpr int LDS = BIAS + BIAS_BYTES;
 
   // Panel y (A: y < FM) of a K tile: the first of its DMA instructions, their
   // number; the panel that goes into its slot when it has been read, and how many
@@ -840,7 +842,8 @@ __global__ __launch_bounds__(G::THREADS, G::THREADS <= 256 && G::LDS > 80 * 1024
     const int lane = threadIdx.x & 63;
     const u32x4 r = lds_dma_rsrc(static_cast<const T*>(p.bias) + n0,
                                  p.bias != nullptr ? (int64_t)(p.n - n0) * (int64_t)sizeof(T) : 0);
-    constexpr int NI = G::BN * (int)sizeof(T) / 256 > 0 ? G::BN * (int)sizeof(T) / 256 : 1;
+    constexpr int NI = (G::BN * (int)sizeof(T) + 255) / 256;
+    static_assert(NI * 256 <= G::BIAS_BYTES, "the DMA of the bias writes all of its words");
 #pragma unroll
     for (int i = 0; i < NI; ++i)
       if (i % (G::NW * G::KG) == gw) {

@@ -393,8 +393,9 @@ int tjk_quantize_f8(const void* x, int x_dtype, int64_t ld_x, void* q, int64_t l
  * results, the exact products in fp16, which take twice as long, summed in fp32.
  * No fp32 output and no residual epilogue: tjk_add_rmsnorm and
  * tjk_add_layernorm add a 2-byte output to an fp32 residual.
- * Requires k % 16 == 0, n % 4 == 0, lda and ldw multiples of 16 (below 2^23),
- * ldc of 4, 16-byte aligned a and w, and bias and c aligned to 4 elements.
+ * Requires k % 16 == 0, n % 4 == 0, lda and ldw multiples of 16, ldc of 4,
+ * 16-byte aligned a and w, and bias and c aligned to 4 elements; lda, ldw and ldc
+ * below 2^23, ld_as and ld_ws below 2^21, and m <= 2^31 - 256.
  * plan_id: -1 chooses, else one of tjk_gemm_f8_plan_count() tiles (0 to 2 for an
  * e4m3 output).  Tiles that split K over groups of
  * waves add up in another order, always the same.

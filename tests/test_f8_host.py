@@ -206,3 +206,12 @@ def test_every_tile_is_some_shapes_choice():
         assert lib.tjk_gemm_f8_default_plan(*bad) == EINVAL
     for plan in (3, 8):
         assert _gemm(out_dtype=E4M3, c_scales=FAKE, ld_cs=1, plan=plan) == EUNSUPPORTED and "0 to 2" in _said()
+
+
+@pytest.mark.parametrize("m", [(1 << 31) - 1, (1 << 31) - 16, (1 << 31) - 255])
+@pytest.mark.parametrize("plan", [-1, 0, 4, 7])
+def test_gemm_refuses_rows_that_tiles_cannot_count(m, plan):
+    """Row counts whose rounding up to a whole tile (256 rows at most) passes
+    31 bits are refused: tiles are counted in 32-bit integers."""
+    assert _gemm(m=m, n=4, k=16, lda=16, ldw=16, ldc=4, ld_as=1, ld_ws=1, plan=plan) == EUNSUPPORTED
+    assert "rows" in _said()

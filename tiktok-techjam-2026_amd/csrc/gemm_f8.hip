@@ -61,6 +61,9 @@ static const F8Plan kPlansF8[] = {
     {Exact32x128k4::BM, Exact32x128k4::BN, 1, Exact32x128k4::KG, {2.560f, 0.000f, 1.267f, 2.279f, 0.000f, 5.344f, 0.163f}}};
 constexpr int kPlanCount = sizeof(kPlans) / sizeof(kPlans[0]), kPlanCountF8 = sizeof(kPlansF8) / sizeof(kPlansF8[0]);
 
+// Rows are rounded up to a whole tile (256 at most) in 32-bit integers.
+constexpr int64_t kMaxRows = (int64_t)INT32_MAX - 255;
+
 // The tile with the least estimate.
 static int auto_plan(int64_t m, int64_t n, int64_t k, bool f8, bool gelu) {
   int best = 0;
@@ -113,7 +116,7 @@ using namespace tjk;
 extern "C" int tjk_gemm_f8_plan_count(void) { return kPlanCount; }
 
 extern "C" int tjk_gemm_f8_default_plan(int64_t m, int64_t n, int64_t k, int out_dtype, int epilogue) {
-  if (m <= 0 || n <= 0 || k < 0 || m > INT32_MAX || n > INT32_MAX || k > INT32_MAX)
+  if (m <= 0 || n <= 0 || k < 0 || m > kMaxRows || n > INT32_MAX || k > INT32_MAX)
     return fail(TJK_EINVAL, "tjk_gemm_f8_default_plan: bad shape");
   if (out_dtype != TJK_F16 && out_dtype != TJK_BF16 && out_dtype != TJK_E4M3)
     return fail(TJK_EINVAL, "tjk_gemm_f8_default_plan: bad output dtype %d", out_dtype);
@@ -139,6 +142,7 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
     return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: an e4m3 output has plans 0 to %d, not %d", kPlanCountF8 - 1, plan_id);
   if ((k && (!a || !w || !a_scales || !w_scales)) || !c || (f8 && !c_scales)) return fail(TJK_EINVAL, "tjk_gemm_f8: null pointer");
   if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: shape exceeds int32");
+  if (m > kMaxRows) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: %lld rows are too many", (long long)m);
   if (k % 16) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: k=%lld must be a multiple of 16", (long long)k);
   if (n % 4) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: n=%lld must be a multiple of 4", (long long)n);
   const int64_t kb = (k + kF8Block - 1) / kF8Block, nb = (n + kF8Block - 1) / kF8Block;
@@ -146,7 +150,8 @@ extern "C" int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, in
     return fail(TJK_EINVAL, "tjk_gemm_f8: leading dimension too small");
   if (lda % 16 || ldw % 16) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: lda/ldw must be multiples of 16");
   if (ldc % 4) return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: ldc must be a multiple of 4");
-  // 256 rows of an operand, of its scales, or 64 of the output within 31-bit byte offsets
+  // 256 rows of an operand or of its scales, or 96 of the output (a wave's), within 31-bit
+  // byte offsets; so n and k, at most ldc and lda, can be rounded up too
   if (ldc > INT32_MAX / 256 || lda > INT32_MAX / 256 || ldw > INT32_MAX / 256 || ld_as > INT32_MAX / 1024 || ld_ws > INT32_MAX / 1024)
     return fail(TJK_EUNSUPPORTED, "tjk_gemm_f8: leading dimension too large");
   const uintptr_t need_c = f8 ? 3 : 7, need_bias = f8 ? 15 : 7;

@@ -391,6 +391,9 @@ int tjk_quantize_f8(const void* x, int x_dtype, int64_t ld_x, void* q, int64_t l
  * its power of two.  That leaves the sums 1.5e-5 off (2-norm, normal operands),
  * well inside a 2-byte rounding.  For an e4m3 output, whose scales are fp32
  * results, the exact products in fp16, which take twice as long, summed in fp32.
+ * GELU(v) of a 2-byte output is off by up to 1.5e-7 |v| (as in tjk_gemm_bias: not
+ * small beside GELU itself below v = -4); of an e4m3 output by up to 8e-6 of its
+ * block's largest value, also where all of the block lie that low.
  * No fp32 output and no residual epilogue: tjk_add_rmsnorm and
  * tjk_add_layernorm add a 2-byte output to an fp32 residual.
  * Requires k % 16 == 0, n % 4 == 0, lda and ldw multiples of 16, ldc of 4,

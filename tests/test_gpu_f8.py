@@ -348,3 +348,66 @@ def test_gemm_f8_output(device, problem, m, n, k, epi, plan):
     _check_quantised(out, scales[:m, :_blocks(n)], v, 1, err)
     assert _untouched(whole, m, n, 2.0)
     assert (scales[m] == 7.0).all() and (scales[:, _blocks(n):] == 7.0).all()
+
+
+def _low_rows(n, device):
+    """(a, w and their scales, bias, pre-activations v): v = a[m, 0] + bias[n] in
+    fp32, the one product of a row being exact, for bias blocks that lie deep in GELU's
+    negative tail, at its edge, and around zeros."""
+    shift = torch.tensor([0.0, 0.25, 3.0, -2.0, -8.0, -1.5, 6.0])
+    m, k = 10 * len(shift), 16
+    bias = torch.empty(n)
+    bias[:128] = torch.linspace(-13, -2.5, 128)
+    bias[128:256] = torch.linspace(-6, -5, 128)
+    bias[200:204] = torch.tensor([0.0, -1e-9, 1e-12, -0.0])  # no value above: no scale from them
+    bias[256:384] = torch.linspace(-9, 0.24, 128)
+    bias[384:512] = torch.randn(128, generator=_gen(11))
+    bias[512:] = torch.tensor([-4.0, -5.0, -5.5, -6.0])
+    a = torch.zeros(m, k)
+    a[:, 0] = shift.repeat(10)
+    w = torch.zeros(n, k)
+    w[:, 0] = 1
+    v = a[:, :1] + bias  # one rounding in fp32, as the kernel's addition of the bias
+    ones = torch.ones(m, 1, device=device), torch.ones(_blocks(n), 1, device=device)
+    return (a.to(F8).to(device), ones[0], w.to(F8).to(device), ones[1], bias.to(device)), v
+
+
+@pytest.mark.parametrize("plan", PLANS_F8)
+def test_gelu_scales_of_blocks_in_the_negative_tail(device, plan):
+    """A block takes its scale from GELU values that may all be small: they have
+    to be right relative to its largest, A.
+
+    GELU takes either form for 32 values of a row, or a block, at a time.  Where the
+    largest |GELU| of them is at least 1 / 32 of the largest |v|: max(v, 0) - |v| h, h off by
+    1.5e-7 (the formula) and 40 U of itself (its roundings, as in _gelu_err), |v| h <= A:
+    32 * 1.5e-7 A + 40 U A.  Elsewhere exp(-v^2 / 2) times a polynomial of 10 terms
+    in 1 / (1 + |v| / 4): 3 U for that quotient, 16 U for 10 steps of one rounding whose
+    terms add up to 1.6 times the polynomial, the fit 1 U, and 11 U for two exponentials of
+    2 U, what their exponent lacks and 6 products: 32 U of the value."""
+    n = 516
+    args, v = _low_rows(n, device)
+    m = v.shape[0]
+    out, whole = _inside(m, n, F8, device, fill=2.0)
+    scales = torch.full((m, _blocks(n)), 7.0, device=device)
+    ops.gemm_f8(*args, out, EPI_BIAS_GELU, out_scales=scales, plan=plan)
+    torch.cuda.synchronize()
+    y = _gelu(v.double())
+    err = torch.empty_like(y)
+    for b in range(_blocks(n)):
+        part = slice(128 * b, 128 * b + 128)
+        err[:, part] = (32 * 1.5e-7 + 40 * U) * y[:, part].abs().amax(dim=1, keepdim=True) + 2.0 ** -149
+    _check_quantised(out, scales, y, 1, err)
+    assert _untouched(whole, m, n, 2.0)
+
+
+@pytest.mark.parametrize("plan", range(3))
+def test_gelu_rows_do_not_depend_on_each_other(device, plan):
+    n = 516
+    (a, a_s, w, w_s, bias), v = _low_rows(n, device)
+    m = v.shape[0]
+    out, scales = torch.empty(m, n, dtype=F8, device=device), torch.empty(m, _blocks(n), device=device)
+    ops.gemm_f8(a, a_s, w, w_s, bias, out, EPI_BIAS_GELU, out_scales=scales, plan=plan)
+    for r in range(7):
+        one, s = torch.empty(1, n, dtype=F8, device=device), torch.empty(1, _blocks(n), device=device)
+        ops.gemm_f8(a[r:r + 1], a_s[r:r + 1], w, w_s, bias, one, EPI_BIAS_GELU, out_scales=s, plan=plan)
+        assert torch.equal(one.view(torch.uint8), out[r:r + 1].view(torch.uint8)) and torch.equal(s, scales[r:r + 1])

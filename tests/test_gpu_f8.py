@@ -411,3 +411,32 @@ def test_gelu_rows_do_not_depend_on_each_other(device, plan):
         one, s = torch.empty(1, n, dtype=F8, device=device), torch.empty(1, _blocks(n), device=device)
         ops.gemm_f8(a[r:r + 1], a_s[r:r + 1], w, w_s, bias, one, EPI_BIAS_GELU, out_scales=s, plan=plan)
         assert torch.equal(one.view(torch.uint8), out[r:r + 1].view(torch.uint8)) and torch.equal(s, scales[r:r + 1])
+
+
+@pytest.mark.parametrize("plan", range(9))
+@pytest.mark.parametrize("m,n,k", [(515, 1040, 144), (2100, 2064, 144)])
+def test_gemm_aligned_outputs(device, problem, m, n, k, plan):
+    """Whole 16-byte pieces of aligned rows: of an output below 4 MB, and of a
+    larger one, which is written through; inside larger buffers that are kept."""
+    (a, a_s), (w, w_s), bias, (v0, err0, err0_f8) = problem(m, n, k)
+    for out_dt, epi in (("bf16", EPI_BIAS), ("f16", EPI_BIAS_GELU)):
+        dt = DT[out_dt]
+        v, err = (v0, err0) if epi == EPI_BIAS else (_gelu(v0), _gelu_err(v0, err0))
+        out, whole = _inside(m, n, dt, device)
+        assert out.data_ptr() % 16 == 0 and out.stride(0) % 16 == 0
+        ops.gemm_f8(a, a_s, w, w_s, bias.to(dt).to(device), out, epi, plan=plan)
+        torch.cuda.synchronize()
+        got, half = out.double().cpu(), torch.finfo(dt).eps / 2
+        over = got.abs() == float("inf")
+        assert (v.abs()[over] >= 65504).all()
+        bad = ~((got - v).abs() <= err + half * (v.abs() + err) + 2.0 ** -25) & ~over
+        assert not bad.any(), f"{out_dt}: {int(bad.sum())} of {m * n} off"
+        assert _untouched(whole, m, n, None)
+    if plan < 3:
+        out, whole = _inside(m, n, F8, device, fill=2.0)
+        assert out.data_ptr() % 16 == 0
+        scales = torch.full((m, _blocks(n)), 7.0, device=device)
+        ops.gemm_f8(a, a_s, w, w_s, bias.to(device), out, out_scales=scales, plan=plan)
+        torch.cuda.synchronize()
+        _check_quantised(out, scales, v0, 1, err0_f8)
+        assert _untouched(whole, m, n, 2.0)

@@ -440,3 +440,66 @@ def test_gemm_aligned_outputs(device, problem, m, n, k, plan):
         torch.cuda.synchronize()
         _check_quantised(out, scales, v0, 1, err0_f8)
         assert _untouched(whole, m, n, 2.0)
+
+
+def _dropped(a, w, a_s, w_s):
+    """64-bit sums of one row a against the rows of w, as they are and with the
+    bits dropped that lie below 2^-13 of the power of two of the largest of each eight
+    products (that power from the operands' own)."""
+    def power(q):
+        return torch.floor(torch.log2(q.abs().clamp(min=2.0 ** -9))).clamp(min=-6)
+
+    n, k = w.shape
+    p = (a * w).view(n, k // 8, 8)
+    e = (power(a) + power(w)).view(n, k // 8, 8)
+    unit = torch.exp2(torch.where(p == 0, -40.0, e).amax(-1, keepdim=True) - 13)
+    f = a_s[None, :] * w_s.repeat_interleave(128, 0)
+    each = [(t.view(n, k // 128, 128).sum(-1) * f).sum(1) for t in (p, torch.trunc(p / unit) * unit)]
+    return each[0], each[1]
+
+
+@pytest.mark.parametrize("spread,stated", [(0.0, 1.5e-5), (0.7, 2.5e-5)])
+@pytest.mark.parametrize("k", [1024, 4096])
+def test_how_exact_the_sums_are(device, k, spread, stated):
+    """The stated 2-norms of the sums' errors: of a 2-byte output for normal
+    operands and with columns that stand out; of an e4m3 output (its scales).
+
+    A bias of minus the result, rounded to fp16, leaves at most 2^-11 of it: the output shows
+    the sum's error to 2^-22 of the sum (and 2^-25).  The error is that of the bits
+    dropped, within a twentieth for what else the matrix unit does with them, and of about
+    20 fp32 additions of a unit in the last place: 20^0.5 * 2 U < 6e-7.
+    A scale's errors in the mean square, in units of U^2 (a rounding to nearest is off by
+    U / 3^0.5): at most 128 additions inside a block, to partial sums of half the
+    block's square on average, 128 / 6; k / 128 <= 32 of the blocks, 32 / 6; six
+    roundings of whole values at most (two of the block's factor and one of its product,
+    the addition of no bias, two of the scale), 6 / 3: 28.7, so 5.4 U = 3.2e-7."""
+    m, n = 33, 2048
+    g = _gen(k)
+
+    def quantised(x, block_rows):
+        b = x.view(x.shape[0] // block_rows, block_rows, k // 128, 128)
+        s = b.abs().amax(dim=(1, 3)) / 448
+        return (b / s[:, None, :, None]).view(x.shape).to(F8), s
+
+    a, a_s = quantised(torch.randn(1, k, generator=g) * torch.exp(spread * torch.randn(1, k, generator=g)), 1)
+    w, w_s = quantised(torch.randn(n, k, generator=g) * 0.02, 128)
+    v, cut = _dropped(a.double(), w.double(), a_s[0].double(), w_s.double())
+    expected = ((cut - v).norm() / v.norm()).item()
+    assert expected <= stated
+    rows = a.expand(m, k).contiguous().to(device), a_s.expand(m, k // 128).contiguous().to(device)
+    bias = (-v).half()
+    for plan in range(9):
+        out = torch.empty(m, n, dtype=torch.float16, device=device)
+        ops.gemm_f8(*rows, w.to(device), w_s.to(device), bias.to(device), out, plan=plan)
+        assert torch.equal(out, out[:1].expand(m, n))
+        error = ((out[0].double().cpu() - (v + bias.double())).norm() / v.norm()).item()
+        print(f"plan {plan}: {error:.3g}, dropped bits {expected:.3g}")
+        assert abs(error - expected) <= expected / 20 + 2.0 ** -22 + 6e-7, (plan, error, expected)
+        assert error <= stated
+    for plan in range(3):
+        out, scales = torch.empty(m, n, dtype=F8, device=device), torch.empty(m, n // 128, device=device)
+        ops.gemm_f8(*rows, w.to(device), w_s.to(device), None, out, out_scales=scales, plan=plan)
+        want = v.view(-1, 128).abs().amax(1) / 448
+        error = ((scales[0].double().cpu() - want).norm() / want.norm()).item()
+        print(f"e4m3 plan {plan}: scales {error:.3g}")
+        assert error <= 3.2e-7

@@ -809,15 +809,15 @@ __device__ __forceinline__ void f8_store(const F8GemmArgs& p, const f32x16 (&acc
   }
 }
 
-// Outputs in e4m3.  A row's largest magnitude over the wave's columns takes one
-// lane exchange; where a block of 128 columns spans several waves they trade
-// theirs through LDS (`red`, BM x WN floats; every wave of the workgroup calls
-// this).  Words are put in rows through `stage` (1024 FM FN bytes of the wave's own),
+// Outputs in e4m3.  A row's largest magnitude over the wave's 64 columns takes
+// one lane exchange; the two waves of a block of 128 trade theirs through LDS
+// (`red`, BM x WN floats; every wave of the workgroup calls this).  Words are put in rows through `stage` (1024 FM FN bytes of the wave's own),
 // the 16-byte piece c of row r at c ^ x(r).
 template <typename G>
 __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&acc)[G::FN][G::FM], int mw, int nw,
                                             int wm, int wn, int lane, float* red, char* stage) {
-  constexpr int FM = G::FM, FN = G::FN, WPB = 128 / G::WTN;
+  constexpr int FM = G::FM, FN = G::FN;
+  static_assert(FN == 2 && G::WN % 2 == 0, "two waves share a block, rows of 64 bytes");
   const int l32 = lane & 31, hi = lane >> 5;
   float top[FM];
 #pragma unroll
@@ -834,26 +834,21 @@ __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&
       }
     top[j] = fmaxf(top[j], __shfl_xor(top[j], 32));
   }
-  if constexpr (WPB > 1) {
-    if (hi == 0) {
+  if (hi == 0) {
 #pragma unroll
-      for (int j = 0; j < FM; ++j) red[wn * G::BM + wm * G::WTM + 32 * j + l32] = top[j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < FM; ++j)
-#pragma unroll
-      for (int o = 0; o < WPB; ++o)
-        top[j] = fmaxf(top[j], red[(wn / WPB * WPB + o) * G::BM + wm * G::WTM + 32 * j + l32]);
+    for (int j = 0; j < FM; ++j) red[wn * G::BM + wm * G::WTM + 32 * j + l32] = top[j];
   }
-  constexpr int LPR = 2 * FN;  // pieces per row: 8 or 4
-  static_assert(LPR == 8 || LPR == 4, "staged rows of 128 or 64 bytes");
-  auto x = [](int r) { return LPR == 8 ? r & 7 : (r >> 1) & 3; };
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < FM; ++j)
+    top[j] = fmaxf(top[j], red[(wn ^ 1) * G::BM + wm * G::WTM + 32 * j + l32]);
+  constexpr int LPR = 4;  // pieces per row
+  auto x = [](int r) { return (r >> 1) & 3; };
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const float s = f8_scale(top[j]), inv = __builtin_amdgcn_rcpf(s);
     const int m = mw + 32 * j + l32;
-    if (hi == 0 && wn % WPB == 0 && m < p.m && nw < p.n) p.cs[(int64_t)m * p.ld_cs + nw / 128] = s;
+    if (hi == 0 && wn % 2 == 0 && m < p.m && nw < p.n) p.cs[(int64_t)m * p.ld_cs + nw / 128] = s;
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll

@@ -342,8 +342,10 @@ int tjk_attn_block_supported(int64_t d_model, int heads, int head_dim, int64_t m
  * ceil(n / 128)]); blocks at the end may be cut short.  Scales have a unit
  * column stride and their own leading dimension.  Quantising a block whose
  * largest magnitude is A takes the scale s = max(A / 448, 2^-126) (to one unit
- * in the last place) and q = x / s rounded to nearest even.  A NaN element
- * stays NaN and does not count in A; a block with an infinity has s = inf.
+ * in the last place) and q = x (1 / s) rounded to nearest even, 1 / s good to one
+ * unit in the last place: an x / s within 2^-22 of the middle between two e4m3
+ * values may become either.  A NaN element stays NaN and does not count in A; a block
+ * with an infinity has s = inf.
  * No counterpart in the reference, which computes in fp16 / bf16 / fp32.
  */
 

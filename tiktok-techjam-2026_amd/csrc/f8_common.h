@@ -22,7 +22,7 @@ __device__ __forceinline__ float f8_scale(float top) { return fmaxf(top * (1.0f 
 // Four values times `inv`, the reciprocal of their block's scale, rounded
 // to nearest even in e4m3, value i in byte i.  A reciprocal good to one unit in
 // the last place leaves |v inv| <= 448 (1 + 2^-22), which rounds to at most
-// 448: nothing saturates.
+// 448: nothing saturates.  A quotient that close to a tie may go either way.
 __device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d, float inv) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);

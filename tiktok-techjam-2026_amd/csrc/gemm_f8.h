@@ -227,8 +227,8 @@ struct F8Geom {
 // fragment, behind the next K tile's first product (its registers are free then).
 // 2048 x 1024 x 4096, one wave per SIMD: 30.1 us, against 35.0 with the conversions
 // in one piece.  Two waves: 4096^3 117 us (1.17 PFLOP/s, the matrix unit busy for
-// 57% of the cycles at 1.95 GHz), 5430 x 4096 x 1024 with GELU 55 us (36 with the
-// e4m3 MFMAs).  Of a K tile there the DMA takes 16% and the conversions 18% beside
+// 57% of the cycles at 1.95 GHz), 5430 x 4096 x 1024 with GELU 57 us (36 with the
+// e4m3 MFMAs).  With a long K or few rows a 2-byte output and quantize_f8 are quicker.  Of a K tile there the DMA takes 16% and the conversions 18% beside
 // the products; with neither it is the products' own time.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,

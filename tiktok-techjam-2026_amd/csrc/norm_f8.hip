@@ -17,10 +17,11 @@ namespace tjk {
 //
 // Bound by memory: residual, addend, sum and quantised row pass once, 7 bytes per
 // element with 2-byte ones.  32768 x 4096 bf16: 165 us, 5.7 TB/s (a copy of 1 GB
-// reaches 4.8); 5430 x 1024 with an fp32 residual: 11.2 us, 5.5 TB/s, as quick from
-// one wave per row (four rows a workgroup) as it gets.  8 x 2048: 2.6 us in a graph,
-// a launch and two passages of memory latency.  gamma is loaded where it is used:
-// requested with the row it takes registers, and 2 to 4% longer.
+// reaches 4.8; to bf16 186 us, to fp32 243); 5430 x 1024 with an fp32 residual: 11.3 us,
+// 5.4 TB/s, as quick from one wave per row (four rows a workgroup) as it gets (to bf16
+// 12.1).  1024 threads a row: 8192 x 16384 bf16 164 us, 5.7 TB/s; 4096 x 32768 190, 5.0.
+// 8 x 2048: 2.6 us in a graph, a launch and two passages of memory latency.  gamma is
+// loaded where it is used: requested with the row it takes registers, and 2 to 4% longer.
 
 struct NormArgs {
   const void* res;

@@ -448,6 +448,8 @@ def gemm_f8(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: 
     [m, ceil(n / 128)]; ``bias`` has a 2-byte out's dtype, else float32.
     Epilogues EPI_BIAS and EPI_BIAS_GELU: a 2-byte output is added to an fp32
     residual by the next ``add_rmsnorm`` or ``add_layernorm``, as its delta.
+    An e4m3 out is the quicker form for hundreds of rows and k up to about 1024;
+    with few rows or a long k a 2-byte out and ``quantize_f8`` are, by up to 1.9 times.
 
     The sums of a 2-byte output are 1.5e-5 off, relative to their 2-norm (2.5e-5 where
     columns of ``a`` stand out; sums that cancel lose 2^-13 of the largest products),

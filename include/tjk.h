@@ -353,7 +353,8 @@ int tjk_attn_block_supported(int64_t d_model, int heads, int head_dim, int64_t m
  * Fused residual-add + RMS norm over rows of length n, in fp32:
  *   x = res (+ delta);  res_out = x (if res_out != NULL), in res_out_dtype
  *   out = x * rsqrt(mean(x^2) + eps) * gamma
- * of the unrounded x.  out_dtype TJK_F32 / F16 / BF16, or TJK_E4M3: out then
+ * of the unrounded x (zeros where the squares' sum passes fp32: an rms above
+ * 1.8e19 / sqrt(n)).  out_dtype TJK_F32 / F16 / BF16, or TJK_E4M3: out then
  * holds the quantised rows and scales [rows, ceil(n / 128)] their scales
  * (scales is not used otherwise).  res, delta and res_out in {TJK_F32,
  * TJK_F16, TJK_BF16}; delta may be NULL.  res_out may alias res or delta only

@@ -228,8 +228,9 @@ struct F8Geom {
 // 2048 x 1024 x 4096, one wave per SIMD: 30.1 us, against 35.0 with the conversions
 // in one piece.  Two waves: 4096^3 117 us (1.17 PFLOP/s, the matrix unit busy for
 // 57% of the cycles at 1.95 GHz), 5430 x 4096 x 1024 with GELU 57 us (36 with the
-// e4m3 MFMAs).  With a long K or few rows a 2-byte output and quantize_f8 are quicker.  Of a K tile there the DMA takes 16% and the conversions 18% beside
-// the products; with neither it is the products' own time.
+// e4m3 MFMAs).  With a long K or few rows a 2-byte output and quantize_f8 are quicker.
+// Of a K tile there the DMA takes 16% and the conversions 18% beside the products; with
+// neither it is the products' own time.
 template <typename G>
 __device__ __forceinline__ void f8_accumulate(char* smem, const F8GemmArgs& p, int m0, int n0,
                                               f32x16 (&acc)[G::FN][G::FM]) {
@@ -591,12 +592,11 @@ __device__ __forceinline__ F8Rows f8_rows(const F8GemmArgs& p, int mw, int nw, i
 // GELU to within 2e-6 of its own value.  gelu_erf's error is absolute, 1.5e-7 |v|,
 // which is 0.4% of GELU(-4) and a quarter of GELU(-6): nothing next to a value
 // of ordinary size, but an e4m3 block whose values all lie there takes its scale
-// from them.  GELU(v) = max(v, 0) - u h, u = |v|,
-// h = erfc(u / sqrt 2) / 2 = exp(-u^2 / 2) R(u); R as a polynomial in
-// t = 1 / (1 + u / 4) without a constant term, fitted for the least largest
-// relative error (3.2e-8) over u >= 0.  exp is the square of 2^-x with 2 x = u^2 log2(e) / 2
-// rounded, corrected by what the rounding left over: x stays above -126 for every
-// result that fp32 holds (a subnormal 2^-2x would be flushed).
+// from them.  GELU(v) = max(v, 0) - u h, u = |v|, h = erfc(u / sqrt 2) / 2 =
+// exp(-u^2 / 2) R(u); R as a polynomial in t = 1 / (1 + u / 4) without a constant term,
+// fitted for the least largest relative error (3.2e-8) over u >= 0.  exp is the square
+// of 2^-x with 2 x = u^2 log2(e) / 2 rounded, corrected by what the rounding left over:
+// 2^-x is a normal number for every result that fp32 holds, 2^-2x would be flushed.
 __device__ __forceinline__ float gelu_low(float v) {
   const float u = fabsf(v), t = __builtin_amdgcn_rcpf(fmaf(u, 0.25f, 1.0f));
   float r = 0.0199038982f;
@@ -811,8 +811,9 @@ __device__ __forceinline__ void f8_store(const F8GemmArgs& p, const f32x16 (&acc
 
 // Outputs in e4m3.  A row's largest magnitude over the wave's 64 columns takes
 // one lane exchange; the two waves of a block of 128 trade theirs through LDS
-// (`red`, BM x WN floats; every wave of the workgroup calls this).  Words are put in rows through `stage` (1024 FM FN bytes of the wave's own),
-// the 16-byte piece c of row r at c ^ x(r).
+// (`red`, BM x WN floats; every wave of the workgroup calls this).  Words are put in
+// rows through `stage` (1024 FM FN bytes of the wave's own), the 16-byte piece c of row
+// r at c ^ x(r).
 template <typename G>
 __device__ __forceinline__ void f8_quantise(const F8GemmArgs& p, const f32x16 (&acc)[G::FN][G::FM], int mw, int nw,
                                             int wm, int wn, int lane, float* red, char* stage) {

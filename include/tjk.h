@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define TJK_ABI_VERSION 11
+#define TJK_ABI_VERSION 12
 
 /* dtypes */
 #define TJK_F32 0
@@ -417,6 +417,125 @@ int tjk_gemm_f8(const void* a, int64_t lda, const float* a_scales, int64_t ld_as
 int tjk_gemm_f8_plan_count(void);
 /* The plan that plan_id -1 takes (host only). */
 int tjk_gemm_f8_default_plan(int64_t m, int64_t n, int64_t k, int out_dtype, int epilogue);
+
+/*
+ * Serving operators: a paged cache of keys and values, and a step of drafted
+ * tokens over it.  No counterpart in the reference, which computes whole
+ * sequences.
+ *
+ * A cache holds `pages` pages of page_size rows (a power of two, 16 to 65536) and
+ * kv_heads heads; row r, head h of page p lies at element p page_stride + h
+ * head_stride + r row_stride of k and of v, head_dim elements of dtype TJK_F16 or
+ * TJK_BF16.  Requires head_dim % 16 == 0, head_dim <= 128, strides that are
+ * multiples of 8, 16-byte aligned k and v, and pages * page_size < 2^31.
+ * Position x of sequence b is row x % page_size of page block_table[b * ld_table + x
+ * / page_size].  An entry that names no page, and positions past table_cols
+ * entries, are never followed: what each call does instead is said there, and it
+ * adds to *index_errors (an int on the device, may be NULL, never reset).
+ *
+ * Trees: a sequence's nodes are rows cu_nodes[b] .. cu_nodes[b + 1] - 1 of the
+ * token arrays, numbered from 0 in each tree, parents before children; node 0
+ * is the last token that is certain.  Counts past max_nodes (<= 64) or the rows
+ * there are cut off; rows that no sequence names are neither read nor written.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t page_stride, head_stride, row_stride; /* elements */
+  int64_t pages;
+  int page_size, kv_heads, head_dim, dtype;
+} tjk_paged_cache;
+
+/*
+ * Queries and keys of `tokens` tokens normalised per head, rotated by their
+ * positions, and keys and values stored in the cache.
+ *   qkv [tokens, heads + 2 kv_heads, head_dim]: the heads' queries, then keys, then
+ *   values (a packed [tokens, 3, heads, head_dim] buffer is one), of dtype.
+ *   x' = x rsqrt(mean(x^2) + eps) gamma     queries with q_gamma, keys with k_gamma
+ *                                           (fp32 [head_dim]; NULL: x' = x)
+ *   y  = the first rot elements of x' turned in pairs (i, i + rot / 2), or with
+ *        interleaved (2 i, 2 i + 1), by the angle whose cosine and sine are
+ *        table[(position * rot / 2 + i) * 2 .. + 1] (fp32); the others as they are
+ * in fp32, rounded once.  Queries go to q_out, keys to k_out (may be NULL) and,
+ * with values, to row slots[t] % page_size of page slots[t] / page_size (cache and
+ * slots may be NULL together).  A negative slot stores nothing.  A position
+ * outside [0, n_positions) makes the token's q_out and k_out rows zero and stores
+ * nothing, a slot past the cache stores nothing; both count in *index_errors.
+ * Two tokens of a call may not share a slot (its row would hold pieces of
+ * either).  q_out may be the queries of qkv and k_out its keys, in place; they may
+ * not overlap qkv otherwise.
+ * Requires rot % 16 == 0, strides that are multiples of 8, and 16-byte aligned
+ * pointers.
+ */
+int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_head, const int32_t* positions,
+                    const float* table, int64_t n_positions, int64_t rot, int interleaved,
+                    void* q_out, int64_t ld_q_token, int64_t ld_q_head,
+                    void* k_out, int64_t ld_k_token, int64_t ld_k_head,
+                    const tjk_paged_cache* cache, const int32_t* slots,
+                    const float* q_gamma, const float* k_gamma, float eps, int* index_errors,
+                    int64_t tokens, int heads, int kv_heads, int head_dim, int dtype, void* stream);
+
+/*
+ * Attention of the trees' nodes: query head h of node i of sequence b attends,
+ * through key head h / (heads / kv_heads), to positions 0 .. ctx_lens[b] - 1 and to
+ * the positions ctx_lens[b] + j of the nodes j whose bit is set in tree_mask[row]
+ * (its own among them, if it is to see itself; NULL: nodes 0 .. i, a chain).
+ *   out[row, h * head_dim ..] = sum_j softmax(scale q . k_j) v_j
+ * Scores, the softmax and the sums over keys are in fp32, the weights given to
+ * the product with the values rounded to the cache's type.  A row that sees
+ * nothing, or only scores of -inf, is zero.  Keys and values that a row does not
+ * see do not reach it, whatever they hold; positions without a page are left
+ * out, and count in *index_errors.
+ * workspace: tjk_tree_attention_bytes() bytes on the device, 16-byte aligned;
+ * calls that share one have to be ordered.
+ * Requires heads % kv_heads == 0, strides that are multiples of 8 and 16-byte
+ * aligned pointers (8 for tree_mask).
+ */
+int tjk_tree_attention(const void* q, int64_t ld_q_token, int64_t ld_q_head,
+                       const tjk_paged_cache* cache, const int32_t* block_table, int64_t ld_table,
+                       int64_t table_cols, const int32_t* ctx_lens, const int32_t* cu_nodes,
+                       const uint64_t* tree_mask, void* out, int64_t ld_out, int64_t tokens,
+                       int batch, int heads, int max_nodes, float scale,
+                       void* workspace, size_t workspace_bytes, int* index_errors, void* stream);
+/* Bytes of workspace that any batch of these sizes needs (0: bad sizes). */
+size_t tjk_tree_attention_bytes(int heads, int kv_heads, int head_dim, int max_nodes);
+
+/*
+ * Verification of drafted tokens.  target and draft [rows, vocab] (fp32) hold for
+ * each node the target's and the draft's distribution of the token behind it;
+ * tokens its token, drawn from the draft's distribution behind its parent;
+ * parents its parent's number (< its own; node 0's is not read); accept_u [rows]
+ * and sample_u [batch] numbers in [0, 1).
+ * From node 0 on, the children of the last accepted node are tried in the order
+ * of their numbers, by rejection sampling: with p and q behind that node,
+ *   r_k = max(p - c_k q, 0), W_k = sum r_k, c_0 = 0, W_0 = 1, c_{k+1} = c_k + W_k,
+ * the k-th child x is accepted if accept_u q(x) W_k < r_k(x).  When none is left,
+ * the next token is the smallest x with r_k(0) + .. + r_k(x) > sample_u sum r_k
+ * (k: the children refused; c_k = 0 if W_k is zero; -1 if p has no weight).  So the
+ * tokens are distributed as the target's.  Products and sums in 64 bits; negative
+ * and NaN weights count as zero.  A child with a token outside [0, vocab) is
+ * refused and counts in *index_errors.
+ * path [batch, max_nodes]: the accepted nodes, node 0 first, then -1; count: how
+ * many; token: the next token.  A sequence without nodes: -1, 0 and -1.
+ */
+int tjk_verify_tree(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
+                    const int32_t* tokens, const int32_t* parents, const float* accept_u,
+                    const float* sample_u, const int32_t* cu_nodes, int32_t* path, int64_t ld_path,
+                    int32_t* count, int32_t* token, int* index_errors, int64_t rows, int64_t vocab,
+                    int batch, int max_nodes, void* stream);
+
+/*
+ * Moves the keys and values of accepted nodes together: position ctx_lens[b] +
+ * path[b, i] to ctx_lens[b] + i for 1 <= i < count[b], in each of `layers` caches
+ * layer_stride elements apart (of k and of v).  path (as tjk_verify_tree writes it)
+ * starts at 0 and increases; an entry below i or past max_nodes, or a position
+ * without a page, moves nothing and counts in *index_errors.  The pages that
+ * nodes lie in belong to one sequence.
+ */
+int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64_t layer_stride,
+                      const int32_t* block_table, int64_t ld_table, int64_t table_cols,
+                      const int32_t* ctx_lens, const int32_t* path, int64_t ld_path, int max_nodes,
+                      const int32_t* count, int* index_errors, int batch, void* stream);
 
 #ifdef __cplusplus
 }

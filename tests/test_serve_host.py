@@ -1,0 +1,283 @@
+"""What the serving operators refuse, through the C-ABI and the Python wrappers
+(no GPU: every call is rejected before a launch), and the rotation's table."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tjkernels import _lib, ops
+from tjkernels._lib import BF16, EINVAL, EUNSUPPORTED, F16, F32, PagedCache, TjkError
+
+FAKE = 1 << 20  # a pointer that is never followed
+
+
+def _cache(**kw):
+    a = dict(k=FAKE, v=FAKE, page_stride=4 * 32 * 64, head_stride=32 * 64, row_stride=64, pages=10, page_size=32, kv_heads=4,
+             head_dim=64, dtype=BF16)
+    a.update(kw)
+    return PagedCache(*a.values())
+
+
+def _call(name, a, kw):
+    cache = {k[6:]: v for k, v in kw.items() if k.startswith("cache_")}
+    a.update({k: v for k, v in kw.items() if not k.startswith("cache_")})
+    if "cache" in a and a["cache"] is not None:
+        a["cache"] = ctypes.byref(_cache(**cache))
+    return getattr(_lib.load(), name)(*a.values())
+
+
+def _append(**kw):
+    return _call("tjk_rope_append", dict(
+        qkv=FAKE, ld_token=1024, ld_head=64, positions=FAKE, table=FAKE, n_positions=100, rot=64, interleaved=0,
+        q_out=FAKE + 4096, ld_q_token=512, ld_q_head=64, k_out=None, ld_k_token=0, ld_k_head=0, cache=1, slots=FAKE,
+        q_gamma=FAKE, k_gamma=None, eps=1e-6, index_errors=None, tokens=5, heads=8, kv_heads=4, head_dim=64, dtype=BF16,
+        stream=None), kw)
+
+
+def _attend(**kw):
+    return _call("tjk_tree_attention", dict(
+        q=FAKE, ld_q_token=512, ld_q_head=64, cache=1, table=FAKE, ld_table=8, table_cols=8, ctx_lens=FAKE, cu_nodes=FAKE,
+        tree_mask=FAKE, out=FAKE, ld_out=512, tokens=5, batch=2, heads=8, max_nodes=4, scale=0.1, workspace=FAKE,
+        workspace_bytes=1 << 40, index_errors=None, stream=None), kw)
+
+
+def _verify(**kw):
+    return _call("tjk_verify_tree", dict(
+        target=FAKE, ld_target=100, draft=FAKE, ld_draft=100, tokens=FAKE, parents=FAKE, accept_u=FAKE, sample_u=FAKE,
+        cu_nodes=FAKE, path=FAKE, ld_path=4, count=FAKE, token=FAKE, index_errors=None, rows=5, vocab=100, batch=2,
+        max_nodes=4, stream=None), kw)
+
+
+def _compact(**kw):
+    return _call("tjk_compact_cache", dict(
+        cache=1, layers=2, layer_stride=1 << 20, table=FAKE, ld_table=8, table_cols=8, ctx_lens=FAKE, path=FAKE, ld_path=4,
+        max_nodes=4, count=FAKE, index_errors=None, batch=2, stream=None), kw)
+
+
+def _said():
+    return _lib.load().tjk_last_error_string().decode()
+
+
+BAD_CACHES = [
+    (dict(cache_k=None), EINVAL, "null"), (dict(cache_v=None), EINVAL, "null"), (dict(cache_dtype=F32), EINVAL, "dtype"),
+    (dict(cache_kv_heads=0), EINVAL, "shape"), (dict(cache_pages=-1), EINVAL, "shape"),
+    (dict(cache_head_dim=72), EUNSUPPORTED, "multiple of 16"), (dict(cache_head_dim=144), EUNSUPPORTED, "128"),
+    (dict(cache_page_size=8), EUNSUPPORTED, "power of two"), (dict(cache_page_size=48), EUNSUPPORTED, "power of two"),
+    (dict(cache_page_size=1 << 17), EUNSUPPORTED, "power of two"),
+    (dict(cache_pages=1 << 26, cache_page_size=32), EUNSUPPORTED, "int32"), (dict(cache_row_stride=56), EINVAL, "strides"),
+    (dict(cache_page_stride=-64), EINVAL, "strides"), (dict(cache_head_stride=100), EUNSUPPORTED, "multiples of 8"),
+    (dict(cache_row_stride=1 << 21), EUNSUPPORTED, "too large"), (dict(cache_k=FAKE + 8), EUNSUPPORTED, "misaligned"),
+]
+
+
+@pytest.mark.parametrize("call", [_append, _attend, _compact])
+@pytest.mark.parametrize("kw,status,word", BAD_CACHES)
+def test_cache_refusals(call, kw, status, word):
+    assert call(**kw) == status and word in _said()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(tokens=-1), EINVAL, "shape"), (dict(heads=0), EINVAL, "shape"), (dict(kv_heads=0), EINVAL, "shape"),
+    (dict(dtype=F32), EINVAL, "dtype"), (dict(dtype=F16), EINVAL, "differ"), (dict(kv_heads=2), EINVAL, "differ"),
+    (dict(head_dim=40), EUNSUPPORTED, "multiple of 16"), (dict(rot=24), EUNSUPPORTED, "rotated"),
+    (dict(rot=80), EUNSUPPORTED, "rotated"), (dict(tokens=1 << 31), EUNSUPPORTED, "large"),
+    (dict(qkv=None), EINVAL, "null"), (dict(positions=None), EINVAL, "null"), (dict(table=None), EINVAL, "null"),
+    (dict(q_out=None), EINVAL, "null"), (dict(slots=None), EINVAL, "null"), (dict(cache=None), EINVAL, "null"),
+    (dict(ld_head=56), EINVAL, "stride"), (dict(ld_q_head=0), EINVAL, "stride"), (dict(ld_token=1020), EUNSUPPORTED, "8"),
+    (dict(ld_q_token=516), EUNSUPPORTED, "8"), (dict(k_out=FAKE + 64, ld_k_head=64, ld_k_token=4), EUNSUPPORTED, "8"),
+    (dict(qkv=FAKE + 8), EUNSUPPORTED, "misaligned"), (dict(table=FAKE + 4), EUNSUPPORTED, "misaligned"),
+    (dict(q_out=FAKE), EINVAL, "in place"), (dict(k_out=FAKE, ld_k_head=64, ld_k_token=1024), EINVAL, "in place"),
+    (dict(k_out=FAKE + 2 * 8 * 64, ld_k_head=64, ld_k_token=256), EINVAL, "in place"),
+])
+def test_append_refusals(kw, status, word):
+    assert _append(**kw) == status and word in _said()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(tokens=-1), EINVAL, "shape"), (dict(batch=-1), EINVAL, "shape"), (dict(heads=0), EINVAL, "shape"),
+    (dict(max_nodes=-1), EINVAL, "shape"), (dict(heads=6), EINVAL, "multiple"), (dict(max_nodes=65), EUNSUPPORTED, "64"),
+    (dict(tokens=1 << 31), EUNSUPPORTED, "large"), (dict(batch=1 << 24), EUNSUPPORTED, "large"),
+    (dict(q=None), EINVAL, "null"), (dict(out=None), EINVAL, "null"), (dict(ctx_lens=None), EINVAL, "null"),
+    (dict(cu_nodes=None), EINVAL, "null"), (dict(table=None), EINVAL, "null"), (dict(ld_table=7), EINVAL, "leading"),
+    (dict(ld_out=504), EINVAL, "leading"), (dict(ld_q_head=56), EINVAL, "leading"),
+    (dict(ld_q_token=513), EUNSUPPORTED, "multiples of 8"), (dict(ld_out=516), EUNSUPPORTED, "multiples of 8"),
+    (dict(q=FAKE + 8), EUNSUPPORTED, "misaligned"), (dict(tree_mask=FAKE + 4), EUNSUPPORTED, "misaligned"),
+    (dict(workspace=FAKE + 8), EUNSUPPORTED, "misaligned"),
+])
+def test_attention_refusals(kw, status, word):
+    assert _attend(**kw) == status and word in _said()
+
+
+def test_attention_refuses_a_small_workspace():
+    need = _lib.load().tjk_tree_attention_bytes(8, 4, 64, 4)
+    if need:
+        assert _attend(workspace_bytes=need - 1) == EINVAL and "workspace" in _said()
+        assert _attend(workspace=None) == EINVAL and "null" in _said()
+    for bad in ((0, 1, 64, 4), (8, 0, 64, 4), (8, 3, 64, 4), (8, 4, 72, 4), (8, 4, 64, 65), (8, 4, 64, 0)):
+        assert _lib.load().tjk_tree_attention_bytes(*bad) == 0
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(rows=-1), EINVAL, "shape"), (dict(vocab=0), EINVAL, "shape"), (dict(batch=-1), EINVAL, "shape"),
+    (dict(max_nodes=0), EINVAL, "shape"), (dict(max_nodes=65, ld_path=65), EUNSUPPORTED, "64"),
+    (dict(vocab=1 << 25, ld_target=1 << 25, ld_draft=1 << 25), EUNSUPPORTED, "large"),
+    (dict(rows=1 << 31), EUNSUPPORTED, "large"), (dict(target=None), EINVAL, "null"), (dict(path=None), EINVAL, "null"),
+    (dict(sample_u=None), EINVAL, "null"), (dict(parents=None), EINVAL, "null"), (dict(ld_draft=99), EINVAL, "leading"),
+    (dict(ld_path=3), EINVAL, "leading"),
+])
+def test_verify_refusals(kw, status, word):
+    assert _verify(**kw) == status and word in _said()
+
+
+@pytest.mark.parametrize("kw,status,word", [
+    (dict(layers=-1), EINVAL, "shape"), (dict(batch=-1), EINVAL, "shape"), (dict(max_nodes=65), EUNSUPPORTED, "64"),
+    (dict(layer_stride=4), EUNSUPPORTED, "8"), (dict(table=None), EINVAL, "null"), (dict(path=None), EINVAL, "null"),
+    (dict(count=None), EINVAL, "null"), (dict(ld_table=7), EINVAL, "leading"), (dict(ld_path=3), EINVAL, "leading"),
+])
+def test_compact_refusals(kw, status, word):
+    assert _compact(**kw) == status and word in _said()
+
+
+def test_nothing_to_do_is_no_error():
+    assert _append(tokens=0, qkv=None) == 0
+    assert _attend(tokens=0, q=None) == 0 and _attend(batch=0, q=None) == 0 and _attend(max_nodes=0, q=None) == 0
+    assert _verify(batch=0, path=None) == 0
+    assert _compact(batch=0, path=None) == 0 and _compact(layers=0) == 0 and _compact(max_nodes=1) == 0
+
+
+# ------------------------------------------------------------ Python wrappers
+
+def _b(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+def _i(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def _py_append(**kw):
+    a = dict(qkv=_b(5, 16, 64), positions=_i(5), table=torch.zeros(100, 32, 2), q_out=_b(5, 8, 64), k_cache=_b(10, 4, 32, 64),
+             v_cache=_b(10, 4, 32, 64), slots=_i(5), k_out=_b(5, 4, 64), q_gamma=torch.ones(64), k_gamma=torch.ones(64))
+    a.update(kw)
+    ops.rope_append(**a)
+
+
+def _py_attend(**kw):
+    a = dict(q=_b(5, 8, 64), k_cache=_b(10, 4, 32, 64), v_cache=_b(10, 4, 32, 64), block_table=_i(2, 8), ctx_lens=_i(2),
+             out=_b(5, 512), cu_nodes=_i(3), max_nodes=4, tree_mask=torch.zeros(5, dtype=torch.int64))
+    a.update(kw)
+    ops.tree_attention(**a)
+
+
+def _py_verify(**kw):
+    a = dict(target=torch.zeros(5, 100), draft=torch.zeros(5, 100), tokens=_i(5), parents=_i(5), accept_u=torch.zeros(5),
+             sample_u=torch.zeros(2), path=_i(2, 4), count=_i(2), token=_i(2), cu_nodes=_i(3))
+    a.update(kw)
+    ops.verify_tree(**a)
+
+
+def _py_compact(**kw):
+    a = dict(k_cache=_b(3, 10, 4, 32, 64), v_cache=_b(3, 10, 4, 32, 64), block_table=_i(2, 8), ctx_lens=_i(2), path=_i(2, 4),
+             count=_i(2))
+    a.update(kw)
+    ops.compact_cache(**a)
+
+
+@pytest.mark.parametrize("call", [_py_append, _py_attend, _py_verify, _py_compact])
+def test_wrappers_take_device_tensors_only(call):
+    with pytest.raises(TjkError, match="device tensors"):
+        call()
+
+
+def test_well_formed_layouts():
+    """Permuted caches, padded rows, single heads, tokens and pages of any
+    stride, no cache, no table, in place: refused last, for the device."""
+    wide = _b(10, 32, 4, 72)
+    packed = _b(5, 3, 4, 64)
+    flat = packed.view(5, 12, 64)
+    for kw in (dict(k_cache=wide[..., :64].transpose(1, 2), v_cache=wide[..., :64].transpose(1, 2)),
+               dict(k_cache=_b(1, 4, 32, 64), v_cache=_b(3, 4, 32, 64)[::3]), dict(k_out=None), dict(table=None),
+               dict(k_cache=None, v_cache=None, slots=None), dict(q_gamma=None), dict(q_out=_b(9, 8, 80)[:7, :, :64]),
+               dict(qkv=flat, q_out=flat[:, :4], k_out=flat[:, 4:8]),
+               dict(qkv=_b(5, 3, 64), q_out=_b(5, 1, 64), k_out=_b(5, 1, 64), k_cache=_b(10, 1, 32, 64),
+                    v_cache=_b(10, 1, 32, 64))):
+        with pytest.raises(TjkError, match="device tensors"):
+            _py_append(**kw)
+    for kw in (dict(tree_mask=None), dict(q=_b(5, 16, 64)[:, ::2]), dict(out=_b(9, 600)[2:, :512]),
+               dict(block_table=_i(2, 16)[:, :3]), dict(workspace=torch.zeros(1 << 27, dtype=torch.uint8))):
+        with pytest.raises(TjkError, match="device tensors"):
+            _py_attend(**kw)
+    for kw in (dict(target=torch.zeros(5, 128)[:, :100]), dict(path=_i(2, 9)[:, :4])):
+        with pytest.raises(TjkError, match="device tensors"):
+            _py_verify(**kw)
+    for kw in (dict(k_cache=_b(10, 4, 32, 64), v_cache=_b(10, 4, 32, 64)), dict(path=_i(2, 9)[:, :4])):
+        with pytest.raises(TjkError, match="device tensors"):
+            _py_compact(**kw)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(qkv=_b(5, 1024)), "qkv must be"), (dict(qkv=_b(5, 64, 16).transpose(1, 2)), "qkv must be"),
+    (dict(qkv=torch.zeros(5, 16, 64, dtype=torch.float64)), "dtype"), (dict(q_out=_b(5, 16, 64)), "left"),
+    (dict(q_out=_b(5, 7, 64)), "left"), (dict(q_out=_b(4, 8, 64)), "q_out must be"), (dict(q_out=_b(5, 8, 32)), "q_out"),
+    (dict(q_out=torch.zeros(5, 8, 64, dtype=torch.float16)), "q_out"), (dict(k_out=_b(5, 3, 64)), "k_out"),
+    (dict(positions=_i(4)), "positions"), (dict(positions=torch.zeros(5, dtype=torch.int64)), "positions"),
+    (dict(table=torch.zeros(100, 64)), "table"), (dict(table=torch.zeros(100, 2, 32).transpose(1, 2)), "table"),
+    (dict(table=_b(100, 32, 2)), "table"), (dict(slots=None), "together"), (dict(v_cache=None), "together"),
+    (dict(slots=_i(6)), "slots"), (dict(k_cache=_b(10, 4, 16, 64)), "differ"),
+    (dict(k_cache=_b(10, 32, 4, 64).transpose(1, 2)), "strides"), (dict(k_cache=_b(1, 10, 4, 32, 64)), "k_cache must be"),
+    (dict(q_gamma=torch.ones(32)), "q_gamma"), (dict(k_gamma=_b(64)), "k_gamma"),
+    (dict(index_errors=torch.zeros(1)), "index_errors"), (dict(qkv=None), "must be a tensor"),
+])
+def test_append_wrapper_refusals(kw, word):
+    with pytest.raises(TjkError, match=word):
+        _py_append(**kw)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(q=_b(5, 8, 32)), "differ"), (dict(q=torch.zeros(5, 8, 64, dtype=torch.float16)), "differ"),
+    (dict(out=_b(5, 256)), "out must be"), (dict(out=_b(4, 512)), "out must be"), (dict(out=torch.zeros(5, 512)), "out must be"),
+    (dict(block_table=_i(2, 8).long()), "block_table"), (dict(block_table=_i(8, 2).t()), "block_table"),
+    (dict(ctx_lens=_i(3)), "ctx_lens"), (dict(cu_nodes=_i(2)), "cu_nodes"), (dict(tree_mask=_i(5)), "tree_mask"),
+    (dict(tree_mask=torch.zeros(6, dtype=torch.int64)), "tree_mask"), (dict(max_nodes=1 << 33, workspace=_i(4)), "max_nodes"),
+    (dict(workspace=torch.zeros(4, 4).t()), "workspace"), (dict(index_errors=_i(0)), "index_errors"),
+])
+def test_attention_wrapper_refusals(kw, word):
+    with pytest.raises(TjkError, match=word):
+        _py_attend(**kw)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(target=_b(5, 100)), "target"), (dict(draft=torch.zeros(5, 99)), "differ"), (dict(draft=torch.zeros(4, 100)), "differ"),
+    (dict(target=torch.zeros(100, 5).t()), "target"), (dict(tokens=_i(4)), "tokens"), (dict(parents=_i(5).long()), "parents"),
+    (dict(accept_u=torch.zeros(5, dtype=torch.float64)), "accept_u"), (dict(sample_u=torch.zeros(3)), "sample_u"),
+    (dict(path=_i(4, 2).t()), "path"), (dict(count=_i(3)), "count"), (dict(token=_i(2).long()), "token"),
+    (dict(cu_nodes=_i(4)), "cu_nodes"),
+])
+def test_verify_wrapper_refusals(kw, word):
+    with pytest.raises(TjkError, match=word):
+        _py_verify(**kw)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(k_cache=_b(3, 10, 4, 32, 64)[:2]), "differ"), (dict(k_cache=_b(1, 3, 10, 4, 32, 64)), "k_cache must be"),
+    (dict(path=_i(3, 4)), "path"), (dict(count=_i(3)), "count"), (dict(ctx_lens=_i(1)), "ctx_lens"),
+])
+def test_compact_wrapper_refusals(kw, word):
+    with pytest.raises(TjkError, match=word):
+        _py_compact(**kw)
+
+
+def test_rope_table():
+    t = ops.rope_table(100000, 64, 500.0)
+    assert t.shape == (100000, 32, 2) and t.dtype == torch.float32 and t.is_contiguous()
+    x = torch.tensor([0, 1, 77, 99999], dtype=torch.float64)
+    for i in (0, 5, 31):
+        angle = x * 500.0 ** (-2 * i / 64)
+        got = t[x.long(), i].double()
+        # a step of the table, and the error of the 64-bit angle itself
+        assert (got[:, 0] - angle.cos()).abs().max() <= 2.0 ** -25 + 1e-10
+        assert (got[:, 1] - angle.sin()).abs().max() <= 2.0 ** -25 + 1e-10
+    assert ops.rope_table(7, 0).shape == (7, 0, 2)
+    with pytest.raises(TjkError, match="pairs"):
+        ops.rope_table(8, 7)

@@ -1,0 +1,300 @@
+// Writing the paged cache: tokens' keys and values appended, with the norms
+// and the position rotation on the way, and the rows of accepted tokens moved
+// together.
+
+#include "paged_cache.h"
+
+namespace tjk {
+
+int check_cache(const char* who, const tjk_paged_cache* c) {
+  if (!c || !c->k || !c->v) return fail(TJK_EINVAL, "%s: null cache", who);
+  if (c->dtype != TJK_F16 && c->dtype != TJK_BF16) return fail(TJK_EINVAL, "%s: bad cache dtype %d", who, c->dtype);
+  if (c->kv_heads <= 0 || c->pages < 0 || c->head_dim <= 0)
+    return fail(TJK_EINVAL, "%s: bad cache shape pages=%lld kv_heads=%d head_dim=%d", who, (long long)c->pages, c->kv_heads,
+                c->head_dim);
+  if (c->head_dim % 16 || c->head_dim > 128)
+    return fail(TJK_EUNSUPPORTED, "%s: head_dim=%d must be a multiple of 16 and <= 128", who, c->head_dim);
+  if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
+    return fail(TJK_EUNSUPPORTED, "%s: page_size=%d must be a power of two from 16 to 65536", who, c->page_size);
+  if (c->pages * c->page_size > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: the cache's rows exceed int32", who);
+  if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < c->head_dim)
+    return fail(TJK_EINVAL, "%s: bad cache strides", who);
+  if (c->page_stride % 8 || c->head_stride % 8 || c->row_stride % 8)
+    return fail(TJK_EUNSUPPORTED, "%s: cache strides must be multiples of 8", who);
+  if (c->row_stride > 1 << 20 || c->row_stride * c->page_size > 1 << 29)
+    return fail(TJK_EUNSUPPORTED, "%s: cache row stride %lld is too large", who, (long long)c->row_stride);
+  if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return fail(TJK_EUNSUPPORTED, "%s: misaligned cache", who);
+  return TJK_OK;
+}
+
+// ------------------------------------------------------------- append
+//
+// One head of one token belongs to G neighbouring lanes (G the power of two from
+// head_dim / 16 up); each holds two 8-element pieces, those that the rotation
+// brings together: pieces p and p + rot / 16 of the halves' form (element i
+// turns with i + rot / 2), and past the rotated ones neighbours.  The norm sums
+// over the G lanes.
+
+struct AppendArgs {
+  const char* qkv;
+  int64_t token_bytes, head_bytes;
+  const int32_t* positions;
+  const float* table;
+  int n_positions;
+  int rot8;  // rotated pieces
+  char* q_out;
+  int64_t q_token_bytes, q_head_bytes;
+  char* k_out;
+  int64_t k_token_bytes, k_head_bytes;
+  Paged cache;
+  const int32_t* slots;
+  const float* q_gamma;
+  const float* k_gamma;
+  float eps;
+  int* index_errors;
+  int64_t tokens;
+  int heads, kv_heads, hd8;  // hd8: pieces of a head
+};
+
+// Sum over groups of G lanes (G <= 8, a power of two), in each of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (G >= 2)
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+  if constexpr (G >= 4)
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+  if constexpr (G >= 8)
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true));
+  return v;
+}
+
+template <typename T, int G, bool INTER>
+__global__ __launch_bounds__(256) void rope_append_kernel(AppendArgs a) {
+  constexpr int HPW = 64 / G;  // heads of a wave
+  const int lane = threadIdx.x & 63, g = lane / G, p = lane % G;
+  const int all = a.heads + 2 * a.kv_heads;
+  const int blocks = (all + HPW - 1) / HPW;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t t = wave / blocks;
+  const int h = (int)(wave - t * blocks) * HPW + g;
+  if (t >= a.tokens) return;
+  const int pos = a.positions[t];
+  const bool placed = pos >= 0 && pos < a.n_positions;
+  int slot = a.slots ? a.slots[t] : -1;
+  const bool stored = placed && slot >= 0 && (slot >> a.cache.shift) < a.cache.pages;
+  if (h == 0 && p == 0 && a.index_errors && (!placed || (slot >= 0 && !stored))) atomicAdd(a.index_errors, 1);
+  const bool in = h < all && 2 * p < a.hd8;
+  const int half = a.rot8 >> 1;
+  const bool turned = p < half;
+  const int c0 = turned && !INTER ? p : 2 * p, c1 = turned && !INTER ? p + half : 2 * p + 1;
+
+  float x[2][8];
+  const T* const src =
+      reinterpret_cast<const T*>(a.qkv + t * a.token_bytes + (int64_t)(in ? h : 0) * a.head_bytes);
+  Oct<T>::to(Oct<T>::load(src + 8 * (in ? c0 : 0)), x[0]);
+  Oct<T>::to(Oct<T>::load(src + 8 * (in ? c1 : 0)), x[1]);
+  if (h < a.heads + a.kv_heads) {
+    const float* const gamma = h < a.heads ? a.q_gamma : a.k_gamma;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i], x[u][i], sum);
+    sum = group_sum<G>(in ? sum : 0.f);
+    if (gamma && in) {
+      const float r = 1.0f / sqrtf(sum / (float)(8 * a.hd8) + a.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[0][i] *= r * gamma[8 * c0 + i];
+        x[1][i] *= r * gamma[8 * c1 + i];
+      }
+    }
+    if (turned && placed && in) {
+      const float2* const cs = reinterpret_cast<const float2*>(a.table) + (int64_t)pos * (4 * a.rot8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // the pair's members: element i of both pieces, or elements 2 j, 2 j + 1 of one
+        float &u = INTER ? x[i >> 2][2 * (i & 3)] : x[0][i], &v = INTER ? x[i >> 2][2 * (i & 3) + 1] : x[1][i];
+        const float2 w = cs[8 * p + i];
+        const float y = u * w.x - v * w.y;
+        v = v * w.x + u * w.y;
+        u = y;
+      }
+    }
+  }
+  if (!in) return;
+  if (!placed) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[0][i] = x[1][i] = 0.f;
+  }
+  auto put = [&](char* row) {
+    reinterpret_cast<uint4*>(row)[c0] = Oct<T>::from(x[0]);
+    reinterpret_cast<uint4*>(row)[c1] = Oct<T>::from(x[1]);
+  };
+  const int kh = h < a.heads + a.kv_heads ? h - a.heads : h - a.heads - a.kv_heads;
+  if (h < a.heads) {
+    put(a.q_out + t * a.q_token_bytes + h * a.q_head_bytes);
+    return;
+  }
+  const bool key = h < a.heads + a.kv_heads;
+  if (key && a.k_out) put(a.k_out + t * a.k_token_bytes + kh * a.k_head_bytes);
+  if (stored)
+    put((key ? a.cache.k : a.cache.v) + (int64_t)(slot >> a.cache.shift) * a.cache.page_bytes + kh * a.cache.head_bytes +
+        (int64_t)(slot & ((1 << a.cache.shift) - 1)) * a.cache.row_bytes);
+}
+
+// ------------------------------------------------------------ compaction
+//
+// A wave moves the rows of one (layer, sequence, head, keys or values), a
+// lane one 16-byte piece of a row: in batches, loads ahead of stores.  Row
+// path[i] >= i goes to row i, so no row is overwritten before it is read.
+
+struct CompactArgs {
+  Paged cache;
+  int64_t layer_bytes;
+  const int32_t* table;
+  int64_t ld_table;
+  int table_cols;
+  const int32_t* ctx_lens;
+  const int32_t* path;
+  int64_t ld_path;
+  int max_nodes;
+  const int32_t* count;
+  int* index_errors;
+  int layers, batch, kv_heads, hd8;
+};
+
+template <int CPR>  // lanes per row
+__global__ __launch_bounds__(256) void compact_kernel(CompactArgs a) {
+  constexpr int RPI = 64 / CPR, U = 4;
+  const int lane = threadIdx.x & 63, r = lane / CPR, c = lane % CPR;
+  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int per = 2 * a.kv_heads;
+  const int64_t lb = wave / per;
+  const int hk = (int)(wave - lb * per);
+  const int layer = (int)(lb / a.batch), b = (int)(lb - (int64_t)layer * a.batch);
+  if (layer >= a.layers) return;
+  const int n = min(a.count[b], a.max_nodes);
+  const int ctx = max(a.ctx_lens[b], 0);
+  char* const base = ((hk & 1) ? a.cache.v : a.cache.k) + layer * a.layer_bytes + (hk >> 1) * a.cache.head_bytes;
+  const int32_t* const row = a.table + b * a.ld_table;
+  const int mask = (1 << a.cache.shift) - 1;
+  auto place = [&](int64_t x) -> char* {  // row of position x, null outside the cache
+    if (x >= (int64_t)a.table_cols << a.cache.shift) return nullptr;
+    const int pg = page_of(row, (int)(x >> a.cache.shift), a.cache.pages);
+    return pg < 0 ? nullptr : base + pg * a.cache.page_bytes + (x & mask) * (int64_t)a.cache.row_bytes;
+  };
+  for (int i0 = 1; i0 < n; i0 += U * RPI) {
+    uint4 v[U];
+    char* dst[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * RPI + r;
+      dst[u] = nullptr;
+      if (i < n && c < a.hd8) {
+        const int from = a.path[b * a.ld_path + i];
+        const char* const src = from >= i && from < a.max_nodes ? place((int64_t)ctx + from) : nullptr;
+        dst[u] = src ? place((int64_t)ctx + i) : nullptr;
+        if (dst[u]) v[u] = reinterpret_cast<const uint4*>(src)[c];
+        else if (layer == 0 && hk == 0 && c == 0 && a.index_errors) atomicAdd(a.index_errors, 1);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (dst[u]) reinterpret_cast<uint4*>(dst[u])[c] = v[u];
+  }
+}
+
+}  // namespace tjk
+
+using namespace tjk;
+
+extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_head, const int32_t* positions,
+                               const float* table, int64_t n_positions, int64_t rot, int interleaved, void* q_out,
+                               int64_t ld_q_token, int64_t ld_q_head, void* k_out, int64_t ld_k_token, int64_t ld_k_head,
+                               const tjk_paged_cache* cache, const int32_t* slots, const float* q_gamma,
+                               const float* k_gamma, float eps, int* index_errors, int64_t tokens, int heads, int kv_heads,
+                               int head_dim, int dtype, void* stream) {
+  const char* const who = "tjk_rope_append";
+  if (tokens < 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || n_positions < 0 || rot < 0)
+    return fail(TJK_EINVAL, "%s: bad shape tokens=%lld heads=%d kv_heads=%d head_dim=%d", who, (long long)tokens, heads,
+                kv_heads, head_dim);
+  if (dtype != TJK_F16 && dtype != TJK_BF16) return fail(TJK_EINVAL, "%s: bad dtype %d", who, dtype);
+  if (head_dim % 16 || head_dim > 128)
+    return fail(TJK_EUNSUPPORTED, "%s: head_dim=%d must be a multiple of 16 and <= 128", who, head_dim);
+  if (rot % 16 || rot > head_dim)
+    return fail(TJK_EUNSUPPORTED, "%s: %lld rotated elements must be a multiple of 16 and <= head_dim", who, (long long)rot);
+  if (heads > 65536 || kv_heads > 65536 || tokens > INT32_MAX || n_positions > INT32_MAX)
+    return fail(TJK_EUNSUPPORTED, "%s: too large", who);
+  if (cache) {
+    if (const int bad = check_cache(who, cache)) return bad;
+    if (cache->dtype != dtype || cache->kv_heads != kv_heads || cache->head_dim != head_dim)
+      return fail(TJK_EINVAL, "%s: the cache's dtype, heads or head_dim differ", who);
+  }
+  if (tokens == 0) return TJK_OK;
+  if (!qkv || !positions || !q_out || (rot > 0 && !table) || (!cache != !slots))
+    return fail(TJK_EINVAL, "%s: null pointer", who);
+  if (ld_head < head_dim || ld_q_head < head_dim || (k_out && ld_k_head < head_dim) || ld_token < 0 || ld_q_token < 0 ||
+      (k_out && ld_k_token < 0))
+    return fail(TJK_EINVAL, "%s: stride too small", who);
+  if (ld_token % 8 || ld_head % 8 || ld_q_token % 8 || ld_q_head % 8 || (k_out && (ld_k_token % 8 || ld_k_head % 8)))
+    return fail(TJK_EUNSUPPORTED, "%s: strides must be multiples of 8", who);
+  if ((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)table | (uintptr_t)q_gamma | (uintptr_t)k_gamma) & 15))
+    return fail(TJK_EUNSUPPORTED, "%s: misaligned pointer", who);
+  // a lane writes what it has read, as long as it lies in the same place
+  const char* const keys = static_cast<const char*>(qkv) + 2 * heads * ld_head;
+  if ((q_out == qkv && (ld_q_token != ld_token || ld_q_head != ld_head)) ||
+      (k_out && ((k_out == keys && (ld_k_token != ld_token || ld_k_head != ld_head)) || k_out == qkv)))
+    return fail(TJK_EINVAL, "%s: outputs may alias qkv only in place", who);
+  AppendArgs a{static_cast<const char*>(qkv), 2 * ld_token, 2 * ld_head, positions, table, (int)n_positions, (int)rot / 8,
+               static_cast<char*>(q_out), 2 * ld_q_token, 2 * ld_q_head, static_cast<char*>(k_out), 2 * ld_k_token,
+               2 * ld_k_head, cache ? paged(*cache) : Paged{}, slots, q_gamma, k_gamma, eps, index_errors, tokens, heads,
+               kv_heads, head_dim / 8};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  auto go = [&](auto elem, auto group, auto inter) -> int {
+    typedef decltype(elem) T;
+    constexpr int G = decltype(group)::value;
+    const int64_t blocks = (heads + 2 * (int64_t)kv_heads + 64 / G - 1) / (64 / G);
+    const int64_t grid = (tokens * blocks + 3) / 4;
+    if (grid > UINT32_MAX / 256) return fail(TJK_EUNSUPPORTED, "%s: %lld tokens are too many", who, (long long)tokens);
+    rope_append_kernel<T, G, decltype(inter)::value><<<(unsigned)grid, 256, 0, s>>>(a);
+    return check_launch(who);
+  };
+  auto with_group = [&](auto elem, auto inter) -> int {
+    if (head_dim <= 16) return go(elem, std::integral_constant<int, 1>{}, inter);
+    if (head_dim <= 32) return go(elem, std::integral_constant<int, 2>{}, inter);
+    if (head_dim <= 64) return go(elem, std::integral_constant<int, 4>{}, inter);
+    return go(elem, std::integral_constant<int, 8>{}, inter);
+  };
+  auto with_form = [&](auto elem) -> int {
+    return interleaved ? with_group(elem, std::true_type{}) : with_group(elem, std::false_type{});
+  };
+  return dtype == TJK_F16 ? with_form(f16(0)) : with_form(bf16(0));
+}
+
+extern "C" int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64_t layer_stride, const int32_t* block_table,
+                                 int64_t ld_table, int64_t table_cols, const int32_t* ctx_lens, const int32_t* path,
+                                 int64_t ld_path, int max_nodes, const int32_t* count, int* index_errors, int batch,
+                                 void* stream) {
+  const char* const who = "tjk_compact_cache";
+  if (const int bad = check_cache(who, cache)) return bad;
+  if (layers < 0 || batch < 0 || max_nodes < 0 || table_cols < 0)
+    return fail(TJK_EINVAL, "%s: bad shape layers=%d batch=%d max_nodes=%d", who, layers, batch, max_nodes);
+  if (max_nodes > 64) return fail(TJK_EUNSUPPORTED, "%s: max_nodes=%d exceeds 64", who, max_nodes);
+  if (table_cols > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: block table too wide", who);
+  if (layers > 1 && (layer_stride < 0 || layer_stride % 8))
+    return fail(TJK_EUNSUPPORTED, "%s: the layers' stride must be a multiple of 8", who);
+  if (layers == 0 || batch == 0 || max_nodes < 2) return TJK_OK;
+  if (!block_table || !ctx_lens || !path || !count) return fail(TJK_EINVAL, "%s: null pointer", who);
+  if (ld_table < table_cols || ld_path < max_nodes) return fail(TJK_EINVAL, "%s: leading dimension too small", who);
+  const int64_t waves = (int64_t)layers * batch * 2 * cache->kv_heads;
+  if ((waves + 3) / 4 > UINT32_MAX / 256) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
+  const CompactArgs a{paged(*cache), 2 * layer_stride, block_table, ld_table, (int)table_cols, ctx_lens, path, ld_path,
+                      max_nodes, count, index_errors, layers, batch, cache->kv_heads, cache->head_dim / 8};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const unsigned grid = (unsigned)((waves + 3) / 4);
+  if (cache->head_dim <= 32) compact_kernel<4><<<grid, 256, 0, s>>>(a);
+  else if (cache->head_dim <= 64) compact_kernel<8><<<grid, 256, 0, s>>>(a);
+  else compact_kernel<16><<<grid, 256, 0, s>>>(a);
+  return check_launch(who);
+}

@@ -16,7 +16,8 @@ import torch  # noqa: F401  (must precede the library load; see module docstring
 
 LIB_PATH = Path(__file__).with_name("libtjk.so")
 F8_PATH = Path(__file__).with_name("_f8.so")
-ABI_VERSION = 11
+SERVE_PATH = Path(__file__).with_name("_serve.so")
+ABI_VERSION = 12
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
 OK, EINVAL, EUNSUPPORTED = 0, -1, -2
@@ -27,6 +28,16 @@ DTYPE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _lib = None
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
+
+
+class PagedCache(ctypes.Structure):
+    """tjk_paged_cache."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
+                ("pages", _i64), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32)]
+
+
+_cache = ctypes.POINTER(PagedCache)
 
 _SIGNATURES = {
     "tjk_abi_version": (_i32, []),
@@ -68,6 +79,14 @@ _SIGNATURES = {
                            _i64, _i32, _i32, _vp]),
     "tjk_gemm_f8_plan_count": (_i32, []),
     "tjk_gemm_f8_default_plan": (_i32, [_i64, _i64, _i64, _i32, _i32]),
+    "tjk_rope_append": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _cache,
+                               _vp, _vp, _vp, _f32, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "tjk_tree_attention": (_i32, [_vp, _i64, _i64, _cache, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32,
+                                  _i32, _f32, _vp, ctypes.c_size_t, _vp, _vp]),
+    "tjk_tree_attention_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32]),
+    "tjk_verify_tree": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64,
+                               _i32, _i32, _vp]),
+    "tjk_compact_cache": (_i32, [_cache, _i32, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
@@ -99,15 +118,27 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+def _require_built(path: Path) -> None:
+    load()
+    if not path.exists():
+        raise TjkError(f"{path} is not built: run `make -C {LIB_PATH.parent.parent / 'csrc'}` "
+                       "or __graft_entry__.build(); tjkernels has no non-HIP fallback")
+
+
 def load_f8():
     """Import (once) the Python calls of the 8-bit operators, which go past
     ctypes; raises if they are not built."""
-    load()
-    if not F8_PATH.exists():
-        raise TjkError(f"{F8_PATH} is not built: run `make -C {LIB_PATH.parent.parent / 'csrc'}` "
-                       "or __graft_entry__.build(); tjkernels has no non-HIP fallback")
+    _require_built(F8_PATH)
     from . import _f8
     return _f8
+
+
+def load_serve():
+    """Import (once) the Python calls of the serving operators, which go past
+    ctypes; raises if they are not built."""
+    _require_built(SERVE_PATH)
+    from . import _serve
+    return _serve
 
 
 def check(status: int, what: str) -> None:

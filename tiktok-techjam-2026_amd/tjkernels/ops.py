@@ -471,3 +471,122 @@ def gemm_plans(dtype: torch.dtype):
                                      ctypes.byref(kg)), "tjk_gemm_plan_info")
         out.append((i, bm.value, bn.value, wv.value, kg.value))
     return out
+
+
+_serve_calls = None
+
+
+def _serve():
+    """The serving operators' calls (csrc/binding_serve.cpp): they check the
+    tensors and launch, raising TjkError."""
+    global _serve_calls
+    if _serve_calls is None:
+        _serve_calls = _lib.load_serve()
+    return _serve_calls
+
+
+def rope_table(positions: int, rotated: int, base: float = 10000.0,
+               device: Optional[torch.device] = None) -> torch.Tensor:
+    """fp32 [positions, rotated / 2, 2]: cosine and sine of position * base^(-2 i /
+    rotated), computed in 64 bits (in 32 the angles of far positions are off by
+    more than a step of the table)."""
+    if rotated < 0 or rotated % 2:
+        raise TjkError(f"rope_table: {rotated} rotated elements are no whole pairs")
+    freq = float(base) ** (-torch.arange(0, rotated, 2, dtype=torch.float64) / max(rotated, 1))
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * freq
+    return torch.stack([angle.cos(), angle.sin()], dim=-1).float().contiguous().to(device)
+
+
+def rope_append(qkv: torch.Tensor, positions: torch.Tensor, table: Optional[torch.Tensor], q_out: torch.Tensor,
+                k_cache: Optional[torch.Tensor] = None, v_cache: Optional[torch.Tensor] = None,
+                slots: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                q_gamma: Optional[torch.Tensor] = None, k_gamma: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                interleaved: bool = False, index_errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Queries and keys normalised per head (RMS, ``q_gamma`` / ``k_gamma`` fp32
+    [hd], optional), rotated by their positions, and keys and values appended to
+    a paged cache, in one pass.
+
+    ``qkv`` [T, heads + 2 kv_heads, hd] holds queries, keys and values of T
+    tokens (``qkv.view(T, 3 * H, hd)`` of a packed buffer); ``positions`` int32
+    [T] index ``table`` (``rope_table``; None: no rotation), which turns the
+    first 2 * table.shape[1] elements of a head, element i with i + half, or
+    2 i with 2 i + 1 when ``interleaved``.  ``q_out`` [T, heads, hd] receives the
+    queries, ``k_out`` [T, kv_heads, hd] (optional) the keys: they may be the
+    views of ``qkv`` itself, as ``flash_attention`` reads them.
+
+    ``k_cache`` and ``v_cache`` are [pages, kv_heads, page_size, hd] with a
+    page_size that is a power of two from 16 up; ``slots`` int32 [T] (page *
+    page_size + row, all different) says where each token goes, a negative one
+    that it goes nowhere.  Without a cache only q_out and k_out are written.  A
+    position outside the table gives zero rows and stores nothing, a slot
+    outside the cache stores nothing; both count in ``index_errors``."""
+    _serve().rope_append(qkv, positions, table, q_out, k_cache, v_cache, slots, k_out, q_gamma, k_gamma, eps,
+                         interleaved, index_errors)
+    return q_out
+
+
+def tree_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, max_nodes: int) -> torch.Tensor:
+    """The workspace of ``tree_attention`` for any batch with these heads and
+    trees of at most max_nodes nodes; calls that share one have to be ordered."""
+    need = _lib.load().tjk_tree_attention_bytes(q.shape[1], k_cache.shape[1], q.shape[2], int(max_nodes))
+    return torch.empty(need, dtype=torch.uint8, device=q.device)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   ctx_lens: torch.Tensor, out: torch.Tensor, cu_nodes: torch.Tensor, max_nodes: int,
+                   tree_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   workspace: Optional[torch.Tensor] = None,
+                   index_errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted tokens over a paged cache: ``q`` [T, heads, hd] holds
+    the nodes of B trees back to back (``cu_nodes`` int32 [B+1], at most
+    ``max_nodes`` <= 64 each), ``out`` is [T, heads * hd].
+
+    Sequence b has ``ctx_lens[b]`` tokens in the cache (``block_table`` int32 [B,
+    pages of a sequence]) and its nodes' keys and values at the positions behind
+    them (``rope_append`` puts them there).  A node sees those tokens and the
+    nodes j whose bit is set in its ``tree_mask`` (int64 [T]: the nodes on its
+    path, itself among them); without a mask the nodes up to itself, a chain: with
+    one node per sequence this is the attention of single tokens.  heads may be a
+    multiple of the cache's kv_heads.
+
+    A row that sees nothing is zero; what a row does not see does not reach it,
+    whatever it holds.  Positions without a page are left out and counted in
+    ``index_errors``.  ``workspace`` (``tree_attention_workspace``) is allocated
+    when it is not given."""
+    if workspace is None:
+        workspace = tree_attention_workspace(q, k_cache, max_nodes)
+    _serve().tree_attention(q, k_cache, v_cache, block_table, ctx_lens, out, cu_nodes, max_nodes, tree_mask,
+                            q.shape[2] ** -0.5 if scale is None else scale, workspace, index_errors)
+    return out
+
+
+def verify_tree(target: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
+                accept_u: torch.Tensor, sample_u: torch.Tensor, path: torch.Tensor, count: torch.Tensor,
+                token: torch.Tensor, cu_nodes: torch.Tensor, index_errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Verifies drafted tokens against the target's probabilities, so that the
+    tokens kept are distributed as the target's.
+
+    ``target`` and ``draft`` fp32 [T, vocab] hold for each node the two models'
+    distributions of the token behind it, ``tokens`` int32 [T] its token (drawn
+    from ``draft`` at its parent), ``parents`` int32 [T] its parent's number in
+    the tree (smaller than its own; node 0's is not read).  From node 0 the
+    children of the last accepted node are tried in order by rejection sampling
+    with ``accept_u`` fp32 [T]; when none is left the next token is drawn from
+    the residual distribution with ``sample_u`` fp32 [B], the lowest that passes.
+
+    Writes ``path`` int32 [B, max_nodes <= 64] (the accepted nodes, 0 first, then
+    -1), ``count`` int32 [B] and ``token`` int32 [B] (-1 without any weight)."""
+    _serve().verify_tree(target, draft, tokens, parents, accept_u, sample_u, path, count, token, cu_nodes, index_errors)
+    return token
+
+
+def compact_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, ctx_lens: torch.Tensor,
+                  path: torch.Tensor, count: torch.Tensor, index_errors: Optional[torch.Tensor] = None) -> None:
+    """Moves the keys and values of accepted nodes together, in place: position
+    ctx_lens[b] + path[b, i] to ctx_lens[b] + i for 1 <= i < count[b] (``path`` and
+    ``count`` as ``verify_tree`` writes them), after which the sequence has
+    ctx_lens[b] + count[b] tokens.  The caches are [pages, kv_heads, page_size, hd],
+    or [layers, pages, kv_heads, page_size, hd] for all layers in one launch.  An
+    entry that no tree can have, or a position without a page, moves nothing and
+    counts in ``index_errors``."""
+    _serve().compact_cache(k_cache, v_cache, block_table, ctx_lens, path, count, index_errors)

@@ -5,6 +5,10 @@
 // positions c .. c + n - 1.  A node sees all of the c tokens and the nodes that
 // its mask names.  Query head h reads key head h / (heads / kv_heads).
 
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
 #include "paged_cache.h"
 
 namespace tjk {
@@ -15,17 +19,19 @@ struct TreeArgs {
   Paged cache;
   const int32_t* table;
   int64_t ld_table;
-  int table_cols;
   const int32_t* ctx_lens;
   const int32_t* cu_nodes;
   const uint64_t* mask;
   char* out;
   int64_t out_bytes;  // of a row
-  float scale;  // with log2(e): scores are exponents of 2
+  float scale;  // its size, with log2(e): scores are exponents of 2
   float* parts;  // workspace: two partial results per workgroup
   int* index_errors;
-  int64_t tokens;
-  int batch, kv_heads, group, hd8, max_nodes;
+  uint32_t flip;  // the signs of two queries' elements, if the scale is negative
+  int room;       // positions that the block table holds
+  int tokens, batch, kv_heads, group, hd8, max_nodes;
+  int most_mbs;   // row blocks of the largest tree
+  int direct;     // an item is one workgroup's
 };
 
 // ---------------------------------------------------------------- work
@@ -42,94 +48,82 @@ constexpr int kTile = 32;     // keys of a tile
 constexpr int kMinTiles = 8;  // least tiles of a workgroup: below, the joining costs more than the splitting gives
 
 struct Seq {
-  int b, n, mbs;       // sequence, its nodes, its row blocks
-  int64_t first;       // its first row
-  int64_t ctx, end;    // tokens behind it, positions that it sees
-  int64_t tiles;       // of an item
-  int64_t before;      // tiles before it
+  int b, n, mbs;  // sequence, its nodes, its row blocks
+  int first;      // its first row
+  int ctx, end;   // tokens behind it, positions that it sees
+  int tiles;      // of an item
+  int before;     // tiles before it
 };
 
-// A lane's sequence b (< batch): everything but `before`.
-__device__ __forceinline__ Seq lane_seq(const TreeArgs& a, int b, int rows) {
+// Sequence b (< batch, else nothing): everything but `before`.
+__device__ __forceinline__ Seq load_seq(const TreeArgs& a, int b, int rows) {
   Seq q{};
   q.b = b;
   if (b < a.batch) {
-    const int lo = max(a.cu_nodes[b], 0), hi = a.cu_nodes[b + 1];
+    const int lo = max(a.cu_nodes[b], 0), hi = max(a.cu_nodes[b + 1], 0);
     q.first = lo;
-    q.n = (int)min((int64_t)min(max((int64_t)hi - lo, (int64_t)0), (int64_t)a.max_nodes), max(a.tokens - lo, (int64_t)0));
-    q.ctx = max(a.ctx_lens[b], 0);
-    q.end = min(q.ctx + q.n, (int64_t)a.table_cols << a.cache.shift);
-    q.tiles = q.n > 0 ? max((q.end + kTile - 1) / kTile, (int64_t)1) : 0;
+    q.n = min(min(max(hi - lo, 0), a.max_nodes), max(a.tokens - lo, 0));
+    q.ctx = min(max(a.ctx_lens[b], 0), INT32_MAX - 128);
+    q.end = min(q.ctx + q.n, a.room);
+    q.tiles = q.n > 0 ? max((q.end + kTile - 1) / kTile, 1) : 0;
     q.mbs = (q.n * a.group + rows - 1) / rows;
   }
   return q;
 }
+__device__ __forceinline__ int seq_tiles(const TreeArgs& a, const Seq& q) { return q.tiles * q.mbs * a.kv_heads; }
 
-__device__ __forceinline__ int64_t lane_i64(int64_t v, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
-__device__ __forceinline__ int64_t wave_sum_i64(int64_t v) {
+__device__ __forceinline__ int wave_sum_int(int v) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return lane_i64(v, 0);
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
-// Tiles of the whole batch.
-__device__ __forceinline__ int64_t all_tiles(const TreeArgs& a, int rows) {
-  int64_t sum = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const Seq q = lane_seq(a, b0 + (int)(threadIdx.x & 63), rows);
-    sum += q.tiles * q.mbs * a.kv_heads;
+// Tiles of the sequences before `stop`.
+__device__ __forceinline__ int tiles_before(const TreeArgs& a, int rows, int stop) {
+  int sum = 0;
+  for (int b0 = 0; b0 < stop; b0 += 64) {
+    const int b = b0 + (int)(threadIdx.x & 63);
+    if (b < stop) sum += seq_tiles(a, load_seq(a, b, rows));
   }
-  return wave_sum_i64(sum);
+  return wave_sum_int(sum);
 }
 
-// The sequence that tile `at` (< all_tiles) belongs to, the same in every lane.
-__device__ __forceinline__ Seq find_seq(const TreeArgs& a, int rows, int64_t at) {
+// The sequence that tile `at` (of all: < total) belongs to, the same in every lane.
+__device__ __forceinline__ Seq find_seq(const TreeArgs& a, int rows, int at) {
   const int lane = threadIdx.x & 63;
-  int64_t base = 0;
+  int base = 0;
   for (int b0 = 0;; b0 += 64) {
-    const Seq q = lane_seq(a, b0 + lane, rows);
-    int64_t incl = q.tiles * q.mbs * a.kv_heads;
-    const int64_t mine = incl;
+    const Seq q = load_seq(a, b0 + lane, rows);
+    const int mine = seq_tiles(a, q);
+    int incl = mine;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t up = __shfl_up(incl, d);
+      const int up = __shfl_up(incl, d);
       incl += lane >= d ? up : 0;
     }
     const uint64_t past = __ballot(base + incl > at);
     if (past != 0 || b0 + 64 >= a.batch) {
       const int l = past ? __ffsll((unsigned long long)past) - 1 : 0;
-      Seq r;
-      r.b = b0 + l;
-      r.n = __builtin_amdgcn_readlane(q.n, l);
-      r.mbs = __builtin_amdgcn_readlane(q.mbs, l);
-      r.first = lane_i64(q.first, l);
-      r.ctx = lane_i64(q.ctx, l);
-      r.end = lane_i64(q.end, l);
-      r.tiles = lane_i64(q.tiles, l);
-      r.before = base + lane_i64(incl - mine, l);
-      return r;
+      return {b0 + l, __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.mbs, l),
+              __builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.ctx, l), __builtin_amdgcn_readlane(q.end, l),
+              __builtin_amdgcn_readlane(q.tiles, l), base + __builtin_amdgcn_readlane(incl - mine, l)};
     }
-    base += lane_i64(incl, 63);
+    base += __builtin_amdgcn_readlane(incl, 63);
   }
 }
 
-// Workgroup w of n takes tiles [share(w), share(w + 1)).
+// Of `total` tiles workgroup w < n takes [share(w), share(w + 1)).
 struct Split {
-  int64_t total;
-  int n;
-  __device__ __forceinline__ Split(int64_t tiles, int most)
-      : total(tiles), n((int)min((int64_t)most, max((tiles + kMinTiles - 1) / kMinTiles, (int64_t)1))) {}
-  __device__ __forceinline__ int64_t share(int w) const { return total * w / n; }
-  // the workgroup whose stretch holds tile x
-  __device__ __forceinline__ int holder(int64_t x) const {
-    int w = (int)((x * n + n - 1) / total);  // the last w with share(w) <= x, or one beside it
-    while (w > 0 && (w >= n || share(w) > x)) --w;
-    while (w + 1 < n && share(w + 1) <= x) ++w;
-    return w;
+  int n, each, more;  // `more` workgroups take each + 1
+  __device__ __forceinline__ Split(int total, int most) {
+    n = min(most, max((total + kMinTiles - 1) / kMinTiles, 1));
+    each = (int)((uint32_t)total / (uint32_t)n);
+    more = total - each * n;
+  }
+  __device__ __forceinline__ int share(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int holder(int x) const {  // of tile x
+    const int big = more * (each + 1);
+    return x < big ? (int)((uint32_t)x / (uint32_t)(each + 1)) : more + (int)((uint32_t)(x - big) / (uint32_t)max(each, 1));
   }
 };
 
@@ -177,11 +171,29 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-__device__ __forceinline__ u32x4 range_of(const char* p, uint32_t bytes) {
-  const uint64_t x = (uint64_t)(uintptr_t)p;
-  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x),
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) & 0xffffu,
-               (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+// N LDS DMA instructions of one descriptor, 1 KB apart in LDS (see lds_dma16).
+// The wait states are in the asm, into which the compiler does not look: five
+// between a VALU write of an SGPR (v_readlane, v_readfirstlane: the descriptor is
+// made of such) and a vector memory instruction that reads it, one between m0 and
+// the copy.
+template <int N>
+__device__ __forceinline__ void copy_rows(u32x4 r, const uint32_t* voff, uint32_t lds) {
+  static_assert(N == 1 || N == 2 || N == 4, "instructions of 16 rows");
+#define TJK_COPY(v) "s_nop 0\n\tbuffer_load_dwordx4 " v ", %0, 0 offen lds"
+#define TJK_STEP "\n\ts_add_u32 m0, m0, 0x400\n\t"
+  if constexpr (N == 1)
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\t" TJK_COPY("%2")::"s"(r), "s"(lds), "v"(voff[0]) : "m0", "scc");
+  else if constexpr (N == 2)
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\t" TJK_COPY("%2") TJK_STEP TJK_COPY("%3")::"s"(r), "s"(lds), "v"(voff[0]),
+                 "v"(voff[1])
+                 : "m0", "scc");
+  else
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\t" TJK_COPY("%2") TJK_STEP TJK_COPY("%3") TJK_STEP TJK_COPY("%4")
+                     TJK_STEP TJK_COPY("%5")::"s"(r),
+                 "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3])
+                 : "m0", "scc");
+#undef TJK_COPY
+#undef TJK_STEP
 }
 
 template <int HD, int NB, int RW, int NST>
@@ -207,25 +219,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
 
-  const int64_t total = all_tiles(a, Sh::ROWS);
-  if (total == 0) return;
-  const Split split(total, gridDim.x);
-  // neighbouring stretches on one XCD
-  const int per = gridDim.x / 8;
-  const int w = (int)(blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (w >= split.n) return;
-  const int64_t stop = split.share(w + 1);
-  int64_t at = split.share(w);
-  if (at >= stop) return;
+  // this workgroup's stretch [at, stop) of all tiles
+  Seq q;
+  int at, stop, w = blockIdx.x;
+  if (a.direct) {
+    const int per = a.kv_heads * a.most_mbs, b = w / per, item = w - b * per;
+    q = load_seq(a, b, Sh::ROWS);
+    q.before = 0;
+    const int kh = item / a.most_mbs, mb = item - kh * a.most_mbs;
+    if (mb >= q.mbs) return;
+    at = (kh * q.mbs + mb) * q.tiles;
+    stop = at + q.tiles;
+  } else {
+    const int total = tiles_before(a, Sh::ROWS, a.batch);
+    if (total == 0) return;
+    const Split split(total, gridDim.x);
+    // neighbouring stretches on one XCD
+    w = (int)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    if (w >= split.n) return;
+    at = split.share(w);
+    stop = split.share(w + 1);
+    q = find_seq(a, Sh::ROWS, at);
+  }
 
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)smem;
   auto swz = [](int r) {
     return CPR == 16 ? ((r >> 3 & 1) | (r & 7) << 1) : ((r >> 3 & 1) | (r & 6));
   };
-  uint32_t voff[NV];
+  // of the DMA instructions of 16 rows (RW = 4: of this wave's)
+  uint32_t voff[RW == 1 ? NV : 1];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int r = i * RPI + lane / CPR, c = (lane % CPR) ^ swz(r);
+  for (int i = 0; i < (RW == 1 ? NV : 1); ++i) {
+    const int r = (RW == 1 ? i : wave % NV) * RPI + lane / CPR, c = (lane % CPR) ^ swz(r);
     voff[i] = (uint32_t)r * a.cache.row_bytes + (c < a.hd8 ? 16u * c : kPast);
   }
   // fragment addresses within a tile
@@ -237,92 +262,89 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 #pragma unroll
   for (int h = 0; h < HT; ++h) vaddr[h] = vrow * RB + (((2 * h + (lane >> 1 & 1)) ^ swz(vrow)) << 4) + 8 * (lane & 1);
 
-  Seq q = find_seq(a, Sh::ROWS, at);
-  int slot = 1;  // of this workgroup's next partial result
   while (at < stop) {
-    if (at >= q.before + q.tiles * q.mbs * a.kv_heads) q = find_seq(a, Sh::ROWS, at);
-    const int64_t off = at - q.before;
-    const int item = (int)(off / q.tiles);
-    const int64_t t0 = off - item * q.tiles, t1 = min(q.tiles, t0 + (stop - at));
+    if (at >= q.before + seq_tiles(a, q)) q = find_seq(a, Sh::ROWS, at);
+    const int off = at - q.before, item = (int)((uint32_t)off / (uint32_t)q.tiles);
+    const int t0 = off - item * q.tiles, t1 = min(q.tiles, t0 + (stop - at));
     at += t1 - t0;
-    const int kh = item / q.mbs, mb = item - kh * q.mbs;
+    const int kh = (int)((uint32_t)item / (uint32_t)q.mbs), mb = item - kh * q.mbs;
     const int rows = q.n * a.group, m0 = mb * Sh::ROWS + (RW == 1 ? 0 : wave * 16 * NB);
-    const int64_t end = q.end;
+    const int end = q.end;
     const char* const kbase = a.cache.k + kh * a.cache.head_bytes;
     const char* const vbase = a.cache.v + kh * a.cache.head_bytes;
     const int32_t* const table = a.table + q.b * a.ld_table;
 
-    // ---- this lane's rows: queries, visible nodes
-    Frag qf[NB][KC];
-    uint64_t bits[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int m = m0 + 16 * i + col;
-      const bool live = m < rows;
-      const int node = live ? m / a.group : 0, head = kh * a.group + (live ? m - node * a.group : 0);
-      const int64_t t = q.first + node;
-      const T* const src = reinterpret_cast<const T*>(a.q + t * a.q_token_bytes + head * a.q_head_bytes);
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const bool in = live && 4 * c + g < a.hd8;
-        Frag f = Mfma<T>::load(src + (4 * c + g < a.hd8 ? 8 * (4 * c + g) : 0));
-        const u32x4 zero = {0, 0, 0, 0};
-        qf[i][c] = in ? f : __builtin_bit_cast(Frag, zero);
-      }
-      bits[i] = a.mask ? a.mask[t] : ~0ull >> (63 - node);
-    }
-
-    // ---- pages of the next 64 tiles: lane j has those of tile first + j * STEP,
-    // the first and the second 16 positions'
+    // ---- places of the next 64 tiles' rows: lane j has the byte offset of tile
+    // first + j * STEP, of its first and its second 16 rows (which may lie in
+    // different pages); hi -1: no page
     constexpr int STEP = RW == 1 ? 4 : 1;
-    const int64_t mine = RW == 1 ? t0 + wave : t0;
-    const int count = mine < t1 ? (int)((t1 - mine + STEP - 1) / STEP) : 0;
-    int page[2];
+    const int mine = RW == 1 ? t0 + wave : t0;
+    const int count = mine < t1 ? (t1 - mine + STEP - 1) / STEP : 0;
+    uint32_t place[2];
+    int place_hi[2];
     auto load_pages = [&](int i0) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int64_t x = (mine + (int64_t)(i0 + lane) * STEP) * kTile + 16 * h;
+        const int x = (mine + (i0 + lane) * STEP) * kTile + 16 * h;
         const bool in = i0 + lane < count && x < end;
-        page[h] = page_of(table, in ? (int)(x >> a.cache.shift) : 0, a.cache.pages);
-        if (in && page[h] < 0 && kh == 0 && mb == 0 && (RW == 1 || wave == 0) && a.index_errors) atomicAdd(a.index_errors, 1);
-        if (!in) page[h] = -1;
+        const int page = page_of(table, in ? x >> a.cache.shift : 0, a.cache.pages);
+        if (in && page < 0 && kh == 0 && mb == 0 && (RW == 1 || wave == 0) && a.index_errors) atomicAdd(a.index_errors, 1);
+        const uint64_t at = (uint64_t)page * (uint64_t)a.cache.page_bytes +
+                            (uint64_t)((uint32_t)(x & ((1 << a.cache.shift) - 1)) * a.cache.row_bytes);
+        const bool there = in && page >= 0;
+        place[h] = there ? (uint32_t)at : 0;
+        place_hi[h] = there ? (int)(at >> 32) : -1;
       }
     };
-    if (kh == 0 && mb == 0 && t0 == 0 && threadIdx.x == 0 && a.index_errors && end < q.ctx + q.n) atomicAdd(a.index_errors, 1);
-    page[0] = page[1] = -1;
+    place[0] = place[1] = 0;
+    place_hi[0] = place_hi[1] = -1;
     if (end > 0) load_pages(0);
-    // 16 rows of keys or values: descriptor of tile i's half h
-    auto half_range = [&](const char* base, int i, int h) {
-      const int pg = __builtin_amdgcn_readlane(page[h], i & 63);
-      const int64_t x = (mine + (int64_t)i * STEP) * kTile + 16 * h;
-      const int left = (int)min(max(end - x, (int64_t)0), (int64_t)16);
-      const char* const p = base + (int64_t)max(pg, 0) * a.cache.page_bytes +
-                            (int64_t)((int)x & ((1 << a.cache.shift) - 1)) * a.cache.row_bytes;
-      return range_of(p, pg < 0 || i >= count ? 0 : (uint32_t)left * a.cache.row_bytes);
-    };
+
+    // ---- this lane's rows: their queries (of a negative scale: their negatives)
+    Frag qf[NB][KC];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int m = min(m0 + 16 * i + col, rows - 1);
+      const int node = (int)((uint32_t)m / (uint32_t)a.group), head = kh * a.group + (m - node * a.group);
+      const char* const src = a.q + (int64_t)(q.first + node) * a.q_token_bytes + head * a.q_head_bytes;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int piece = 4 * c + g;
+        u32x4 f = reinterpret_cast<const u32x4*>(src)[min(piece, a.hd8 - 1)];
+        if (piece >= a.hd8) f = u32x4{0, 0, 0, 0};
+        f ^= a.flip;
+        qf[i][c] = __builtin_bit_cast(Frag, f);
+      }
+    }
+    if (kh == 0 && mb == 0 && t0 == 0 && threadIdx.x == 0 && a.index_errors && end < q.ctx + q.n) atomicAdd(a.index_errors, 1);
+
     // halves of tile i without a page: bits 0 and 1
     auto pageless = [&](int i) {
-      return (__builtin_amdgcn_readlane(page[0], i & 63) < 0 ? 1 : 0) | (__builtin_amdgcn_readlane(page[1], i & 63) < 0 ? 2 : 0);
+      return (__builtin_amdgcn_readlane(place_hi[0], i & 63) < 0 ? 1 : 0) |
+             (__builtin_amdgcn_readlane(place_hi[1], i & 63) < 0 ? 2 : 0);
+    };
+    // descriptor of the 16 rows of tile i's half h
+    auto half_range = [&](const char* base, int i, int h) __attribute__((always_inline)) {
+      const uint32_t lo = __builtin_amdgcn_readlane((int)place[h], i & 63);
+      const int hi = __builtin_amdgcn_readlane(place_hi[h], i & 63);
+      const int left = min(max(end - ((mine + i * STEP) * kTile + 16 * h), 0), 16);
+      const uint64_t p = (uint64_t)(uintptr_t)base + ((uint64_t)(uint32_t)max(hi, 0) << 32 | lo);
+      const uint32_t bytes = hi < 0 || i >= count ? 0 : (uint32_t)left * a.cache.row_bytes;
+      return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)p), (uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu,
+                   (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
     };
     // tile i's keys (or values) to LDS byte `to`
-    auto copy = [&](const char* base, int i, uint32_t to) {
+    auto copy = [&](const char* base, int i, uint32_t to) __attribute__((always_inline)) {
       if constexpr (RW == 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const u32x4 r = half_range(base, i, h);
-#pragma unroll
-          for (int u = 0; u < NV; ++u) lds_dma16(r, voff[u], to + (h * NV + u) * 1024);
+          copy_rows<NV>(half_range(base, i, h), voff, to + h * NV * 1024);
         }
       } else {
+        static_assert(NK == 4 || NK == 8, "a wave copies one or two pieces of a tile");
 #pragma unroll
-        for (int u = 0; u < (NK + 3) / 4; ++u) {
-          const int k = wave + 4 * u;
-          const u32x4 r = half_range(base, i, k / NV);
-          uint32_t v = voff[0];
-#pragma unroll
-          for (int j = 1; j < NV; ++j) v = k % NV == j ? voff[j] : v;
-          lds_dma16(r, v, to + k * 1024);
-        }
+        for (int u = 0; u < NK / 4; ++u)
+          copy_rows<1>(half_range(base, i, NK == 8 ? u : wave >> 1), voff, to + (wave + 4 * u) * 1024);
       }
     };
 
@@ -352,37 +374,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
           for (int c = 0; c < KC; ++c) s[i][b] = Mfma16<T>::mma(kf[b][c], qf[i][c], s[i][b]);
         }
     };
-    // whether this lane's row i sees key x + k (k: of the tile)
-    auto sees = [&](int i, int64_t x, int k, int none) {
-      const int64_t p = x + k;
-      const bool tree = p < q.ctx || (p - q.ctx < 64 && (bits[i] >> ((p - q.ctx) & 63) & 1));
-      return p < end && tree && !(none >> (k >> 4) & 1);
+    // the nodes that this lane's row i sees, of the tile from position x on: bit k for
+    // key k (a tile of the c tokens has them all)
+    auto visible = [&](int i, int x, int none) {
+      const int m = min(m0 + 16 * i + col, rows - 1), node = (int)((uint32_t)m / (uint32_t)a.group);
+      const uint64_t bits = a.mask ? a.mask[q.first + node] : ~0ull >> (63 - node);
+      const int d = x - q.ctx;  // the tile's first key as a node
+      uint32_t keys = d >= 64 ? 0u : d >= 0 ? (uint32_t)(bits >> d) : d <= -32 ? ~0u : (uint32_t)(bits << -d) | ((1u << -d) - 1);
+      if (end - x < 32) keys &= (1u << max(end - x, 0)) - 1;
+      return keys & ~((none & 1 ? 0xffffu : 0u) | (none & 2 ? 0xffff0000u : 0u));
     };
-    auto softmax = [&](f32x4 (&s)[NB][2], Frag (&p)[NB], int64_t x, bool masked, int none) {
+    auto softmax = [&](f32x4 (&s)[NB][2], Frag (&p)[NB]) {
       bool moves = false;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         float top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = s[i][b][r] * a.scale;
-            if (masked) v = sees(i, x, 16 * b + 4 * g + r, none) ? v : -INFINITY;
-            s[i][b][r] = v;
-            top = fmaxf(top, v);
-          }
-        moves |= top > m_off[i] + kLazy;
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[i][j >> 2][j & 3]);
+        moves |= top * a.scale > m_off[i] + kLazy;
       }
       if (__any(moves)) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           float top = -INFINITY;
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[i][b][r]);
-          const float m = fmaxf(m_off[i], column_max(top));
+          for (int j = 0; j < 8; ++j) top = fmaxf(top, s[i][j >> 2][j & 3]);
+          const float m = fmaxf(m_off[i], column_max(top * a.scale));
           const float keep = m_off[i] == m ? 1.f : __builtin_amdgcn_exp2f(m_off[i] - m);
           m_off[i] = m;
           l[i] *= keep;
@@ -392,14 +409,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       }
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const float base = m_off[i] == -INFINITY ? 0.f : m_off[i];
+        const float base = m_off[i] == -INFINITY ? 0.f : -m_off[i];
         float e[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(s[i][j >> 2][j & 3] - base);
+        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[i][j >> 2][j & 3], a.scale, base));
         p[i] = Mfma<T>::pack(e);
         // sums of the rounded weights, those that the product uses
         l[i] = Mfma<T>::sum8(p[i], l[i]);
       }
+    };
+    auto hide = [&](f32x4 (&s)[NB][2], const uint32_t (&keys)[NB]) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          s[i][j >> 2][j & 3] = keys[i] >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1 ? s[i][j >> 2][j & 3] : -INFINITY;
     };
     // Infinities and NaN among a tile's values: a weight of zero would not keep them
     // from a row that does not see them.  They are added to the rows that do, and
@@ -420,13 +444,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       for (uint64_t x = m; x; x &= x - 1) keys |= 1u << ((__ffsll((unsigned long long)x) - 1) >> 1);
       return keys;
     };
-    auto add_bad = [&](const char* vt, uint32_t keys, int64_t x, int none) {
-      for (; keys; keys &= keys - 1) {
-        const int k = __ffs(keys) - 1;
+    auto add_bad = [&](const char* vt, uint32_t bad, const uint32_t (&keys)[NB]) {
+      for (; bad; bad &= bad - 1) {
+        const int k = __ffs(bad) - 1;
         const int sw = swz(k & 15);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const bool seen = sees(i, x, k, none);
+          const bool seen = keys[i] >> k & 1;
 #pragma unroll
           for (int h = 0; h < HT; ++h) {
             const int c = 2 * h + (g >> 1);
@@ -485,9 +509,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
           if (NST > 1 && i >= count) break;
           char* const kt = mem + s * 2 * TB;
           char* const vt = kt + TB;
-          const int64_t x = (mine + (int64_t)i * STEP) * kTile;
-          const int none = lost[s];
+          const int x = (mine + i * STEP) * kTile, none = lost[s];
           const bool masked = x + kTile > q.ctx || none != 0;
+          uint32_t keys[NB];
           if (((i + NST) & 63) == 0 && i + NST < count) load_pages(i + NST);
           f32x4 sc[NB][2];
           Frag p[NB];
@@ -496,12 +520,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           copy(kbase, i + NST, ring + s * 2 * TB);
           lost[s] = pageless(i + NST);
-          softmax(sc, p, x, masked, none);
+          if (masked) {
+#pragma unroll
+            for (int u = 0; u < NB; ++u) keys[u] = visible(u, x, none);
+            hide(sc, keys);
+          }
+          softmax(sc, p);
           asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK * (2 * NST - 1)) : "memory");
           if (masked) {
-            const uint32_t keys = bad_values(vt);
-            if (keys) {
-              add_bad(vt, keys, x, none);
+            const uint32_t bad = bad_values(vt);
+            if (bad) {
+              add_bad(vt, bad, keys);
               clear_bad(vt);
               asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
@@ -559,8 +588,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       }
       int s = 0;
       for (int i = 0; i < count; ++i) {
-        const int64_t x = (mine + i) * kTile;
-        const int none = lost[0];
+        const int x = (mine + i) * kTile, none = lost[0];
         const bool masked = x + kTile > q.ctx || none != 0;
         if (((i + NST - 1) & 63) == 0 && i + NST - 1 < count) load_pages(i + NST - 1);
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NI * (NST - 2)) : "memory");
@@ -575,11 +603,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         f32x4 sc[NB][2];
         Frag p[NB];
         scores(kt, sc);
-        softmax(sc, p, x, masked, none);
+        uint32_t keys[NB];
         if (masked) {
-          const uint32_t keys = bad_values(vt);  // the same in every wave
-          if (keys) {
-            add_bad(vt, keys, x, none);
+#pragma unroll
+          for (int u = 0; u < NB; ++u) keys[u] = visible(u, x, none);
+          hide(sc, keys);
+        }
+        softmax(sc, p);
+        if (masked) {
+          const uint32_t bad = bad_values(vt);  // the same in every wave
+          if (bad) {
+            add_bad(vt, bad, keys);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (wave == 0) clear_bad(vt);
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -594,8 +628,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     // ---- the rows, or what the joining launch needs of them
     const bool whole = t0 == 0 && t1 == q.tiles;
     if (RW == 1 && wave != 0) continue;
-    const int64_t part = 2 * (int64_t)w + (t0 == 0 ? 1 : 0);
-    (void)slot;
+    const int64_t part = 2 * w + (t0 == 0 ? 1 : 0);
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int m = m0 + 16 * i + col;
@@ -622,74 +655,66 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   }
 }
 
-// Joins the stretches of an item: a workgroup takes kJoinRows rows of it, 16
-// lanes a row (eight or four columns each), the stretches in turn over its
-// row groups.  The order is that of the keys, whoever finished first.
-constexpr int kJoinRows = 16;
-
+// Joins the stretches of an item.  A wave takes R rows, HD / 4 lanes a row; the
+// four waves of a workgroup take the stretches in turn, four loads in flight, and
+// join theirs at last.  The order is that of the keys, whoever finished first.
 template <typename T, int HD, int ROWS>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int most) {
-  constexpr int V = HD / 16, PART = ROWS * (HD + 2);
-  const int64_t total = all_tiles(a, ROWS);
-  if (total == 0) return;
-  const Split split(total, most);
-  const int blocks = (ROWS + kJoinRows - 1) / kJoinRows;
-  const int mbs = (a.max_nodes * a.group + ROWS - 1) / ROWS;
+  constexpr int L = HD / 4, R = 64 / L, PART = ROWS * (HD + 2), BLOCKS = ROWS / R, U = 4;
+  __shared__ float4 so[3][64];
+  __shared__ float2 sm[3][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int rest = blockIdx.x;
-  const int rb = rest % blocks;
-  rest /= blocks;
-  const int mb = rest % mbs;
-  rest /= mbs;
+  const int rb = rest % BLOCKS;
+  rest /= BLOCKS;
+  const int mb = rest % a.most_mbs;
+  rest /= a.most_mbs;
   const int kh = rest % a.kv_heads, b = rest / a.kv_heads;
-  // this sequence, and the tiles before it
-  int64_t before = 0;
-  for (int b0 = 0; b0 < b; b0 += 64) {
-    const int l = b0 + (int)(threadIdx.x & 63);
-    if (l < b) {
-      const Seq q = lane_seq(a, l, ROWS);
-      before += q.tiles * q.mbs * a.kv_heads;
-    }
-  }
-  before = wave_sum_i64(before);
-  const Seq q = lane_seq(a, b, ROWS);
-  const int row = rb * kJoinRows + (threadIdx.x >> 4);
-  const int m = mb * ROWS + row;
-  if (q.n == 0 || mb >= q.mbs) return;
-  const int64_t first = before + ((int64_t)kh * q.mbs + mb) * q.tiles, last = first + q.tiles - 1;
-  const int w0 = split.holder(first), w1 = split.holder(last);
+  const Seq q = load_seq(a, b, ROWS);
+  if (mb * ROWS + rb * R >= q.n * a.group) return;
+  const int before = tiles_before(a, ROWS, b);
+  const Split split(tiles_before(a, ROWS, a.batch), most);
+  const int first = before + (kh * q.mbs + mb) * q.tiles;
+  const int w0 = split.holder(first), w1 = split.holder(first + q.tiles - 1);
   if (w0 == w1) return;  // one workgroup had all of it
-  if (row >= ROWS || m >= q.n * a.group) return;
-  const int c0 = (threadIdx.x & 15) * V;
-  float top = -INFINITY, sum = 0.f, o[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = 0.f;
-  for (int w = w0; w <= w1; ++w) {
-    // the first stretch may begin in the middle of its workgroup's
-    const float* const part = a.parts + (2 * (int64_t)w + (w == w0 ? 1 : 0)) * PART;
-    const float2 ml = *reinterpret_cast<const float2*>(part + ROWS * HD + 2 * row);
+  const int row = rb * R + lane / L, c0 = lane % L * 4, m = mb * ROWS + row;
+  float top = -INFINITY, sum = 0.f;
+  float4 o = make_float4(0, 0, 0, 0);
+  auto add = [&](float2 ml, float4 v) {
     const float t = fmaxf(top, ml.x);
     const float f1 = top == t ? 1.f : __builtin_amdgcn_exp2f(top - t), f2 = ml.x == t ? 1.f : __builtin_amdgcn_exp2f(ml.x - t);
     top = t;
     sum = sum * f1 + ml.y * f2;
-    const float4* const src = reinterpret_cast<const float4*>(part + row * HD + c0);
+    o = make_float4(o.x * f1 + v.x * f2, o.y * f1 + v.y * f2, o.z * f1 + v.z * f2, o.w * f1 + v.w * f2);
+  };
+  for (int x = w0 + wave; x <= w1; x += 4 * U) {
+    float2 ml[U];
+    float4 v[U];
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const float4 v = src[i / 4];
-      o[i] = o[i] * f1 + v.x * f2;
-      o[i + 1] = o[i + 1] * f1 + v.y * f2;
-      o[i + 2] = o[i + 2] * f1 + v.z * f2;
-      o[i + 3] = o[i + 3] * f1 + v.w * f2;
+    for (int u = 0; u < U; ++u) {
+      const int w = min(x + 4 * u, w1);
+      // the first stretch may be the end of its workgroup's
+      const float* const part = a.parts + (int64_t)(2 * w + (w == w0 ? 1 : 0)) * PART;
+      ml[u] = *reinterpret_cast<const float2*>(part + ROWS * HD + 2 * row);
+      v[u] = *reinterpret_cast<const float4*>(part + row * HD + c0);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (x + 4 * u <= w1) add(ml[u], v[u]);
   }
+  if (wave > 0) {
+    so[wave - 1][lane] = o;
+    sm[wave - 1][lane] = make_float2(top, sum);
+  }
+  __syncthreads();
+  if (wave > 0 || m >= q.n * a.group) return;
+#pragma unroll
+  for (int u = 0; u < 3; ++u) add(sm[u][lane], so[u][lane]);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int node = m / a.group, head = kh * a.group + m - node * a.group;
-  T* const dst = reinterpret_cast<T*>(a.out + (q.first + node) * a.out_bytes) + (int64_t)head * (8 * a.hd8);
-  if (c0 < 8 * a.hd8) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4)
-      *reinterpret_cast<typename Quad<T>::raw*>(dst + c0 + i) =
-          Quad<T>::from(make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv));
-  }
+  T* const dst = reinterpret_cast<T*>(a.out + (int64_t)(q.first + node) * a.out_bytes) + head * (8 * a.hd8);
+  if (c0 < 8 * a.hd8)
+    *reinterpret_cast<typename Quad<T>::raw*>(dst + c0) = Quad<T>::from(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 // ---------------------------------------------------------------- variants
@@ -722,13 +747,22 @@ static auto with_variant(int head_dim, int rows, F&& f) {
   return f(Variant<128, 4, 4, 3, 2>{});
 }
 
+// Tiles of the longest context that the block table holds up to which each item
+// is one workgroup's.
+constexpr int kDirectTiles = 32;
+
 template <typename T, typename V>
-static int launch_tree(const TreeArgs& a, hipStream_t s) {
+static int launch_tree(TreeArgs a, hipStream_t s) {
   constexpr int ROWS = V::Sh::ROWS;
-  tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC><<<V::GRID, 256, 0, s>>>(a);
+  a.most_mbs = (a.max_nodes * a.group + ROWS - 1) / ROWS;
+  const int64_t items = (int64_t)a.batch * a.kv_heads * a.most_mbs, tiles = (a.room + kTile - 1) / kTile;
+  if (items * std::max<int64_t>(tiles, 1) > INT32_MAX || items * (ROWS / 2) > INT32_MAX / 256)
+    return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
+  a.direct = tiles <= kDirectTiles;
+  tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);
   if (const int bad = check_launch("tjk_tree_attention")) return bad;
-  const int64_t mbs = (a.max_nodes * a.group + ROWS - 1) / ROWS;
-  const int64_t grid = (int64_t)a.batch * a.kv_heads * mbs * ((ROWS + kJoinRows - 1) / kJoinRows);
+  if (a.direct) return TJK_OK;
+  const int64_t grid = items * (ROWS * (V::HD / 4) / 64);
   tree_join_kernel<T, V::HD, ROWS><<<(unsigned)grid, 256, 0, s>>>(a, V::GRID);
   return check_launch("tjk_tree_attention");
 }
@@ -773,10 +807,12 @@ extern "C" int tjk_tree_attention(const void* q, int64_t ld_q_token, int64_t ld_
   if (workspace_bytes < need)
     return fail(TJK_EINVAL, "%s: a workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
   const float log2e = 1.44269504088896340736f;
-  const TreeArgs a{static_cast<const char*>(q), 2 * ld_q_token, 2 * ld_q_head, paged(*cache), block_table, ld_table,
-                   (int)table_cols, ctx_lens, cu_nodes, tree_mask, static_cast<char*>(out), 2 * ld_out, scale * log2e,
-                   static_cast<float*>(workspace), index_errors, tokens, batch, cache->kv_heads, heads / cache->kv_heads,
-                   cache->head_dim / 8, max_nodes};
+  const int64_t room = std::min<int64_t>(table_cols * cache->page_size, INT32_MAX - 128);
+  // (a scale of zero would make no number of what is hidden, -inf)
+  const TreeArgs a{static_cast<const char*>(q), 2 * ld_q_token, 2 * ld_q_head, paged(*cache), block_table, ld_table, ctx_lens,
+                   cu_nodes, tree_mask, static_cast<char*>(out), 2 * ld_out, std::max(std::fabs(scale) * log2e, FLT_MIN),
+                   static_cast<float*>(workspace), index_errors, scale < 0 ? 0x80008000u : 0u, (int)room, (int)tokens, batch,
+                   cache->kv_heads, heads / cache->kv_heads, cache->head_dim / 8, max_nodes, 0, 0};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return with_variant(cache->head_dim, max_nodes * a.group, [&](auto v) {
     return cache->dtype == TJK_F16 ? launch_tree<f16, decltype(v)>(a, s) : launch_tree<bf16, decltype(v)>(a, s);

@@ -486,11 +486,13 @@ int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_head, const in
  * nothing, or only scores of -inf, is zero.  Keys and values that a row does not
  * see do not reach it, whatever they hold; positions without a page are left
  * out, and count in *index_errors.
- * workspace: tjk_tree_attention_bytes() bytes on the device, 16-byte aligned;
- * calls that share one have to be ordered.
+ * workspace: tjk_tree_attention_bytes() bytes on the device, 16-byte aligned, of
+ * which the first TJK_TREE_COUNTERS have to be zero before the first call; each
+ * call leaves them so.  Calls that share a workspace have to be ordered.
  * Requires heads % kv_heads == 0, strides that are multiples of 8 and 16-byte
  * aligned pointers (8 for tree_mask).
  */
+#define TJK_TREE_COUNTERS 12288
 int tjk_tree_attention(const void* q, int64_t ld_q_token, int64_t ld_q_head,
                        const tjk_paged_cache* cache, const int32_t* block_table, int64_t ld_table,
                        int64_t table_cols, const int32_t* ctx_lens, const int32_t* cu_nodes,

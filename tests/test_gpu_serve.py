@@ -423,14 +423,15 @@ def test_attention_layouts(device):
 
 
 def test_attention_repeats(device):
-    """The same bits again, with a workspace full of rubbish, and on another
-    stream than the tensors'."""
+    """The same bits again, with a workspace full of rubbish behind its counters,
+    and on another stream than the tensors'; the counters are left at zero."""
     t = Trees([3000, 5, 777], [6, 1, 30], 8, 2, 128, 32, torch.bfloat16, 20)
     want = t.run(device)
     ws = ops.tree_attention_workspace(t.q.to(device), t.k, t.max_nodes)
     for fill in (0, 255):
-        ws.fill_(fill)
+        ws[12288:].fill_(fill)
         assert torch.equal(t.run(device, workspace=ws), want)
+        assert (ws[:12288] == 0).all()
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):

@@ -25,7 +25,8 @@ struct TreeArgs {
   char* out;
   int64_t out_bytes;  // of a row
   float scale;  // its size, with log2(e): scores are exponents of 2
-  float* parts;  // workspace: two partial results per workgroup
+  int* counters;  // workspace: two per workgroup and level of joining, zero between launches
+  float* parts;   // two partial results per workgroup
   int* index_errors;
   uint32_t flip;  // the signs of two queries' elements, if the scale is negative
   int room;       // positions that the block table holds
@@ -37,22 +38,29 @@ struct TreeArgs {
 // ---------------------------------------------------------------- work
 //
 // An item is a block of rows of one (sequence, key head): rows m = node * group +
-// query head, ROWS of them.  Its keys are cut into tiles of 32, all items' tiles
-// are numbered through, and every workgroup takes an equal stretch of them:
-// lengths are known on the device only, and a long sequence next to short ones
-// is split as finely as it needs.  A stretch that is a whole item writes its rows;
-// else it leaves the rows' sums, with their exponent offset, in the workspace, and
-// a second launch joins them.
+// query head, ROWS of them.  Its keys are cut into tiles of 32.  An item counts
+// kItemCost units, for what it costs beside its tiles, and one for each tile; all
+// items' units are numbered through, and every workgroup takes an equal stretch of
+// them: lengths are known on the device only, and a long sequence next to short
+// ones is split as finely as it needs.  A stretch that is a whole item writes its rows;
+// else it leaves the rows' sums, with their exponent offset, in the workspace.  Of
+// eight neighbouring stretches of an item the workgroup that comes last (a counter
+// says which) joins the eight, of eight such eights the last one them, and so on;
+// always in the order of the keys.  Nobody waits for another, and the counters are
+// left at zero.  (One workgroup joining all 64 stretches of an item took 25 us of 70
+// for 2 x 99995 tokens.)
 
 constexpr int kTile = 32;     // keys of a tile
-constexpr int kMinTiles = 8;  // least tiles of a workgroup: below, the joining costs more than the splitting gives
+constexpr int kJoin = 8;      // sums that are joined at a time
+constexpr int kItemCost = 8;  // an item's start and end take as long as about so many tiles
+constexpr int kMinUnits = 8;  // of a workgroup: below, the joining costs more than the splitting gives
 
 struct Seq {
   int b, n, mbs;  // sequence, its nodes, its row blocks
   int first;      // its first row
   int ctx, end;   // tokens behind it, positions that it sees
   int tiles;      // of an item
-  int before;     // tiles before it
+  int before;     // units before it
 };
 
 // Sequence b (< batch, else nothing): everything but `before`.
@@ -70,58 +78,67 @@ __device__ __forceinline__ Seq load_seq(const TreeArgs& a, int b, int rows) {
   }
   return q;
 }
-__device__ __forceinline__ int seq_tiles(const TreeArgs& a, const Seq& q) { return q.tiles * q.mbs * a.kv_heads; }
+__device__ __forceinline__ int seq_units(const TreeArgs& a, const Seq& q) { return (q.tiles + kItemCost) * q.mbs * a.kv_heads; }
 
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return __builtin_amdgcn_readfirstlane(v);
-}
-
-// Tiles of the sequences before `stop`.
-__device__ __forceinline__ int tiles_before(const TreeArgs& a, int rows, int stop) {
-  int sum = 0;
-  for (int b0 = 0; b0 < stop; b0 += 64) {
-    const int b = b0 + (int)(threadIdx.x & 63);
-    if (b < stop) sum += seq_tiles(a, load_seq(a, b, rows));
-  }
-  return wave_sum_int(sum);
-}
-
-// The sequence that tile `at` (of all: < total) belongs to, the same in every lane.
-__device__ __forceinline__ Seq find_seq(const TreeArgs& a, int rows, int at) {
+// Inclusive sum over the lanes.
+__device__ __forceinline__ int wave_scan(int v) {
   const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int b0 = 0;; b0 += 64) {
-    const Seq q = load_seq(a, b0 + lane, rows);
-    const int mine = seq_tiles(a, q);
-    int incl = mine;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(incl, d);
-      incl += lane >= d ? up : 0;
-    }
-    const uint64_t past = __ballot(base + incl > at);
-    if (past != 0 || b0 + 64 >= a.batch) {
-      const int l = past ? __ffsll((unsigned long long)past) - 1 : 0;
-      return {b0 + l, __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.mbs, l),
-              __builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.ctx, l), __builtin_amdgcn_readlane(q.end, l),
-              __builtin_amdgcn_readlane(q.tiles, l), base + __builtin_amdgcn_readlane(incl - mine, l)};
-    }
-    base += __builtin_amdgcn_readlane(incl, 63);
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(v, d);
+    v += lane >= d ? up : 0;
   }
+  return v;
 }
 
-// Of `total` tiles workgroup w < n takes [share(w), share(w + 1)).
+// The sequences of a batch, 64 at a time, and the units before and of them.
+struct Plan {
+  Seq q;  // lane l: sequence first + l
+  int first, incl, base;
+  __device__ __forceinline__ void load(const TreeArgs& a, int rows, int b0) {
+    first = b0;
+    q = load_seq(a, b0 + (int)(threadIdx.x & 63), rows);
+    incl = wave_scan(seq_units(a, q));
+  }
+  // all of the batch's units; the first 64 sequences are left loaded
+  __device__ __forceinline__ int total(const TreeArgs& a, int rows) {
+    int sum = 0;
+    for (int b0 = (a.batch - 1) / 64 * 64; b0 >= 0; b0 -= 64) {
+      load(a, rows, b0);
+      sum += __builtin_amdgcn_readlane(incl, 63);
+    }
+    base = 0;
+    return sum;
+  }
+  // The sequence that unit `at` (< total, not before the last one asked for) belongs
+  // to, the same in every lane.
+  __device__ __forceinline__ Seq find(const TreeArgs& a, int rows, int at) {
+    while (true) {
+      const uint64_t past = __ballot(base + incl > at);
+      if (past != 0 || first + 64 >= a.batch) {
+        const int l = past ? __ffsll((unsigned long long)past) - 1 : 0;
+        return {first + l, __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.mbs, l),
+                __builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.ctx, l),
+                __builtin_amdgcn_readlane(q.end, l), __builtin_amdgcn_readlane(q.tiles, l),
+                base + __builtin_amdgcn_readlane(incl - seq_units(a, q), l)};
+      }
+      base += __builtin_amdgcn_readlane(incl, 63);
+      load(a, rows, first + 64);
+    }
+  }
+};
+
+// Of `total` units workgroup w < n takes [share(w), share(w + 1)).
 struct Split {
   int n, each, more;  // `more` workgroups take each + 1
+  Split() = default;
   __device__ __forceinline__ Split(int total, int most) {
-    n = min(most, max((total + kMinTiles - 1) / kMinTiles, 1));
+    n = min(most, max((total + kMinUnits - 1) / kMinUnits, 1));
     each = (int)((uint32_t)total / (uint32_t)n);
     more = total - each * n;
   }
   __device__ __forceinline__ int share(int w) const { return w * each + min(w, more); }
-  __device__ __forceinline__ int holder(int x) const {  // of tile x
+  __device__ __forceinline__ int holder(int x) const {  // of unit x
     const int big = more * (each + 1);
     return x < big ? (int)((uint32_t)x / (uint32_t)(each + 1)) : more + (int)((uint32_t)(x - big) / (uint32_t)max(each, 1));
   }
@@ -147,6 +164,8 @@ struct Split {
 // and share the tiles, in a ring of NST, one barrier a tile.
 
 constexpr uint32_t kPast = 0x80000000u;  // beyond any descriptor's range
+// Cache policies: stores through to memory, loads from it, past an XCD's own L2.
+constexpr int kThrough = 17, kCoherent = 16;
 constexpr float kLazy = 8.0f;            // a row's offset follows its scores when they pass it by 2^8
 
 template <typename T> struct Mfma16;
@@ -219,8 +238,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
 
-  // this workgroup's stretch [at, stop) of all tiles
+  // this workgroup's stretch [at, stop) of all units
   Seq q;
+  int first64 = 0, base64 = 0;  // the 64 sequences that hold q, the units before them
+  Split split{};
   int at, stop, w = blockIdx.x;
   if (a.direct) {
     const int per = a.kv_heads * a.most_mbs, b = w / per, item = w - b * per;
@@ -228,23 +249,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     q.before = 0;
     const int kh = item / a.most_mbs, mb = item - kh * a.most_mbs;
     if (mb >= q.mbs) return;
-    at = (kh * q.mbs + mb) * q.tiles;
-    stop = at + q.tiles;
+    at = (kh * q.mbs + mb) * (q.tiles + kItemCost);
+    stop = at + q.tiles + kItemCost;
   } else {
-    const int total = tiles_before(a, Sh::ROWS, a.batch);
+    Plan plan;
+    const int total = plan.total(a, Sh::ROWS);
     if (total == 0) return;
-    const Split split(total, gridDim.x);
+    split = Split(total, gridDim.x);
     // neighbouring stretches on one XCD
     w = (int)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
     if (w >= split.n) return;
     at = split.share(w);
     stop = split.share(w + 1);
-    q = find_seq(a, Sh::ROWS, at);
+    q = plan.find(a, Sh::ROWS, at);
+    first64 = plan.first;
+    base64 = plan.base;
   }
 
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)smem;
+  // Keys are read one piece of 16 rows at a time, values two neighbouring pieces of
+  // 8 rows: neither meets a bank twice, in halves of 128 bytes or in whole passes.
   auto swz = [](int r) {
-    return CPR == 16 ? ((r >> 3 & 1) | (r & 7) << 1) : ((r >> 3 & 1) | (r & 6));
+    const int r0 = r & 1, r1 = r >> 1 & 1, r2 = r >> 2 & 1, r3 = r >> 3 & 1;
+    return CPR == 16 ? (r2 ^ r3) | r0 << 1 | r1 << 2 | r2 << 3 : (r0 ^ r3) | r1 << 1 | (r0 ^ r2) << 2;
   };
   // of the DMA instructions of 16 rows (RW = 4: of this wave's)
   uint32_t voff[RW == 1 ? NV : 1];
@@ -262,11 +289,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 #pragma unroll
   for (int h = 0; h < HT; ++h) vaddr[h] = vrow * RB + (((2 * h + (lane >> 1 & 1)) ^ swz(vrow)) << 4) + 8 * (lane & 1);
 
+  const __amdgpu_buffer_rsrc_t parts = wave_rsrc(a.parts, (int64_t)2 * gridDim.x * Sh::PART * 4);
+  // where row m of key head kh of sequence q goes
+  auto out_row = [&](int m, int kh) {
+    const int node = (int)((uint32_t)m / (uint32_t)a.group);
+    return reinterpret_cast<T*>(a.out + (int64_t)(q.first + node) * a.out_bytes) +
+           (int64_t)(kh * a.group + m - node * a.group) * (8 * a.hd8);
+  };
   while (at < stop) {
-    if (at >= q.before + seq_tiles(a, q)) q = find_seq(a, Sh::ROWS, at);
-    const int off = at - q.before, item = (int)((uint32_t)off / (uint32_t)q.tiles);
-    const int t0 = off - item * q.tiles, t1 = min(q.tiles, t0 + (stop - at));
-    at += t1 - t0;
+    if (at >= q.before + seq_units(a, q)) {  // (loaded again: kept over the tiles, it would take their registers)
+      Plan plan;
+      plan.load(a, Sh::ROWS, first64);
+      plan.base = base64;
+      q = plan.find(a, Sh::ROWS, at);
+      first64 = plan.first;
+      base64 = plan.base;
+    }
+    const int units = q.tiles + kItemCost, off = at - q.before, item = (int)((uint32_t)off / (uint32_t)units);
+    const int u0 = off - item * units, u1 = min(units, u0 + (stop - at));
+    const int x0 = at - u0 + kItemCost;  // the unit of the item's first tile
+    const int t0 = max(u0 - kItemCost, 0), t1 = max(u1 - kItemCost, 0);
+    at += u1 - u0;
+    if (t0 == t1) continue;  // its tiles are the next workgroup's
     const int kh = (int)((uint32_t)item / (uint32_t)q.mbs), mb = item - kh * q.mbs;
     const int rows = q.n * a.group, m0 = mb * Sh::ROWS + (RW == 1 ? 0 : wave * 16 * NB);
     const int end = q.end;
@@ -625,96 +669,123 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
-    // ---- the rows, or what the joining launch needs of them
+    // ---- the rows, or their sums for who comes last
     const bool whole = t0 == 0 && t1 == q.tiles;
-    if (RW == 1 && wave != 0) continue;
-    const int64_t part = 2 * w + (t0 == 0 ? 1 : 0);
+    const int part = 2 * w + (t0 == 0 ? 1 : 0);  // a stretch ends in the first part of an item at most once
+    if (RW > 1 || wave == 0) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int m = m0 + 16 * i + col;
-      const float sum = column_sum(l[i]);
-      if (m >= rows) continue;
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-        const int node = m / a.group, head = kh * a.group + m - node * a.group;
-        T* const dst = reinterpret_cast<T*>(a.out + (q.first + node) * a.out_bytes) + (int64_t)head * (8 * a.hd8);
+      for (int i = 0; i < NB; ++i) {
+        const int m = m0 + 16 * i + col, r = m - mb * Sh::ROWS;
+        const float sum = column_sum(l[i]);
+        if (m >= rows) continue;
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          T* const dst = out_row(m, kh);
 #pragma unroll
-        for (int h = 0; h < HT; ++h)
-          if (16 * h < 8 * a.hd8)
-            *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) =
-                Quad<T>::from(make_float4(o[i][h][0] * inv, o[i][h][1] * inv, o[i][h][2] * inv, o[i][h][3] * inv));
-      } else {
-        float* const dst = a.parts + part * Sh::PART + (int64_t)(m - mb * Sh::ROWS) * HD;
+          for (int h = 0; h < HT; ++h)
+            if (2 * h < a.hd8)
+              *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) =
+                  Quad<T>::from(make_float4(o[i][h][0] * inv, o[i][h][1] * inv, o[i][h][2] * inv, o[i][h][3] * inv));
+        } else {
 #pragma unroll
-        for (int h = 0; h < HT; ++h)
-          *reinterpret_cast<float4*>(dst + 16 * h + 4 * g) = make_float4(o[i][h][0], o[i][h][1], o[i][h][2], o[i][h][3]);
-        float* const ml = a.parts + part * Sh::PART + Sh::ROWS * HD + 2 * (m - mb * Sh::ROWS);
-        if (g == 0) *reinterpret_cast<float2*>(ml) = make_float2(m_off[i], sum);
+          for (int h = 0; h < HT; ++h)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o[i][h]), parts,
+                                                   4 * (part * Sh::PART + r * HD + 16 * h + 4 * g), 0, kThrough);
+          if (g == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m_off[i]), __float_as_uint(sum)}, parts,
+                                                  4 * (part * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kThrough);
+        }
+      }
+    }
+    if (whole) continue;
+
+    // ---- the last of eight joins them, until the item is whole
+    const int w0 = split.holder(x0);
+    const int stretches = split.holder(x0 + q.tiles - 1) - w0 + 1;
+    auto part_of = [&](int z) { return 2 * (w0 + z) + (z == 0 ? 1 : 0); };  // of stretch z
+    const int live = min(rows - mb * Sh::ROWS, Sh::ROWS);
+    // Joins n sums, of stretches first, first + span, ...: into the rows if that is
+    // all of the item, else in the place of the first.  L lanes a row; where rows
+    // leave lanes free, `shares` groups of lanes take the stretches in turn.
+    auto join_parts = [&](int first, int span, int n, bool whole) __attribute__((always_inline)) {
+      constexpr int L = HD / 4, GROUPS = 256 / L;
+      int wide = GROUPS;
+      while (wide / 2 >= live) wide /= 2;
+      const int shares = GROUPS / wide, group = threadIdx.x / L, c0 = threadIdx.x % L * 4, share = group / wide;
+      for (int r0 = 0; r0 < live; r0 += wide) {
+        const int r = min(r0 + group % wide, live - 1);
+        u32x2 ml[kJoin];
+        u32x4 v[kJoin];
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u) {
+          const int p = part_of(first + min(share + u * shares, n - 1) * span);
+          if (u * shares < n) {
+            ml[u] = __builtin_amdgcn_raw_buffer_load_b64(parts, 4 * (p * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kCoherent);
+            v[u] = __builtin_amdgcn_raw_buffer_load_b128(parts, 4 * (p * Sh::PART + r * HD + c0), 0, kCoherent);
+          }
+        }
+        float top = -INFINITY, sum = 0.f;
+        f32x4 y = {0, 0, 0, 0};
+        auto add = [&](float m2, float l2, f32x4 v2) {
+          const float t = fmaxf(top, m2);
+          const float f1 = top == t ? 1.f : __builtin_amdgcn_exp2f(top - t), f2 = m2 == t ? 1.f : __builtin_amdgcn_exp2f(m2 - t);
+          top = t;
+          sum = sum * f1 + l2 * f2;
+          y = y * f1 + v2 * f2;
+        };
+#pragma unroll
+        for (int u = 0; u < kJoin; ++u)
+          if (share + u * shares < n) add(__uint_as_float(ml[u][0]), __uint_as_float(ml[u][1]), __builtin_bit_cast(f32x4, v[u]));
+        if (shares > 1) {  // (then one round of rows)
+          f32x4* const so = reinterpret_cast<f32x4*>(smem);
+          float2* const sm = reinterpret_cast<float2*>(smem + 4096);
+          so[threadIdx.x] = y;
+          sm[threadIdx.x] = make_float2(top, sum);
+          __syncthreads();
+          if (share == 0)
+            for (int u = 1; u < min(shares, n); ++u) {
+              const int other = threadIdx.x + u * wide * L;
+              add(sm[other].x, sm[other].y, so[other]);
+            }
+          __syncthreads();
+        }
+        if (share != 0 || r0 + group % wide >= live) continue;
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+          if (c0 < 8 * a.hd8)
+            *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r, kh) + c0) =
+                Quad<T>::from(make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
+        } else {
+          const int p = part_of(first);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, 4 * (p * Sh::PART + r * HD + c0), 0, kThrough);
+          if (c0 == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(top), __float_as_uint(sum)}, parts,
+                                                  4 * (p * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kThrough);
+        }
+      }
+    };
+    int* const word = reinterpret_cast<int*>(smem);
+    for (int span = 1, level = 0; span < stretches; span *= kJoin, ++level) {
+      // stretches first, first + span, ... of this group hold its sums
+      const int first = (w - w0) / (span * kJoin) * (span * kJoin);
+      const int n = min(kJoin, (stretches - first + span - 1) / span);
+      if (n > 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this one's sums are in memory
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          int* const counter = a.counters + level * (2 * gridDim.x) + part_of(first);
+          const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+          if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          *word = last;
+        }
+        __syncthreads();
+        const bool joins = *word != 0;
+        __syncthreads();
+        if (!joins) break;
+        join_parts(first, span, n, span * kJoin >= stretches);
       }
     }
   }
-}
-
-// Joins the stretches of an item.  A wave takes R rows, HD / 4 lanes a row; the
-// four waves of a workgroup take the stretches in turn, four loads in flight, and
-// join theirs at last.  The order is that of the keys, whoever finished first.
-template <typename T, int HD, int ROWS>
-__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int most) {
-  constexpr int L = HD / 4, R = 64 / L, PART = ROWS * (HD + 2), BLOCKS = ROWS / R, U = 4;
-  __shared__ float4 so[3][64];
-  __shared__ float2 sm[3][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int rest = blockIdx.x;
-  const int rb = rest % BLOCKS;
-  rest /= BLOCKS;
-  const int mb = rest % a.most_mbs;
-  rest /= a.most_mbs;
-  const int kh = rest % a.kv_heads, b = rest / a.kv_heads;
-  const Seq q = load_seq(a, b, ROWS);
-  if (mb * ROWS + rb * R >= q.n * a.group) return;
-  const int before = tiles_before(a, ROWS, b);
-  const Split split(tiles_before(a, ROWS, a.batch), most);
-  const int first = before + (kh * q.mbs + mb) * q.tiles;
-  const int w0 = split.holder(first), w1 = split.holder(first + q.tiles - 1);
-  if (w0 == w1) return;  // one workgroup had all of it
-  const int row = rb * R + lane / L, c0 = lane % L * 4, m = mb * ROWS + row;
-  float top = -INFINITY, sum = 0.f;
-  float4 o = make_float4(0, 0, 0, 0);
-  auto add = [&](float2 ml, float4 v) {
-    const float t = fmaxf(top, ml.x);
-    const float f1 = top == t ? 1.f : __builtin_amdgcn_exp2f(top - t), f2 = ml.x == t ? 1.f : __builtin_amdgcn_exp2f(ml.x - t);
-    top = t;
-    sum = sum * f1 + ml.y * f2;
-    o = make_float4(o.x * f1 + v.x * f2, o.y * f1 + v.y * f2, o.z * f1 + v.z * f2, o.w * f1 + v.w * f2);
-  };
-  for (int x = w0 + wave; x <= w1; x += 4 * U) {
-    float2 ml[U];
-    float4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int w = min(x + 4 * u, w1);
-      // the first stretch may be the end of its workgroup's
-      const float* const part = a.parts + (int64_t)(2 * w + (w == w0 ? 1 : 0)) * PART;
-      ml[u] = *reinterpret_cast<const float2*>(part + ROWS * HD + 2 * row);
-      v[u] = *reinterpret_cast<const float4*>(part + row * HD + c0);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (x + 4 * u <= w1) add(ml[u], v[u]);
-  }
-  if (wave > 0) {
-    so[wave - 1][lane] = o;
-    sm[wave - 1][lane] = make_float2(top, sum);
-  }
-  __syncthreads();
-  if (wave > 0 || m >= q.n * a.group) return;
-#pragma unroll
-  for (int u = 0; u < 3; ++u) add(sm[u][lane], so[u][lane]);
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  const int node = m / a.group, head = kh * a.group + m - node * a.group;
-  T* const dst = reinterpret_cast<T*>(a.out + (int64_t)(q.first + node) * a.out_bytes) + head * (8 * a.hd8);
-  if (c0 < 8 * a.hd8)
-    *reinterpret_cast<typename Quad<T>::raw*>(dst + c0) = Quad<T>::from(make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
 }
 
 // ---------------------------------------------------------------- variants
@@ -727,7 +798,8 @@ struct Variant {
   static constexpr int HD = HD_, NB = NB_, RW = RW_, NST = NST_, OCC = OCC_;
   typedef TreeShape<HD, NB, RW, NST> Sh;
   static constexpr int GRID = kCus * OCC;
-  static constexpr size_t BYTES = (size_t)2 * GRID * Sh::PART * sizeof(float);
+  static constexpr size_t BYTES = TJK_TREE_COUNTERS + (size_t)2 * GRID * Sh::PART * sizeof(float);
+  static_assert(GRID <= kJoin * kJoin * kJoin && 3 * 2 * GRID * 4 <= TJK_TREE_COUNTERS && BYTES < 0x7fffffff, "counters and 32-bit offsets");
 };
 
 // Calls f with the variant for a head_dim and the rows of the largest tree.
@@ -743,27 +815,30 @@ static auto with_variant(int head_dim, int rows, F&& f) {
   if (rows <= 16) return f(Variant<128, 1, 1, 1, 2>{});
   if (rows <= 32) return f(Variant<128, 2, 1, 1, 2>{});
   if (rows <= 64) return f(Variant<128, 4, 1, 2, 1>{});
-  if (rows <= 128) return f(Variant<128, 2, 4, 3, 2>{});
-  return f(Variant<128, 4, 4, 3, 2>{});
+  return f(Variant<128, 2, 4, 3, 2>{});
 }
 
-// Tiles of the longest context that the block table holds up to which each item
-// is one workgroup's.
-constexpr int kDirectTiles = 32;
+// Whether each item is one workgroup's, with no plan and no joining: by the tiles of
+// the longest context that the block table holds, the lengths being on the device.
+// A workgroup takes about 0.3 us a tile, plan and joining 5 to 10 us.  Bounds at which
+// both take as long, contexts spread from an eighth of the table up, us whole / split:
+// 8 items of 32 tiles 12 / 11, 32 items 12 / 14 (head_dim 64) and 15 / 17 (128), of 63
+// tiles 19 / 15 and 22 / 19; 128 items of 63 tiles 21 / 19 and 23 / 25; 256 items of 65
+// tiles 23 / 28; 512 items of 63 tiles 39 / 41 and 67 / 71, of 125 tiles 67 / 65 and
+// 118 / 118.
+static bool whole_items(int64_t items, int64_t tiles) {
+  return tiles <= std::min<int64_t>(std::max<int64_t>(32, 24 + items / 4), 96);
+}
 
 template <typename T, typename V>
 static int launch_tree(TreeArgs a, hipStream_t s) {
   constexpr int ROWS = V::Sh::ROWS;
   a.most_mbs = (a.max_nodes * a.group + ROWS - 1) / ROWS;
   const int64_t items = (int64_t)a.batch * a.kv_heads * a.most_mbs, tiles = (a.room + kTile - 1) / kTile;
-  if (items * std::max<int64_t>(tiles, 1) > INT32_MAX || items * (ROWS / 2) > INT32_MAX / 256)
+  if (items * (std::max<int64_t>(tiles, 1) + kItemCost) > INT32_MAX || items > INT32_MAX / 256)
     return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
-  a.direct = tiles <= kDirectTiles;
+  a.direct = whole_items(items, tiles);
   tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);
-  if (const int bad = check_launch("tjk_tree_attention")) return bad;
-  if (a.direct) return TJK_OK;
-  const int64_t grid = items * (ROWS * (V::HD / 4) / 64);
-  tree_join_kernel<T, V::HD, ROWS><<<(unsigned)grid, 256, 0, s>>>(a, V::GRID);
   return check_launch("tjk_tree_attention");
 }
 
@@ -811,7 +886,7 @@ extern "C" int tjk_tree_attention(const void* q, int64_t ld_q_token, int64_t ld_
   // (a scale of zero would make no number of what is hidden, -inf)
   const TreeArgs a{static_cast<const char*>(q), 2 * ld_q_token, 2 * ld_q_head, paged(*cache), block_table, ld_table, ctx_lens,
                    cu_nodes, tree_mask, static_cast<char*>(out), 2 * ld_out, std::max(std::fabs(scale) * log2e, FLT_MIN),
-                   static_cast<float*>(workspace), index_errors, scale < 0 ? 0x80008000u : 0u, (int)room, (int)tokens, batch,
+                   static_cast<int*>(workspace), reinterpret_cast<float*>(static_cast<char*>(workspace) + TJK_TREE_COUNTERS), index_errors, scale < 0 ? 0x80008000u : 0u, (int)room, (int)tokens, batch,
                    cache->kv_heads, heads / cache->kv_heads, cache->head_dim / 8, max_nodes, 0, 0};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return with_variant(cache->head_dim, max_nodes * a.group, [&](auto v) {

@@ -21,6 +21,7 @@ ABI_VERSION = 12
 
 F32, F16, BF16, E4M3 = 0, 1, 2, 3
 OK, EINVAL, EUNSUPPORTED = 0, -1, -2
+TREE_COUNTERS = 12288  # bytes of a tree attention's workspace that start at zero
 EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESIDUAL = 0, 1, 2
 
 DTYPE_CODES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}

@@ -527,9 +527,12 @@ def rope_append(qkv: torch.Tensor, positions: torch.Tensor, table: Optional[torc
 
 def tree_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, max_nodes: int) -> torch.Tensor:
     """The workspace of ``tree_attention`` for any batch with these heads and
-    trees of at most max_nodes nodes; calls that share one have to be ordered."""
+    trees of at most max_nodes nodes; calls that share one have to be ordered.
+    Its counters start at zero, and each call leaves them there."""
     need = _lib.load().tjk_tree_attention_bytes(q.shape[1], k_cache.shape[1], q.shape[2], int(max_nodes))
-    return torch.empty(need, dtype=torch.uint8, device=q.device)
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    workspace[:_lib.TREE_COUNTERS].zero_()
+    return workspace
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,

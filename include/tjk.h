@@ -519,12 +519,16 @@ size_t tjk_tree_attention_bytes(int heads, int kv_heads, int head_dim, int max_n
  * refused and counts in *index_errors.
  * path [batch, max_nodes]: the accepted nodes, node 0 first, then -1; count: how
  * many; token: the next token.  A sequence without nodes: -1, 0 and -1.
+ * workspace: tjk_verify_tree_bytes() bytes (which may be 0) on the device, 16-byte
+ * aligned, whatever they hold; calls that share one have to be ordered.
  */
 int tjk_verify_tree(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
                     const int32_t* tokens, const int32_t* parents, const float* accept_u,
                     const float* sample_u, const int32_t* cu_nodes, int32_t* path, int64_t ld_path,
                     int32_t* count, int32_t* token, int* index_errors, int64_t rows, int64_t vocab,
-                    int batch, int max_nodes, void* stream);
+                    int batch, int max_nodes, void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace (0 also for bad sizes). */
+size_t tjk_verify_tree_bytes(int64_t vocab, int batch);
 
 /*
  * Moves the keys and values of accepted nodes together: position ctx_lens[b] +

@@ -46,7 +46,7 @@ def _verify(**kw):
     return _call("tjk_verify_tree", dict(
         target=FAKE, ld_target=100, draft=FAKE, ld_draft=100, tokens=FAKE, parents=FAKE, accept_u=FAKE, sample_u=FAKE,
         cu_nodes=FAKE, path=FAKE, ld_path=4, count=FAKE, token=FAKE, index_errors=None, rows=5, vocab=100, batch=2,
-        max_nodes=4, stream=None), kw)
+        max_nodes=4, workspace=FAKE, workspace_bytes=1 << 40, stream=None), kw)
 
 
 def _compact(**kw):
@@ -124,10 +124,20 @@ def test_attention_refuses_a_small_workspace():
     (dict(vocab=1 << 25, ld_target=1 << 25, ld_draft=1 << 25), EUNSUPPORTED, "large"),
     (dict(rows=1 << 31), EUNSUPPORTED, "large"), (dict(target=None), EINVAL, "null"), (dict(path=None), EINVAL, "null"),
     (dict(sample_u=None), EINVAL, "null"), (dict(parents=None), EINVAL, "null"), (dict(ld_draft=99), EINVAL, "leading"),
-    (dict(ld_path=3), EINVAL, "leading"),
+    (dict(ld_path=3), EINVAL, "leading"), (dict(workspace=FAKE + 8), EUNSUPPORTED, "misaligned"),
 ])
 def test_verify_refusals(kw, status, word):
     assert _verify(**kw) == status and word in _said()
+
+
+def test_verify_refuses_a_small_workspace():
+    big = dict(vocab=200000, ld_target=200000, ld_draft=200000)
+    need = _lib.load().tjk_verify_tree_bytes(200000, 2)
+    assert need > 0 and _lib.load().tjk_verify_tree_bytes(100, 2) == 0
+    assert _verify(workspace_bytes=need - 1, **big) == EINVAL and "workspace" in _said()
+    assert _verify(workspace=None, **big) == EINVAL and "workspace" in _said()
+    for bad in ((0, 2), (100000, 0), (1 << 25, 2)):
+        assert _lib.load().tjk_verify_tree_bytes(*bad) == 0
 
 
 @pytest.mark.parametrize("kw,status,word", [

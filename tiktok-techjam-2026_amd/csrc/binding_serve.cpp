@@ -5,6 +5,8 @@
 
 #include "binding.h"
 
+#include <ATen/ops/empty.h>
+
 namespace {
 
 // [tokens, heads, head_dim] with a unit stride of the last dimension.
@@ -183,15 +185,15 @@ PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t given) {
   });
 }
 
-// (target, draft, tokens, parents, accept_u, sample_u, path, count, token, cu_nodes, index_errors)
+// (target, draft, tokens, parents, accept_u, sample_u, path, count, token, cu_nodes, workspace, index_errors)
 PyObject* verify_tree(PyObject*, PyObject* const* args, Py_ssize_t given) {
-  return guarded(given, 11, [&] {
+  return guarded(given, 12, [&] {
     const at::Tensor &p_t = tensor(args[0], "target"), &q_t = tensor(args[1], "draft"), &tok_t = tensor(args[2], "tokens"),
                      &par_t = tensor(args[3], "parents"), &au_t = tensor(args[4], "accept_u"),
                      &su_t = tensor(args[5], "sample_u"), &path_t = tensor(args[6], "path"),
                      &count_t = tensor(args[7], "count"), &next_t = tensor(args[8], "token"),
                      &cu_t = tensor(args[9], "cu_nodes");
-    const at::Tensor* err_t = tensor_or_none(args[10], "index_errors");
+    const at::Tensor *given_t = tensor_or_none(args[10], "workspace"), *err_t = tensor_or_none(args[11], "index_errors");
     int64_t rows, vocab, ld_p, rows_q, vocab_q, ld_q;
     const float* const p = probabilities(p_t, &rows, &vocab, &ld_p, "target");
     const float* const q = probabilities(q_t, &rows_q, &vocab_q, &ld_q, "draft");
@@ -204,11 +206,17 @@ PyObject* verify_tree(PyObject*, PyObject* const* args, Py_ssize_t given) {
     const float* const au = static_cast<const float*>(vector_of(au_t, rows, at::kFloat, "accept_u"));
     const float* const su = static_cast<const float*>(vector_of(su_t, path.rows, at::kFloat, "sample_u"));
     int* const err = errors_of(err_t);
+    if (given_t && !given_t->is_contiguous()) refuse("workspace must be contiguous");
     const c10::DeviceIndex device =
-        one_device({&p_t, &q_t, &tok_t, &par_t, &au_t, &su_t, &path_t, &count_t, &next_t, &cu_t, err_t});
+        one_device({&p_t, &q_t, &tok_t, &par_t, &au_t, &su_t, &path_t, &count_t, &next_t, &cu_t, given_t, err_t});
+    at::Tensor own;  // freed behind the launch, in the order of the stream
+    const size_t need = tjk_verify_tree_bytes(vocab, (int)path.rows);
+    if (!given_t && need > 0) own = at::empty({(int64_t)need}, p_t.options().dtype(at::kByte));
+    const at::Tensor* const ws_t = given_t ? given_t : need > 0 ? &own : nullptr;
     return launch(device, "tjk_verify_tree", [&](void* stream) {
       return tjk_verify_tree(p, ld_p, q, ld_q, tok, par, au, su, cu, path.data, path.ld, count, next, err, rows, vocab,
-                             (int)path.rows, (int)path.cols, stream);
+                             (int)path.rows, (int)path.cols, ws_t ? ws_t->data_ptr() : nullptr, ws_t ? ws_t->nbytes() : 0,
+                             stream);
     });
   });
 }

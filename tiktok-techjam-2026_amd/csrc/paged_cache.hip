@@ -9,7 +9,7 @@ namespace tjk {
 int check_cache(const char* who, const tjk_paged_cache* c) {
   if (!c || !c->k || !c->v) return fail(TJK_EINVAL, "%s: null cache", who);
   if (c->dtype != TJK_F16 && c->dtype != TJK_BF16) return fail(TJK_EINVAL, "%s: bad cache dtype %d", who, c->dtype);
-  if (c->kv_heads <= 0 || c->pages < 0 || c->head_dim <= 0)
+  if (c->kv_heads <= 0 || c->pages <= 0 || c->head_dim <= 0)
     return fail(TJK_EINVAL, "%s: bad cache shape pages=%lld kv_heads=%d head_dim=%d", who, (long long)c->pages, c->kv_heads,
                 c->head_dim);
   if (c->head_dim % 16 || c->head_dim > 128)
@@ -73,53 +73,70 @@ __global__ __launch_bounds__(256) void rope_append_kernel(AppendArgs a) {
   constexpr int HPW = 64 / G;  // heads of a wave
   const int lane = threadIdx.x & 63, g = lane / G, p = lane % G;
   const int all = a.heads + 2 * a.kv_heads;
-  const int blocks = (all + HPW - 1) / HPW;
-  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t t = wave / blocks;
-  const int h = (int)(wave - t * blocks) * HPW + g;
-  if (t >= a.tokens) return;
+  const uint32_t blocks = (uint32_t)(all + HPW - 1) / HPW;
+  const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), tok = wave / blocks;
+  const int h = (int)(wave - tok * blocks) * HPW + g;
+  if ((int)tok >= a.tokens) return;
+  const int64_t t = tok;
   const int pos = a.positions[t];
-  const bool placed = pos >= 0 && pos < a.n_positions;
-  int slot = a.slots ? a.slots[t] : -1;
-  const bool stored = placed && slot >= 0 && (slot >> a.cache.shift) < a.cache.pages;
-  if (h == 0 && p == 0 && a.index_errors && (!placed || (slot >= 0 && !stored))) atomicAdd(a.index_errors, 1);
+  const int slot = a.slots ? a.slots[t] : -1;
   const bool in = h < all && 2 * p < a.hd8;
   const int half = a.rot8 >> 1;
   const bool turned = p < half;
-  const int c0 = turned && !INTER ? p : 2 * p, c1 = turned && !INTER ? p + half : 2 * p + 1;
+  const int c0 = !in ? 0 : turned && !INTER ? p : 2 * p, c1 = !in ? 0 : turned && !INTER ? p + half : 2 * p + 1;
+
+  // every load goes out before the first is waited for, but for the angles, which
+  // lie where the position says
+  const T* const src = reinterpret_cast<const T*>(a.qkv + t * a.token_bytes + (int64_t)(in ? h : 0) * a.head_bytes);
+  const typename Oct<T>::raw r0 = Oct<T>::load(src + 8 * c0), r1 = Oct<T>::load(src + 8 * c1);
+  const float* const gamma = h < a.heads ? a.q_gamma : h < a.heads + a.kv_heads ? a.k_gamma : nullptr;
+  Oct<float>::raw g0{}, g1{};
+  if (gamma) {
+    g0 = Oct<float>::load(gamma + 8 * c0);
+    g1 = Oct<float>::load(gamma + 8 * c1);
+  }
+  const bool placed = pos >= 0 && pos < a.n_positions;
+  const bool stored = placed && slot >= 0 && (slot >> a.cache.shift) < a.cache.pages;
+  const bool turns = in && turned && placed && h < a.heads + a.kv_heads;
+  Oct<float>::raw w0{}, w1{};
+  if (turns) {
+    const float* const cs = a.table + ((int64_t)pos * (4 * a.rot8) + 8 * p) * 2;
+    w0 = Oct<float>::load(cs);
+    w1 = Oct<float>::load(cs + 8);
+  }
+  if (h == 0 && p == 0 && a.index_errors && (!placed || (slot >= 0 && !stored))) atomicAdd(a.index_errors, 1);
 
   float x[2][8];
-  const T* const src =
-      reinterpret_cast<const T*>(a.qkv + t * a.token_bytes + (int64_t)(in ? h : 0) * a.head_bytes);
-  Oct<T>::to(Oct<T>::load(src + 8 * (in ? c0 : 0)), x[0]);
-  Oct<T>::to(Oct<T>::load(src + 8 * (in ? c1 : 0)), x[1]);
-  if (h < a.heads + a.kv_heads) {
-    const float* const gamma = h < a.heads ? a.q_gamma : a.k_gamma;
-    float sum = 0.f;
+  Oct<T>::to(r0, x[0]);
+  Oct<T>::to(r1, x[1]);
+  float sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i], x[u][i], sum);
+  sum = group_sum<G>(in ? sum : 0.f);
+  if (gamma) {
+    const float r = 1.0f / sqrtf(sum / (float)(8 * a.hd8) + a.eps);
+    float f[2][8];
+    Oct<float>::to(g0, f[0]);
+    Oct<float>::to(g1, f[1]);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(x[u][i], x[u][i], sum);
-    sum = group_sum<G>(in ? sum : 0.f);
-    if (gamma && in) {
-      const float r = 1.0f / sqrtf(sum / (float)(8 * a.hd8) + a.eps);
+      for (int i = 0; i < 8; ++i) x[u][i] *= r * f[u][i];
+  }
+  if (turns) {
+    float w[2][8];
+    Oct<float>::to(w0, w[0]);
+    Oct<float>::to(w1, w[1]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[0][i] *= r * gamma[8 * c0 + i];
-        x[1][i] *= r * gamma[8 * c1 + i];
-      }
-    }
-    if (turned && placed && in) {
-      const float2* const cs = reinterpret_cast<const float2*>(a.table) + (int64_t)pos * (4 * a.rot8);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // the pair's members: element i of both pieces, or elements 2 j, 2 j + 1 of one
-        float &u = INTER ? x[i >> 2][2 * (i & 3)] : x[0][i], &v = INTER ? x[i >> 2][2 * (i & 3) + 1] : x[1][i];
-        const float2 w = cs[8 * p + i];
-        const float y = u * w.x - v * w.y;
-        v = v * w.x + u * w.y;
-        u = y;
-      }
+    for (int i = 0; i < 8; ++i) {
+      // the pair's members: element i of both pieces, or elements 2 j, 2 j + 1 of one
+      float &u = INTER ? x[i >> 2][2 * (i & 3)] : x[0][i], &v = INTER ? x[i >> 2][2 * (i & 3) + 1] : x[1][i];
+      const float c = w[i >> 2][2 * (i & 3)], s = w[i >> 2][2 * (i & 3) + 1];
+      const float y = u * c - v * s;
+      v = v * c + u * s;
+      u = y;
     }
   }
   if (!in) return;
@@ -131,12 +148,12 @@ __global__ __launch_bounds__(256) void rope_append_kernel(AppendArgs a) {
     reinterpret_cast<uint4*>(row)[c0] = Oct<T>::from(x[0]);
     reinterpret_cast<uint4*>(row)[c1] = Oct<T>::from(x[1]);
   };
-  const int kh = h < a.heads + a.kv_heads ? h - a.heads : h - a.heads - a.kv_heads;
   if (h < a.heads) {
     put(a.q_out + t * a.q_token_bytes + h * a.q_head_bytes);
     return;
   }
   const bool key = h < a.heads + a.kv_heads;
+  const int kh = key ? h - a.heads : h - a.heads - a.kv_heads;
   if (key && a.k_out) put(a.k_out + t * a.k_token_bytes + kh * a.k_head_bytes);
   if (stored)
     put((key ? a.cache.k : a.cache.v) + (int64_t)(slot >> a.cache.shift) * a.cache.page_bytes + kh * a.cache.head_bytes +
@@ -145,9 +162,17 @@ __global__ __launch_bounds__(256) void rope_append_kernel(AppendArgs a) {
 
 // ------------------------------------------------------------ compaction
 //
-// A wave moves the rows of one (layer, sequence, head, keys or values), a
-// lane one 16-byte piece of a row: in batches, loads ahead of stores.  Row
+// A wave moves the keys and the values of one (layer, sequence, head), a lane one
+// 16-byte piece of a row: the places first, then the loads, then the stores.  Row
 // path[i] >= i goes to row i, so no row is overwritten before it is read.
+//
+// Bound by latency (counts and path, places, rows: three passages of memory one
+// after the other), then by memory, which does not like 256 bytes here and 256
+// there: 24 layers x 64 sequences x 8 heads of 128, 7 rows each, 27 us, 3.5 TB/s read
+// and written; four layers of 8 sequences 5 us.  Keys and values in waves of their
+// own 29 and 6 us, two instructions of rows in flight instead of four 28.5 and 4.4.
+// Loads where nothing moves, from one place for all, to spare the lanes' conditions:
+// 40 and 13.
 
 struct CompactArgs {
   Paged cache;
@@ -166,42 +191,61 @@ struct CompactArgs {
 
 template <int CPR>  // lanes per row
 __global__ __launch_bounds__(256) void compact_kernel(CompactArgs a) {
-  constexpr int RPI = 64 / CPR, U = 4;
+  constexpr int RPI = 64 / CPR, U = 4;  // rows of an instruction, instructions in flight
   const int lane = threadIdx.x & 63, r = lane / CPR, c = lane % CPR;
-  const int64_t wave = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int per = 2 * a.kv_heads;
-  const int64_t lb = wave / per;
-  const int hk = (int)(wave - lb * per);
-  const int layer = (int)(lb / a.batch), b = (int)(lb - (int64_t)layer * a.batch);
+  const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), lb = wave / (uint32_t)a.kv_heads;
+  const int h = (int)(wave - lb * a.kv_heads), layer = (int)(lb / (uint32_t)a.batch), b = (int)(lb - layer * a.batch);
   if (layer >= a.layers) return;
+  char* const kb = a.cache.k + layer * a.layer_bytes + h * a.cache.head_bytes;
+  char* const vb = a.cache.v + layer * a.layer_bytes + h * a.cache.head_bytes;
   const int n = min(a.count[b], a.max_nodes);
-  const int ctx = max(a.ctx_lens[b], 0);
-  char* const base = ((hk & 1) ? a.cache.v : a.cache.k) + layer * a.layer_bytes + (hk >> 1) * a.cache.head_bytes;
+  const int64_t ctx = max(a.ctx_lens[b], 0);
   const int32_t* const row = a.table + b * a.ld_table;
+  const int32_t* const path = a.path + b * a.ld_path;
+  const int64_t room = (int64_t)a.table_cols << a.cache.shift;
   const int mask = (1 << a.cache.shift) - 1;
-  auto place = [&](int64_t x) -> char* {  // row of position x, null outside the cache
-    if (x >= (int64_t)a.table_cols << a.cache.shift) return nullptr;
-    const int pg = page_of(row, (int)(x >> a.cache.shift), a.cache.pages);
-    return pg < 0 ? nullptr : base + pg * a.cache.page_bytes + (x & mask) * (int64_t)a.cache.row_bytes;
-  };
   for (int i0 = 1; i0 < n; i0 += U * RPI) {
-    uint4 v[U];
-    char* dst[U];
+    int64_t src[U], dst[U];
+    int from[U], ps[U], pd[U];
+    bool named[U], moves[U], lost = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) from[u] = path[min(i0 + u * RPI + r, a.max_nodes - 1)];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * RPI + r;
-      dst[u] = nullptr;
-      if (i < n && c < a.hd8) {
-        const int from = a.path[b * a.ld_path + i];
-        const char* const src = from >= i && from < a.max_nodes ? place((int64_t)ctx + from) : nullptr;
-        dst[u] = src ? place((int64_t)ctx + i) : nullptr;
-        if (dst[u]) v[u] = reinterpret_cast<const uint4*>(src)[c];
-        else if (layer == 0 && hk == 0 && c == 0 && a.index_errors) atomicAdd(a.index_errors, 1);
+      named[u] = i < n && from[u] >= i && from[u] < a.max_nodes && ctx + from[u] < room;  // (and ctx + i, which is less)
+      ps[u] = page_of(row, named[u] ? (int)((ctx + from[u]) >> a.cache.shift) : 0, a.cache.pages);
+      pd[u] = page_of(row, named[u] ? (int)((ctx + i) >> a.cache.shift) : 0, a.cache.pages);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * RPI + r;
+      const bool there = named[u] && ps[u] >= 0 && pd[u] >= 0;
+      moves[u] = there && c < a.hd8;
+      lost |= i < n && !there;
+      src[u] = ps[u] * a.cache.page_bytes + ((ctx + from[u]) & mask) * a.cache.row_bytes + 16 * c;
+      dst[u] = pd[u] * a.cache.page_bytes + ((ctx + i) & mask) * a.cache.row_bytes + 16 * c;
+    }
+    uint4 k[U], v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k[u] = v[u] = make_uint4(0, 0, 0, 0);
+      if (moves[u]) {
+        k[u] = *reinterpret_cast<const uint4*>(kb + src[u]);
+        v[u] = *reinterpret_cast<const uint4*>(vb + src[u]);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (dst[u]) reinterpret_cast<uint4*>(dst[u])[c] = v[u];
+      if (moves[u]) {
+        *reinterpret_cast<uint4*>(kb + dst[u]) = k[u];
+        *reinterpret_cast<uint4*>(vb + dst[u]) = v[u];
+      }
+    if (lost && layer == 0 && h == 0 && c == 0 && a.index_errors) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * RPI + r < n && !moves[u]) atomicAdd(a.index_errors, 1);
+    }
   }
 }
 
@@ -256,7 +300,7 @@ extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_hea
     constexpr int G = decltype(group)::value;
     const int64_t blocks = (heads + 2 * (int64_t)kv_heads + 64 / G - 1) / (64 / G);
     const int64_t grid = (tokens * blocks + 3) / 4;
-    if (grid > UINT32_MAX / 256) return fail(TJK_EUNSUPPORTED, "%s: %lld tokens are too many", who, (long long)tokens);
+    if (grid > UINT32_MAX / 256 || tokens * blocks > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: %lld tokens are too many", who, (long long)tokens);
     rope_append_kernel<T, G, decltype(inter)::value><<<(unsigned)grid, 256, 0, s>>>(a);
     return check_launch(who);
   };
@@ -284,17 +328,18 @@ extern "C" int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64
   if (table_cols > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: block table too wide", who);
   if (layers > 1 && (layer_stride < 0 || layer_stride % 8))
     return fail(TJK_EUNSUPPORTED, "%s: the layers' stride must be a multiple of 8", who);
-  if (layers == 0 || batch == 0 || max_nodes < 2) return TJK_OK;
+  if (layers == 0 || batch == 0 || max_nodes < 2 || table_cols == 0) return TJK_OK;
   if (!block_table || !ctx_lens || !path || !count) return fail(TJK_EINVAL, "%s: null pointer", who);
   if (ld_table < table_cols || ld_path < max_nodes) return fail(TJK_EINVAL, "%s: leading dimension too small", who);
-  const int64_t waves = (int64_t)layers * batch * 2 * cache->kv_heads;
-  if ((waves + 3) / 4 > UINT32_MAX / 256) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
+  const int64_t waves = (int64_t)layers * batch * cache->kv_heads;
+  if (waves > INT32_MAX / 64) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
   const CompactArgs a{paged(*cache), 2 * layer_stride, block_table, ld_table, (int)table_cols, ctx_lens, path, ld_path,
                       max_nodes, count, index_errors, layers, batch, cache->kv_heads, cache->head_dim / 8};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const unsigned grid = (unsigned)((waves + 3) / 4);
-  if (cache->head_dim <= 32) compact_kernel<4><<<grid, 256, 0, s>>>(a);
-  else if (cache->head_dim <= 64) compact_kernel<8><<<grid, 256, 0, s>>>(a);
-  else compact_kernel<16><<<grid, 256, 0, s>>>(a);
+  auto go = [&](auto lanes) { compact_kernel<decltype(lanes)::value><<<grid, 256, 0, s>>>(a); };
+  if (cache->head_dim <= 32) go(std::integral_constant<int, 4>{});
+  else if (cache->head_dim <= 64) go(std::integral_constant<int, 8>{});
+  else go(std::integral_constant<int, 16>{});
   return check_launch(who);
 }

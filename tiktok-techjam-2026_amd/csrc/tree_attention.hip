@@ -267,11 +267,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   }
 
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_void*)smem;
-  // Keys are read one piece of 16 rows at a time, values two neighbouring pieces of
-  // 8 rows: neither meets a bank twice, in halves of 128 bytes or in whole passes.
+  // A 16-byte read serves lanes 0 - 3, 12 - 15 and 20 - 27 together (then 4 - 11, 16 -
+  // 19, 28 - 31, and so in the other half): a piece of rows 0 - 3 and 12 - 15 and its
+  // neighbour of rows 4 - 11.  A transposing read serves 32 lanes, two neighbouring
+  // pieces of 8 rows.  Neither meets a bank twice.
   auto swz = [](int r) {
     const int r0 = r & 1, r1 = r >> 1 & 1, r2 = r >> 2 & 1, r3 = r >> 3 & 1;
-    return CPR == 16 ? (r2 ^ r3) | r0 << 1 | r1 << 2 | r2 << 3 : (r0 ^ r3) | r1 << 1 | (r0 ^ r2) << 2;
+    return CPR == 16 ? r2 | r0 << 1 | r1 << 2 | (r2 ^ r3) << 3 : r2 | r1 << 1 | (r2 ^ r3) << 2;
   };
   // of the DMA instructions of 16 rows (RW = 4: of this wave's)
   uint32_t voff[RW == 1 ? NV : 1];

@@ -10,6 +10,8 @@
 // token is drawn from r_k.  Products and sums in 64 bits: a decision at a border
 // does not hang on the order of a sum.
 
+#include <algorithm>
+
 #include "tjk_common.h"
 
 namespace tjk {
@@ -28,11 +30,33 @@ struct VerifyArgs {
   int32_t* count;
   int32_t* token;
   int* index_errors;
+  struct Slot* slots;  // [batch][2][parts]
   int64_t rows;
-  int max_nodes, vocab;
+  int batch, max_nodes, vocab;
+  int parts, part;  // workgroups of a sequence, elements of each
 };
 
-constexpr int kVerifyThreads = 1024;
+// The walk needs p and q at the drafted tokens only, which the lanes of a wave
+// gather at once, and a pass over the vocabulary for each refusal: the sum W_k.
+// The last such sum also says where the next token lies, so that only the part
+// that holds it is read again.  A sequence's vocabulary is cut into `parts`, a
+// workgroup each; every one walks the same walk from the same numbers and meets
+// the others at the sums only: each puts its own in the workspace and reads
+// theirs.  It waits a bounded time: a sum that does not come (workgroups of other
+// work may hold the chip) it computes itself, in the same order, so nothing hangs on
+// who was there.
+
+constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kMostParts = 64;
+constexpr int kMostGroups = 256;  // workgroups of a launch
+constexpr int kPartElements = 16384;  // least of a part
+constexpr int kPolls = 256;  // of a missing sum: about 50 us
+
+struct Slot {  // of a workgroup's sum: its halves, each with the round it belongs to
+  uint64_t half[2];
+};
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may begin anywhere
 
 __device__ __forceinline__ double residual(float p, double c, float q) {
   const double r = (double)p - c * (double)q;
@@ -45,116 +69,265 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-__global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
-  constexpr int NW = kVerifyThreads / 64;
-  __shared__ double part[NW];
-  __shared__ int found[NW];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Four weights from x on (x + 4 past `end`: what there is).
+__device__ __forceinline__ void weights4(const float* p, const float* q, double c, int x, int end, double (&w)[4]) {
+  float a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
+  if (x + 4 <= end) {
+    const f32x4u v = *reinterpret_cast<const f32x4u*>(p + x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = v[i];
+    if (c != 0) {
+      const f32x4u u = *reinterpret_cast<const f32x4u*>(q + x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b[i] = u[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (x + i < end) a[i] = p[x + i], b[i] = c != 0 ? q[x + i] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = residual(a[i], c, b[i]);
+}
+
+__global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
+  __shared__ double wave_sums[2][kWaves], part_sums[kMostParts];
+  __shared__ int missing;
+  const int b = blockIdx.x % a.batch, part = blockIdx.x / a.batch;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t first = max(a.cu_nodes[b], 0);
-  const int n = (int)min((int64_t)min(max(a.cu_nodes[b + 1] - a.cu_nodes[b], 0), a.max_nodes), max(a.rows - first, (int64_t)0));
-  const int parent = lane > 0 && lane < n ? a.parents[first + lane] : -1;
+  const int n = (int)min((int64_t)min(max(a.cu_nodes[b + 1] - (int)first, 0), a.max_nodes), max(a.rows - first, (int64_t)0));
   int32_t* const path = a.path + b * a.ld_path;
+  const bool writes = part == 0 && tid == 0;
   if (n == 0) {
-    for (int i = tid; i < a.max_nodes; i += kVerifyThreads) path[i] = -1;
-    if (tid == 0) a.count[b] = 0, a.token[b] = -1;
+    if (part == 0)
+      for (int i = tid; i < a.max_nodes; i += kThreads) path[i] = -1;
+    if (writes) a.count[b] = 0, a.token[b] = -1;
     return;
   }
-  // a thread's elements lie together, so the threads' sums are in order
-  const int per = (a.vocab + kVerifyThreads - 1) / kVerifyThreads;
-  const int lo = min(tid * per, a.vocab), hi = min(lo + per, a.vocab);
-  auto thread_sum = [&](const float* p, const float* q, double c) {
+  // lane j: node j, and p and q of its token behind its parent
+  int parent = -1;
+  float pj = 0.f, qj = 0.f, uj = 0.f;
+  if (lane > 0 && lane < n) {
+    parent = a.parents[first + lane];
+    const int x = a.tokens[first + lane];
+    uj = a.accept_u[first + lane];
+    if (parent < 0 || parent >= lane) {
+      parent = -1;
+    } else if (x >= 0 && x < a.vocab) {
+      pj = a.target[(first + parent) * a.ld_target + x];
+      qj = a.draft[(first + parent) * a.ld_draft + x];
+    } else {
+      pj = -1.f;  // of no token: refused
+      if (part == 0 && wave == 0 && a.index_errors) atomicAdd(a.index_errors, 1);
+    }
+  }
+  const float *p = a.target + first * a.ld_target, *q = a.draft + first * a.ld_draft;
+
+  // A part's sum: its waves' stretches, each 256 elements at a time.
+  int flip = 0;
+  auto sum_part = [&](int which, double c) {
+    const int lo = which * a.part + wave * (a.part / kWaves), end = min(min(lo + a.part / kWaves, (which + 1) * a.part), a.vocab);
     double s = 0;
-    for (int x = lo; x < hi; ++x) s += residual(p[x], c, c == 0 ? 0.f : q[x]);
-    return s;
-  };
-  auto block_sum = [&](double s) {
+    int x = lo + 4 * lane;
+    for (; x - 4 * lane + 1024 <= end; x += 1024) {
+      double w[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) weights4(p, q, c, x + 256 * u, end, w[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += (w[u][0] + w[u][1]) + (w[u][2] + w[u][3]);
+    }
+    for (; x < end; x += 256) {
+      double w[4];
+      weights4(p, q, c, x, end, w);
+      s += (w[0] + w[1]) + (w[2] + w[3]);
+    }
     s = wave_sum64(s);
-    __syncthreads();
-    if (lane == 0) part[wave] = s;
+    flip ^= 1;  // (the last sums may still be read)
+    if (lane == 0) wave_sums[flip][wave] = s;
     __syncthreads();
     s = 0;
-    for (int w = 0; w < NW; ++w) s += part[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s += wave_sums[flip][w];
     return s;
   };
+  int round = 0;
+  // The whole sum at (p, q, c); part_sums has the parts'.
+  auto sum_all = [&](double c) {
+    ++round;
+    const double mine = sum_part(part, c);
+    if (a.parts == 1) {
+      if (tid == 0) part_sums[0] = mine;
+      __syncthreads();
+      return mine;
+    }
+    Slot* const slots = a.slots + (b * 2 + (round & 1)) * a.parts;
+    const uint64_t bits = __builtin_bit_cast(uint64_t, mine), tag = (uint64_t)round << 32;
+    if (tid == 0) {
+      __hip_atomic_store(&slots[part].half[0], tag | (uint32_t)bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&slots[part].half[1], tag | bits >> 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      missing = 0;
+    }
+    __syncthreads();
+    if (tid < a.parts) {
+      uint64_t lo = tag | (uint32_t)bits, hi = tag | bits >> 32;
+      if (tid != part) {
+        for (int i = 0; i < kPolls; ++i) {
+          lo = __hip_atomic_load(&slots[tid].half[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          hi = __hip_atomic_load(&slots[tid].half[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (lo >> 32 == (uint64_t)round && hi >> 32 == (uint64_t)round) break;
+          __builtin_amdgcn_s_sleep(1);
+        }
+      }
+      if (lo >> 32 == (uint64_t)round && hi >> 32 == (uint64_t)round)
+        part_sums[tid] = __builtin_bit_cast(double, hi << 32 | (uint32_t)lo);
+      else
+        part_sums[tid] = -1, missing = 1;
+    }
+    __syncthreads();
+    if (missing) {
+      for (int i = 0; i < a.parts; ++i) {
+        if (part_sums[i] >= 0) continue;  // (the same in every thread)
+        const double s = sum_part(i, c);
+        __syncthreads();
+        if (tid == 0) part_sums[i] = s;
+        __syncthreads();
+      }
+      sum_part(part, c);  // its waves' sums again, which the search wants
+    }
+    double s = 0;
+    for (int i = 0; i < a.parts; ++i) s += part_sums[i];
+    return s;
+  };
+
   int cur = 0, done = 1, tried = 0;
-  if (tid == 0) path[0] = 0;
+  if (writes) path[0] = 0;
   double c = 0, mass = 1;
-  const float *p = a.target + first * a.ld_target, *q = a.draft + first * a.ld_draft;
+  bool summed = false;  // mass is the sum at c
   while (true) {
     const uint64_t left = __ballot(parent == cur && lane > tried);
     if (left == 0) break;
     const int j = __ffsll((unsigned long long)left) - 1;
     tried = j;
-    const int x = a.tokens[first + j];
-    bool taken = false;
-    if (x >= 0 && x < a.vocab)
-      taken = (double)a.accept_u[first + j] * (double)q[x] * mass < residual(p[x], c, c == 0 ? 0.f : q[x]);
-    else if (tid == 0 && a.index_errors)
-      atomicAdd(a.index_errors, 1);
-    if (taken) {
-      if (tid == 0) path[done] = j;
+    const float pt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, pj), j));
+    const float qt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, qj), j));
+    const float ut = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, uj), j));
+    if ((double)ut * (double)qt * mass < residual(pt, c, c == 0 ? 0.f : qt)) {
+      if (writes) path[done] = j;
       ++done;
       cur = j;
       c = 0;
       mass = 1;
+      summed = false;
       p = a.target + (first + j) * a.ld_target;
       q = a.draft + (first + j) * a.ld_draft;
     } else {
       c += mass;
-      mass = block_sum(thread_sum(p, q, c));
+      mass = sum_all(c);
+      summed = true;
     }
   }
-  for (int i = done + tid; i < a.max_nodes; i += kVerifyThreads) path[i] = -1;
-  double mine = thread_sum(p, q, c), sum = block_sum(mine);
-  if (!(sum > 0)) {
+  if (part == 0)
+    for (int i = done + tid; i < a.max_nodes; i += kThreads) path[i] = -1;
+  if (!summed) mass = sum_all(c);
+  if (!(mass > 0) && c != 0) {
     c = 0;
-    mine = thread_sum(p, q, c);
-    sum = block_sum(mine);
+    mass = sum_all(c);
   }
-  // running sums: of the waves before, of the lanes before
-  double before = 0;
-  for (int w = 0; w < wave; ++w) before += part[w];
-  double incl = mine;
+  if (writes) a.count[b] = done;
+  if (!(mass > 0)) {
+    if (writes) a.token[b] = -1;
+    return;
+  }
+  // the part, and in it the wave, whose sum passes the point; if rounding leaves
+  // none, the last with any weight
+  const double point = (double)a.sample_u[b] * mass;
+  double before = 0, cum = 0;
+  int where = -1;
+  for (int i = 0; i < a.parts; ++i) {
+    if (part_sums[i] > 0) where = i, before = cum;
+    cum += part_sums[i];
+    if (cum > point && part_sums[i] > 0) break;
+  }
+  if (where != part) return;
+  cum = before;
+  int at = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    const double s = wave_sums[flip][w];
+    if (s > 0) at = w, before = cum;
+    cum += s;
+    if (cum > point && s > 0) break;
+  }
+  if (at != wave) return;
+  // 1024 elements at a time, 16 to a lane
+  const int lo = part * a.part + wave * (a.part / kWaves), end = min(min(lo + a.part / kWaves, (part + 1) * a.part), a.vocab);
+  int last = -1;
+  for (int x0 = lo; x0 < end; x0 += 1024) {
+    const int x = x0 + 16 * lane;
+    double w[4][4], s = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double up = __shfl_up(incl, d);
-    if (lane >= d) incl += up;
-  }
-  double at = before + incl - mine;
-  const double point = (double)a.sample_u[b] * sum;
-  int mine_first = INT32_MAX, last = -1;
-  for (int x = lo; x < hi; ++x) {
-    const double r = residual(p[x], c, c == 0 ? 0.f : q[x]);
-    at += r;
-    if (r > 0) last = x;
-    if (at > point && r > 0) {
-      mine_first = x;
-      break;
+    for (int u = 0; u < 4; ++u) weights4(p, q, c, x + 4 * u, end, w[u]);
+    int mine = -1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s += w[i >> 2][i & 3];
+      if (w[i >> 2][i & 3] > 0) mine = x + i;
     }
+    double incl = s;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double up = __shfl_up(incl, d);
+      if (lane >= d) incl += up;
+    }
+    const uint64_t some = __ballot(mine >= 0), past = __ballot(before + incl > point && s > 0);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      if (lane == l) {
+        double run = before + incl - s;
+        int token = mine;
+#pragma unroll
+        for (int i = 15; i >= 0; --i) {
+          double upto = run;
+#pragma unroll
+          for (int k = 0; k <= i; ++k) upto += w[k >> 2][k & 3];
+          if (upto > point && w[i >> 2][i & 3] > 0) token = x + i;
+        }
+        a.token[b] = token;
+      }
+      return;
+    }
+    if (some) last = __builtin_amdgcn_readlane(mine, 63 - __builtin_clzll(some));
+    before += __shfl(incl, 63);
   }
-  // the first token past the point; if rounding leaves none, the last with any weight
-  for (int d = 1; d < 64; d <<= 1) {
-    mine_first = min(mine_first, __shfl_xor(mine_first, d));
-    last = max(last, __shfl_xor(last, d));
-  }
-  __shared__ int lasts[NW];
-  if (lane == 0) found[wave] = mine_first, lasts[wave] = last;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < NW; ++w) mine_first = min(mine_first, found[w]), last = max(last, lasts[w]);
-    a.count[b] = done;
-    a.token[b] = mine_first != INT32_MAX ? mine_first : last;
-  }
+  if (lane == 0) a.token[b] = last;
+}
+
+__global__ __launch_bounds__(256) void clear_slots_kernel(uint64_t* p, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
+// Workgroups of a sequence.
+static int verify_parts(int64_t vocab, int batch) {
+  const int64_t most = std::min<int64_t>(kMostParts, batch > 0 ? kMostGroups / batch : 1);
+  return (int)std::max<int64_t>(1, std::min(most, vocab / kPartElements));
 }
 
 }  // namespace tjk
 
 using namespace tjk;
 
+extern "C" size_t tjk_verify_tree_bytes(int64_t vocab, int batch) {
+  if (vocab <= 0 || vocab > 1 << 24 || batch <= 0 || batch > 1 << 20) return 0;
+  const int parts = verify_parts(vocab, batch);
+  return parts > 1 ? (size_t)batch * 2 * parts * sizeof(Slot) : 0;
+}
+
 extern "C" int tjk_verify_tree(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
                                const int32_t* tokens, const int32_t* parents, const float* accept_u, const float* sample_u,
                                const int32_t* cu_nodes, int32_t* path, int64_t ld_path, int32_t* count, int32_t* token,
-                               int* index_errors, int64_t rows, int64_t vocab, int batch, int max_nodes, void* stream) {
+                               int* index_errors, int64_t rows, int64_t vocab, int batch, int max_nodes, void* workspace,
+                               size_t workspace_bytes, void* stream) {
   const char* const who = "tjk_verify_tree";
   if (rows < 0 || vocab <= 0 || batch < 0 || max_nodes <= 0)
     return fail(TJK_EINVAL, "%s: bad shape rows=%lld vocab=%lld batch=%d max_nodes=%d", who, (long long)rows,
@@ -167,8 +340,20 @@ extern "C" int tjk_verify_tree(const float* target, int64_t ld_target, const flo
     return fail(TJK_EINVAL, "%s: null pointer", who);
   if (ld_target < vocab || ld_draft < vocab || ld_path < max_nodes)
     return fail(TJK_EINVAL, "%s: leading dimension too small", who);
+  const size_t need = tjk_verify_tree_bytes(vocab, batch);
+  if (workspace_bytes < need || (need > 0 && !workspace))
+    return fail(TJK_EINVAL, "%s: a workspace of %zu bytes, %zu needed", who, workspace ? workspace_bytes : 0, need);
+  if ((uintptr_t)workspace & 15) return fail(TJK_EUNSUPPORTED, "%s: misaligned workspace", who);
+  const int parts = verify_parts(vocab, batch);
+  const int64_t part = ((vocab + parts - 1) / parts + 256 * kWaves - 1) / (256 * kWaves) * (256 * kWaves);
   const VerifyArgs a{target, draft, ld_target, ld_draft, tokens, parents, accept_u, sample_u, cu_nodes, path, ld_path, count,
-                     token, index_errors, rows, max_nodes, (int)vocab};
-  verify_kernel<<<(unsigned)batch, kVerifyThreads, 0, reinterpret_cast<hipStream_t>(stream)>>>(a);
+                     token, index_errors, static_cast<Slot*>(workspace), rows, batch, max_nodes, (int)vocab, parts, (int)part};
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (parts > 1) {
+    const int words = (int)(need / sizeof(uint64_t));
+    clear_slots_kernel<<<(unsigned)((words + 255) / 256), 256, 0, s>>>(static_cast<uint64_t*>(workspace), words);
+    if (const int bad = check_launch(who)) return bad;
+  }
+  verify_kernel<<<(unsigned)(batch * parts), kThreads, 0, s>>>(a);
   return check_launch(who);
 }

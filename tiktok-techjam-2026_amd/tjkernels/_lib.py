@@ -86,7 +86,8 @@ _SIGNATURES = {
                                   _i32, _f32, _vp, ctypes.c_size_t, _vp, _vp]),
     "tjk_tree_attention_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32]),
     "tjk_verify_tree": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64,
-                               _i32, _i32, _vp]),
+                               _i32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "tjk_verify_tree_bytes": (ctypes.c_size_t, [_i64, _i32]),
     "tjk_compact_cache": (_i32, [_cache, _i32, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp]),
 }
 

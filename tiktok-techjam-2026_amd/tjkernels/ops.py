@@ -565,7 +565,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 
 def verify_tree(target: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor,
                 accept_u: torch.Tensor, sample_u: torch.Tensor, path: torch.Tensor, count: torch.Tensor,
-                token: torch.Tensor, cu_nodes: torch.Tensor, index_errors: Optional[torch.Tensor] = None) -> torch.Tensor:
+                token: torch.Tensor, cu_nodes: torch.Tensor, workspace: Optional[torch.Tensor] = None,
+                index_errors: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Verifies drafted tokens against the target's probabilities, so that the
     tokens kept are distributed as the target's.
 
@@ -578,8 +579,12 @@ def verify_tree(target: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor,
     the residual distribution with ``sample_u`` fp32 [B], the lowest that passes.
 
     Writes ``path`` int32 [B, max_nodes <= 64] (the accepted nodes, 0 first, then
-    -1), ``count`` int32 [B] and ``token`` int32 [B] (-1 without any weight)."""
-    _serve().verify_tree(target, draft, tokens, parents, accept_u, sample_u, path, count, token, cu_nodes, index_errors)
+    -1), ``count`` int32 [B] and ``token`` int32 [B] (-1 without any weight).
+    ``workspace`` (uint8, tjk_verify_tree_bytes of the vocabulary and the batch, which
+    may be none) is allocated when it is not given; calls that share one have to
+    be ordered."""
+    _serve().verify_tree(target, draft, tokens, parents, accept_u, sample_u, path, count, token, cu_nodes, workspace,
+                         index_errors)
     return token
 
 

@@ -39,7 +39,7 @@ struct TreeArgs {
 //
 // An item is a block of rows of one (sequence, key head): rows m = node * group +
 // query head, ROWS of them.  Its keys are cut into tiles of 32.  An item counts
-// kItemCost units, for what it costs beside its tiles, and one for each tile; all
+// COST units, for what it costs beside its tiles, and one for each tile; all
 // items' units are numbered through, and every workgroup takes an equal stretch of
 // them: lengths are known on the device only, and a long sequence next to short
 // ones is split as finely as it needs.  A stretch that is a whole item writes its rows;
@@ -52,8 +52,20 @@ struct TreeArgs {
 
 constexpr int kTile = 32;     // keys of a tile
 constexpr int kJoin = 8;      // sums that are joined at a time
-constexpr int kItemCost = 8;  // an item's start and end take as long as about so many tiles
 constexpr int kMinUnits = 8;  // of a workgroup: below, the joining costs more than the splitting gives
+
+// The launch's arguments, loaded again: kept over the tiles' loop, they would take
+// its scalar registers, and the loop reload them from lanes of a vector register.
+typedef const __attribute__((address_space(4))) TreeArgs ConstArgs;
+__device__ __forceinline__ ConstArgs& fresh_args() {
+  ConstArgs* p = (ConstArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+}
+template <typename T>
+__device__ __forceinline__ T* in_memory(T* p) {  // (a pointer out of the arguments is one to device memory)
+  return (T*)(__attribute__((address_space(1))) T*)p;
+}
 
 struct Seq {
   int b, n, mbs;  // sequence, its nodes, its row blocks
@@ -64,21 +76,23 @@ struct Seq {
 };
 
 // Sequence b (< batch, else nothing): everything but `before`.
-__device__ __forceinline__ Seq load_seq(const TreeArgs& a, int b, int rows) {
+template <typename A>
+__device__ __forceinline__ Seq load_seq(const A& a, int b, int rows) {
   Seq q{};
   q.b = b;
   if (b < a.batch) {
-    const int lo = max(a.cu_nodes[b], 0), hi = max(a.cu_nodes[b + 1], 0);
+    const int lo = max(in_memory(a.cu_nodes)[b], 0), hi = max(in_memory(a.cu_nodes)[b + 1], 0);
     q.first = lo;
     q.n = min(min(max(hi - lo, 0), a.max_nodes), max(a.tokens - lo, 0));
-    q.ctx = min(max(a.ctx_lens[b], 0), INT32_MAX - 128);
+    q.ctx = min(max(in_memory(a.ctx_lens)[b], 0), INT32_MAX - 128);
     q.end = min(q.ctx + q.n, a.room);
     q.tiles = q.n > 0 ? max((q.end + kTile - 1) / kTile, 1) : 0;
     q.mbs = (q.n * a.group + rows - 1) / rows;
   }
   return q;
 }
-__device__ __forceinline__ int seq_units(const TreeArgs& a, const Seq& q) { return (q.tiles + kItemCost) * q.mbs * a.kv_heads; }
+template <typename A>
+__device__ __forceinline__ int seq_units(const A& a, const Seq& q, int cost) { return (q.tiles + cost) * q.mbs * a.kv_heads; }
 
 // Inclusive sum over the lanes.
 __device__ __forceinline__ int wave_scan(int v) {
@@ -92,19 +106,22 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // The sequences of a batch, 64 at a time, and the units before and of them.
+template <typename Sh>
 struct Plan {
   Seq q;  // lane l: sequence first + l
   int first, incl, base;
-  __device__ __forceinline__ void load(const TreeArgs& a, int rows, int b0) {
+  template <typename A>
+  __device__ __forceinline__ void load(const A& a, int b0) {
     first = b0;
-    q = load_seq(a, b0 + (int)(threadIdx.x & 63), rows);
-    incl = wave_scan(seq_units(a, q));
+    q = load_seq(a, b0 + (int)(threadIdx.x & 63), Sh::ROWS);
+    incl = wave_scan(seq_units(a, q, Sh::COST));
   }
   // all of the batch's units; the first 64 sequences are left loaded
-  __device__ __forceinline__ int total(const TreeArgs& a, int rows) {
+  template <typename A>
+  __device__ __forceinline__ int total(const A& a) {
     int sum = 0;
     for (int b0 = (a.batch - 1) / 64 * 64; b0 >= 0; b0 -= 64) {
-      load(a, rows, b0);
+      load(a, b0);
       sum += __builtin_amdgcn_readlane(incl, 63);
     }
     base = 0;
@@ -112,7 +129,8 @@ struct Plan {
   }
   // The sequence that unit `at` (< total, not before the last one asked for) belongs
   // to, the same in every lane.
-  __device__ __forceinline__ Seq find(const TreeArgs& a, int rows, int at) {
+  template <typename A>
+  __device__ __forceinline__ Seq find(const A& a, int at) {
     while (true) {
       const uint64_t past = __ballot(base + incl > at);
       if (past != 0 || first + 64 >= a.batch) {
@@ -120,10 +138,10 @@ struct Plan {
         return {first + l, __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.mbs, l),
                 __builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.ctx, l),
                 __builtin_amdgcn_readlane(q.end, l), __builtin_amdgcn_readlane(q.tiles, l),
-                base + __builtin_amdgcn_readlane(incl - seq_units(a, q), l)};
+                base + __builtin_amdgcn_readlane(incl - seq_units(a, q, Sh::COST), l)};
       }
       base += __builtin_amdgcn_readlane(incl, 63);
-      load(a, rows, first + 64);
+      load(a, first + 64);
     }
   }
 };
@@ -190,45 +208,31 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// N LDS DMA instructions of one descriptor, 1 KB apart in LDS (see lds_dma16).
-// The wait states are in the asm, into which the compiler does not look: five
-// between a VALU write of an SGPR (v_readlane, v_readfirstlane: the descriptor is
-// made of such) and a vector memory instruction that reads it, one between m0 and
-// the copy.
-template <int N>
-__device__ __forceinline__ void copy_rows(u32x4 r, const uint32_t* voff, uint32_t lds) {
-  static_assert(N == 1 || N == 2 || N == 4, "instructions of 16 rows");
-#define TJK_COPY(v) "s_nop 0\n\tbuffer_load_dwordx4 " v ", %0, 0 offen lds"
-#define TJK_STEP "\n\ts_add_u32 m0, m0, 0x400\n\t"
-  if constexpr (N == 1)
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\t" TJK_COPY("%2")::"s"(r), "s"(lds), "v"(voff[0]) : "m0", "scc");
-  else if constexpr (N == 2)
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\t" TJK_COPY("%2") TJK_STEP TJK_COPY("%3")::"s"(r), "s"(lds), "v"(voff[0]),
-                 "v"(voff[1])
-                 : "m0", "scc");
-  else
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %1\n\t" TJK_COPY("%2") TJK_STEP TJK_COPY("%3") TJK_STEP TJK_COPY("%4")
-                     TJK_STEP TJK_COPY("%5")::"s"(r),
-                 "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3])
-                 : "m0", "scc");
-#undef TJK_COPY
-#undef TJK_STEP
+// lds_dma16 with wait states of its own: the compiler does not look into inline asm.
+// Five lie between a VALU write of an SGPR (v_readlane, v_readfirstlane: the
+// descriptors are made of such) and a vector memory instruction that reads it, one
+// between a write of m0 and a copy into LDS.
+__device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t voff, uint32_t lds_addr) {
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "{m0}"(lds_addr));
 }
 
-template <int HD, int NB, int RW, int NST>
+// SUB: tiles of a stage of the shared ring (RW = 4).
+template <int HD, int NB, int RW, int NST, int SUB>
 struct TreeShape {
   static constexpr int ROWS = 16 * NB * RW;
+  static constexpr int COST = RW == 1 ? 8 : 16;  // units of an item beside its tiles'
   static constexpr int RB = 2 * HD;             // bytes of a row in LDS
   static constexpr int TB = kTile * RB;         // of a tile's keys or values
-  static constexpr int RING = (RW == 1 ? 4 : 1) * NST * 2 * TB;
+  static constexpr int RING = (RW == 1 ? 4 : SUB) * NST * 2 * TB;
   static constexpr int JOIN = RW == 1 ? 2 * (NB * HD * 64 + NB * 512) : 0;  // two waves' sums
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
   static constexpr int PART = ROWS * (HD + 2);  // floats of a partial result
 };
 
-template <typename T, int HD, int NB, int RW, int NST, int OCC>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void tree_attention_kernel(TreeArgs a) {
-  typedef TreeShape<HD, NB, RW, NST> Sh;
+template <typename T, int HD, int NB, int RW, int NST, int OCC, int SUB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC))) void tree_attention_kernel(TreeArgs args) {
+  ConstArgs& a = fresh_args();
+  typedef TreeShape<HD, NB, RW, NST, SUB> Sh;
   typedef typename Mfma<T>::frag Frag;
   constexpr int RB = Sh::RB, TB = Sh::TB, CPR = RB / 16, RPI = 64 / CPR;
   constexpr int KC = HD / 32, HT = HD / 16;
@@ -249,11 +253,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     q.before = 0;
     const int kh = item / a.most_mbs, mb = item - kh * a.most_mbs;
     if (mb >= q.mbs) return;
-    at = (kh * q.mbs + mb) * (q.tiles + kItemCost);
-    stop = at + q.tiles + kItemCost;
+    at = (kh * q.mbs + mb) * (q.tiles + Sh::COST);
+    stop = at + q.tiles + Sh::COST;
   } else {
-    Plan plan;
-    const int total = plan.total(a, Sh::ROWS);
+    Plan<Sh> plan;
+    const int total = plan.total(a);
     if (total == 0) return;
     split = Split(total, gridDim.x);
     // neighbouring stretches on one XCD
@@ -261,7 +265,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     if (w >= split.n) return;
     at = split.share(w);
     stop = split.share(w + 1);
-    q = plan.find(a, Sh::ROWS, at);
+    q = plan.find(a, at);
     first64 = plan.first;
     base64 = plan.base;
   }
@@ -291,26 +295,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 #pragma unroll
   for (int h = 0; h < HT; ++h) vaddr[h] = vrow * RB + (((2 * h + (lane >> 1 & 1)) ^ swz(vrow)) << 4) + 8 * (lane & 1);
 
-  const __amdgpu_buffer_rsrc_t parts = wave_rsrc(a.parts, (int64_t)2 * gridDim.x * Sh::PART * 4);
-  // where row m of key head kh of sequence q goes
-  auto out_row = [&](int m, int kh) {
-    const int node = (int)((uint32_t)m / (uint32_t)a.group);
-    return reinterpret_cast<T*>(a.out + (int64_t)(q.first + node) * a.out_bytes) +
-           (int64_t)(kh * a.group + m - node * a.group) * (8 * a.hd8);
-  };
   while (at < stop) {
-    if (at >= q.before + seq_units(a, q)) {  // (loaded again: kept over the tiles, it would take their registers)
-      Plan plan;
-      plan.load(a, Sh::ROWS, first64);
+    ConstArgs& a = fresh_args();
+    if (at >= q.before + seq_units(a, q, Sh::COST)) {  // (loaded again: kept over the tiles, it would take their registers)
+      Plan<Sh> plan;
+      plan.load(a, first64);
       plan.base = base64;
-      q = plan.find(a, Sh::ROWS, at);
+      q = plan.find(a, at);
       first64 = plan.first;
       base64 = plan.base;
     }
-    const int units = q.tiles + kItemCost, off = at - q.before, item = (int)((uint32_t)off / (uint32_t)units);
+    const int units = q.tiles + Sh::COST, off = at - q.before, item = (int)((uint32_t)off / (uint32_t)units);
     const int u0 = off - item * units, u1 = min(units, u0 + (stop - at));
-    const int x0 = at - u0 + kItemCost;  // the unit of the item's first tile
-    const int t0 = max(u0 - kItemCost, 0), t1 = max(u1 - kItemCost, 0);
+    const int x0 = at - u0 + Sh::COST;  // the unit of the item's first tile
+    const int t0 = max(u0 - Sh::COST, 0), t1 = max(u1 - Sh::COST, 0);
     at += u1 - u0;
     if (t0 == t1) continue;  // its tiles are the next workgroup's
     const int kh = (int)((uint32_t)item / (uint32_t)q.mbs), mb = item - kh * q.mbs;
@@ -318,32 +316,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     const int end = q.end;
     const char* const kbase = a.cache.k + kh * a.cache.head_bytes;
     const char* const vbase = a.cache.v + kh * a.cache.head_bytes;
-    const int32_t* const table = a.table + q.b * a.ld_table;
+    const int32_t* const table = in_memory(a.table) + q.b * a.ld_table;
+    const float scale = a.scale;
 
-    // ---- places of the next 64 tiles' rows: lane j has the byte offset of tile
-    // first + j * STEP, of its first and its second 16 rows (which may lie in
-    // different pages); hi -1: no page
+    // ---- places of the next 64 tiles' rows: lane j has, of the tile first + j * STEP,
+    // the byte offsets of its first and its second 16 rows (which may lie in different
+    // pages) and the bytes from there to the last row that is to be read (0: none)
     constexpr int STEP = RW == 1 ? 4 : 1;
     const int mine = RW == 1 ? t0 + wave : t0;
     const int count = mine < t1 ? (t1 - mine + STEP - 1) / STEP : 0;
-    uint32_t place[2];
-    int place_hi[2];
+    uint32_t place[2], place_hi[2], reach[2];
     auto load_pages = [&](int i0) {
+      ConstArgs& a = fresh_args();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int x = (mine + (i0 + lane) * STEP) * kTile + 16 * h;
         const bool in = i0 + lane < count && x < end;
         const int page = page_of(table, in ? x >> a.cache.shift : 0, a.cache.pages);
-        if (in && page < 0 && kh == 0 && mb == 0 && (RW == 1 || wave == 0) && a.index_errors) atomicAdd(a.index_errors, 1);
-        const uint64_t at = (uint64_t)page * (uint64_t)a.cache.page_bytes +
-                            (uint64_t)((uint32_t)(x & ((1 << a.cache.shift) - 1)) * a.cache.row_bytes);
+        if (in && page < 0 && kh == 0 && mb == 0 && (RW == 1 || wave == 0) && a.index_errors) atomicAdd(in_memory(a.index_errors), 1);
         const bool there = in && page >= 0;
-        place[h] = there ? (uint32_t)at : 0;
-        place_hi[h] = there ? (int)(at >> 32) : -1;
+        const uint64_t at = there ? (uint64_t)page * (uint64_t)a.cache.page_bytes +
+                                        (uint64_t)((uint32_t)(x & ((1 << a.cache.shift) - 1)) * a.cache.row_bytes)
+                                  : 0;
+        place[h] = (uint32_t)at;
+        place_hi[h] = (uint32_t)(at >> 32);
+        reach[h] = there ? (uint32_t)min(end - x, 16) * a.cache.row_bytes : 0;
       }
     };
-    place[0] = place[1] = 0;
-    place_hi[0] = place_hi[1] = -1;
+    place[0] = place[1] = place_hi[0] = place_hi[1] = reach[0] = reach[1] = 0;
     if (end > 0) load_pages(0);
 
     // ---- this lane's rows: their queries (of a negative scale: their negatives)
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     for (int i = 0; i < NB; ++i) {
       const int m = min(m0 + 16 * i + col, rows - 1);
       const int node = (int)((uint32_t)m / (uint32_t)a.group), head = kh * a.group + (m - node * a.group);
-      const char* const src = a.q + (int64_t)(q.first + node) * a.q_token_bytes + head * a.q_head_bytes;
+      const char* const src = in_memory(a.q) + (int64_t)(q.first + node) * a.q_token_bytes + head * a.q_head_bytes;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const int piece = 4 * c + g;
@@ -362,35 +362,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         qf[i][c] = __builtin_bit_cast(Frag, f);
       }
     }
-    if (kh == 0 && mb == 0 && t0 == 0 && threadIdx.x == 0 && a.index_errors && end < q.ctx + q.n) atomicAdd(a.index_errors, 1);
+    if (kh == 0 && mb == 0 && t0 == 0 && threadIdx.x == 0 && a.index_errors && end < q.ctx + q.n) atomicAdd(in_memory(a.index_errors), 1);
 
-    // halves of tile i without a page: bits 0 and 1
-    auto pageless = [&](int i) {
-      return (__builtin_amdgcn_readlane(place_hi[0], i & 63) < 0 ? 1 : 0) |
-             (__builtin_amdgcn_readlane(place_hi[1], i & 63) < 0 ? 2 : 0);
+    // halves of tile i with nothing to read, for want of a page or past the end: bits 0
+    // and 1
+    auto empty = [&](int i) {
+      return (__builtin_amdgcn_readlane((int)reach[0], i & 63) == 0 ? 1 : 0) |
+             (__builtin_amdgcn_readlane((int)reach[1], i & 63) == 0 ? 2 : 0);
     };
     // descriptor of the 16 rows of tile i's half h
     auto half_range = [&](const char* base, int i, int h) __attribute__((always_inline)) {
-      const uint32_t lo = __builtin_amdgcn_readlane((int)place[h], i & 63);
-      const int hi = __builtin_amdgcn_readlane(place_hi[h], i & 63);
-      const int left = min(max(end - ((mine + i * STEP) * kTile + 16 * h), 0), 16);
-      const uint64_t p = (uint64_t)(uintptr_t)base + ((uint64_t)(uint32_t)max(hi, 0) << 32 | lo);
-      const uint32_t bytes = hi < 0 || i >= count ? 0 : (uint32_t)left * a.cache.row_bytes;
+      const uint32_t lo = __builtin_amdgcn_readlane((int)place[h], i & 63), hi = __builtin_amdgcn_readlane((int)place_hi[h], i & 63);
+      const uint32_t bytes = __builtin_amdgcn_readlane((int)reach[h], i & 63);
+      const uint64_t p = (uint64_t)(uintptr_t)base + ((uint64_t)hi << 32 | lo);
       return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)p), (uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) & 0xffffu,
-                   (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+                   i < count ? bytes : 0, 0x00020000u};
     };
     // tile i's keys (or values) to LDS byte `to`
     auto copy = [&](const char* base, int i, uint32_t to) __attribute__((always_inline)) {
       if constexpr (RW == 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          copy_rows<NV>(half_range(base, i, h), voff, to + h * NV * 1024);
+          const u32x4 r = half_range(base, i, h);
+#pragma unroll
+          for (int u = 0; u < NV; ++u) copy16(r, voff[u], to + (h * NV + u) * 1024);
         }
       } else {
         static_assert(NK == 4 || NK == 8, "a wave copies one or two pieces of a tile");
 #pragma unroll
         for (int u = 0; u < NK / 4; ++u)
-          copy_rows<1>(half_range(base, i, NK == 8 ? u : wave >> 1), voff, to + (wave + 4 * u) * 1024);
+          copy16(half_range(base, i, NK == 8 ? u : wave >> 1), voff[0], to + (wave + 4 * u) * 1024);
       }
     };
 
@@ -423,29 +424,35 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     // the nodes that this lane's row i sees, of the tile from position x on: bit k for
     // key k (a tile of the c tokens has them all)
     auto visible = [&](int i, int x, int none) {
-      const int m = min(m0 + 16 * i + col, rows - 1), node = (int)((uint32_t)m / (uint32_t)a.group);
-      const uint64_t bits = a.mask ? a.mask[q.first + node] : ~0ull >> (63 - node);
+      int m = min(m0 + 16 * i + col, rows - 1);
+      asm volatile("" : "+v"(m));  // computed here, not kept over the tiles that need none of it
+      ConstArgs& a = fresh_args();
+      const int node = (int)((uint32_t)m / (uint32_t)a.group);
+      const uint64_t bits = a.mask ? in_memory(a.mask)[q.first + node] : ~0ull >> (63 - node);
       const int d = x - q.ctx;  // the tile's first key as a node
       uint32_t keys = d >= 64 ? 0u : d >= 0 ? (uint32_t)(bits >> d) : d <= -32 ? ~0u : (uint32_t)(bits << -d) | ((1u << -d) - 1);
       if (end - x < 32) keys &= (1u << max(end - x, 0)) - 1;
       return keys & ~((none & 1 ? 0xffffu : 0u) | (none & 2 ? 0xffff0000u : 0u));
     };
-    auto softmax = [&](f32x4 (&s)[NB][2], Frag (&p)[NB]) {
+    // weights p of n tiles' scores s, the rows' offsets and sums
+    auto softmax = [&](auto n, f32x4 (*s)[NB][2], Frag (*p)[NB]) __attribute__((always_inline)) {
+      constexpr int N = decltype(n)::value;
+      float top[NB];
       bool moves = false;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        float top = -INFINITY;
+        top[i] = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[i][j >> 2][j & 3]);
-        moves |= top * a.scale > m_off[i] + kLazy;
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top[i] = fmaxf(top[i], s[u][i][j >> 2][j & 3]);
+        top[i] *= scale;
+        moves |= top[i] > m_off[i] + kLazy;
       }
       if (__any(moves)) {
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          float top = -INFINITY;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = fmaxf(top, s[i][j >> 2][j & 3]);
-          const float m = fmaxf(m_off[i], column_max(top * a.scale));
+          const float m = fmaxf(m_off[i], column_max(top[i]));
           const float keep = m_off[i] == m ? 1.f : __builtin_amdgcn_exp2f(m_off[i] - m);
           m_off[i] = m;
           l[i] *= keep;
@@ -454,29 +461,34 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         }
       }
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const float base = m_off[i] == -INFINITY ? 0.f : -m_off[i];
-        float e[8];
+      for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[i][j >> 2][j & 3], a.scale, base));
-        p[i] = Mfma<T>::pack(e);
-        // sums of the rounded weights, those that the product uses
-        l[i] = Mfma<T>::sum8(p[i], l[i]);
-      }
+        for (int i = 0; i < NB; ++i) {
+          const float base = m_off[i] == -INFINITY ? 0.f : -m_off[i];
+          float e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[u][i][j >> 2][j & 3], scale, base));
+          p[u][i] = Mfma<T>::pack(e);
+          // sums of the rounded weights, those that the product uses
+          l[i] = Mfma<T>::sum8(p[u][i], l[i]);
+        }
     };
     auto hide = [&](f32x4 (&s)[NB][2], const uint32_t (&keys)[NB]) {
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t mine = keys[i] >> (4 * g);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          s[i][j >> 2][j & 3] = keys[i] >> (16 * (j >> 2) + 4 * g + (j & 3)) & 1 ? s[i][j >> 2][j & 3] : -INFINITY;
+          s[i][j >> 2][j & 3] = mine >> (16 * (j >> 2) + (j & 3)) & 1 ? s[i][j >> 2][j & 3] : -INFINITY;
+      }
     };
     // Infinities and NaN among a tile's values: a weight of zero would not keep them
     // from a row that does not see them.  They are added to the rows that do, and
     // the product finds zeros in their place.  (Tiles of the c tokens need none of
     // this: every row sees those.)
     auto bad_values = [&](const char* vt) -> uint32_t {
-      const int row = lane >> 1;
+      int row = lane >> 1;
+      asm volatile("" : "+v"(row));
       bool bad = false;
 #pragma unroll
       for (int c = 0; c < CPR / 2; ++c) {
@@ -511,7 +523,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       }
     };
     auto clear_bad = [&](char* vt) {
-      const int row = lane >> 1;
+      int row = lane >> 1;
+      asm volatile("" : "+v"(row));
       for (int c = 0; c < CPR / 2; ++c) {
         u32x4* const at = reinterpret_cast<u32x4*>(vt + row * RB + ((lane & 1) * (CPR / 2) + c) * 16);
         u32x4 v = *at;
@@ -524,68 +537,74 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         *at = v;
       }
     };
+    auto values = [&](const char* vt, int h) {
+      typedef short v4s __attribute__((ext_vector_type(4)));
+      typedef short v8s __attribute__((ext_vector_type(8)));
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(vt + vaddr[h]));
+      const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(vt + vaddr[h] + 16 * RB));
+      const v8s both = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      return __builtin_bit_cast(Frag, both);
+    };
+    auto product = [&](int h, const Frag& vf, const Frag (&p)[NB]) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) o[i][h] = Mfma16<T>::mma(vf, p[i], o[i][h]);
+    };
     auto products = [&](const char* vt, const Frag (&p)[NB]) {
 #pragma unroll
-      for (int h = 0; h < HT; ++h) {
-        typedef short v4s __attribute__((ext_vector_type(4)));
-        typedef short v8s __attribute__((ext_vector_type(8)));
-        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(vt + vaddr[h]));
-        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)(vt + vaddr[h] + 16 * RB));
-        const v8s both = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        const Frag vf = __builtin_bit_cast(Frag, both);
-#pragma unroll
-        for (int i = 0; i < NB; ++i) o[i][h] = Mfma16<T>::mma(vf, p[i], o[i][h]);
-      }
+      for (int h = 0; h < HT; ++h) product(h, values(vt, h), p);
     };
 
+    // Tiles of the c tokens, which every row sees whole, run a loop without any of the
+    // masks' work, up to one without a page; the others a second one.
+    const int plain = min(max((q.ctx / kTile - mine + STEP - 1) / STEP, 0), count);
+    int lost[NST];  // empty() of tile i and those behind it
     if constexpr (RW == 1) {
       const uint32_t ring = lds + wave * (NST * 2 * TB);
       char* const mem = smem + wave * (NST * 2 * TB);
-      int lost[NST];  // of the tiles in the slots
 #pragma unroll
       for (int s = 0; s < NST; ++s) {
         copy(kbase, s, ring + s * 2 * TB);
         copy(vbase, s, ring + s * 2 * TB + TB);
-        lost[s] = pageless(s);
+        lost[s] = empty(s);
       }
-      for (int i0 = 0; i0 < count; i0 += NST) {
+      auto step = [&](int i, auto hides) __attribute__((always_inline)) {
+        const int slot = i % NST * (2 * TB);
+        char* const kt = mem + slot;
+        char* const vt = kt + TB;
+        f32x4 sc[NB][2];
+        Frag p[NB];
+        const int none = lost[0];
+        if (((i + NST) & 63) == 0 && i + NST < count) load_pages(i + NST);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK * (2 * NST - 1)) : "memory");
+        scores(kt, sc);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        copy(kbase, i + NST, ring + slot);
 #pragma unroll
-        for (int s = 0; s < NST; ++s) {
-          const int i = i0 + s;
-          if (NST > 1 && i >= count) break;
-          char* const kt = mem + s * 2 * TB;
-          char* const vt = kt + TB;
-          const int x = (mine + i * STEP) * kTile, none = lost[s];
-          const bool masked = x + kTile > q.ctx || none != 0;
-          uint32_t keys[NB];
-          if (((i + NST) & 63) == 0 && i + NST < count) load_pages(i + NST);
-          f32x4 sc[NB][2];
-          Frag p[NB];
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK * (2 * NST - 1)) : "memory");
-          scores(kt, sc);
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          copy(kbase, i + NST, ring + s * 2 * TB);
-          lost[s] = pageless(i + NST);
-          if (masked) {
+        for (int j = 0; j + 1 < NST; ++j) lost[j] = lost[j + 1];
+        lost[NST - 1] = empty(i + NST);
+        uint32_t keys[NB];
+        if constexpr (decltype(hides)::value) {
 #pragma unroll
-            for (int u = 0; u < NB; ++u) keys[u] = visible(u, x, none);
-            hide(sc, keys);
-          }
-          softmax(sc, p);
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK * (2 * NST - 1)) : "memory");
-          if (masked) {
-            const uint32_t bad = bad_values(vt);
-            if (bad) {
-              add_bad(vt, bad, keys);
-              clear_bad(vt);
-              asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            }
-          }
-          products(vt, p);
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          copy(vbase, i + NST, ring + s * 2 * TB + TB);
+          for (int u = 0; u < NB; ++u) keys[u] = visible(u, (mine + i * STEP) * kTile, none);
+          hide(sc, keys);
         }
-      }
+        softmax(std::integral_constant<int, 1>{}, &sc, &p);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NK * (2 * NST - 1)) : "memory");
+        if constexpr (decltype(hides)::value) {
+          const uint32_t bad = bad_values(vt);
+          if (bad) {
+            add_bad(vt, bad, keys);
+            clear_bad(vt);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          }
+        }
+        products(vt, p);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        copy(vbase, i + NST, ring + slot + TB);
+      };
+      int i = 0;
+      for (; i < plain && lost[0] == 0; ++i) step(i, std::false_type{});
+      for (; i < count; ++i) step(i, std::true_type{});
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       // ---- join the four waves' sums: 2 and 3 into 0 and 1, then 1 into 0
       __syncthreads();
@@ -624,54 +643,78 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         __syncthreads();
       }
     } else {
-      constexpr int NI = 2 * ((NK + 3) / 4);  // a wave's DMA instructions of a tile
-      int lost[NST];  // of tile i and those behind it
+      constexpr int NI = SUB * 2 * ((NK + 3) / 4);  // a wave's DMA instructions of a stage
+      // tiles i .. i + SUB - 1 to stage st, and their empty halves
+      auto fetch = [&](int i, int st) __attribute__((always_inline)) {
+        int none = 0;
 #pragma unroll
-      for (int s = 0; s < NST - 1; ++s) {
-        copy(kbase, s, lds + s * 2 * TB);
-        copy(vbase, s, lds + s * 2 * TB + TB);
-        lost[s] = pageless(s);
-      }
-      int s = 0;
-      for (int i = 0; i < count; ++i) {
-        const int x = (mine + i) * kTile, none = lost[0];
-        const bool masked = x + kTile > q.ctx || none != 0;
-        if (((i + NST - 1) & 63) == 0 && i + NST - 1 < count) load_pages(i + NST - 1);
+        for (int u = 0; u < SUB; ++u) {
+          copy(kbase, i + u, lds + (st * SUB + u) * 2 * TB);
+          copy(vbase, i + u, lds + (st * SUB + u) * 2 * TB + TB);
+          none |= empty(i + u) << (2 * u);
+        }
+        return none;
+      };
+#pragma unroll
+      for (int s = 0; s < NST - 1; ++s) lost[s] = fetch(s * SUB, s);
+      int st = 0;
+      auto step = [&](int i, auto hides) __attribute__((always_inline)) {
+        const int none = lost[0], ahead = i + (NST - 1) * SUB;
+        if ((ahead & 63) == 0 && ahead < count) load_pages(ahead);
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NI * (NST - 2)) : "memory");
-        const int next = s == 0 ? NST - 1 : s - 1;
-        copy(kbase, i + NST - 1, lds + next * 2 * TB);
-        copy(vbase, i + NST - 1, lds + next * 2 * TB + TB);
-        lost[NST - 1] = pageless(i + NST - 1);
+        lost[NST - 1] = fetch(ahead, st == 0 ? NST - 1 : st - 1);
 #pragma unroll
         for (int j = 0; j < NST - 1; ++j) lost[j] = lost[j + 1];
-        char* const kt = smem + s * 2 * TB;
-        char* const vt = kt + TB;
-        f32x4 sc[NB][2];
-        Frag p[NB];
-        scores(kt, sc);
-        uint32_t keys[NB];
-        if (masked) {
+        auto keys_at = [&](int u) { return smem + (st * SUB + u) * 2 * TB; };
+        if constexpr (!decltype(hides)::value) {
+          // a stage's scores together: longer runs of the matrix unit, one look at the
+          // rows' offsets
+          f32x4 sc[SUB][NB][2];
+          Frag p[SUB][NB];
 #pragma unroll
-          for (int u = 0; u < NB; ++u) keys[u] = visible(u, x, none);
-          hide(sc, keys);
-        }
-        softmax(sc, p);
-        if (masked) {
-          const uint32_t bad = bad_values(vt);  // the same in every wave
-          if (bad) {
-            add_bad(vt, bad, keys);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (wave == 0) clear_bad(vt);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          for (int u = 0; u < SUB; ++u) scores(keys_at(u), sc[u]);
+          softmax(std::integral_constant<int, SUB>{}, sc, p);
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) products(keys_at(u) + TB, p[u]);
+        } else {
+          for (int u = 0; u < SUB && i + u < count; ++u) {
+            char* const kt = keys_at(u);
+            char* const vt = kt + TB;
+            f32x4 sc[NB][2];
+            Frag p[NB];
+            scores(kt, sc);
+            uint32_t keys[NB];
+#pragma unroll
+            for (int j = 0; j < NB; ++j) keys[j] = visible(j, (mine + i + u) * kTile, none >> (2 * u));
+            hide(sc, keys);
+            softmax(std::integral_constant<int, 1>{}, &sc, &p);
+            const uint32_t bad = bad_values(vt);  // the same in every wave
+            if (bad) {
+              add_bad(vt, bad, keys);
+              asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+              if (wave == 0) clear_bad(vt);
+              asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+            products(vt, p);
           }
         }
-        products(vt, p);
-        s = s == NST - 1 ? 0 : s + 1;
-      }
+        st = st == NST - 1 ? 0 : st + 1;
+      };
+      int i = 0;
+      for (; i + SUB <= plain && lost[0] == 0; i += SUB) step(i, std::false_type{});
+      for (; i < count; i += SUB) step(i, std::true_type{});
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     }
 
     // ---- the rows, or their sums for who comes last
+    ConstArgs& z = fresh_args();
+    const __amdgpu_buffer_rsrc_t parts = wave_rsrc(z.parts, (int64_t)2 * gridDim.x * Sh::PART * 4);
+    // where row m goes
+    auto out_row = [&](int m) {
+      const int node = (int)((uint32_t)m / (uint32_t)z.group);
+      return reinterpret_cast<T*>(in_memory(z.out) + (int64_t)(q.first + node) * z.out_bytes) +
+             (int64_t)(kh * z.group + m - node * z.group) * (8 * z.hd8);
+    };
     const bool whole = t0 == 0 && t1 == q.tiles;
     const int part = 2 * w + (t0 == 0 ? 1 : 0);  // a stretch ends in the first part of an item at most once
     if (RW > 1 || wave == 0) {
@@ -682,10 +725,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         if (m >= rows) continue;
         if (whole) {
           const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-          T* const dst = out_row(m, kh);
+          T* const dst = out_row(m);
 #pragma unroll
           for (int h = 0; h < HT; ++h)
-            if (2 * h < a.hd8)
+            if (2 * h < z.hd8)
               *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) =
                   Quad<T>::from(make_float4(o[i][h][0] * inv, o[i][h][1] * inv, o[i][h][2] * inv, o[i][h][3] * inv));
         } else {
@@ -754,8 +797,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         if (share != 0 || r0 + group % wide >= live) continue;
         if (whole) {
           const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-          if (c0 < 8 * a.hd8)
-            *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r, kh) + c0) =
+          if (c0 < 8 * z.hd8)
+            *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) =
                 Quad<T>::from(make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
         } else {
           const int p = part_of(first);
@@ -775,7 +818,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this one's sums are in memory
         __syncthreads();
         if (threadIdx.x == 0) {
-          int* const counter = a.counters + level * (2 * gridDim.x) + part_of(first);
+          int* const counter = in_memory(z.counters) + level * (2 * gridDim.x) + part_of(first);
           const bool last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
           if (last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           *word = last;
@@ -795,10 +838,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 // Workgroups of a launch: the CUs times those that a CU holds.
 constexpr int kCus = 256;
 
-template <int HD_, int NB_, int RW_, int NST_, int OCC_>
+template <int HD_, int NB_, int RW_, int NST_, int OCC_, int SUB_ = 1>
 struct Variant {
-  static constexpr int HD = HD_, NB = NB_, RW = RW_, NST = NST_, OCC = OCC_;
-  typedef TreeShape<HD, NB, RW, NST> Sh;
+  static constexpr int HD = HD_, NB = NB_, RW = RW_, NST = NST_, OCC = OCC_, SUB = SUB_;
+  typedef TreeShape<HD, NB, RW, NST, SUB> Sh;
   static constexpr int GRID = kCus * OCC;
   static constexpr size_t BYTES = TJK_TREE_COUNTERS + (size_t)2 * GRID * Sh::PART * sizeof(float);
   static_assert(GRID <= kJoin * kJoin * kJoin && 3 * 2 * GRID * 4 <= TJK_TREE_COUNTERS && BYTES < 0x7fffffff, "counters and 32-bit offsets");
@@ -811,13 +854,13 @@ static auto with_variant(int head_dim, int rows, F&& f) {
     if (rows <= 16) return f(Variant<64, 1, 1, 2, 2>{});
     if (rows <= 32) return f(Variant<64, 2, 1, 2, 2>{});
     if (rows <= 64) return f(Variant<64, 4, 1, 2, 2>{});
-    if (rows <= 128) return f(Variant<64, 2, 4, 3, 2>{});
-    return f(Variant<64, 4, 4, 3, 2>{});
+    if (rows <= 128) return f(Variant<64, 2, 4, 2, 2, 2>{});
+    return f(Variant<64, 4, 4, 2, 2, 2>{});
   }
   if (rows <= 16) return f(Variant<128, 1, 1, 1, 2>{});
   if (rows <= 32) return f(Variant<128, 2, 1, 1, 2>{});
   if (rows <= 64) return f(Variant<128, 4, 1, 2, 1>{});
-  return f(Variant<128, 2, 4, 3, 2>{});
+  return f(Variant<128, 2, 4, 2, 2, 2>{});
 }
 
 // Whether each item is one workgroup's, with no plan and no joining: by the tiles of
@@ -837,10 +880,10 @@ static int launch_tree(TreeArgs a, hipStream_t s) {
   constexpr int ROWS = V::Sh::ROWS;
   a.most_mbs = (a.max_nodes * a.group + ROWS - 1) / ROWS;
   const int64_t items = (int64_t)a.batch * a.kv_heads * a.most_mbs, tiles = (a.room + kTile - 1) / kTile;
-  if (items * (std::max<int64_t>(tiles, 1) + kItemCost) > INT32_MAX || items > INT32_MAX / 256)
+  if (items * (std::max<int64_t>(tiles, 1) + V::Sh::COST) > INT32_MAX || items > INT32_MAX / 256)
     return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
   a.direct = whole_items(items, tiles);
-  tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);
+  tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC, V::SUB><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);
   return check_launch("tjk_tree_attention");
 }
 

@@ -33,7 +33,12 @@ int check_cache(const char* who, const tjk_paged_cache* c) {
 // head_dim / 16 up); each holds two 8-element pieces, those that the rotation
 // brings together: pieces p and p + rot / 16 of the halves' form (element i
 // turns with i + rot / 2), and past the rotated ones neighbours.  The norm sums
-// over the G lanes.
+// over the G lanes.  A wave takes 64 / G heads of one token.
+//
+// Bound by memory: 65536 tokens of 16 + 2 x 16 heads of 64 with norms, bf16, 157 us,
+// 5.2 TB/s (a copy of 1 GB: 5.1); 4096 tokens of 32 + 2 x 8 heads of 128 22.3 us, 4.6; 1003
+// of them 7.0 us.  8 tokens: 3.5 us, a launch and two passages of memory (position and
+// row, then the angles).
 
 struct AppendArgs {
   const char* qkv;

@@ -179,12 +179,29 @@ struct Split {
 // RW = 1 (up to 64 rows): the four waves take tiles in turn, each with NST slots of its
 // own, and meet only to join their sums: no barrier in the loop.  Copies run ahead
 // by NST tiles, K and V apart.  RW = 4 (more rows): the waves have 16 NB rows each
-// and share the tiles, in a ring of NST, one barrier a tile.
+// and share the tiles, in a ring of NST stages of SUB, one barrier a stage.
+//
+// Weights go to the product with V in the cache's type, as in flash_pipe_kernel: half
+// a step of 2^-8 (bf16) each, 2.2e-3 of the result (2-norm) where its own rounding
+// is 1.7e-3; a product in two parts would double it.  Everything summed is fp32, the
+// sum of the weights that of the rounded ones.
+//
+// Few rows are bound by memory: 64 single tokens over 512 to 4096, 16 heads of 128
+// bf16, 215 us, 5.6 TB/s (a copy of 1 GB reaches 5.1); 2 x 99995 tokens, 4 key heads of
+// 64, 56 us, of which the stretches take 34 to 46, the joining 12.  8 single tokens
+// over up to 512: 9.4 us, launch and passages of memory one after the other (places 2,
+// first tiles 1.5, the rest of them 3, joining of the waves 1).  Many rows are bound
+// by issue: 32 trees of 64 nodes, 8 heads of 128 to a key head, 230 us, 680 TFLOP/s
+// (770 in long stretches): matrix unit 27% of the time, vector unit 36%, LDS 21%; 48
+// rows a wave take 238 to 253, 64 rows 261 (one wave a SIMD; two do not fit), three
+// waves a SIMD do not fit.
 
 constexpr uint32_t kPast = 0x80000000u;  // beyond any descriptor's range
 // Cache policies: stores through to memory, loads from it, past an XCD's own L2.
 constexpr int kThrough = 17, kCoherent = 16;
-constexpr float kLazy = 8.0f;            // a row's offset follows its scores when they pass it by 2^8
+// A row's offset follows its scores when they pass it by 2^8: most tiles rescale
+// nothing, and a weight of up to 256 is no harm in either type.
+constexpr float kLazy = 8.0f;
 
 template <typename T> struct Mfma16;
 template <> struct Mfma16<bf16> {
@@ -208,8 +225,8 @@ __device__ __forceinline__ float column_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// lds_dma16 with wait states of its own: the compiler does not look into inline asm.
-// Five lie between a VALU write of an SGPR (v_readlane, v_readfirstlane: the
+// One LDS DMA (see lds_dma16) with wait states of its own: the compiler does not look
+// into inline asm.  Five lie between a VALU write of an SGPR (v_readlane, v_readfirstlane: the
 // descriptors are made of such) and a vector memory instruction that reads it, one
 // between a write of m0 and a copy into LDS.
 __device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t voff, uint32_t lds_addr) {
@@ -220,7 +237,10 @@ __device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t voff, uint32_t lds_a
 template <int HD, int NB, int RW, int NST, int SUB>
 struct TreeShape {
   static constexpr int ROWS = 16 * NB * RW;
-  static constexpr int COST = RW == 1 ? 8 : 16;  // units of an item beside its tiles'
+  // Units of an item beside its tiles': 9 single tokens over 29 to 4921, 8 heads of 80,
+  // 56 us with 0, 30 with 2, 25.6 with 4, 23.9 with 8; 16 trees of 64 nodes, 2 heads of
+  // 128 to a key head, 96 with 8, 79 with 16.
+  static constexpr int COST = RW == 1 ? 8 : 16;
   static constexpr int RB = 2 * HD;             // bytes of a row in LDS
   static constexpr int TB = kTile * RB;         // of a tile's keys or values
   static constexpr int RING = (RW == 1 ? 4 : SUB) * NST * 2 * TB;
@@ -847,7 +867,11 @@ struct Variant {
   static_assert(GRID <= kJoin * kJoin * kJoin && 3 * 2 * GRID * 4 <= TJK_TREE_COUNTERS && BYTES < 0x7fffffff, "counters and 32-bit offsets");
 };
 
-// Calls f with the variant for a head_dim and the rows of the largest tree.
+// Calls f with the variant for a head_dim and the rows of the largest tree: as few
+// 16-row blocks as hold them, so that a wave holds the sums of no rows that are not
+// there; from 64 rows on four waves with rows of their own (64 rows of 128 in four
+// waves that share the tiles: 105 to 108 us either way at 16 x 2000 to 4000 tokens, 16
+// key heads; of 64: 60 and 62).
 template <typename F>
 static auto with_variant(int head_dim, int rows, F&& f) {
   if (head_dim <= 64) {

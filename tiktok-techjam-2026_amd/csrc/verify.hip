@@ -42,14 +42,23 @@ struct VerifyArgs {
 // that holds it is read again.  A sequence's vocabulary is cut into `parts`, a
 // workgroup each; every one walks the same walk from the same numbers and meets
 // the others at the sums only: each puts its own in the workspace and reads
-// theirs.  It waits a bounded time: a sum that does not come (workgroups of other
+// theirs.  64 trees of up to 32 nodes over 128257 tokens: 32 us (one workgroup a
+// sequence 77), of which the clearing of the sums' places 3; the distributions of the last
+// nodes alone are 13 at a copy's rate, but a tree with five refusals makes five passes,
+// one after the other, of about 5 us: 128 KB by one CU, the waves' sums, and two
+// passages of memory to the other parts and back.  Four chains of six over 32000: 10 us.  It waits a bounded time: a sum that does not come (workgroups of other
 // work may hold the chip) it computes itself, in the same order, so nothing hangs on
 // who was there.
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kMostParts = 64;
-constexpr int kMostGroups = 256;  // workgroups of a launch
-constexpr int kPartElements = 16384;  // least of a part
+// Workgroups of a launch: one per CU, so that they are all there.  64 trees over 128257:
+// 38 us with 256 or 512, 810 with 1024, which are not and run out of patience.
+constexpr int kMostGroups = 256;
+// Least elements of a part, us with 4096 / 8192 / 16384: chain over 32000 10.9 / 10.8 / 9.3 (no
+// meeting), 16 trees over 50000 20.4 / 21.1 / 22.2, 4 over 128000 19.1 / 16.9 / 17.5, 64 over
+// 10000 17.3 / 13.0 / 13.0.
+constexpr int kPartElements = 16384;
 constexpr int kPolls = 256;  // of a missing sum: about 50 us
 
 struct Slot {  // of a workgroup's sum: its halves, each with the round it belongs to

@@ -123,6 +123,21 @@ def test_append_in_place_without_cache(device, hd, rot, interleaved):
     assert torch.equal(packed[:, 2 * heads:].cpu(), qkv[:, 2 * heads:])
 
 
+@pytest.mark.parametrize("t,heads", [(1, 4), (37, 1), (1, 1)])
+def test_append_in_place_of_one(device, t, heads):
+    """One token, one head: their views' strides say nothing, the rows are the
+    same."""
+    hd = 64
+    qkv, table, pos, qg, kg, y, err = _append_case(t, heads, heads, hd, hd, True, False, torch.bfloat16, 13)
+    padded = torch.full((t, 3 * heads, 72), 7.0, dtype=torch.bfloat16, device=device)
+    padded[..., :hd] = qkv.to(device)
+    rows = padded[..., :hd]
+    ops.rope_append(rows, pos.to(device), table.to(device), rows[:, :heads], k_out=rows[:, heads:2 * heads],
+                    q_gamma=qg.to(device), k_gamma=kg.to(device))
+    _within(rows[:, :2 * heads], y, err, torch.bfloat16)
+    assert torch.equal(rows[:, 2 * heads:].cpu(), qkv[:, 2 * heads:]) and (padded[..., hd:] == 7).all()
+
+
 def test_append_cache_orders(device):
     """[pages, page, heads, hd] seen as [pages, heads, page, hd], keys and values
     side by side in one buffer, a strided qkv: the same rows."""

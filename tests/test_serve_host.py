@@ -291,3 +291,12 @@ def test_rope_table():
     assert ops.rope_table(7, 0).shape == (7, 0, 2)
     with pytest.raises(TjkError, match="pairs"):
         ops.rope_table(8, 7)
+
+
+def test_append_in_place_of_one_head():
+    """In place, the head stride of a single head is of no meaning: with that in order
+    the call is found too large, the last thing looked at."""
+    one = dict(q_out=FAKE, cache=None, slots=None, heads=1, kv_heads=16, tokens=1 << 30, head_dim=128, rot=0, ld_head=136,
+               ld_token=4488, ld_q_token=4488, ld_q_head=128)
+    assert _append(**one) == EUNSUPPORTED and "too many" in _said()
+    assert _append(**dict(one, ld_q_token=4480)) == EINVAL and "in place" in _said()

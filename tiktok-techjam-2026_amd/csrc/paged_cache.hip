@@ -290,10 +290,14 @@ extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_hea
     return fail(TJK_EUNSUPPORTED, "%s: strides must be multiples of 8", who);
   if ((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)table | (uintptr_t)q_gamma | (uintptr_t)k_gamma) & 15))
     return fail(TJK_EUNSUPPORTED, "%s: misaligned pointer", who);
-  // a lane writes what it has read, as long as it lies in the same place
+  // a lane writes what it has read, as long as it lies in the same place (a stride of
+  // which there is one step only says nothing)
   const char* const keys = static_cast<const char*>(qkv) + 2 * heads * ld_head;
-  if ((q_out == qkv && (ld_q_token != ld_token || ld_q_head != ld_head)) ||
-      (k_out && ((k_out == keys && (ld_k_token != ld_token || ld_k_head != ld_head)) || k_out == qkv)))
+  auto elsewhere = [&](int64_t token, int64_t head, int rows) {
+    return (tokens > 1 && token != ld_token) || (rows > 1 && head != ld_head);
+  };
+  if ((q_out == qkv && elsewhere(ld_q_token, ld_q_head, heads)) ||
+      (k_out && ((k_out == keys && elsewhere(ld_k_token, ld_k_head, kv_heads)) || k_out == qkv)))
     return fail(TJK_EINVAL, "%s: outputs may alias qkv only in place", who);
   AppendArgs a{static_cast<const char*>(qkv), 2 * ld_token, 2 * ld_head, positions, table, (int)n_positions, (int)rot / 8,
                static_cast<char*>(q_out), 2 * ld_q_token, 2 * ld_q_head, static_cast<char*>(k_out), 2 * ld_k_token,

@@ -620,6 +620,16 @@ def test_verify_strides_and_bad_offsets(device):
     assert d.run(device) == d.want() and d.run(device)[1] == [1]
 
 
+def test_verify_offsets_at_the_ends_of_32_bits(device):
+    """An offset of -2^31 behind a positive one: no nodes."""
+    d = Drafts([6, 9, 4], 500, "tree", 7)
+    path, count, token = d.run(device)
+    d.cu = [0, 6, -2 ** 31, 2 ** 31 - 1]
+    got = d.run(device)
+    assert got[0][0] == path[0] and got[0][1] == [-1] * 9
+    assert got[1][:2] == [count[0], 0] and got[2][:2] == [token[0], -1]
+
+
 # --------------------------------------------------------------- compaction
 
 @pytest.mark.parametrize("layers,kv,hd,page", [(1, 1, 16, 16), (3, 4, 64, 16), (2, 2, 128, 32), (1, 3, 80, 16), (5, 2, 48, 64)])

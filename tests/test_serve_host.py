@@ -300,3 +300,10 @@ def test_append_in_place_of_one_head():
                ld_token=4488, ld_q_token=4488, ld_q_head=128)
     assert _append(**one) == EUNSUPPORTED and "too many" in _said()
     assert _append(**dict(one, ld_q_token=4480)) == EINVAL and "in place" in _said()
+
+
+def test_attention_refuses_more_work_than_32_bits_number():
+    """63 items of 34087042 units are 2^31 - 2, which the division among the
+    workgroups, rounding up, would carry past 32 bits."""
+    kw = dict(batch=63, heads=1, cache_kv_heads=1, ld_table=1 << 26)
+    assert _attend(table_cols=34087042 - 8, **kw) == EUNSUPPORTED and "too large" in _said()

@@ -904,7 +904,7 @@ static int launch_tree(TreeArgs a, hipStream_t s) {
   constexpr int ROWS = V::Sh::ROWS;
   a.most_mbs = (a.max_nodes * a.group + ROWS - 1) / ROWS;
   const int64_t items = (int64_t)a.batch * a.kv_heads * a.most_mbs, tiles = (a.room + kTile - 1) / kTile;
-  if (items * (std::max<int64_t>(tiles, 1) + V::Sh::COST) > INT32_MAX || items > INT32_MAX / 256)
+  if (items * (std::max<int64_t>(tiles, 1) + V::Sh::COST) > INT32_MAX - kMinUnits || items > INT32_MAX / 256)
     return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
   a.direct = whole_items(items, tiles);
   tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC, V::SUB><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   const int b = blockIdx.x % a.batch, part = blockIdx.x / a.batch;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t first = max(a.cu_nodes[b], 0);
-  const int n = (int)min((int64_t)min(max(a.cu_nodes[b + 1] - (int)first, 0), a.max_nodes), max(a.rows - first, (int64_t)0));
+  const int n = (int)min((int64_t)min(max(max(a.cu_nodes[b + 1], 0) - (int)first, 0), a.max_nodes), max(a.rows - first, (int64_t)0));
   int32_t* const path = a.path + b * a.ld_path;
   const bool writes = part == 0 && tid == 0;
   if (n == 0) {

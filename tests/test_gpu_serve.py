@@ -304,6 +304,35 @@ def test_long_contexts(device, contexts, counts, heads, kv, hd, dt):
     Trees(contexts, counts, heads, kv, hd, 64, DT[dt], 1).check(device)
 
 
+@pytest.mark.parametrize("context,nodes,heads,kv", [(20000, 2, 1, 1), (17003, 64, 4, 2), (18001, 17, 2, 1)])
+def test_contexts_joined_in_several_levels(device, context, nodes, heads, kv):
+    """More than 64 stretches of an item, joined eight by eight by eight; pages that
+    are not there in the midst of it, all positions of which are left out, and
+    counted by halves of a tile: four to a page."""
+    t = Trees([context], [nodes], heads, kv, 16, 64, torch.float16, 30)
+    want = t.check(device)
+    assert torch.equal(t.run(device), want)
+    t.table[0, 100], t.table[0, 171] = -1, t.pages
+    errors = torch.zeros(1, dtype=torch.int32, device=device)
+    got = t.run(device, errors=errors)
+    exact, err = t.exact()
+    _within(got, exact, err, t.dt)
+    assert int(errors) == 8
+
+
+def test_many_heads_of_one_key_head(device):
+    """64 heads of a key head and 64 nodes: 4096 rows."""
+    Trees([40, 3], [64, 5], 64, 1, 64, 16, torch.bfloat16, 31).check(device)
+
+
+def test_many_sequences_of_unequal_length(device):
+    """130 sequences, more than twice the lanes of a wave, cut into stretches that
+    cross them, one of them long."""
+    contexts, counts = [(i * 29) % 70 for i in range(130)], [(i * 5) % 4 for i in range(130)]
+    contexts[77], counts[77] = 5000, 3
+    Trees(contexts, counts, 2, 1, 32, 16, torch.bfloat16, 32).check(device)
+
+
 def test_many_sequences(device):
     """More sequences than lanes of a wave, ragged, some without nodes."""
     counts = [(i * 7) % 5 for i in range(150)]
@@ -597,6 +626,13 @@ def test_verify_edges(device):
     e.q[0], e.p[0] = 1 / 64, 1 / 128
     e.au[:] = 0.9
     assert e.run(device) == e.want() and e.run(device)[1] == [1]
+
+
+@pytest.mark.parametrize("counts,vocab", [([20, 9], 128257), ([30], 300001), ([5] * 100, 33000)])
+def test_verify_over_several_workgroups(device, counts, vocab):
+    for seed in range(2):
+        d = Drafts(counts, vocab, "tree", seed, noise=(1.0, 4.0)[seed])
+        assert d.run(device) == d.want()
 
 
 def test_verify_strides_and_bad_offsets(device):

@@ -4,7 +4,7 @@ steps of drafted tokens, graphs, two calls at once."""
 import pytest
 import torch
 
-from tjkernels import ops
+from tjkernels import _lib, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -262,3 +262,75 @@ def test_two_calls_at_once(device):
     for d, want in zip(jobs, wants):
         for k in ("q", "out", "path", "count", "token"):
             assert torch.equal(d[k], want[k]), k
+
+
+def _verification(device, seed, batch=3, vocab=150001):
+    """Arguments of a verification that several workgroups share."""
+    g = _gen(seed)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    logits = torch.randn(5 * batch, vocab, generator=g)
+    a = [torch.softmax(logits, 1), torch.softmax(logits + 2 * torch.randn(5 * batch, vocab, generator=g), 1),
+         torch.randint(0, vocab, (5 * batch,), generator=g).int(), i32([-1, 0, 0, 0, 1] * batch),
+         torch.rand(5 * batch, generator=g), torch.rand(batch, generator=g)]
+    a[2][1::5] = a[0][0::5].argmax(1).int()
+    return [x.to(device) for x in a], i32([5 * b for b in range(batch + 1)]).to(device)
+
+
+def _verified(device, a, cu, workspace=None):
+    batch = cu.numel() - 1
+    path = torch.zeros(batch, 5, dtype=torch.int32, device=device)
+    count, token = torch.zeros_like(path[:, 0]).contiguous(), torch.zeros_like(path[:, 0]).contiguous()
+    ops.verify_tree(*a, path, count, token, cu_nodes=cu, workspace=workspace)
+    return path, count, token
+
+
+@pytest.mark.parametrize("own_workspace", [True, False])
+def test_captured_verification_of_several_workgroups(device, own_workspace):
+    """Replayed on other distributions and numbers, with eager calls in between."""
+    a, cu = _verification(device, 1)
+    need = _lib.load().tjk_verify_tree_bytes(150001, 3)
+    assert need > 0
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=device) if own_workspace else None
+    _verified(device, a, cu, ws)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _verified(device, a, cu, ws)
+    seen = set()
+    for seed in range(2, 7):
+        new, _ = _verification(device, seed)
+        for x, y in zip(a, new):
+            x.copy_(y)
+        graph.replay()
+        want = _verified(device, new, cu)
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y), seed
+        seen |= set(want[2].tolist())
+    assert len(seen) > 10
+
+
+def test_verifications_at_once(device):
+    """Two streams' verifications share the chip, beside attention over long
+    contexts that may hold its workgroups up: the same results."""
+    jobs = [_verification(device, seed, batch, vocab) for seed, batch, vocab in ((21, 3, 150001), (22, 16, 60001))]
+    wants = [_verified(device, *job) for job in jobs]
+    d = _inputs(device, 23, context=(1800, 1700))
+    want = torch.empty_like(d["out"])
+    attend = lambda out: ops.tree_attention(d["q"], d["k"][0], d["v"][0], d["blocks"], d["ctx"], out, cu_nodes=d["cu"],  # noqa: E731
+                                            max_nodes=9)
+    d["q"].normal_()
+    attend(want)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for job, stream in zip(jobs, streams):
+            with torch.cuda.stream(stream):
+                got.append(_verified(device, *job))
+        with torch.cuda.stream(streams[2]):
+            attend(d["out"])
+    torch.cuda.synchronize()
+    for i, result in enumerate(got):
+        for x, y in zip(result, wants[i % 2]):
+            assert torch.equal(x, y)
+    assert torch.equal(d["out"], want)

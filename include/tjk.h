@@ -485,7 +485,9 @@ int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_head, const in
  * the product with the values rounded to the cache's type.  A row that sees
  * nothing, or only scores of -inf, is zero.  Keys and values that a row does not
  * see do not reach it, whatever they hold; positions without a page are left
- * out, and count in *index_errors.
+ * out, and count in *index_errors.  Of a tree of more than max_nodes nodes, or that
+ * runs past `tokens`, the first rows count; rows that no sequence names stay.  out
+ * may not overlap q or the cache.
  * workspace: tjk_tree_attention_bytes() bytes on the device, 16-byte aligned, of
  * which the first TJK_TREE_COUNTERS have to be zero before the first call; each
  * call leaves them so.  Calls that share a workspace have to be ordered.
@@ -516,7 +518,8 @@ size_t tjk_tree_attention_bytes(int heads, int kv_heads, int head_dim, int max_n
  * (k: the children refused; c_k = 0 if W_k is zero; -1 if p has no weight).  So the
  * tokens are distributed as the target's.  Products and sums in 64 bits; negative
  * and NaN weights count as zero.  A child with a token outside [0, vocab) is
- * refused and counts in *index_errors.
+ * refused and counts in *index_errors; a node whose parent is none before it is
+ * not reached, nor are those past max_nodes or rows.
  * path [batch, max_nodes]: the accepted nodes, node 0 first, then -1; count: how
  * many; token: the next token.  A sequence without nodes: -1, 0 and -1.
  * workspace: tjk_verify_tree_bytes() bytes (which may be 0) on the device, 16-byte
@@ -535,8 +538,8 @@ size_t tjk_verify_tree_bytes(int64_t vocab, int batch);
  * path[b, i] to ctx_lens[b] + i for 1 <= i < count[b], in each of `layers` caches
  * layer_stride elements apart (of k and of v).  path (as tjk_verify_tree writes it)
  * starts at 0 and increases; an entry below i or past max_nodes, or a position
- * without a page, moves nothing and counts in *index_errors.  The pages that
- * nodes lie in belong to one sequence.
+ * without a page, moves nothing and counts in *index_errors (a table of no columns:
+ * nothing moves or counts).  The pages that nodes lie in belong to one sequence.
  */
 int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64_t layer_stride,
                       const int32_t* block_table, int64_t ld_table, int64_t table_cols,

@@ -307,3 +307,32 @@ def test_attention_refuses_more_work_than_32_bits_number():
     workgroups, rounding up, would carry past 32 bits."""
     kw = dict(batch=63, heads=1, cache_kv_heads=1, ld_table=1 << 26)
     assert _attend(table_cols=34087042 - 8, **kw) == EUNSUPPORTED and "too large" in _said()
+
+
+@pytest.mark.parametrize("call", [_append, _compact])
+@pytest.mark.parametrize("kw", [dict(cache_page_stride=0), dict(cache_head_stride=0), dict(cache_head_stride=32)])
+def test_written_caches_do_not_overlap(call, kw):
+    assert call(**kw) == EINVAL and "overlap" in _said()
+    assert _attend(workspace=None, **kw) == EINVAL and "null workspace" in _said()  # one that is read may
+
+
+def test_outputs_do_not_overlap():
+    assert _append(ld_q_token=0) == EINVAL and "stride" in _said()
+    assert _append(k_out=FAKE + 64, ld_k_head=64, ld_k_token=0) == EINVAL and "stride" in _said()
+    assert _compact(layer_stride=0) == EUNSUPPORTED and "row" in _said()
+    assert _attend(q=FAKE, out=FAKE) == EINVAL and "out may not be q" in _said()
+
+
+def test_wrappers_refuse_expanded_outputs():
+    with pytest.raises(TjkError):
+        _py_append(q_out=_b(1, 8, 64).expand(5, 8, 64))
+    with pytest.raises(TjkError):
+        _py_compact(k_cache=_b(1, 10, 4, 32, 64).expand(3, 10, 4, 32, 64), v_cache=_b(1, 10, 4, 32, 64).expand(3, 10, 4, 32, 64))
+
+
+@pytest.mark.parametrize("kw", [dict(q=_b(5, 512)), dict(k_cache=_b(10, 32, 64)), dict(q=_b(5)), dict(q=_b(1, 5, 8, 64))])
+def test_attention_shapes_are_refused_before_the_workspace(kw):
+    with pytest.raises(TjkError):
+        _py_attend(**kw)
+    with pytest.raises(TjkError):
+        _py_attend(workspace=torch.zeros(64, dtype=torch.uint8), **kw)

@@ -27,8 +27,9 @@ inline Paged paged(const tjk_paged_cache& c) {
           (uint32_t)(2 * c.row_stride), (int)c.pages, shift};
 }
 
-// Status of a cache that an entry point `who` is given.
-int check_cache(const char* who, const tjk_paged_cache* c);
+// Status of a cache that an entry point `who` is given; one that it writes may not
+// hold two rows in one place.
+int check_cache(const char* who, const tjk_paged_cache* c, bool writes);
 
 // A page that a block table names, -1 if the cache holds no such page.
 __device__ __forceinline__ int page_of(const int32_t* table_row, int at, int pages) {

@@ -6,7 +6,7 @@
 
 namespace tjk {
 
-int check_cache(const char* who, const tjk_paged_cache* c) {
+int check_cache(const char* who, const tjk_paged_cache* c, bool writes) {
   if (!c || !c->k || !c->v) return fail(TJK_EINVAL, "%s: null cache", who);
   if (c->dtype != TJK_F16 && c->dtype != TJK_BF16) return fail(TJK_EINVAL, "%s: bad cache dtype %d", who, c->dtype);
   if (c->kv_heads <= 0 || c->pages <= 0 || c->head_dim <= 0)
@@ -19,6 +19,8 @@ int check_cache(const char* who, const tjk_paged_cache* c) {
   if (c->pages * c->page_size > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: the cache's rows exceed int32", who);
   if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < c->head_dim)
     return fail(TJK_EINVAL, "%s: bad cache strides", who);
+  if (writes && ((c->pages > 1 && c->page_stride < c->head_dim) || (c->kv_heads > 1 && c->head_stride < c->head_dim)))
+    return fail(TJK_EINVAL, "%s: rows of the cache overlap", who);
   if (c->page_stride % 8 || c->head_stride % 8 || c->row_stride % 8)
     return fail(TJK_EUNSUPPORTED, "%s: cache strides must be multiples of 8", who);
   if (c->row_stride > 1 << 20 || c->row_stride * c->page_size > 1 << 29)
@@ -276,7 +278,7 @@ extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_hea
   if (heads > 65536 || kv_heads > 65536 || tokens > INT32_MAX || n_positions > INT32_MAX)
     return fail(TJK_EUNSUPPORTED, "%s: too large", who);
   if (cache) {
-    if (const int bad = check_cache(who, cache)) return bad;
+    if (const int bad = check_cache(who, cache, true)) return bad;
     if (cache->dtype != dtype || cache->kv_heads != kv_heads || cache->head_dim != head_dim)
       return fail(TJK_EINVAL, "%s: the cache's dtype, heads or head_dim differ", who);
   }
@@ -288,6 +290,8 @@ extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_hea
     return fail(TJK_EINVAL, "%s: stride too small", who);
   if (ld_token % 8 || ld_head % 8 || ld_q_token % 8 || ld_q_head % 8 || (k_out && (ld_k_token % 8 || ld_k_head % 8)))
     return fail(TJK_EUNSUPPORTED, "%s: strides must be multiples of 8", who);
+  if (tokens > 1 && (ld_q_token < head_dim || (k_out && ld_k_token < head_dim)))
+    return fail(TJK_EINVAL, "%s: a stride too small for a row of its own", who);
   if ((((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)table | (uintptr_t)q_gamma | (uintptr_t)k_gamma) & 15))
     return fail(TJK_EUNSUPPORTED, "%s: misaligned pointer", who);
   // a lane writes what it has read, as long as it lies in the same place (a stride of
@@ -330,13 +334,13 @@ extern "C" int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64
                                  int64_t ld_path, int max_nodes, const int32_t* count, int* index_errors, int batch,
                                  void* stream) {
   const char* const who = "tjk_compact_cache";
-  if (const int bad = check_cache(who, cache)) return bad;
+  if (const int bad = check_cache(who, cache, true)) return bad;
   if (layers < 0 || batch < 0 || max_nodes < 0 || table_cols < 0)
     return fail(TJK_EINVAL, "%s: bad shape layers=%d batch=%d max_nodes=%d", who, layers, batch, max_nodes);
   if (max_nodes > 64) return fail(TJK_EUNSUPPORTED, "%s: max_nodes=%d exceeds 64", who, max_nodes);
   if (table_cols > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: block table too wide", who);
-  if (layers > 1 && (layer_stride < 0 || layer_stride % 8))
-    return fail(TJK_EUNSUPPORTED, "%s: the layers' stride must be a multiple of 8", who);
+  if (layers > 1 && (layer_stride < cache->head_dim || layer_stride % 8))
+    return fail(TJK_EUNSUPPORTED, "%s: the layers' stride must be a multiple of 8 and hold a row", who);
   if (layers == 0 || batch == 0 || max_nodes < 2 || table_cols == 0) return TJK_OK;
   if (!block_table || !ctx_lens || !path || !count) return fail(TJK_EINVAL, "%s: null pointer", who);
   if (ld_table < table_cols || ld_path < max_nodes) return fail(TJK_EINVAL, "%s: leading dimension too small", who);

@@ -906,6 +906,7 @@ static int launch_tree(TreeArgs a, hipStream_t s) {
   const int64_t items = (int64_t)a.batch * a.kv_heads * a.most_mbs, tiles = (a.room + kTile - 1) / kTile;
   if (items * (std::max<int64_t>(tiles, 1) + V::Sh::COST) > INT32_MAX - kMinUnits || items > INT32_MAX / 256)
     return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
+  if (a.out == a.q) return fail(TJK_EINVAL, "tjk_tree_attention: out may not be q, which other workgroups still read");
   a.direct = whole_items(items, tiles);
   tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC, V::SUB><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);
   return check_launch("tjk_tree_attention");
@@ -928,7 +929,7 @@ extern "C" int tjk_tree_attention(const void* q, int64_t ld_q_token, int64_t ld_
                                   int64_t ld_out, int64_t tokens, int batch, int heads, int max_nodes, float scale,
                                   void* workspace, size_t workspace_bytes, int* index_errors, void* stream) {
   const char* const who = "tjk_tree_attention";
-  if (const int bad = check_cache(who, cache)) return bad;
+  if (const int bad = check_cache(who, cache, false)) return bad;
   if (tokens < 0 || batch < 0 || heads <= 0 || max_nodes < 0 || table_cols < 0)
     return fail(TJK_EINVAL, "%s: bad shape tokens=%lld batch=%d heads=%d max_nodes=%d", who, (long long)tokens, batch, heads,
                 max_nodes);

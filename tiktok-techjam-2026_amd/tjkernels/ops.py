@@ -529,6 +529,8 @@ def tree_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor, max_nodes: 
     """The workspace of ``tree_attention`` for any batch with these heads and
     trees of at most max_nodes nodes; calls that share one have to be ordered.
     Its counters start at zero, and each call leaves them there."""
+    if q.dim() != 3 or k_cache.dim() != 4:
+        raise TjkError("q must be [tokens, heads, head_dim], k_cache [pages, kv_heads, page_size, head_dim]")
     need = _lib.load().tjk_tree_attention_bytes(q.shape[1], k_cache.shape[1], q.shape[2], int(max_nodes))
     workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     workspace[:_lib.TREE_COUNTERS].zero_()
@@ -553,13 +555,13 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     multiple of the cache's kv_heads.
 
     A row that sees nothing is zero; what a row does not see does not reach it,
-    whatever it holds.  Positions without a page are left out and counted in
+    whatever it holds.  ``out`` may not overlap ``q``.  Positions without a page are left out and counted in
     ``index_errors``.  ``workspace`` (``tree_attention_workspace``) is allocated
     when it is not given."""
     if workspace is None:
         workspace = tree_attention_workspace(q, k_cache, max_nodes)
     _serve().tree_attention(q, k_cache, v_cache, block_table, ctx_lens, out, cu_nodes, max_nodes, tree_mask,
-                            q.shape[2] ** -0.5 if scale is None else scale, workspace, index_errors)
+                            q.shape[-1] ** -0.5 if scale is None else scale, workspace, index_errors)
     return out
 
 
@@ -579,7 +581,8 @@ def verify_tree(target: torch.Tensor, draft: torch.Tensor, tokens: torch.Tensor,
     the residual distribution with ``sample_u`` fp32 [B], the lowest that passes.
 
     Writes ``path`` int32 [B, max_nodes <= 64] (the accepted nodes, 0 first, then
-    -1), ``count`` int32 [B] and ``token`` int32 [B] (-1 without any weight).
+    -1), ``count`` int32 [B] and ``token`` int32 [B] (-1 without any weight).  A
+    token outside the vocabulary is refused and counts in ``index_errors``.
     ``workspace`` (uint8, tjk_verify_tree_bytes of the vocabulary and the batch, which
     may be none) is allocated when it is not given; calls that share one have to
     be ordered."""

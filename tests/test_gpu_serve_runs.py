@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from tjkernels import _lib, ops
+from tjkernels.graphs import CapturedGraph
 
 pytestmark = pytest.mark.gpu
 
@@ -191,6 +192,28 @@ def _step(d, ws=None):
 
 
 OUT = ("q", "out", "path", "count", "token", "k", "v")
+
+
+def test_step_captured_beside_a_graph_of_inference_mode(device):
+    """The engine's callers are under inference_mode, and so are its captures; while
+    such a graph lives, a step can be captured outside of it, and in it."""
+    x = torch.ones(4, device=device)
+    with torch.inference_mode():
+        kept = CapturedGraph(lambda: x.add_(1), device)
+    d = _inputs(device, 1)
+    _step(d)
+    for mode in (False, True):
+        with torch.inference_mode(mode):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                ops.tree_attention(d["q"], d["k"][0], d["v"][0], d["blocks"], d["ctx"], d["out"], cu_nodes=d["cu"], max_nodes=9)
+        want = ops.tree_attention(d["q"], d["k"][0], d["v"][0], d["blocks"], d["ctx"], torch.empty_like(d["out"]),
+                                  cu_nodes=d["cu"], max_nodes=9)
+        d["out"].zero_()
+        graph.replay()
+        assert torch.equal(d["out"], want)
+    kept.replay()
+    assert (x == 3).all()
 
 
 @pytest.mark.parametrize("own_workspace", [True, False])

@@ -17,6 +17,7 @@ allocation, no host sync, no memset).
 
 from __future__ import annotations
 
+import contextlib
 import warnings
 from collections import OrderedDict
 from typing import Callable, Hashable, Optional, Tuple
@@ -47,7 +48,13 @@ class CapturedGraph:
         origin.wait_stream(side)
         torch.cuda.synchronize(device)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        # The first capture makes torch's own tensors for the generator's state, which
+        # live as long as any graph: made under inference_mode, in which the engine's
+        # callers are, they would refuse every capture of the program's outside of it.
+        capture = torch.cuda.graph(self.graph)
+        with contextlib.ExitStack() as stack:
+            with torch.inference_mode(False):
+                stack.enter_context(capture)
             body()
         # device buffers the recorded kernels read or write (row maps,
         # schedules, workspaces): held for as long as the graph can replay

@@ -333,6 +333,40 @@ def test_many_sequences_of_unequal_length(device):
     Trees(contexts, counts, 2, 1, 32, 16, torch.bfloat16, 32).check(device)
 
 
+@pytest.mark.parametrize("long", [0, 4000])
+@pytest.mark.parametrize("batch,heads,kv,hd", [(70, 6, 1, 64), (9, 8, 2, 128), (66, 12, 4, 32)])
+def test_row_blocks_of_ragged_trees(device, batch, heads, kv, hd, long):
+    """Trees of no, one and several row blocks side by side, more than 64 of them, with
+    a long context among them (stretches) and without one (whole items)."""
+    contexts, counts = [(i * 31) % 75 for i in range(batch)], [(i * 23) % 65 for i in range(batch)]
+    contexts[batch // 2] += long
+    counts[batch // 2] = 64
+    Trees(contexts, counts, heads, kv, hd, 16, torch.bfloat16, 33).check(device)
+
+
+@pytest.mark.parametrize("heads,kv,hd,most", [(8, 8, 64, 3), (16, 8, 128, 9), (32, 8, 64, 12), (32, 8, 128, 15), (9, 9, 48, 1)])
+def test_more_items_than_workgroups(device, heads, kv, hd, most):
+    """A wave has a sequence's key head for itself."""
+    batch = 90
+    contexts, counts = [(i * 41) % 420 for i in range(batch)], [1 + (i * 3) % most if i % 7 else 0 for i in range(batch)]
+    contexts[5], counts[5] = 0, most
+    t = Trees(contexts, counts, heads, kv, hd, 16, torch.bfloat16, 34)
+    want = t.check(device)
+    assert torch.equal(t.run(device), want)
+    t.mask[t.cu[5]] = 0
+    t.table[3, 2], t.table[8, 0] = -1, t.pages
+    t.v[0], t.k[0] = float("nan"), float("inf")  # the page of nobody
+    t.table = t.table[:, :13].contiguous()  # 208 positions
+    errors = torch.zeros(1, dtype=torch.int32, device=device)
+    got = t.run(device, errors=errors)
+    exact, err = t.exact()
+    _within(got, exact, err, t.dt)
+    # halves of tiles of a lost page, which is one of 16, and each sequence that the table cuts off
+    lost = sum(1 for b, col in ((3, 2), (8, 0)) if counts[b] and contexts[b] + counts[b] > 16 * col)
+    assert int(errors) == lost + sum(1 for c, n in zip(contexts, counts) if n and c + n > 208)
+    assert (got[int(t.cu[5])] == 0).all()
+
+
 def test_many_sequences(device):
     """More sequences than lanes of a wave, ragged, some without nodes."""
     counts = [(i * 7) % 5 for i in range(150)]

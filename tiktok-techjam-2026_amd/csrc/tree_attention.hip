@@ -40,7 +40,8 @@ struct TreeArgs {
 // An item is a block of rows of one (sequence, key head): rows m = node * group +
 // query head, ROWS of them.  Its keys are cut into tiles of 32.  An item counts
 // COST units, for what it costs beside its tiles, and one for each tile; all
-// items' units are numbered through, and every workgroup takes an equal stretch of
+// items' units are numbered through (all first row blocks, then all second ones, and so
+// on; in each the sequences, their key heads and tiles), and every workgroup takes an equal stretch of
 // them: lengths are known on the device only, and a long sequence next to short
 // ones is split as finely as it needs.  A stretch that is a whole item writes its rows;
 // else it leaves the rows' sums, with their exponent offset, in the workspace.  Of
@@ -69,10 +70,11 @@ __device__ __forceinline__ T* in_memory(T* p) {  // (a pointer out of the argume
 
 struct Seq {
   int b, n, mbs;  // sequence, its nodes, its row blocks
+  int mb;         // the row block that is meant
   int first;      // its first row
   int ctx, end;   // tokens behind it, positions that it sees
   int tiles;      // of an item
-  int before;     // units before it
+  int before;     // units before it, in front of those of its row block mb
 };
 
 // Sequence b (< batch, else nothing): everything but `before`.
@@ -91,8 +93,9 @@ __device__ __forceinline__ Seq load_seq(const A& a, int b, int rows) {
   }
   return q;
 }
+// Units of one of its row blocks.
 template <typename A>
-__device__ __forceinline__ int seq_units(const A& a, const Seq& q, int cost) { return (q.tiles + cost) * q.mbs * a.kv_heads; }
+__device__ __forceinline__ int seq_units(const A& a, const Seq& q, int cost) { return (q.tiles + cost) * a.kv_heads; }
 
 // Inclusive sum over the lanes.
 __device__ __forceinline__ int wave_scan(int v) {
@@ -105,43 +108,50 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// The sequences of a batch, 64 at a time, and the units before and of them.
+// The sequences of a batch, 64 at a time, and the units before and of them: first
+// those of all sequences' first row blocks, then of the second ones, and so on.
 template <typename Sh>
 struct Plan {
   Seq q;  // lane l: sequence first + l
-  int first, incl, base;
+  int first, incl, base, mb;
+  template <typename A>
+  __device__ __forceinline__ int units(const A& a) const { return q.mbs > mb ? seq_units(a, q, Sh::COST) : 0; }
   template <typename A>
   __device__ __forceinline__ void load(const A& a, int b0) {
     first = b0;
     q = load_seq(a, b0 + (int)(threadIdx.x & 63), Sh::ROWS);
-    incl = wave_scan(seq_units(a, q, Sh::COST));
+    incl = wave_scan(units(a));
   }
   // all of the batch's units; the first 64 sequences are left loaded
   template <typename A>
   __device__ __forceinline__ int total(const A& a) {
     int sum = 0;
+    mb = 0;
     for (int b0 = (a.batch - 1) / 64 * 64; b0 >= 0; b0 -= 64) {
       load(a, b0);
-      sum += __builtin_amdgcn_readlane(incl, 63);
+      sum += __builtin_amdgcn_readlane(Sh::MANY ? wave_scan(seq_units(a, q, Sh::COST) * q.mbs) : incl, 63);
     }
     base = 0;
     return sum;
   }
-  // The sequence that unit `at` (< total, not before the last one asked for) belongs
-  // to, the same in every lane.
+  // The sequence and row block that unit `at` (< total, not before the last one asked
+  // for) belongs to, the same in every lane.
   template <typename A>
   __device__ __forceinline__ Seq find(const A& a, int at) {
     while (true) {
       const uint64_t past = __ballot(base + incl > at);
-      if (past != 0 || first + 64 >= a.batch) {
+      const bool end = first + 64 >= a.batch;
+      if (past != 0 || (end && (!Sh::MANY || mb + 1 >= a.most_mbs))) {
         const int l = past ? __ffsll((unsigned long long)past) - 1 : 0;
-        return {first + l, __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.mbs, l),
+        return {first + l, __builtin_amdgcn_readlane(q.n, l), __builtin_amdgcn_readlane(q.mbs, l), mb,
                 __builtin_amdgcn_readlane(q.first, l), __builtin_amdgcn_readlane(q.ctx, l),
                 __builtin_amdgcn_readlane(q.end, l), __builtin_amdgcn_readlane(q.tiles, l),
-                base + __builtin_amdgcn_readlane(incl - seq_units(a, q, Sh::COST), l)};
+                base + __builtin_amdgcn_readlane(incl - units(a), l)};
       }
       base += __builtin_amdgcn_readlane(incl, 63);
-      load(a, first + 64);
+      mb += end;
+      if (end && first == 0) incl = wave_scan(units(a));
+      else load(a, end ? 0 : first + 64);
     }
   }
 };
@@ -178,7 +188,8 @@ struct Split {
 //
 // RW = 1 (up to 64 rows): the four waves take tiles in turn, each with NST slots of its
 // own, and meet only to join their sums: no barrier in the loop.  Copies run ahead
-// by NST tiles, K and V apart.  RW = 4 (more rows): the waves have 16 NB rows each
+// by NST tiles, K and V apart.  RW = 0: the same, but each wave has an item of its own, and
+// they do not meet at all (many items of few tiles).  RW = 4 (more rows): the waves have 16 NB rows each
 // and share the tiles, in a ring of NST stages of SUB, one barrier a stage.
 //
 // Weights go to the product with V in the cache's type, as in flash_pipe_kernel: half
@@ -236,14 +247,15 @@ __device__ __forceinline__ void copy16(u32x4 rsrc, uint32_t voff, uint32_t lds_a
 // SUB: tiles of a stage of the shared ring (RW = 4).
 template <int HD, int NB, int RW, int NST, int SUB>
 struct TreeShape {
-  static constexpr int ROWS = 16 * NB * RW;
+  static constexpr int ROWS = 16 * NB * (RW > 1 ? RW : 1);
+  static constexpr bool MANY = RW > 1;  // trees of more than one row block
   // Units of an item beside its tiles': 9 single tokens over 29 to 4921, 8 heads of 80,
   // 56 us with 0, 30 with 2, 25.6 with 4, 23.9 with 8; 16 trees of 64 nodes, 2 heads of
   // 128 to a key head, 96 with 8, 79 with 16.
-  static constexpr int COST = RW == 1 ? 8 : 16;
+  static constexpr int COST = RW <= 1 ? 8 : 16;
   static constexpr int RB = 2 * HD;             // bytes of a row in LDS
   static constexpr int TB = kTile * RB;         // of a tile's keys or values
-  static constexpr int RING = (RW == 1 ? 4 : SUB) * NST * 2 * TB;
+  static constexpr int RING = (RW <= 1 ? 4 : SUB) * NST * 2 * TB;
   static constexpr int JOIN = RW == 1 ? 2 * (NB * HD * 64 + NB * 512) : 0;  // two waves' sums
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
   static constexpr int PART = ROWS * (HD + 2);  // floats of a partial result
@@ -266,22 +278,39 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   Seq q;
   int first64 = 0, base64 = 0;  // the 64 sequences that hold q, the units before them
   Split split{};
-  int at, stop, w = blockIdx.x;
-  if (a.direct) {
-    const int per = a.kv_heads * a.most_mbs, b = w / per, item = w - b * per;
+  int at, stop, w;
+  // Workgroups of one XCD have neighbouring stretches, so that the row blocks of a key
+  // head, which read the same keys and values, read them at the same time from its
+  // cache: 32 trees of 64 nodes over 1000 to 8192, 8 heads of 128 to a key head, 227 us with row
+  // blocks side by side, 216 so; 64 trees over 4000 334 and 313; 256 over 450 257 and 242.
+  const int xcd = blockIdx.x % 8, j = blockIdx.x / 8;
+  if constexpr (RW == 0) {
+    const int pair = blockIdx.x * 4 + wave, b = pair / a.kv_heads, kh = pair - b * a.kv_heads;
+    q = load_seq(a, b, Sh::ROWS);
+    if (q.mbs == 0) return;
+    at = kh * (q.tiles + Sh::COST);
+    stop = at + q.tiles + Sh::COST;
+    w = 0;
+  } else if (a.direct) {
+    const int mbs = Sh::MANY ? a.most_mbs : 1, pair = j / mbs * 8 + xcd, b = pair / a.kv_heads, kh = pair - b * a.kv_heads;
     q = load_seq(a, b, Sh::ROWS);
     q.before = 0;
-    const int kh = item / a.most_mbs, mb = item - kh * a.most_mbs;
-    if (mb >= q.mbs) return;
-    at = (kh * q.mbs + mb) * (q.tiles + Sh::COST);
+    q.mb = j - j / mbs * mbs;
+    if (q.mb >= q.mbs) return;
+    at = kh * (q.tiles + Sh::COST);
     stop = at + q.tiles + Sh::COST;
+    w = 0;
   } else {
     Plan<Sh> plan;
     const int total = plan.total(a);
     if (total == 0) return;
     split = Split(total, gridDim.x);
-    // neighbouring stretches on one XCD
-    w = (int)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    const int each = gridDim.x / 8;
+    w = xcd * each + j;
+    if (Sh::MANY) {  // stretches that are as far into the units of each row block
+      const int mbs = min(a.most_mbs, each), per = each / mbs, round = j / mbs;
+      w = round < per ? (j - round * mbs) * (8 * per) + xcd * per + round : j * 8 + xcd;
+    }
     if (w >= split.n) return;
     at = split.share(w);
     stop = split.share(w + 1);
@@ -300,10 +329,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     return CPR == 16 ? r2 | r0 << 1 | r1 << 2 | (r2 ^ r3) << 3 : r2 | r1 << 1 | (r2 ^ r3) << 2;
   };
   // of the DMA instructions of 16 rows (RW = 4: of this wave's)
-  uint32_t voff[RW == 1 ? NV : 1];
+  uint32_t voff[RW <= 1 ? NV : 1];
 #pragma unroll
-  for (int i = 0; i < (RW == 1 ? NV : 1); ++i) {
-    const int r = (RW == 1 ? i : wave % NV) * RPI + lane / CPR, c = (lane % CPR) ^ swz(r);
+  for (int i = 0; i < (RW <= 1 ? NV : 1); ++i) {
+    const int r = (RW <= 1 ? i : wave % NV) * RPI + lane / CPR, c = (lane % CPR) ^ swz(r);
     voff[i] = (uint32_t)r * a.cache.row_bytes + (c < a.hd8 ? 16u * c : kPast);
   }
   // fragment addresses within a tile
@@ -319,20 +348,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     ConstArgs& a = fresh_args();
     if (at >= q.before + seq_units(a, q, Sh::COST)) {  // (loaded again: kept over the tiles, it would take their registers)
       Plan<Sh> plan;
+      plan.mb = q.mb;
       plan.load(a, first64);
       plan.base = base64;
       q = plan.find(a, at);
       first64 = plan.first;
       base64 = plan.base;
     }
-    const int units = q.tiles + Sh::COST, off = at - q.before, item = (int)((uint32_t)off / (uint32_t)units);
-    const int u0 = off - item * units, u1 = min(units, u0 + (stop - at));
+    const int units = q.tiles + Sh::COST, off = at - q.before, kh = (int)((uint32_t)off / (uint32_t)units);
+    const int u0 = off - kh * units, u1 = min(units, u0 + (stop - at));
     const int x0 = at - u0 + Sh::COST;  // the unit of the item's first tile
     const int t0 = max(u0 - Sh::COST, 0), t1 = max(u1 - Sh::COST, 0);
     at += u1 - u0;
     if (t0 == t1) continue;  // its tiles are the next workgroup's
-    const int kh = (int)((uint32_t)item / (uint32_t)q.mbs), mb = item - kh * q.mbs;
-    const int rows = q.n * a.group, m0 = mb * Sh::ROWS + (RW == 1 ? 0 : wave * 16 * NB);
+    const int mb = Sh::MANY ? q.mb : 0;
+    const int rows = q.n * a.group, m0 = mb * Sh::ROWS + (RW <= 1 ? 0 : wave * 16 * NB);
     const int end = q.end;
     const char* const kbase = a.cache.k + kh * a.cache.head_bytes;
     const char* const vbase = a.cache.v + kh * a.cache.head_bytes;
@@ -353,7 +383,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         const int x = (mine + (i0 + lane) * STEP) * kTile + 16 * h;
         const bool in = i0 + lane < count && x < end;
         const int page = page_of(table, in ? x >> a.cache.shift : 0, a.cache.pages);
-        if (in && page < 0 && kh == 0 && mb == 0 && (RW == 1 || wave == 0) && a.index_errors) atomicAdd(in_memory(a.index_errors), 1);
+        if (in && page < 0 && kh == 0 && mb == 0 && (RW <= 1 || wave == 0) && a.index_errors) atomicAdd(in_memory(a.index_errors), 1);
         const bool there = in && page >= 0;
         const uint64_t at = there ? (uint64_t)page * (uint64_t)a.cache.page_bytes +
                                         (uint64_t)((uint32_t)(x & ((1 << a.cache.shift) - 1)) * a.cache.row_bytes)
@@ -382,7 +412,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         qf[i][c] = __builtin_bit_cast(Frag, f);
       }
     }
-    if (kh == 0 && mb == 0 && t0 == 0 && threadIdx.x == 0 && a.index_errors && end < q.ctx + q.n) atomicAdd(in_memory(a.index_errors), 1);
+    if (kh == 0 && mb == 0 && t0 == 0 && (RW == 0 ? lane : threadIdx.x) == 0 && a.index_errors && end < q.ctx + q.n) atomicAdd(in_memory(a.index_errors), 1);
 
     // halves of tile i with nothing to read, for want of a page or past the end: bits 0
     // and 1
@@ -400,7 +430,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     };
     // tile i's keys (or values) to LDS byte `to`
     auto copy = [&](const char* base, int i, uint32_t to) __attribute__((always_inline)) {
-      if constexpr (RW == 1) {
+      if constexpr (RW <= 1) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const u32x4 r = half_range(base, i, h);
@@ -578,7 +608,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     // masks' work, up to one without a page; the others a second one.
     const int plain = min(max((q.ctx / kTile - mine + STEP - 1) / STEP, 0), count);
     int lost[NST];  // empty() of tile i and those behind it
-    if constexpr (RW == 1) {
+    if constexpr (RW <= 1) {
       const uint32_t ring = lds + wave * (NST * 2 * TB);
       char* const mem = smem + wave * (NST * 2 * TB);
 #pragma unroll
@@ -626,41 +656,43 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       for (; i < plain && lost[0] == 0; ++i) step(i, std::false_type{});
       for (; i < count; ++i) step(i, std::true_type{});
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      // ---- join the four waves' sums: 2 and 3 into 0 and 1, then 1 into 0
-      __syncthreads();
-#pragma unroll
-      for (int half = 2; half >= 1; half >>= 1) {
-        float4* const xo = reinterpret_cast<float4*>(smem + (wave & (half - 1)) * (NB * HD * 64 + NB * 512));
-        float* const xm = reinterpret_cast<float*>(xo + NB * HT * 64);
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-#pragma unroll
-            for (int h = 0; h < HT; ++h) xo[(i * HT + h) * 64 + lane] = make_float4(o[i][h][0], o[i][h][1], o[i][h][2], o[i][h][3]);
-            xm[i * 128 + lane] = m_off[i];
-            xm[i * 128 + 64 + lane] = l[i];
-          }
-        }
+      if constexpr (RW == 1) {
+        // ---- join the four waves' sums: 2 and 3 into 0 and 1, then 1 into 0
         __syncthreads();
-        if (wave < half) {
 #pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const float m2 = xm[i * 128 + lane], m = fmaxf(m_off[i], m2);
-            const float f1 = m_off[i] == m ? 1.f : __builtin_amdgcn_exp2f(m_off[i] - m);
-            const float f2 = m2 == m ? 1.f : __builtin_amdgcn_exp2f(m2 - m);
-            m_off[i] = m;
-            l[i] = l[i] * f1 + xm[i * 128 + 64 + lane] * f2;
+        for (int half = 2; half >= 1; half >>= 1) {
+          float4* const xo = reinterpret_cast<float4*>(smem + (wave & (half - 1)) * (NB * HD * 64 + NB * 512));
+          float* const xm = reinterpret_cast<float*>(xo + NB * HT * 64);
+          if (wave >= half && wave < 2 * half) {
 #pragma unroll
-            for (int h = 0; h < HT; ++h) {
-              const float4 v = xo[(i * HT + h) * 64 + lane];
-              o[i][h][0] = o[i][h][0] * f1 + v.x * f2;
-              o[i][h][1] = o[i][h][1] * f1 + v.y * f2;
-              o[i][h][2] = o[i][h][2] * f1 + v.z * f2;
-              o[i][h][3] = o[i][h][3] * f1 + v.w * f2;
+            for (int i = 0; i < NB; ++i) {
+#pragma unroll
+              for (int h = 0; h < HT; ++h) xo[(i * HT + h) * 64 + lane] = make_float4(o[i][h][0], o[i][h][1], o[i][h][2], o[i][h][3]);
+              xm[i * 128 + lane] = m_off[i];
+              xm[i * 128 + 64 + lane] = l[i];
             }
           }
+          __syncthreads();
+          if (wave < half) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+              const float m2 = xm[i * 128 + lane], m = fmaxf(m_off[i], m2);
+              const float f1 = m_off[i] == m ? 1.f : __builtin_amdgcn_exp2f(m_off[i] - m);
+              const float f2 = m2 == m ? 1.f : __builtin_amdgcn_exp2f(m2 - m);
+              m_off[i] = m;
+              l[i] = l[i] * f1 + xm[i * 128 + 64 + lane] * f2;
+#pragma unroll
+              for (int h = 0; h < HT; ++h) {
+                const float4 v = xo[(i * HT + h) * 64 + lane];
+                o[i][h][0] = o[i][h][0] * f1 + v.x * f2;
+                o[i][h][1] = o[i][h][1] * f1 + v.y * f2;
+                o[i][h][2] = o[i][h][2] * f1 + v.z * f2;
+                o[i][h][3] = o[i][h][3] * f1 + v.w * f2;
+              }
+            }
+          }
+          __syncthreads();
         }
-        __syncthreads();
       }
     } else {
       constexpr int NI = SUB * 2 * ((NK + 3) / 4);  // a wave's DMA instructions of a stage
@@ -737,7 +769,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     };
     const bool whole = t0 == 0 && t1 == q.tiles;
     const int part = 2 * w + (t0 == 0 ? 1 : 0);  // a stretch ends in the first part of an item at most once
-    if (RW > 1 || wave == 0) {
+    if (RW != 1 || wave == 0) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const int m = m0 + 16 * i + col, r = m - mb * Sh::ROWS;
@@ -762,7 +794,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         }
       }
     }
-    if (whole) continue;
+    if (RW == 0 || whole) continue;
 
     // ---- the last of eight joins them, until the item is whole
     const int w0 = split.holder(x0);
@@ -899,6 +931,19 @@ static bool whole_items(int64_t items, int64_t tiles) {
   return tiles <= std::min<int64_t>(std::max<int64_t>(32, 24 + items / 4), 96);
 }
 
+// Whether a wave has an item for itself: where there are more items than workgroups at
+// once and few tiles for four waves.  us by workgroups / by waves, contexts spread from an
+// eighth of the table up, head_dim 64 (128): 512 items of 8 tiles 11.6 / 12.1 (15.0 / 14.7),
+// of 16 14.6 / 16.6 (20.3 / 21.3); 1024 of 2 14.5 / 8.3 (17.9 / 11.0), of 16 22.7 / 19.5
+// (39.1 / 38.0), of 32 38.9 / 37.5 (65.7 / 67.6); 8192 of 2 93 / 29 (119 / 47), of 16 149 /
+// 114 (228 / 213).
+static bool one_wave(int64_t items, int64_t tiles, int64_t groups) { return items > groups && tiles <= 24; }
+
+template <typename T, int HD, int NB, int RW, int NST, int OCC, int SUB>
+static void start_tree(const TreeArgs& a, int64_t groups, hipStream_t s) {
+  tree_attention_kernel<T, HD, NB, RW, NST, OCC, SUB><<<(unsigned)groups, 256, 0, s>>>(a);
+}
+
 template <typename T, typename V>
 static int launch_tree(TreeArgs a, hipStream_t s) {
   constexpr int ROWS = V::Sh::ROWS;
@@ -908,7 +953,15 @@ static int launch_tree(TreeArgs a, hipStream_t s) {
     return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
   if (a.out == a.q) return fail(TJK_EINVAL, "tjk_tree_attention: out may not be q, which other workgroups still read");
   a.direct = whole_items(items, tiles);
-  tree_attention_kernel<T, V::HD, V::NB, V::RW, V::NST, V::OCC, V::SUB><<<a.direct ? (unsigned)items : V::GRID, 256, 0, s>>>(a);
+  if constexpr (V::RW == 1) {
+    if (a.direct && one_wave(items, tiles, V::GRID)) {
+      start_tree<T, V::HD, V::NB, 0, V::NST, V::OCC, V::SUB>(a, (items + 3) / 4, s);
+      return check_launch("tjk_tree_attention");
+    }
+  }
+  // whole items: eight key heads, an XCD each, and their row blocks
+  const int64_t groups = a.direct ? ((int64_t)a.batch * a.kv_heads + 7) / 8 * 8 * a.most_mbs : V::GRID;
+  start_tree<T, V::HD, V::NB, V::RW, V::NST, V::OCC, V::SUB>(a, groups, s);
   return check_launch("tjk_tree_attention");
 }
 

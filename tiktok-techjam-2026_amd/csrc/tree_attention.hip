@@ -202,10 +202,15 @@ struct Split {
 // 64, 56 us, of which the stretches take 34 to 46, the joining 12.  8 single tokens
 // over up to 512: 9.4 us, launch and passages of memory one after the other (places 2,
 // first tiles 1.5, the rest of them 3, joining of the waves 1).  Many rows are bound
-// by issue: 32 trees of 64 nodes, 8 heads of 128 to a key head, 230 us, 680 TFLOP/s
-// (770 in long stretches): matrix unit 27% of the time, vector unit 36%, LDS 21%; 48
-// rows a wave take 238 to 253, 64 rows 261 (one wave a SIMD; two do not fit), three
-// waves a SIMD do not fit.
+// by the matrix and the vector unit and by power: 32 trees of 64 nodes over 1000 to 8192,
+// 8 heads of 128 to a key head, 200 to 216 us, 720 to 780 TFLOP/s (64 over
+// 4000: 313 us, 870); matrix
+// unit 31% of the time, vector unit 36%, LDS 21%.  (Before row blocks lay side by side,
+// 336 us for the latter: 280 if every page lay in L2, and 280 if keys and values were
+// zeros, at the same traffic.)  Per wave 48 rows take 5 to 10% longer than 32, 64
+// (one wave a SIMD; two do not fit) 15%, three waves a SIMD do not fit; the next tile's
+// scores ahead of the softmax, with a barrier a tile for it, 8 to 15% longer;
+// fragments loaded further ahead and wave priorities, no difference.
 
 constexpr uint32_t kPast = 0x80000000u;  // beyond any descriptor's range
 // Cache policies: stores through to memory, loads from it, past an XCD's own L2.
@@ -281,8 +286,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
   int at, stop, w;
   // Workgroups of one XCD have neighbouring stretches, so that the row blocks of a key
   // head, which read the same keys and values, read them at the same time from its
-  // cache: 32 trees of 64 nodes over 1000 to 8192, 8 heads of 128 to a key head, 227 us with row
-  // blocks side by side, 216 so; 64 trees over 4000 334 and 313; 256 over 450 257 and 242.
+  // cache: 32 trees of 64 nodes over 1000 to 8192, 8 heads of 128 to a key head, 227 us with
+  // row blocks one after the other, 216 and a third of the reads from memory so; 64 trees
+  // over 4000 334 and 313; 256 over 450 257 and 242.
   const int xcd = blockIdx.x % 8, j = blockIdx.x / 8;
   if constexpr (RW == 0) {
     const int pair = blockIdx.x * 4 + wave, b = pair / a.kv_heads, kh = pair - b * a.kv_heads;

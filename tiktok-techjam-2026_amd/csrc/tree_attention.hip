@@ -809,61 +809,74 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     const int live = min(rows - mb * Sh::ROWS, Sh::ROWS);
     // Joins n sums, of stretches first, first + span, ...: into the rows if that is
     // all of the item, else in the place of the first.  L lanes a row; where rows
-    // leave lanes free, `shares` groups of lanes take the stretches in turn.
-    auto join_parts = [&](int first, int span, int n, bool whole) __attribute__((always_inline)) {
-      constexpr int L = HD / 4, GROUPS = 256 / L;
-      int wide = GROUPS;
-      while (wide / 2 >= live) wide /= 2;
-      const int shares = GROUPS / wide, group = threadIdx.x / L, c0 = threadIdx.x % L * 4, share = group / wide;
-      for (int r0 = 0; r0 < live; r0 += wide) {
-        const int r = min(r0 + group % wide, live - 1);
-        u32x2 ml[kJoin];
-        u32x4 v[kJoin];
+    // leave lanes free, `shares` groups of lanes take the stretches in turn.  Of many rows,
+    // the fewer the stretches the more are asked for together (Q of them for N
+    // stretches): 17 sequences over up to 12239, 4 to 10 nodes, 16 heads of 128 to a key
+    // head, 105 us with one row of each lane at a time, 95 so; 64-node trees over 1000
+    // to 8192 204 and 201.  Fewer rows gain nothing, and lose 1 to 4% by the longer code.
+    constexpr int L = HD / 4, GROUPS = 256 / L;
+    int wide = GROUPS;
+    while (wide / 2 >= live) wide /= 2;
+    const int shares = GROUPS / wide, group = threadIdx.x / L, c0 = threadIdx.x % L * 4, share = group / wide;
+    auto join_parts = [&](auto most, auto together, int first, int span, int n, bool whole) __attribute__((always_inline)) {
+      constexpr int N = decltype(most)::value, Q = decltype(together)::value;
+      for (int r0 = group % wide; r0 - group % wide < live; r0 += wide * Q) {
+        u32x2 ml[Q][N];
+        u32x4 v[Q][N];
 #pragma unroll
-        for (int u = 0; u < kJoin; ++u) {
+        for (int u = 0; u < N; ++u) {
           const int p = part_of(first + min(share + u * shares, n - 1) * span);
           if (u * shares < n) {
-            ml[u] = __builtin_amdgcn_raw_buffer_load_b64(parts, 4 * (p * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kCoherent);
-            v[u] = __builtin_amdgcn_raw_buffer_load_b128(parts, 4 * (p * Sh::PART + r * HD + c0), 0, kCoherent);
+#pragma unroll
+            for (int k = 0; k < Q; ++k) {
+              const int r = min(r0 + k * wide, live - 1);
+              ml[k][u] = __builtin_amdgcn_raw_buffer_load_b64(parts, 4 * (p * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kCoherent);
+              v[k][u] = __builtin_amdgcn_raw_buffer_load_b128(parts, 4 * (p * Sh::PART + r * HD + c0), 0, kCoherent);
+            }
           }
         }
-        float top = -INFINITY, sum = 0.f;
-        f32x4 y = {0, 0, 0, 0};
-        auto add = [&](float m2, float l2, f32x4 v2) {
-          const float t = fmaxf(top, m2);
-          const float f1 = top == t ? 1.f : __builtin_amdgcn_exp2f(top - t), f2 = m2 == t ? 1.f : __builtin_amdgcn_exp2f(m2 - t);
-          top = t;
-          sum = sum * f1 + l2 * f2;
-          y = y * f1 + v2 * f2;
-        };
 #pragma unroll
-        for (int u = 0; u < kJoin; ++u)
-          if (share + u * shares < n) add(__uint_as_float(ml[u][0]), __uint_as_float(ml[u][1]), __builtin_bit_cast(f32x4, v[u]));
-        if (shares > 1) {  // (then one round of rows)
-          f32x4* const so = reinterpret_cast<f32x4*>(smem);
-          float2* const sm = reinterpret_cast<float2*>(smem + 4096);
-          so[threadIdx.x] = y;
-          sm[threadIdx.x] = make_float2(top, sum);
-          __syncthreads();
-          if (share == 0)
-            for (int u = 1; u < min(shares, n); ++u) {
-              const int other = threadIdx.x + u * wide * L;
-              add(sm[other].x, sm[other].y, so[other]);
-            }
-          __syncthreads();
-        }
-        if (share != 0 || r0 + group % wide >= live) continue;
-        if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-          if (c0 < 8 * z.hd8)
-            *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) =
-                Quad<T>::from(make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
-        } else {
-          const int p = part_of(first);
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, 4 * (p * Sh::PART + r * HD + c0), 0, kThrough);
-          if (c0 == 0)
-            __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(top), __float_as_uint(sum)}, parts,
-                                                  4 * (p * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kThrough);
+        for (int k = 0; k < Q; ++k) {
+          const int r = r0 + k * wide;
+          float top = -INFINITY, sum = 0.f;
+          f32x4 y = {0, 0, 0, 0};
+          auto add = [&](float m2, float l2, f32x4 v2) {
+            const float t = fmaxf(top, m2);
+            const float f1 = top == t ? 1.f : __builtin_amdgcn_exp2f(top - t), f2 = m2 == t ? 1.f : __builtin_amdgcn_exp2f(m2 - t);
+            top = t;
+            sum = sum * f1 + l2 * f2;
+            y = y * f1 + v2 * f2;
+          };
+#pragma unroll
+          for (int u = 0; u < N; ++u)
+            if (share + u * shares < n)
+              add(__uint_as_float(ml[k][u][0]), __uint_as_float(ml[k][u][1]), __builtin_bit_cast(f32x4, v[k][u]));
+          if (Q == 1 && shares > 1) {  // (then one round of rows)
+            f32x4* const so = reinterpret_cast<f32x4*>(smem);
+            float2* const sm = reinterpret_cast<float2*>(smem + 4096);
+            so[threadIdx.x] = y;
+            sm[threadIdx.x] = make_float2(top, sum);
+            __syncthreads();
+            if (share == 0)
+              for (int u = 1; u < min(shares, n); ++u) {
+                const int other = threadIdx.x + u * wide * L;
+                add(sm[other].x, sm[other].y, so[other]);
+              }
+            __syncthreads();
+          }
+          if (share != 0 || r >= live) continue;
+          if (whole) {
+            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            if (c0 < 8 * z.hd8)
+              *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) =
+                  Quad<T>::from(make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
+          } else {
+            const int p = part_of(first);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, 4 * (p * Sh::PART + r * HD + c0), 0, kThrough);
+            if (c0 == 0)
+              __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(top), __float_as_uint(sum)}, parts,
+                                                    4 * (p * Sh::PART + Sh::ROWS * HD + 2 * r), 0, kThrough);
+          }
         }
       }
     };
@@ -885,7 +898,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         const bool joins = *word != 0;
         __syncthreads();
         if (!joins) break;
-        join_parts(first, span, n, span * kJoin >= stretches);
+        const bool all = span * kJoin >= stretches;
+        typedef std::integral_constant<int, 1> One;
+        if (!Sh::MANY || shares > 1) join_parts(std::integral_constant<int, kJoin>{}, One{}, first, span, n, all);
+        else if constexpr (Sh::MANY) {
+          if (n <= 2) join_parts(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{}, first, span, n, all);
+          else if (n <= 4) join_parts(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}, first, span, n, all);
+          else join_parts(std::integral_constant<int, kJoin>{}, std::integral_constant<int, 16 / kJoin>{}, first, span, n, all);
+        }
       }
     }
   }

@@ -42,13 +42,17 @@ struct VerifyArgs {
 // that holds it is read again.  A sequence's vocabulary is cut into `parts`, a
 // workgroup each; every one walks the same walk from the same numbers and meets
 // the others at the sums only: each puts its own in the workspace and reads
-// theirs.  64 trees of up to 32 nodes over 128257 tokens: 32 us (one workgroup a
-// sequence 77), of which the clearing of the sums' places 3; the distributions of the last
-// nodes alone are 13 at a copy's rate, but a tree with five refusals makes five passes,
-// one after the other, of about 5 us: 128 KB by one CU, the waves' sums, and two
-// passages of memory to the other parts and back.  Four chains of six over 32000: 10 us.  It waits a bounded time: a sum that does not come (workgroups of other
+// theirs.  It waits a bounded time: a sum that does not come (workgroups of other
 // work may hold the chip) it computes itself, in the same order, so nothing hangs on
 // who was there.
+//
+// 64 trees of up to 32 nodes over 128257 tokens: 32 to 36 us (one workgroup a sequence
+// 77), of which the clearing of the sums' places 3 to 5; the distributions of the last
+// nodes alone are 13 at a copy's rate, but a tree with five refusals makes five
+// passes, one after the other, of about 5 us: 128 KB by one CU, the waves' sums, and two
+// passages of memory to the other parts and back.  A part's p and q held in registers
+// for a second refusal at a node took 4 us off that, and added 0.6 to the 11 of four
+// chains of six over 32000.
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kMostParts = 64;

@@ -517,7 +517,7 @@ size_t tjk_tree_attention_bytes(int heads, int kv_heads, int head_dim, int max_n
  * the next token is the smallest x with r_k(0) + .. + r_k(x) > sample_u sum r_k
  * (k: the children refused; c_k = 0 if W_k is zero; -1 if p has no weight).  So the
  * tokens are distributed as the target's.  Products and sums in 64 bits; negative
- * and NaN weights count as zero.  A child with a token outside [0, vocab) is
+ * and NaN weights, p's and q's, count as zero.  A child with a token outside [0, vocab) is
  * refused and counts in *index_errors; a node whose parent is none before it is
  * not reached, nor are those past max_nodes or rows.
  * path [batch, max_nodes]: the accepted nodes, node 0 first, then -1; count: how

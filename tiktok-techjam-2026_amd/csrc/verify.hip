@@ -71,8 +71,11 @@ struct Slot {  // of a workgroup's sum: its halves, each with the round it belon
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may begin anywhere
 
+// A draft's weight: none if it is negative or NaN, which could otherwise take a token
+// that the target excludes.
+__device__ __forceinline__ float drafted(float q) { return fmaxf(q, 0.f); }
 __device__ __forceinline__ double residual(float p, double c, float q) {
-  const double r = (double)p - c * (double)q;
+  const double r = (double)p - c * (double)drafted(q);
   return r > 0 ? r : 0;  // NaN: no weight
 }
 
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
       parent = -1;
     } else if (x >= 0 && x < a.vocab) {
       pj = a.target[(first + parent) * a.ld_target + x];
-      qj = a.draft[(first + parent) * a.ld_draft + x];
+      qj = drafted(a.draft[(first + parent) * a.ld_draft + x]);
     } else {
       pj = -1.f;  // of no token: refused
       if (part == 0 && wave == 0 && a.index_errors) atomicAdd(a.index_errors, 1);

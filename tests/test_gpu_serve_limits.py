@@ -1,9 +1,12 @@
-"""The serving operators where their numbers end: weights that are none."""
+"""The serving operators where their numbers end: weights that are none, weights far
+below a row's largest."""
 
 import pytest
 import torch
 
-from test_gpu_serve import Drafts, _verify_oracle
+from tjkernels import ops
+
+from test_gpu_serve import U, Drafts, Trees, _half, _verify_oracle, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +30,56 @@ def test_negative_and_nan_draft_weights_are_zero(device, vocab, shape):
         d.tokens = torch.randint(0, vocab, (t,), generator=g).tolist()
         want = _verify_oracle(d.p, d.q.nan_to_num(0, neginf=0).clamp(min=0), d.tokens, d.parents, d.au, d.su, d.cu, d.n_max)
         assert d.run(device) == want
+
+
+def _set_scores(t, b, scores):
+    """Keys of sequence b with these scores, for a scale of 1: the queries are the
+    first unit vector."""
+    x = torch.arange(len(scores))
+    t.q.zero_()
+    t.q[..., 0] = 1
+    t.k[t.table[b][x // t.page].long(), 0, x % t.page, 0] = scores.to(t.dt)
+
+
+@pytest.mark.parametrize("low,high", [(-18.2, -17.4), (-18.0, -9.7), (-22.0, -18.0)])
+@pytest.mark.parametrize("sink", [0.0, 0.37, 1.0])
+@pytest.mark.parametrize("nodes,heads,batch", [(1, 1, 600), (64, 2, 300)])
+def test_far_smaller_weights_of_many_keys(device, low, high, sink, nodes, heads, batch):
+    """One key takes most of a row, and 99995 others, 2^14 to 2^32 below it, give what
+    its value, zero, leaves.  So many sequences share the pages that each is one
+    workgroup's, and every key of a wave is held against the same offset.  fp16 weights
+    are off by half a step, and by 2^-25 at least, where the largest is 2^7 or more: by
+    2^-32 of it, in the weights' sum too."""
+    n = 99995
+    t = Trees([n - 1], [nodes], heads, 1, 16, 64, torch.float16, 40)
+    t.mask[:] = 1  # the first node
+    s = low + (high - low) * torch.rand(n, generator=t.g)
+    s[int(sink * (n - 1))] = 0
+    _set_scores(t, 0, s)
+    t.v = (0.5 + 0.5 * torch.rand(t.v.shape, generator=t.g)).half()
+    at = int(sink * (n - 1))
+    t.v[t.table[0, at // 64], :, at % 64] = 0
+    x = torch.arange(n)
+    page, row = t.table[0][x // 64].long(), x % 64
+    k, v = t.k[page, 0, row, 0].double(), t.v[page, 0, row].double()
+    p = torch.softmax(k, 0)
+    want = p @ v
+    # (see Trees.exact: scores are exact here, the weights' arguments and sums are not)
+    err = want * (2 * (((k.max() - k.min()) * 1.45 + 6) * U + _half(t.dt)) + 2 * (n + 8) * U) + 2 * 2.0 ** -32 * p.max() * v.sum(0)
+    got = ops.tree_attention(t.q.repeat(batch, 1, 1).to(device), t.k.to(device), t.v.to(device),
+                             t.table.repeat(batch, 1).to(device), t.ctx.repeat(batch).to(device),
+                             torch.full((batch * nodes, heads * 16), 7.0, dtype=t.dt, device=device),
+                             cu_nodes=torch.arange(0, batch * nodes + 1, nodes, dtype=torch.int32, device=device),
+                             max_nodes=nodes, tree_mask=t.mask.repeat(batch).to(device), scale=1.0)
+    _within(got.view(-1, 16), want, err, t.dt)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_scores_that_rise_along_a_row(device, dt):
+    """Slowly, so that weights grow far past 1 before the row's offset follows: none
+    passes the type's range."""
+    for span in (5.5, 60.0, 700.0):
+        t = Trees([3001, 40, 20000], [1, 1, 1], 2, 1, 16, 64, dt, 42, mask=None)
+        for b, c in enumerate(t.contexts):
+            _set_scores(t, b, torch.linspace(-span, 0, c + 1))
+        t.check(device, scale=1.0)

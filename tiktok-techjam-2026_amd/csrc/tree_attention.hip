@@ -218,6 +218,12 @@ constexpr int kThrough = 17, kCoherent = 16;
 // A row's offset follows its scores when they pass it by 2^8: most tiles rescale
 // nothing, and a weight of up to 256 is no harm in either type.
 constexpr float kLazy = 8.0f;
+// Weights are 2^kLift above what the offset makes of them (it cancels in the result,
+// and all parts of an item share it).  fp16 weights are whole multiples of 2^-24, and
+// with the largest at 1 a row of one large weight and 99995 of 2^-25 and less lost them
+// all; of 2^7 to 2^15 the largest, the rounding is 2^-32 of it.
+template <typename T>
+constexpr float kLift = std::is_same<T, f16>::value ? 7.0f : 0.0f;
 
 template <typename T> struct Mfma16;
 template <> struct Mfma16<bf16> {
@@ -520,7 +526,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const float base = m_off[i] == -INFINITY ? 0.f : -m_off[i];
+          const float base = m_off[i] == -INFINITY ? 0.f : kLift<T> - m_off[i];
           float e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[u][i][j >> 2][j & 3], scale, base));

@@ -75,8 +75,7 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows m
 // that the target excludes.
 __device__ __forceinline__ float drafted(float q) { return fmaxf(q, 0.f); }
 __device__ __forceinline__ double residual(float p, double c, float q) {
-  const double r = (double)p - c * (double)drafted(q);
-  return r > 0 ? r : 0;  // NaN: no weight
+  return fmax((double)p - c * (double)drafted(q), 0.);  // NaN: no weight
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -85,10 +84,11 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// Four weights from x on (x + 4 past `end`: what there is).
+// Four weights from x on (WHOLE: all before `end`; else what there is).
+template <bool WHOLE = false>
 __device__ __forceinline__ void weights4(const float* p, const float* q, double c, int x, int end, double (&w)[4]) {
   float a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
-  if (x + 4 <= end) {
+  if (WHOLE || x + 4 <= end) {
     const f32x4u v = *reinterpret_cast<const f32x4u*>(p + x);
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = v[i];
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     for (; x - 4 * lane + 1024 <= end; x += 1024) {
       double w[4][4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) weights4(p, q, c, x + 256 * u, end, w[u]);
+      for (int u = 0; u < 4; ++u) weights4<true>(p, q, c, x + 256 * u, end, w[u]);
 #pragma unroll
       for (int u = 0; u < 4; ++u) s += (w[u][0] + w[u][1]) + (w[u][2] + w[u][3]);
     }

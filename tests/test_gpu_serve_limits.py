@@ -1,5 +1,5 @@
 """The serving operators where their numbers end: weights that are none, weights far
-below a row's largest."""
+below a row's largest, scores and values that are not finite."""
 
 import pytest
 import torch
@@ -83,3 +83,18 @@ def test_scores_that_rise_along_a_row(device, dt):
         for b, c in enumerate(t.contexts):
             _set_scores(t, b, torch.linspace(-span, 0, c + 1))
         t.check(device, scale=1.0)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("contexts,counts,heads,kv,hd", [([70, 0], [3, 5], 4, 2, 64), ([5000, 1], [1, 1], 1, 1, 64),
+                                                         ([90, 200], [64, 40], 8, 2, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_of_infinitely_low_scores_are_zero(device, dt, contexts, counts, heads, kv, hd, bad):
+    """Keys that take every row to -inf give a row of zeros, whatever their values
+    hold."""
+    t = Trees(contexts, counts, heads, kv, hd, 16, dt, 41)
+    t.q = t.q.abs() + 1
+    t.k[:] = -float("inf")
+    t.v[:, :, ::3] = bad
+    got = t.run(device)
+    assert (got == 0).all()

@@ -779,6 +779,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       return reinterpret_cast<T*>(in_memory(z.out) + (int64_t)(q.first + node) * z.out_bytes) +
              (int64_t)(kh * z.group + m - node * z.group) * (8 * z.hd8);
     };
+    // four elements of a row, of the weighted and of the weights' sum; zeros if there is
+    // no weight (weights of zero may have met values that are not finite)
+    auto result = [&](const f32x4& y, float sum) {
+      const float inv = 1.0f / sum;
+      return Quad<T>::from(sum == 0.f ? make_float4(0, 0, 0, 0) : make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
+    };
     const bool whole = t0 == 0 && t1 == q.tiles;
     const int part = 2 * w + (t0 == 0 ? 1 : 0);  // a stretch ends in the first part of an item at most once
     if (RW != 1 || wave == 0) {
@@ -788,13 +794,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         const float sum = column_sum(l[i]);
         if (m >= rows) continue;
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
           T* const dst = out_row(m);
 #pragma unroll
           for (int h = 0; h < HT; ++h)
-            if (2 * h < z.hd8)
-              *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) =
-                  Quad<T>::from(make_float4(o[i][h][0] * inv, o[i][h][1] * inv, o[i][h][2] * inv, o[i][h][3] * inv));
+            if (2 * h < z.hd8) *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) = result(o[i][h], sum);
         } else {
 #pragma unroll
           for (int h = 0; h < HT; ++h)
@@ -872,10 +875,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
           }
           if (share != 0 || r >= live) continue;
           if (whole) {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
             if (c0 < 8 * z.hd8)
-              *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) =
-                  Quad<T>::from(make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
+              *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) = result(y, sum);
           } else {
             const int p = part_of(first);
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, 4 * (p * Sh::PART + r * HD + c0), 0, kThrough);

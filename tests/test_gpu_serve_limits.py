@@ -1,10 +1,12 @@
 """The serving operators where their numbers end: weights that are none, weights far
-below a row's largest, scores and values that are not finite."""
+below a row's largest, scores and values that are not finite, sums that do not come."""
+
+import ctypes
 
 import pytest
 import torch
 
-from tjkernels import ops
+from tjkernels import _lib, ops
 
 from test_gpu_serve import U, Drafts, Trees, _half, _verify_oracle, _within
 
@@ -30,6 +32,48 @@ def test_negative_and_nan_draft_weights_are_zero(device, vocab, shape):
         d.tokens = torch.randint(0, vocab, (t,), generator=g).tolist()
         want = _verify_oracle(d.p, d.q.nan_to_num(0, neginf=0).clamp(min=0), d.tokens, d.parents, d.au, d.su, d.cu, d.n_max)
         assert d.run(device) == want
+
+
+def _run_with_polls(d, device, polls):
+    """d.run(device) where a workgroup looks `polls` times for another's sum."""
+    call = _lib.load().tjk_verify_tree_polls
+    types = _lib._SIGNATURES["tjk_verify_tree"][1]
+    call.restype, call.argtypes = ctypes.c_int, types[:-1] + [ctypes.c_int] + types[-1:]
+    batch, vocab, rows = len(d.counts), d.p.shape[1], len(d.tokens)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    need = _lib.load().tjk_verify_tree_bytes(vocab, batch)
+    assert need > 0  # several workgroups
+    workspace = torch.full((need,), 255, dtype=torch.uint8, device=device)
+    path = torch.full((batch, d.n_max), 99, dtype=torch.int32, device=device)
+    out = [path, i32([99] * batch), i32([99] * batch)]
+    put = [x.to(device) for x in (d.p, d.q, d.au, d.su)] + [i32(d.tokens), i32(d.parents), i32(d.cu)]
+    p, q, au, su, tokens, parents, cu = [x.data_ptr() for x in put]
+    assert call(p, vocab, q, vocab, tokens, parents, au, su, cu, path.data_ptr(), d.n_max, out[1].data_ptr(), out[2].data_ptr(),
+                None, rows, vocab, batch, d.n_max, workspace.data_ptr(), need, polls,
+                torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    return tuple(x.tolist() for x in out)
+
+
+@pytest.mark.parametrize("polls", [0, 1, 2, 5])
+@pytest.mark.parametrize("counts,vocab", [([12, 20], 128257), ([64], 300001), ([9, 1, 0, 17] * 10, 50001)])
+def test_verify_without_the_others_sums(device, polls, counts, vocab):
+    """Workgroups that miss some or all of the others' sums compute them themselves:
+    the same paths and tokens, with many refusals, without any, and where a residual is
+    nothing."""
+    assert _lib.load().tjk_verify_tree_bytes(vocab, len(counts)) > 0
+    for seed in range(3):
+        d = Drafts(counts, vocab, "tree", seed, noise=(1.0, 4.0, 0.1)[seed])
+        if seed == 1:
+            d.au = 1 - d.au / 8  # refusals
+            b = counts[0]
+            d.p[:b], d.q[:b] = 1 / (2 * vocab), 1 / vocab  # p below q everywhere
+        assert _run_with_polls(d, device, polls) == d.want()
+    d = Drafts([64] if len(counts) == 1 else [64, 3], vocab, "chain", 7, noise=3.0)
+    d.parents = [-1] + [0] * 63 + ([] if len(counts) == 1 else [-1, 0, 0])  # 63 children of the root, most refused
+    d.tokens[1:64] = (d.q[0] - d.p[0]).topk(63).indices.tolist()
+    d.au[1:64] = 1 - 2.0 ** -20
+    assert _run_with_polls(d, device, polls) == d.want()
 
 
 def _set_scores(t, b, scores):

@@ -30,10 +30,11 @@ struct VerifyArgs {
   int32_t* count;
   int32_t* token;
   int* index_errors;
-  struct Slot* slots;  // [batch][2][parts]
+  struct Slot* slots;  // [batch][max_nodes][parts]
   int64_t rows;
   int batch, max_nodes, vocab;
   int parts, part;  // workgroups of a sequence, elements of each
+  int polls;        // of a missing sum
 };
 
 // The walk needs p and q at the drafted tokens only, which the lanes of a wave
@@ -44,7 +45,10 @@ struct VerifyArgs {
 // the others at the sums only: each puts its own in the workspace and reads
 // theirs.  It waits a bounded time: a sum that does not come (workgroups of other
 // work may hold the chip) it computes itself, in the same order, so nothing hangs on
-// who was there.
+// who was there; a part that was missed once is looked for only once at the next
+// sums, until it is there again.  Each of a sequence's sums has places of its own (a
+// refusal takes one, and the end one: max_nodes at most), so that a workgroup that comes
+// late finds all that the others left.
 //
 // 64 trees of up to 32 nodes over 128257 tokens: 32 to 36 us (one workgroup a sequence
 // 77), of which the clearing of the sums' places 3 to 5; the distributions of the last
@@ -56,8 +60,10 @@ struct VerifyArgs {
 
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kMostParts = 64;
-// Workgroups of a launch: one per CU, so that they are all there.  64 trees over 128257:
-// 38 us with 256 or 512, 810 with 1024, which are not and run out of patience.
+// Workgroups of a launch: one per CU, so that they are all there, beside other work
+// too.  64 trees over 128257: 37.7 us with 256, 34.8 with 512 (parts of 8192), 119 with
+// 1024 (parts of 4096), which are not all there (298 while late ones did not find the
+// sums that they had missed).
 constexpr int kMostGroups = 256;
 // Least elements of a part, us with 4096 / 8192 / 16384: chain over 32000 10.9 / 10.8 / 9.3 (no
 // meeting), 16 trees over 50000 20.4 / 21.1 / 22.2, 4 over 128000 19.1 / 16.9 / 17.5, 64 over
@@ -65,7 +71,9 @@ constexpr int kMostGroups = 256;
 constexpr int kPartElements = 16384;
 constexpr int kPolls = 256;  // of a missing sum: about 50 us
 
-struct Slot {  // of a workgroup's sum: its halves, each with the round it belongs to
+constexpr int kMostNodes = 64;
+
+struct Slot {  // of a workgroup's sum: its halves, each with the number of the sum; zeros before
   uint64_t half[2];
 };
 
@@ -168,6 +176,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     return s;
   };
   int round = 0;
+  bool late = false;  // thread i < parts: part i's last sum did not come
   // The whole sum at (p, q, c); part_sums has the parts'.
   auto sum_all = [&](double c) {
     ++round;
@@ -177,7 +186,7 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
       __syncthreads();
       return mine;
     }
-    Slot* const slots = a.slots + (b * 2 + (round & 1)) * a.parts;
+    Slot* const slots = a.slots + ((int64_t)b * a.max_nodes + round - 1) * a.parts;
     const uint64_t bits = __builtin_bit_cast(uint64_t, mine), tag = (uint64_t)round << 32;
     if (tid == 0) {
       __hip_atomic_store(&slots[part].half[0], tag | (uint32_t)bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -186,19 +195,22 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
     }
     __syncthreads();
     if (tid < a.parts) {
-      uint64_t lo = tag | (uint32_t)bits, hi = tag | bits >> 32;
+      double sum = mine;
       if (tid != part) {
-        for (int i = 0; i < kPolls; ++i) {
+        uint64_t lo = 0, hi = 0;
+        bool there = false;
+        const int polls = late ? min(a.polls, 1) : a.polls;
+        for (int i = 0; i < polls && !there; ++i) {
+          if (i > 0) __builtin_amdgcn_s_sleep(1);
           lo = __hip_atomic_load(&slots[tid].half[0], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           hi = __hip_atomic_load(&slots[tid].half[1], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          if (lo >> 32 == (uint64_t)round && hi >> 32 == (uint64_t)round) break;
-          __builtin_amdgcn_s_sleep(1);
+          there = lo >> 32 == (uint64_t)round && hi >> 32 == (uint64_t)round;
         }
+        late = !there;
+        sum = there ? __builtin_bit_cast(double, hi << 32 | (uint32_t)lo) : -1;
+        if (late) missing = 1;
       }
-      if (lo >> 32 == (uint64_t)round && hi >> 32 == (uint64_t)round)
-        part_sums[tid] = __builtin_bit_cast(double, hi << 32 | (uint32_t)lo);
-      else
-        part_sums[tid] = -1, missing = 1;
+      part_sums[tid] = sum;
     }
     __syncthreads();
     if (missing) {
@@ -318,9 +330,9 @@ __global__ __launch_bounds__(kThreads) void verify_kernel(VerifyArgs a) {
   if (lane == 0) a.token[b] = last;
 }
 
-__global__ __launch_bounds__(256) void clear_slots_kernel(uint64_t* p, int n) {
+__global__ __launch_bounds__(256) void clear_slots_kernel(Slot* p, int n) {
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n) p[i] = 0;
+  if (i < n) *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
 }
 
 // Workgroups of a sequence.
@@ -336,19 +348,19 @@ using namespace tjk;
 extern "C" size_t tjk_verify_tree_bytes(int64_t vocab, int batch) {
   if (vocab <= 0 || vocab > 1 << 24 || batch <= 0 || batch > 1 << 20) return 0;
   const int parts = verify_parts(vocab, batch);
-  return parts > 1 ? (size_t)batch * 2 * parts * sizeof(Slot) : 0;
+  return parts > 1 ? (size_t)batch * kMostNodes * parts * sizeof(Slot) : 0;
 }
 
-extern "C" int tjk_verify_tree(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
-                               const int32_t* tokens, const int32_t* parents, const float* accept_u, const float* sample_u,
-                               const int32_t* cu_nodes, int32_t* path, int64_t ld_path, int32_t* count, int32_t* token,
-                               int* index_errors, int64_t rows, int64_t vocab, int batch, int max_nodes, void* workspace,
-                               size_t workspace_bytes, void* stream) {
+static int verify_tree(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
+                       const int32_t* tokens, const int32_t* parents, const float* accept_u, const float* sample_u,
+                       const int32_t* cu_nodes, int32_t* path, int64_t ld_path, int32_t* count, int32_t* token,
+                       int* index_errors, int64_t rows, int64_t vocab, int batch, int max_nodes, void* workspace,
+                       size_t workspace_bytes, int polls, void* stream) {
   const char* const who = "tjk_verify_tree";
   if (rows < 0 || vocab <= 0 || batch < 0 || max_nodes <= 0)
     return fail(TJK_EINVAL, "%s: bad shape rows=%lld vocab=%lld batch=%d max_nodes=%d", who, (long long)rows,
                 (long long)vocab, batch, max_nodes);
-  if (max_nodes > 64) return fail(TJK_EUNSUPPORTED, "%s: max_nodes=%d exceeds 64", who, max_nodes);
+  if (max_nodes > kMostNodes) return fail(TJK_EUNSUPPORTED, "%s: max_nodes=%d exceeds 64", who, max_nodes);
   if (rows > INT32_MAX || vocab > 1 << 24 || batch > 1 << 20) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
   if (batch == 0) return TJK_OK;
   if (!cu_nodes || !path || !count || !token || !sample_u ||
@@ -363,13 +375,33 @@ extern "C" int tjk_verify_tree(const float* target, int64_t ld_target, const flo
   const int parts = verify_parts(vocab, batch);
   const int64_t part = ((vocab + parts - 1) / parts + 256 * kWaves - 1) / (256 * kWaves) * (256 * kWaves);
   const VerifyArgs a{target, draft, ld_target, ld_draft, tokens, parents, accept_u, sample_u, cu_nodes, path, ld_path, count,
-                     token, index_errors, static_cast<Slot*>(workspace), rows, batch, max_nodes, (int)vocab, parts, (int)part};
+                     token, index_errors, static_cast<Slot*>(workspace), rows, batch, max_nodes, (int)vocab, parts, (int)part, polls};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (parts > 1) {
-    const int words = (int)(need / sizeof(uint64_t));
-    clear_slots_kernel<<<(unsigned)((words + 255) / 256), 256, 0, s>>>(static_cast<uint64_t*>(workspace), words);
+    const int slots = batch * max_nodes * parts;
+    clear_slots_kernel<<<(unsigned)((slots + 255) / 256), 256, 0, s>>>(a.slots, slots);
     if (const int bad = check_launch(who)) return bad;
   }
   verify_kernel<<<(unsigned)(batch * parts), kThreads, 0, s>>>(a);
   return check_launch(who);
+}
+
+extern "C" int tjk_verify_tree(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
+                               const int32_t* tokens, const int32_t* parents, const float* accept_u, const float* sample_u,
+                               const int32_t* cu_nodes, int32_t* path, int64_t ld_path, int32_t* count, int32_t* token,
+                               int* index_errors, int64_t rows, int64_t vocab, int batch, int max_nodes, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return verify_tree(target, ld_target, draft, ld_draft, tokens, parents, accept_u, sample_u, cu_nodes, path, ld_path, count,
+                     token, index_errors, rows, vocab, batch, max_nodes, workspace, workspace_bytes, kPolls, stream);
+}
+
+// The same for tests, with the looks at a missing sum given: with none every workgroup
+// computes every sum itself.
+extern "C" int tjk_verify_tree_polls(const float* target, int64_t ld_target, const float* draft, int64_t ld_draft,
+                                     const int32_t* tokens, const int32_t* parents, const float* accept_u,
+                                     const float* sample_u, const int32_t* cu_nodes, int32_t* path, int64_t ld_path,
+                                     int32_t* count, int32_t* token, int* index_errors, int64_t rows, int64_t vocab, int batch,
+                                     int max_nodes, void* workspace, size_t workspace_bytes, int polls, void* stream) {
+  return verify_tree(target, ld_target, draft, ld_draft, tokens, parents, accept_u, sample_u, cu_nodes, path, ld_path, count,
+                     token, index_errors, rows, vocab, batch, max_nodes, workspace, workspace_bytes, polls, stream);
 }

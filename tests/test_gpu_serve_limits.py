@@ -1,5 +1,6 @@
 """The serving operators where their numbers end: weights that are none, weights far
-below a row's largest, scores and values that are not finite, sums that do not come."""
+below a row's largest, scores and values that are not finite, sums that do not
+come, rows in unusual places."""
 
 import ctypes
 
@@ -7,6 +8,7 @@ import pytest
 import torch
 
 from tjkernels import _lib, ops
+from tjkernels._lib import TjkError
 
 from test_gpu_serve import U, Drafts, Trees, _half, _verify_oracle, _within
 
@@ -142,3 +144,39 @@ def test_rows_of_infinitely_low_scores_are_zero(device, dt, contexts, counts, he
     t.v[:, :, ::3] = bad
     got = t.run(device)
     assert (got == 0).all()
+
+
+def test_cache_of_steps_that_do_not_nest(device):
+    """Heads between the rows of pages that lie closer than a page's heads reach: no
+    two share a place, so the cache is as good as another."""
+    t = Trees([11, 6], [3, 2], 6, 3, 16, 16, torch.bfloat16, 43)
+    t.table = torch.tensor([[1], [0]], dtype=torch.int32)
+    t.k, t.v, t.pages = t.k[:2].contiguous(), t.v[:2].contiguous(), 2
+    want = t.run(device)
+    odd = [torch.full((16 * 128,), 7.0, dtype=t.dt, device=device).as_strided((2, 3, 16, 16), (48, 32, 128, 1)) for _ in range(2)]
+    # each position of the two sequences, appended
+    x = torch.cat([torch.arange(14), torch.arange(8)])
+    page = torch.tensor([1] * 14 + [0] * 8)
+    rows = torch.cat([t.k[page, :, x], t.k[page, :, x], t.k[page, :, x], t.v[page, :, x]], dim=1).to(device)
+    ops.rope_append(rows, x.int().to(device), None, torch.empty_like(rows[:, :6]), *odd, (page * 16 + x).int().to(device))
+    assert torch.equal(t.run(device, k_cache=odd[0], v_cache=odd[1]), want)
+
+
+def test_queries_and_output_in_one_buffer(device):
+    """Side by side in its rows: the same bits; over each other: refused."""
+    t = Trees([90, 33], [5, 12], 4, 2, 64, 16, torch.float16, 44)
+    want = t.run(device)
+    both = torch.full((t.t, 2, 256), 7.0, dtype=t.dt, device=device)
+    both[:, 1] = t.q.view(t.t, 256).to(device)
+    q = both[:, 1].unflatten(1, (4, 64))
+    assert torch.equal(t.run(device, q=q, out=both[:, 0]), want)
+    assert torch.equal(both[:, 1].cpu(), t.q.view(t.t, 256))
+    with pytest.raises(TjkError, match="overlap"):
+        t.run(device, q=q, out=both.view(-1)[248:].as_strided((t.t, 256), (512, 1)))
+    k = t.k.to(device)
+    args = [torch.zeros(3, dtype=torch.int32, device=device)] * 2
+    qkv = torch.zeros(3, 8, 64, dtype=t.dt, device=device)
+    with pytest.raises(TjkError, match="keys and values overlap"):
+        ops.rope_append(qkv, args[0], None, torch.empty_like(qkv[:, :4]), k, k, args[1])
+    with pytest.raises(TjkError, match="q_out and k_out overlap"):
+        ops.rope_append(qkv, args[0], None, k.view(-1, 4, 64)[:3], k_out=k.view(-1, 2, 64)[1:4])

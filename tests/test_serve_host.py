@@ -336,3 +336,112 @@ def test_attention_shapes_are_refused_before_the_workspace(kw):
         _py_attend(**kw)
     with pytest.raises(TjkError):
         _py_attend(workspace=torch.zeros(64, dtype=torch.uint8), **kw)
+
+
+# ------------------------------------------------------------ rows that overlap
+
+def _starts(base, *steps):
+    at = [base]
+    for stride, n in steps:
+        at = [x + i * stride for x in at for i in range(n)]
+    return at
+
+
+def _overlap(rows, size):
+    rows = sorted(rows)
+    return any(b - a < size for a, b in zip(rows, rows[1:]))
+
+
+# with every other check passed, the last thing looked at: too many tokens
+MANY = dict(qkv=1 << 40, tokens=1 << 30, heads=1, kv_heads=16, head_dim=128, rot=0, ld_token=33 * 128, ld_head=128,
+            q_out=1 << 50, ld_q_token=128, ld_q_head=128, cache=None, slots=None)
+
+
+def test_written_caches_of_any_strides():
+    """A cache is refused if two of its rows share an element, and only then."""
+    g = torch.Generator()
+    g.manual_seed(0)
+    r = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+    found = [0, 0]
+    for _ in range(3000):
+        hd, heads, pages = 16 * (1 + r(3)), 1 + r(4), 1 + r(5)
+        short, wide = hd + 8 * r(4), hd + 8 * r(60)
+        strides = [short, wide, (heads + r(2)) * short if r(2) else wide * 16 + 8 * r(3)]
+        order = torch.randperm(3, generator=g).tolist()
+        page, head, row = [strides[i] for i in order]
+        bad = _overlap(_starts(0, (page, pages), (head, heads), (row, 16)), hd)
+        kw = dict(cache=1, cache_k=1 << 53, cache_v=1 << 54, cache_page_stride=page, cache_head_stride=head, cache_row_stride=row,
+                  cache_pages=pages, cache_page_size=16, cache_kv_heads=heads, cache_head_dim=hd)
+        many = dict(MANY, slots=FAKE, head_dim=hd, kv_heads=heads, heads=1000, ld_head=hd, ld_token=(1000 + 2 * heads) * hd,
+                    ld_q_token=1000 * hd, ld_q_head=hd, tokens=1 << 28, **kw)
+        status = _append(**many)
+        said = _said()
+        assert (status == EINVAL and "rows of the cache overlap" in said) if bad else \
+            (status == EUNSUPPORTED and "too many" in said), (page, head, row, pages, heads, hd, said)
+        layer = 8 * (hd // 8 + r(pages * 16 * heads * 16))
+        bad = _overlap(_starts(0, (layer, 3), (page, pages), (head, heads), (row, 16)), hd)
+        status = _compact(layers=3, layer_stride=layer, batch=1 << 25, **kw)
+        said = _said()
+        assert (status == EINVAL and "rows of the cache overlap" in said) if bad else \
+            (status == EUNSUPPORTED and "too large" in said), (layer, page, head, row, pages, heads, hd, said)
+        found[bad] += 1
+    assert min(found) > 100
+
+
+def test_pages_whose_keys_are_values():
+    cache = dict(cache=1, slots=FAKE, heads=1000, kv_heads=4, ld_token=1008 * 64, ld_head=64, head_dim=64, ld_q_token=64000,
+                 ld_q_head=64, tokens=1 << 28, cache_k=1 << 53)
+    many = {k: v for k, v in MANY.items() if k not in cache}
+    rows = 2 * 64  # bytes
+    for apart, bad in ((0, True), (rows - 16, True), (rows, True), (31 * rows, True), (128 * rows, False), (-rows, True),
+                       (-128 * rows, False), (127 * rows + 16, True), (10 * 128 * rows, False)):
+        status = _append(**many, **cache, cache_v=(1 << 53) + apart)
+        assert (status == EINVAL and "keys and values overlap" in _said()) if bad else \
+            (status == EUNSUPPORTED and "too many" in _said()), (apart, _said())
+
+
+def test_outputs_beside_their_inputs():
+    """q_out and k_out may lie in one buffer with qkv, between its rows, but in no
+    place of theirs or of each other's other than their own."""
+    g = torch.Generator()
+    g.manual_seed(1)
+    r = lambda n: int(torch.randint(0, n, (1,), generator=g))  # noqa: E731
+    many = dict(MANY, head_dim=16, heads=700, kv_heads=50, tokens=1 << 28)
+    found = [0, 0]
+    for _ in range(1500):
+        token = 16 * (800 + r(2) * 800)
+        kw = dict(ld_token=token, ld_head=16, ld_q_token=token, ld_q_head=16, k_out=None, ld_k_token=token, ld_k_head=16)
+        at = 8 * r(2 * token // 8)
+        kw["q_out"] = MANY["qkv"] + 2 * (0 if r(8) == 0 else at)
+        if r(2):
+            kw["k_out"] = MANY["qkv"] + 2 * (700 * 16 if r(3) == 0 else 8 * r(2 * token // 8))
+        # whether rows meet depends on the difference of their tokens: seven say all
+        pieces = lambda p, n: {x // 8 + i for x in _starts((p - MANY["qkv"]) // 2, (token, 7), (16, n)) for i in (0, 1)}  # noqa: E731
+        qkv, q = pieces(MANY["qkv"], 800), pieces(kw["q_out"], 700)
+        k = pieces(kw["k_out"], 50) if kw["k_out"] else set()
+        bad = (kw["q_out"] != MANY["qkv"] and q & qkv) or (kw["k_out"] != MANY["qkv"] + 2 * 700 * 16 and k & qkv) or q & k
+        if kw["k_out"] == MANY["qkv"]:
+            bad = True
+        status = _append(**dict(many, **kw))
+        assert (status == EINVAL) if bad else (status == EUNSUPPORTED and "too many" in _said()), (kw, _said())
+        found[bool(bad)] += 1
+    assert min(found) > 30
+
+
+def test_outputs_whose_own_rows_overlap():
+    for kw, bad in ((dict(heads=4, ld_q_token=256, ld_q_head=128), True), (dict(heads=4, ld_q_token=512, ld_q_head=128), False),
+                    (dict(heads=4, ld_q_token=128, ld_q_head=128 << 30), False), (dict(heads=4, ld_q_token=128, ld_q_head=256), True),
+                    (dict(heads=1, ld_q_token=128, k_out=1 << 51, ld_k_head=128, ld_k_token=1920), True),
+                    (dict(heads=1, ld_q_token=128, k_out=1 << 51, ld_k_head=128, ld_k_token=2048), False)):
+        status = _append(**dict(MANY, ld_token=36 * 128, **kw))
+        assert (status == EINVAL and "rows of an output overlap" in _said()) if bad else \
+            (status == EUNSUPPORTED and "too many" in _said()), (kw, _said())
+
+
+def test_attention_output_over_its_queries():
+    """Anywhere in their rows, not only at their beginning."""
+    for out in (FAKE - 2 * 512 + 16, FAKE + 16, FAKE + 2 * 512, FAKE + 2 * (4 * 512 + 448), FAKE - 2 * (4 * 512 + 8)):
+        assert _attend(out=out) == EINVAL and "overlap" in _said()
+    wide = dict(ld_q_token=1024, ld_out=1024)
+    assert _attend(out=FAKE + 2 * 504, **wide) == EINVAL and "overlap" in _said()
+    assert _attend(out=FAKE - 2 * 520, **wide, ld_q_head=72) == EINVAL and "overlap" in _said()

@@ -8,6 +8,7 @@
 #pragma once
 
 #include "f8_common.h"
+#include "strided_rows.h"
 
 namespace tjk {
 
@@ -27,9 +28,10 @@ inline Paged paged(const tjk_paged_cache& c) {
           (uint32_t)(2 * c.row_stride), (int)c.pages, shift};
 }
 
-// Status of a cache that an entry point `who` is given; one that it writes may not
-// hold two rows in one place.
+// Status of a cache that an entry point `who` is given.
 int check_cache(const char* who, const tjk_paged_cache* c, bool writes);
+// Status of one that it writes, `layers` of them, besides: no two rows in one place.
+int check_written(const char* who, const tjk_paged_cache* c, int layers, int64_t layer_stride);
 
 // A page that a block table names, -1 if the cache holds no such page.
 __device__ __forceinline__ int page_of(const int32_t* table_row, int at, int pages) {

@@ -29,6 +29,16 @@ int check_cache(const char* who, const tjk_paged_cache* c, bool writes) {
   return TJK_OK;
 }
 
+int check_written(const char* who, const tjk_paged_cache* c, int layers, int64_t layer_stride) {
+  const StridedRows rows = StridedRows(c->k, 2 * c->head_dim)
+                               .by(2 * c->page_stride, c->pages)
+                               .by(2 * c->head_stride, c->kv_heads)
+                               .by(2 * c->row_stride, c->page_size)
+                               .by(2 * layer_stride, layers);
+  if (rows_overlap(rows)) return fail(TJK_EINVAL, "%s: rows of the cache overlap", who);
+  return TJK_OK;
+}
+
 // ------------------------------------------------------------- append
 //
 // One head of one token belongs to G neighbouring lanes (G the power of two from
@@ -303,6 +313,22 @@ extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_hea
   if ((q_out == qkv && elsewhere(ld_q_token, ld_q_head, heads)) ||
       (k_out && ((k_out == keys && elsewhere(ld_k_token, ld_k_head, kv_heads)) || k_out == qkv)))
     return fail(TJK_EINVAL, "%s: outputs may alias qkv only in place", who);
+  auto rows = [&](const void* base, int64_t token, int64_t head, int n) {
+    return StridedRows(base, 2 * head_dim).by(2 * token, tokens).by(2 * head, n);
+  };
+  const StridedRows in = rows(qkv, ld_token, ld_head, heads + 2 * kv_heads), q_rows = rows(q_out, ld_q_token, ld_q_head, heads),
+                    k_rows = rows(k_out, ld_k_token, ld_k_head, kv_heads);
+  if (rows_overlap(q_rows) || (k_out && rows_overlap(k_rows))) return fail(TJK_EINVAL, "%s: rows of an output overlap", who);
+  if ((q_out != qkv && rows_meet(q_rows, in)) || (k_out && k_out != keys && rows_meet(k_rows, in)))
+    return fail(TJK_EINVAL, "%s: outputs may overlap qkv only in place", who);
+  if (k_out && rows_meet(q_rows, k_rows)) return fail(TJK_EINVAL, "%s: q_out and k_out overlap", who);
+  if (cache) {
+    if (const int bad = check_written(who, cache, 1, 0)) return bad;
+    auto page = [&](const void* base) {
+      return StridedRows(base, 2 * head_dim).by(2 * cache->head_stride, kv_heads).by(2 * cache->row_stride, cache->page_size);
+    };
+    if (rows_meet(page(cache->k), page(cache->v))) return fail(TJK_EINVAL, "%s: a page's keys and values overlap", who);
+  }
   AppendArgs a{static_cast<const char*>(qkv), 2 * ld_token, 2 * ld_head, positions, table, (int)n_positions, (int)rot / 8,
                static_cast<char*>(q_out), 2 * ld_q_token, 2 * ld_q_head, static_cast<char*>(k_out), 2 * ld_k_token,
                2 * ld_k_head, cache ? paged(*cache) : Paged{}, slots, q_gamma, k_gamma, eps, index_errors, tokens, heads,
@@ -344,6 +370,7 @@ extern "C" int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64
   if (layers == 0 || batch == 0 || max_nodes < 2 || table_cols == 0) return TJK_OK;
   if (!block_table || !ctx_lens || !path || !count) return fail(TJK_EINVAL, "%s: null pointer", who);
   if (ld_table < table_cols || ld_path < max_nodes) return fail(TJK_EINVAL, "%s: leading dimension too small", who);
+  if (const int bad = check_written(who, cache, layers, layer_stride)) return bad;
   const int64_t waves = (int64_t)layers * batch * cache->kv_heads;
   if (waves > INT32_MAX / 64) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
   const CompactArgs a{paged(*cache), 2 * layer_stride, block_table, ld_table, (int)table_cols, ctx_lens, path, ld_path,

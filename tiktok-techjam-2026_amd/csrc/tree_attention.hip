@@ -984,7 +984,10 @@ static int launch_tree(TreeArgs a, hipStream_t s) {
   const int64_t items = (int64_t)a.batch * a.kv_heads * a.most_mbs, tiles = (a.room + kTile - 1) / kTile;
   if (items * (std::max<int64_t>(tiles, 1) + V::Sh::COST) > INT32_MAX - kMinUnits || items > INT32_MAX / 256)
     return fail(TJK_EUNSUPPORTED, "tjk_tree_attention: the batch's sequences, heads and table are too large");
-  if (a.out == a.q) return fail(TJK_EINVAL, "tjk_tree_attention: out may not be q, which other workgroups still read");
+  const int64_t hd2 = 16 * a.hd8, heads = (int64_t)a.kv_heads * a.group;
+  if (rows_meet(StridedRows(a.q, hd2).by(a.q_token_bytes, a.tokens).by(a.q_head_bytes, heads),
+                StridedRows(a.out, heads * hd2).by(a.out_bytes, a.tokens)))
+    return fail(TJK_EINVAL, "tjk_tree_attention: out may not be q, which other workgroups still read, or overlap it");
   a.direct = whole_items(items, tiles);
   if constexpr (V::RW == 1) {
     if (a.direct && one_wave(items, tiles, V::GRID)) {

@@ -526,7 +526,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          const float base = m_off[i] == -INFINITY ? 0.f : kLift<T> - m_off[i];
+          const float base = m_off[i] == -INFINITY ? 0.f : kLift<T> == 0.f ? -m_off[i] : kLift<T> - m_off[i];
           float e[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[u][i][j >> 2][j & 3], scale, base));
@@ -781,9 +781,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
     };
     // four elements of a row, of the weighted and of the weights' sum; zeros if there is
     // no weight (weights of zero may have met values that are not finite)
-    auto result = [&](const f32x4& y, float sum) {
-      const float inv = 1.0f / sum;
-      return Quad<T>::from(sum == 0.f ? make_float4(0, 0, 0, 0) : make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
+    auto result = [&](const f32x4& y, bool none, float inv) {
+      return Quad<T>::from(none ? make_float4(0, 0, 0, 0) : make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv));
     };
     const bool whole = t0 == 0 && t1 == q.tiles;
     const int part = 2 * w + (t0 == 0 ? 1 : 0);  // a stretch ends in the first part of an item at most once
@@ -795,9 +794,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
         if (m >= rows) continue;
         if (whole) {
           T* const dst = out_row(m);
+          const bool none = sum == 0.f;
+          const float inv = 1.0f / sum;
 #pragma unroll
           for (int h = 0; h < HT; ++h)
-            if (2 * h < z.hd8) *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) = result(o[i][h], sum);
+            if (2 * h < z.hd8) *reinterpret_cast<typename Quad<T>::raw*>(dst + 16 * h + 4 * g) = result(o[i][h], none, inv);
         } else {
 #pragma unroll
           for (int h = 0; h < HT; ++h)
@@ -876,7 +877,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
           if (share != 0 || r >= live) continue;
           if (whole) {
             if (c0 < 8 * z.hd8)
-              *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) = result(y, sum);
+              *reinterpret_cast<typename Quad<T>::raw*>(out_row(mb * Sh::ROWS + r) + c0) = result(y, sum == 0.f, 1.0f / sum);
           } else {
             const int p = part_of(first);
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), parts, 4 * (p * Sh::PART + r * HD + c0), 0, kThrough);

@@ -445,3 +445,15 @@ def test_attention_output_over_its_queries():
     wide = dict(ld_q_token=1024, ld_out=1024)
     assert _attend(out=FAKE + 2 * 504, **wide) == EINVAL and "overlap" in _said()
     assert _attend(out=FAKE - 2 * 520, **wide, ld_q_head=72) == EINVAL and "overlap" in _said()
+
+
+@pytest.mark.parametrize("call", [_append, _attend, _compact])
+def test_pages_whose_rows_pass_64_bits(call):
+    for pages in (1 << 59, (1 << 59) + 1, 1 << 62):
+        assert call(cache_pages=pages, cache_page_size=32) == EUNSUPPORTED and "int32" in _said()
+
+
+def test_compactions_whose_waves_pass_64_bits():
+    kw = dict(cache_kv_heads=16, cache_page_stride=16 * 32 * 64)
+    for layers, batch in ((1 << 30, 1 << 30), (2 ** 31 - 1, 2 ** 31 - 1), (1 << 30, 1 << 29)):
+        assert _compact(layers=layers, batch=batch, **kw) == EUNSUPPORTED and "too large" in _said()

@@ -16,7 +16,7 @@ int check_cache(const char* who, const tjk_paged_cache* c, bool writes) {
     return fail(TJK_EUNSUPPORTED, "%s: head_dim=%d must be a multiple of 16 and <= 128", who, c->head_dim);
   if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)))
     return fail(TJK_EUNSUPPORTED, "%s: page_size=%d must be a power of two from 16 to 65536", who, c->page_size);
-  if (c->pages * c->page_size > INT32_MAX) return fail(TJK_EUNSUPPORTED, "%s: the cache's rows exceed int32", who);
+  if (c->pages > INT32_MAX / c->page_size) return fail(TJK_EUNSUPPORTED, "%s: the cache's rows exceed int32", who);
   if (c->page_stride < 0 || c->head_stride < 0 || c->row_stride < c->head_dim)
     return fail(TJK_EINVAL, "%s: bad cache strides", who);
   if (writes && ((c->pages > 1 && c->page_stride < c->head_dim) || (c->kv_heads > 1 && c->head_stride < c->head_dim)))
@@ -371,8 +371,8 @@ extern "C" int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64
   if (!block_table || !ctx_lens || !path || !count) return fail(TJK_EINVAL, "%s: null pointer", who);
   if (ld_table < table_cols || ld_path < max_nodes) return fail(TJK_EINVAL, "%s: leading dimension too small", who);
   if (const int bad = check_written(who, cache, layers, layer_stride)) return bad;
-  const int64_t waves = (int64_t)layers * batch * cache->kv_heads;
-  if (waves > INT32_MAX / 64) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
+  const int64_t pairs = (int64_t)layers * batch, waves = pairs * cache->kv_heads;
+  if (pairs > INT32_MAX || waves > INT32_MAX / 64) return fail(TJK_EUNSUPPORTED, "%s: too large", who);
   const CompactArgs a{paged(*cache), 2 * layer_stride, block_table, ld_table, (int)table_cols, ctx_lens, path, ld_path,
                       max_nodes, count, index_errors, layers, batch, cache->kv_heads, cache->head_dim / 8};
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -457,3 +457,9 @@ def test_compactions_whose_waves_pass_64_bits():
     kw = dict(cache_kv_heads=16, cache_page_stride=16 * 32 * 64)
     for layers, batch in ((1 << 30, 1 << 30), (2 ** 31 - 1, 2 ** 31 - 1), (1 << 30, 1 << 29)):
         assert _compact(layers=layers, batch=batch, **kw) == EUNSUPPORTED and "too large" in _said()
+
+
+@pytest.mark.parametrize("q", [_b(5, 8, 0), torch.zeros((), dtype=torch.bfloat16)])
+def test_queries_without_elements_are_refused(q):
+    with pytest.raises(TjkError):
+        _py_attend(q=q, workspace=torch.zeros(64, dtype=torch.uint8))

@@ -555,13 +555,15 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     multiple of the cache's kv_heads.
 
     A row that sees nothing is zero; what a row does not see does not reach it,
-    whatever it holds.  ``out`` may not overlap ``q``.  Positions without a page are left out and counted in
-    ``index_errors``.  ``workspace`` (``tree_attention_workspace``) is allocated
+    whatever it holds.  ``out`` may not overlap ``q``.  Positions without a page
+    are left out and counted in ``index_errors``.  ``workspace`` (``tree_attention_workspace``) is allocated
     when it is not given."""
     if workspace is None:
         workspace = tree_attention_workspace(q, k_cache, max_nodes)
-    _serve().tree_attention(q, k_cache, v_cache, block_table, ctx_lens, out, cu_nodes, max_nodes, tree_mask,
-                            q.shape[-1] ** -0.5 if scale is None else scale, workspace, index_errors)
+    if scale is None:  # (no elements: refused by the call)
+        scale = q.shape[-1] ** -0.5 if q.dim() > 0 and q.shape[-1] > 0 else 1.0
+    _serve().tree_attention(q, k_cache, v_cache, block_table, ctx_lens, out, cu_nodes, max_nodes, tree_mask, scale, workspace,
+                            index_errors)
     return out
 
 

@@ -463,3 +463,17 @@ def test_compactions_whose_waves_pass_64_bits():
 def test_queries_without_elements_are_refused(q):
     with pytest.raises(TjkError):
         _py_attend(q=q, workspace=torch.zeros(64, dtype=torch.uint8))
+
+
+def test_append_in_place_of_tokens_that_overlap():
+    """A token's values that are the next one's queries may be read, but not while
+    those are written."""
+    one = dict(MANY, heads=2, ld_token=34 * 128 - 256, ld_q_token=256)
+    assert _append(**one) == EUNSUPPORTED and "too many" in _said()
+    place = dict(q_out=MANY["qkv"], ld_q_token=one["ld_token"])
+    assert _append(**dict(one, **place)) == EINVAL and "overlap" in _said()
+    keys = dict(k_out=MANY["qkv"] + 2 * 2 * 128, ld_k_token=one["ld_token"], ld_k_head=128, ld_q_token=256)
+    assert _append(**dict(one, **keys)) == EINVAL and "overlap" in _said()
+    for apart in (dict(one, **place), dict(one, **keys)):
+        apart.update(ld_token=34 * 128, **{k: 34 * 128 for k in ("ld_q_token", "ld_k_token")})
+        assert _append(**apart) == EUNSUPPORTED and "too many" in _said()

@@ -319,7 +319,8 @@ extern "C" int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_hea
   const StridedRows in = rows(qkv, ld_token, ld_head, heads + 2 * kv_heads), q_rows = rows(q_out, ld_q_token, ld_q_head, heads),
                     k_rows = rows(k_out, ld_k_token, ld_k_head, kv_heads);
   if (rows_overlap(q_rows) || (k_out && rows_overlap(k_rows))) return fail(TJK_EINVAL, "%s: rows of an output overlap", who);
-  if ((q_out != qkv && rows_meet(q_rows, in)) || (k_out && k_out != keys && rows_meet(k_rows, in)))
+  const bool in_place = q_out == qkv || (k_out && k_out == keys);
+  if ((q_out != qkv && rows_meet(q_rows, in)) || (k_out && k_out != keys && rows_meet(k_rows, in)) || (in_place && rows_overlap(in)))
     return fail(TJK_EINVAL, "%s: outputs may overlap qkv only in place", who);
   if (k_out && rows_meet(q_rows, k_rows)) return fail(TJK_EINVAL, "%s: q_out and k_out overlap", who);
   if (cache) {

@@ -180,3 +180,40 @@ def test_queries_and_output_in_one_buffer(device):
         ops.rope_append(qkv, args[0], None, torch.empty_like(qkv[:, :4]), k, k, args[1])
     with pytest.raises(TjkError, match="q_out and k_out overlap"):
         ops.rope_append(qkv, args[0], None, k.view(-1, 4, 64)[:3], k_out=k.view(-1, 2, 64)[1:4])
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("context", [2 ** 31 - 1, 2 ** 31 - 130])
+def test_contexts_at_the_end_of_32_bits(device, dt, context):
+    """A table of 2^31 positions, all of them rows of one page, and a context that
+    reaches the last whole tile that 32 bits number, or past it: no row without a key is
+    counted, which all of the keys, far below its score of zero, would vanish beside."""
+    k = torch.zeros(1, 1, 65536, 16, dtype=dt, device=device)
+    k[..., 0] = -100
+    v = torch.ones_like(k)
+    q = torch.zeros(1, 1, 16, dtype=dt, device=device)
+    q[..., 0] = 1
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=device)  # noqa: E731
+    errors = i32(0)
+    out = torch.full((1, 16), 7.0, dtype=dt, device=device)
+    ops.tree_attention(q, k, v, torch.zeros(1, 32768, dtype=torch.int32, device=device), i32(context), out, cu_nodes=i32(0, 1),
+                       max_nodes=1, scale=1.0, index_errors=errors)
+    assert (out == 1).all()
+    assert int(errors) == (context + 1 > 2 ** 31 - 129)  # what is past it is cut off
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_append_keeps_the_bits_of_what_it_copies(device, dt):
+    """Every number of the type, subnormals and infinities among them, as a value, and
+    as a query and a key without norm and rotation; NaN stays NaN."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dt).view(512, 1, 128)
+    qkv = bits.repeat(1, 3, 1).to(device)
+    k, v = [torch.zeros(32, 1, 16, 128, dtype=dt, device=device) for _ in range(2)]
+    at = torch.arange(512, dtype=torch.int32, device=device)
+    q, k_out = torch.zeros_like(qkv[:, :1]), torch.zeros_like(qkv[:, :1])
+    ops.rope_append(qkv, at, None, q, k, v, at, k_out=k_out)
+    nan = torch.isnan(bits).flatten()
+    want = bits.view(torch.int16).flatten()[~nan]
+    for got in (q, k_out, k, v):
+        got = got.cpu().flatten()
+        assert torch.isnan(got[nan]).all() and torch.equal(got.view(torch.int16)[~nan], want)

@@ -462,8 +462,9 @@ typedef struct {
  * outside [0, n_positions) makes the token's q_out and k_out rows zero and stores
  * nothing, a slot past the cache stores nothing; both count in *index_errors.
  * Two tokens of a call may not share a slot (its row would hold pieces of
- * either).  q_out may be the queries of qkv and k_out its keys, in place; they may
- * not overlap qkv otherwise.
+ * either).  q_out may be the queries of qkv and k_out its keys, in place (rows of
+ * qkv's own that overlap are refused then); they may not overlap qkv otherwise, nor each
+ * other, nor may the rows of a cache that is written, or a page's keys and values.
  * Requires rot % 16 == 0, strides that are multiples of 8, and 16-byte aligned
  * pointers.
  */
@@ -482,8 +483,10 @@ int tjk_rope_append(const void* qkv, int64_t ld_token, int64_t ld_head, const in
  * (its own among them, if it is to see itself; NULL: nodes 0 .. i, a chain).
  *   out[row, h * head_dim ..] = sum_j softmax(scale q . k_j) v_j
  * Scores, the softmax and the sums over keys are in fp32, the weights given to
- * the product with the values rounded to the cache's type.  A row that sees
- * nothing, or only scores of -inf, is zero.  Keys and values that a row does not
+ * the product with the values rounded to the cache's type (in fp16 the least are
+ * multiples of 2^-31 of a row's largest, or less).  Weights reach 2^8, in fp16 2^15, before
+ * the division by their sum: the weighted values' sums have to stay in fp32's range.  A
+ * row that sees nothing, or only scores of -inf, is zero.  Keys and values that a row does not
  * see do not reach it, whatever they hold; positions without a page are left
  * out, and count in *index_errors.  Of a tree of more than max_nodes nodes, or that
  * runs past `tokens`, the first rows count; rows that no sequence names stay.  out
@@ -540,6 +543,7 @@ size_t tjk_verify_tree_bytes(int64_t vocab, int batch);
  * starts at 0 and increases; an entry below i or past max_nodes, or a position
  * without a page, moves nothing and counts in *index_errors (a table of no columns:
  * nothing moves or counts).  The pages that nodes lie in belong to one sequence.
+ * Rows that overlap, of a cache or of two layers, are refused.
  */
 int tjk_compact_cache(const tjk_paged_cache* cache, int layers, int64_t layer_stride,
                       const int32_t* block_table, int64_t ld_table, int64_t table_cols,

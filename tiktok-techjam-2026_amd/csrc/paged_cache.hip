@@ -49,7 +49,7 @@ int check_written(const char* who, const tjk_paged_cache* c, int layers, int64_t
 //
 // Bound by memory: 65536 tokens of 16 + 2 x 16 heads of 64 with norms, bf16, 157 us,
 // 5.2 TB/s (a copy of 1 GB: 5.1); 4096 tokens of 32 + 2 x 8 heads of 128 22.3 us, 4.6; 1003
-// of them 7.0 us.  8 tokens: 3.5 us, a launch and two passages of memory (position and
+// of them 6.2 to 7.0 us.  8 tokens: 3.3 to 4 us, a launch and two passages of memory (position and
 // row, then the angles).
 
 struct AppendArgs {
@@ -185,9 +185,10 @@ __global__ __launch_bounds__(256) void rope_append_kernel(AppendArgs a) {
 //
 // Bound by latency (counts and path, places, rows: three passages of memory one
 // after the other), then by memory, which does not like 256 bytes here and 256
-// there: 24 layers x 64 sequences x 8 heads of 128, 7 rows each, 27 us, 3.5 TB/s read
-// and written; four layers of 8 sequences 5 us.  Keys and values in waves of their
-// own 29 and 6 us, two instructions of rows in flight instead of four 28.5 and 4.4.
+// there: 24 layers x 64 sequences x 8 heads of 128, 7 rows each, 25.5 us, 3.7 TB/s read
+// and written (21.5 on the same rows again); four layers of 8 sequences 3.6 us.  Where
+// this took 27 and 5, keys and values in waves of their own took 29 and 6 us, two
+// instructions of rows in flight instead of four 28.5 and 4.4.
 // Loads where nothing moves, from one place for all, to spare the lanes' conditions:
 // 40 and 13.
 

@@ -192,20 +192,20 @@ struct Split {
 // they do not meet at all (many items of few tiles).  RW = 4 (more rows): the waves have 16 NB rows each
 // and share the tiles, in a ring of NST stages of SUB, one barrier a stage.
 //
-// Weights go to the product with V in the cache's type, as in flash_pipe_kernel: half
-// a step of 2^-8 (bf16) each, 2.2e-3 of the result (2-norm) where its own rounding
-// is 1.7e-3; a product in two parts would double it.  Everything summed is fp32, the
+// Weights go to the product with V in the cache's type, as in flash_pipe_kernel: off by
+// 2^-8 (bf16) at most each, 2.2e-3 of the result (2-norm) where its own rounding
+// is 1.7e-3 (fp16 2.5e-4 and 2.1e-4); a product in two parts would double it.  Everything summed is fp32, the
 // sum of the weights that of the rounded ones.
 //
 // Few rows are bound by memory: 64 single tokens over 512 to 4096, 16 heads of 128
-// bf16, 215 us, 5.6 TB/s (a copy of 1 GB reaches 5.1); 2 x 99995 tokens, 4 key heads of
-// 64, 56 us, of which the stretches take 34 to 46, the joining 12.  8 single tokens
-// over up to 512: 9.4 us, launch and passages of memory one after the other (places 2,
+// bf16, 213 us, 5.6 TB/s (a copy of 1 GB reaches 5.1); 2 x 99995 tokens, 4 key heads of
+// 64, 57 us (48 on the same ones again), of which the joining takes 12.  8 single tokens
+// over up to 512: 8.8 us, launch and passages of memory one after the other (places 2,
 // first tiles 1.5, the rest of them 3, joining of the waves 1).  Many rows are bound
 // by the matrix and the vector unit and by power: 32 trees of 64 nodes over 1000 to 8192,
-// 8 heads of 128 to a key head, 200 to 216 us, 720 to 780 TFLOP/s (64 over
-// 4000: 313 us, 870); matrix
-// unit 31% of the time, vector unit 36%, LDS 21%.  (Before row blocks lay side by side,
+// 8 heads of 128 to a key head, 200 to 210 us, 740 to 780 TFLOP/s, and 212 to 262 in the
+// first milliseconds after a pause, until the clock has settled (64 over 4000: 313 us,
+// 870); matrix unit 32% of the time, vector unit 41%, LDS 18%.  (Before row blocks lay side by side,
 // 336 us for the latter: 280 if every page lay in L2, and 280 if keys and values were
 // zeros, at the same traffic.)  Per wave 48 rows take 5 to 10% longer than 32, 64
 // (one wave a SIMD; two do not fit) 15%, three waves a SIMD do not fit; the next tile's
@@ -933,11 +933,11 @@ struct Variant {
   static_assert(GRID <= kJoin * kJoin * kJoin && 3 * 2 * GRID * 4 <= TJK_TREE_COUNTERS && BYTES < 0x7fffffff, "counters and 32-bit offsets");
 };
 
-// Calls f with the variant for a head_dim and the rows of the largest tree: as few
-// 16-row blocks as hold them, so that a wave holds the sums of no rows that are not
-// there; from 64 rows on four waves with rows of their own (64 rows of 128 in four
-// waves that share the tiles: 105 to 108 us either way at 16 x 2000 to 4000 tokens, 16
-// key heads; of 64: 60 and 62).
+// Calls f with the variant for a head_dim and the rows of the largest tree: up to 64
+// rows, one, two or four blocks of 16 that each of the four waves holds whole (33 to 48
+// rows hold a block of none), above that waves with rows of their own that share the
+// tiles (64 rows of 128 so: 105 to 108 us either way at 16 x 2000 to 4000 tokens, 16 key
+// heads; of 64: 60 and 62).
 template <typename F>
 static auto with_variant(int head_dim, int rows, F&& f) {
   if (head_dim <= 64) {

@@ -50,11 +50,11 @@ struct VerifyArgs {
 // refusal takes one, and the end one: max_nodes at most), so that a workgroup that comes
 // late finds all that the others left.
 //
-// 64 trees of up to 32 nodes over 128257 tokens: 32 to 36 us (one workgroup a sequence
+// 64 trees of up to 32 nodes over 128257 tokens: 36 to 38 us (one workgroup a sequence
 // 77), of which the clearing of the sums' places 3 to 5; the distributions of the last
 // nodes alone are 13 at a copy's rate, but a tree with five refusals makes five
-// passes, one after the other, of about 5 us: 128 KB by one CU, the waves' sums, and two
-// passages of memory to the other parts and back.  A part's p and q held in registers
+// passes, one after the other, of about 5 us: 128 KB of p and as much of q by one CU,
+// the waves' sums, and two passages of memory to the other parts and back.  A part's p and q held in registers
 // for a second refusal at a node took 4 us off that, and added 0.6 to the 11 of four
 // chains of six over 32000.
 
@@ -65,9 +65,9 @@ constexpr int kMostParts = 64;
 // 1024 (parts of 4096), which are not all there (298 while late ones did not find the
 // sums that they had missed).
 constexpr int kMostGroups = 256;
-// Least elements of a part, us with 4096 / 8192 / 16384: chain over 32000 10.9 / 10.8 / 9.3 (no
-// meeting), 16 trees over 50000 20.4 / 21.1 / 22.2, 4 over 128000 19.1 / 16.9 / 17.5, 64 over
-// 10000 17.3 / 13.0 / 13.0.
+// Least elements of a part, us with 4096 / 8192 / 16384: chain over 32000 11.1 / 10.9 / 9.2 (no
+// meeting), 16 trees over 50000 21.6 / 21.1 / 22.8, 4 over 128000 19.5 / 17.0 / 17.8, 64 over
+// 10000 18.1 / 13.2 / 13.1, 4 chains over 32000 11.6 / 12.1 / 11.4, 64 12.6 / 14.2 / 14.0.
 constexpr int kPartElements = 16384;
 constexpr int kPolls = 256;  // of a missing sum: about 50 us
 
